@@ -91,6 +91,11 @@ _SIGS = [
     ("g4h_attn_decode_window", _int, [_vp, _vp, _vp, _int, _int, _int, _int, _int, _int, _int, _vp, _vp, _sz, _vp]),
     ("g4h_attn_prefill", _int, [_vp, _vp, _vp, _int, _int, _int, _int, _int, _int, _vp, _vp, _sz, _vp]),
     ("g4h_attn_prefill_workspace_bytes", _sz, [_int, _int, _int, _int]),
+    ("g4h_paged_pool_bytes", _sz, [_int, _int, _int, _int, _i64]),
+    ("g4h_paged_append", _int, [_vp, _vp, _vp, _int, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
+    ("g4h_paged_read", _int, [_vp, _vp, _int, _vp, _vp, _vp]),
+    ("g4h_paged_attn_workspace_bytes", _sz, [_vp, _vp, _int]),
+    ("g4h_paged_attn", _int, [_vp, _vp, _int, _vp, _sz, C.c_float, C.c_float, _int, _vp, _sz, _vp, _sz, _vp]),
     ("g4h_kv_store", _int, [_int, _vp, _vp, _int, _int, _sz, _vp]),
     ("g4h_model_create", _int, [_vp, C.c_uint64, C.POINTER(_vp)]),
     ("g4h_model_free", _int, [_vp]),
@@ -458,6 +463,107 @@ def attn_prefill(q, kc, vc, kv_type: int, n_head: int, n_kv: int, hd: int, pos0:
 
 def kv_store(kv_type: int, src, dst, hd: int, rows: int = 1, dst_stride: int = 0, stream=None) -> None:
     check(lib().g4h_kv_store(kv_type, _p(src), _p(dst), hd, rows, dst_stride, stream))
+
+
+# ------------------------------------------------------------ paged KV cache
+# g4h_paged_kv.status_dev flags
+PAGED_BAD_PAGE, PAGED_BAD_BATCH = 1, 2
+
+
+class _PagedKV(C.Structure):
+    _fields_ = [("kv_type", _int), ("n_kv", _int), ("hd", _int), ("page", _int), ("n_pages", _i64), ("k_dev", _vp), ("v_dev", _vp),
+                ("status_dev", _vp)]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [("n_seq", _int), ("n_tok", _int), ("q_off_dev", _vp), ("len_dev", _vp), ("table_dev", _vp), ("table_stride", _int),
+                ("max_len", _int), ("n_prefix", _int), ("prefix_dev", _vp)]
+
+
+class _Rope(C.Structure):
+    _fields_ = [("n_rot", _int), ("interleaved", _int), ("base", C.c_double), ("factor_dev", _vp)]
+
+
+def paged_pool_bytes(kv_type: int, n_kv: int, hd: int, page: int, n_pages: int) -> int:
+    return lib().g4h_paged_pool_bytes(kv_type, n_kv, hd, page, n_pages)
+
+
+class PagedKV:
+    """The pools of a paged KV cache (g4h_paged_kv): k and v are device memory
+    of paged_pool_bytes each (allocated here if not given), and a status word."""
+
+    def __init__(self, kv_type: int, n_kv: int, hd: int, page: int, n_pages: int, k=None, v=None, status=None):
+        nbytes = paged_pool_bytes(kv_type, n_kv, hd, page, n_pages)
+        if not nbytes:
+            raise G4HError(ERR_SHAPE, lib().g4h_last_error().decode())
+        init()
+        self.k = Buffer(nbytes) if k is None else k
+        self.v = Buffer(nbytes) if v is None else v
+        if status is None:
+            status = Buffer.from_array(np.zeros(1, np.int32))
+        self.status_word = status
+        self.struct = _PagedKV(kv_type, n_kv, hd, page, n_pages, _p(self.k), _p(self.v), _p(status))
+        self.ref = C.byref(self.struct)
+
+    def status(self, stream=None) -> int:
+        """The PAGED_* flags that calls have set since the last query
+        (synchronizes the stream); clears them."""
+        word = np.empty(1, np.int32)
+        check(lib().g4h_memcpy_d2h(word.ctypes.data_as(_vp), self.struct.status_dev, 4, stream))
+        if word[0]:
+            check(lib().g4h_memset(self.struct.status_dev, 0, 4, stream))
+        return int(word[0])
+
+
+class PagedBatch:
+    """A batch of sequences over a paged KV cache (g4h_paged_batch); lens,
+    table, q_off and prefix are device arrays of int32."""
+
+    def __init__(self, n_seq: int, n_tok: int, lens, table, table_stride: int, max_len: int, q_off=None, n_prefix: int = 0, prefix=None):
+        self.keep = (lens, table, q_off, prefix)
+        self.struct = _PagedBatch(n_seq, n_tok, _p(q_off), _p(lens), _p(table), table_stride, max_len, n_prefix, _p(prefix))
+        self.ref = C.byref(self.struct)
+
+
+class Rope:
+    """RoPE settings (g4h_rope); factors: a device array of n_rot / 2 floats."""
+
+    def __init__(self, n_rot: int, base: float, interleaved: bool = False, factors=None):
+        self.keep = factors
+        self.struct = _Rope(n_rot, 1 if interleaved else 0, base, _p(factors))
+        self.ref = C.byref(self.struct)
+
+
+def paged_append(kv: PagedKV, batch: PagedBatch, k, v, q=None, q_out=None, n_head: int = 0, rope=None, q_stride: int = 0,
+                 q_out_stride: int = 0, k_stride: int = 0, v_stride: int = 0, stream=None) -> None:
+    """Rotate and store the batch's new key and value rows; with n_head, rotate
+    its queries into q_out."""
+    check(lib().g4h_paged_append(kv.ref, batch.ref, rope.ref if rope else None, n_head, _p(q), q_stride, _p(q_out), q_out_stride,
+                                 _p(k), k_stride, _p(v), v_stride, stream))
+
+
+def paged_read(kv: PagedKV, batch: PagedBatch, k_out=None, v_out=None, out_type: int = F32, stream=None) -> None:
+    """The cached rows of the batch's new tokens as values."""
+    check(lib().g4h_paged_read(kv.ref, batch.ref, out_type, _p(k_out), _p(v_out), stream))
+
+
+def paged_attn_workspace_bytes(kv: PagedKV, batch: PagedBatch, n_head: int) -> int:
+    return lib().g4h_paged_attn_workspace_bytes(kv.ref, batch.ref, n_head)
+
+
+def paged_attn(kv: PagedKV, batch: PagedBatch, q, n_head: int, out, scale: float = 1.0, softcap: float = 0.0, window: int = 0, ws=None,
+               q_stride: int = 0, out_stride: int = 0, stream=None) -> None:
+    """Attention of the batch's new tokens over the paged cache; ws: a Buffer of
+    paged_attn_workspace_bytes (allocated here, and the stream waited for, if
+    not given)."""
+    need = 0 if isinstance(ws, Buffer) else paged_attn_workspace_bytes(kv, batch, n_head)
+    made = ws is None and need > 0
+    if made:
+        ws = Buffer(need)
+    check(lib().g4h_paged_attn(kv.ref, batch.ref, n_head, _p(q), q_stride, scale, softcap, window, _p(out), out_stride, _p(ws),
+                               ws.nbytes if isinstance(ws, Buffer) else need, stream))
+    if made:
+        synchronize(stream)                          # before the workspace goes
 
 
 # ---------------------------------------------------------------- decode step

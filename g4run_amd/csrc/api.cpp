@@ -3,6 +3,7 @@
 #include "../../include/g4hip.h"
 
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -10,6 +11,7 @@
 #include <unordered_map>
 
 #include "kernels.h"
+#include "paged.h"
 
 using namespace g4;
 
@@ -907,5 +909,177 @@ extern "C" int g4h_kv_store(int kv_type, const float *src, void *dst, int hd, in
     if ((uintptr_t)dst % 2 || dst_stride % 2) return fail(G4H_ERR_ARG, "g4h_kv_store: destination must be 2-byte aligned");
     if (rows == 0) return G4H_OK;
     G4_HIP(launch_kv_store(kv_type, src, (uint8_t *)dst, hd, rows, dst_stride, (hipStream_t)stream));
+    return G4H_OK;
+}
+
+// ------------------------------------------------------ paged KV cache ----
+// Arguments are checked before the device is, so that refusals are the same
+// with and without one.
+static int check_paged_shape(const char *fn, int kv_type, int n_kv, int hd, int page, int64_t n_pages) {
+    if (kv_type != F16 && kv_type != Q8_0 && kv_type != Q4_0)
+        return fail(G4H_ERR_TYPE, "%s: KV type %d unsupported (f16, q8_0, q4_0)", fn, kv_type);
+    if (hd != 64 && hd != 128 && hd != 256 && hd != 512) return fail(G4H_ERR_SHAPE, "%s: hd=%d (64, 128, 256 or 512)", fn, hd);
+    if (page < 16 || page % 16 || page > PAGED_MAX_PAGE) return fail(G4H_ERR_SHAPE, "%s: page=%d (a multiple of 16 up to %d)", fn, page, PAGED_MAX_PAGE);
+    if (n_kv < 1 || (int64_t)n_kv * page * hd * 2 > 0x7fffffff) return fail(G4H_ERR_SHAPE, "%s: n_kv=%d (a page must stay below 2 GiB)", fn, n_kv);
+    if (n_pages < 1 || n_pages > 0x7fffffff) return fail(G4H_ERR_ARG, "%s: n_pages=%lld", fn, (long long)n_pages);
+    return G4H_OK;
+}
+static size_t paged_page_bytes(int kv_type, int n_kv, int hd, int page) {
+    return (size_t)n_kv * page * (paged_row_bytes(kv_type, hd) + (kv_type == F16 ? 0 : hd / 16));
+}
+extern "C" size_t g4h_paged_pool_bytes(int kv_type, int n_kv, int hd, int page, int64_t n_pages) {
+    if (check_paged_shape("g4h_paged_pool_bytes", kv_type, n_kv, hd, page, n_pages)) return 0;
+    return paged_page_bytes(kv_type, n_kv, hd, page) * (size_t)n_pages;
+}
+// the pools and the batch of a call
+static int paged_args(const char *fn, const g4h_paged_kv *kv, const g4h_paged_batch *batch, PagedPool &p, PagedBatch &b, bool sizes_only = false) {
+    if (!kv || !batch) return fail(G4H_ERR_ARG, "%s: null pointer", fn);
+    if (int rc = check_paged_shape(fn, kv->kv_type, kv->n_kv, kv->hd, kv->page, kv->n_pages)) return rc;
+    if (batch->n_seq < 0 || batch->n_tok < 0 || batch->table_stride < 0 || batch->max_len < 0 || batch->max_len > PAGED_MAX_POS ||
+        batch->n_prefix < 0 || batch->n_prefix > PAGED_MAX_POS)
+        return fail(G4H_ERR_ARG, "%s: n_seq=%d n_tok=%d table_stride=%d max_len=%d n_prefix=%d", fn, batch->n_seq, batch->n_tok,
+                    batch->table_stride, batch->max_len, batch->n_prefix);
+    if (batch->n_tok > 1 << 24 || (int64_t)batch->n_seq * kv->n_kv > 1 << 22)
+        return fail(G4H_ERR_ARG, "%s: n_tok=%d (up to 2^24), n_seq=%d (n_seq * n_kv up to 2^22)", fn, batch->n_tok, batch->n_seq);
+    if (!sizes_only) {
+        if (!kv->k_dev || !kv->v_dev || (uintptr_t)kv->k_dev % 16 || (uintptr_t)kv->v_dev % 16)
+            return fail(G4H_ERR_ARG, "%s: pools must be 16-byte aligned device memory", fn);
+        if (batch->n_seq && batch->n_tok && (!batch->len_dev || !batch->table_dev)) return fail(G4H_ERR_ARG, "%s: null lengths or page table", fn);
+        if ((uintptr_t)batch->len_dev % 4 || (uintptr_t)batch->table_dev % 4 || (uintptr_t)batch->q_off_dev % 4 || (uintptr_t)batch->prefix_dev % 4 ||
+            (uintptr_t)kv->status_dev % 4)
+            return fail(G4H_ERR_ARG, "%s: index arrays must be 4-byte aligned", fn);
+    }
+    p.k = (uint8_t *)kv->k_dev;
+    p.v = (uint8_t *)kv->v_dev;
+    p.n_pages = kv->n_pages;
+    p.page_bytes = paged_page_bytes(kv->kv_type, kv->n_kv, kv->hd, kv->page);
+    p.type = kv->kv_type;
+    p.n_kv = kv->n_kv;
+    p.hd = kv->hd;
+    p.page = kv->page;
+    p.units = kv->page / 16;
+    p.inv = p.units == 1 ? 0 : (uint32_t)(0x100000000ull / p.units + 1);
+    p.sc_off = kv->kv_type == F16 ? 0 : (uint32_t)((size_t)kv->n_kv * kv->page * paged_row_bytes(kv->kv_type, kv->hd));
+    p.status = kv->status_dev;
+    b.n_seq = batch->n_seq;
+    b.n_tok = batch->n_tok;
+    b.q_off = batch->q_off_dev;
+    b.len = batch->len_dev;
+    b.table = batch->table_dev;
+    b.table_stride = batch->table_stride;
+    b.max_len = batch->max_len;
+    b.n_prefix = batch->n_prefix;
+    b.prefix = batch->prefix_dev;
+    return G4H_OK;
+}
+// a row array's stride: packed for 0, else at least a row; 4-byte aligned
+static int paged_rows(const char *fn, const char *what, const void *ptr, size_t &stride, size_t row, int n_tok) {
+    if (!ptr || (uintptr_t)ptr % 4) return fail(G4H_ERR_ARG, "%s: %s must be 4-byte aligned device memory", fn, what);
+    if (stride == 0) stride = row;
+    if (stride < row && n_tok > 1) return fail(G4H_ERR_ARG, "%s: %s stride %zu is smaller than a row of %zu", fn, what, stride, row);
+    return G4H_OK;
+}
+
+extern "C" int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_rope *rope, int n_head, const float *q,
+                                size_t q_stride, float *q_out, size_t q_out_stride, const float *k, size_t k_stride, const float *v,
+                                size_t v_stride, void *stream) {
+    const char *fn = "g4h_paged_append";
+    PagedAppend a;
+    if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
+    if (n_head < 0 || n_head > 65536) return fail(G4H_ERR_ARG, "%s: n_head=%d", fn, n_head);
+    const size_t row = (size_t)a.p.n_kv * a.p.hd, qrow = (size_t)n_head * a.p.hd;
+    if (int rc = paged_rows(fn, "k", k, k_stride, row, a.b.n_tok)) return rc;
+    if (int rc = paged_rows(fn, "v", v, v_stride, row, a.b.n_tok)) return rc;
+    if (n_head) {
+        if (int rc = paged_rows(fn, "q", q, q_stride, qrow, a.b.n_tok)) return rc;
+        if (int rc = paged_rows(fn, "q_out", q_out, q_out_stride, qrow, a.b.n_tok)) return rc;
+        if (q == q_out && q_stride != q_out_stride && a.b.n_tok > 1) return fail(G4H_ERR_ARG, "%s: q rotated in place keeps its stride", fn);
+    }
+    a.r.n_rot = 0;
+    a.r.interleaved = 0;
+    a.r.log2_base = 0.0;
+    a.r.factor = nullptr;
+    if (rope && rope->n_rot) {
+        if (rope->n_rot < 0 || rope->n_rot % 8 || rope->n_rot > a.p.hd)
+            return fail(G4H_ERR_SHAPE, "%s: n_rot=%d (a multiple of 8 up to hd=%d)", fn, rope->n_rot, a.p.hd);
+        if (!(rope->base > 0.0) || !std::isfinite(rope->base)) return fail(G4H_ERR_ARG, "%s: rope base %g", fn, rope->base);
+        if ((uintptr_t)rope->factor_dev % 4) return fail(G4H_ERR_ARG, "%s: rope factors must be 4-byte aligned", fn);
+        a.r.n_rot = rope->n_rot;
+        a.r.interleaved = rope->interleaved != 0;
+        a.r.log2_base = std::log2(rope->base);
+        a.r.factor = rope->factor_dev;
+    }
+    a.n_head = n_head;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.qs = q_stride;
+    a.qos = q_out_stride;
+    a.ks = k_stride;
+    a.vs = v_stride;
+    G4_NEED_INIT();
+    G4_HIP(launch_paged_append(a, (hipStream_t)stream));
+    return G4H_OK;
+}
+
+extern "C" int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out_type, void *k_out, void *v_out, void *stream) {
+    const char *fn = "g4h_paged_read";
+    PagedRead a;
+    if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
+    if (out_type != F16 && out_type != F32) return fail(G4H_ERR_TYPE, "%s: output type %d unsupported (f32, f16)", fn, out_type);
+    const uintptr_t al = out_type == F16 ? 2 : 4;
+    if ((!k_out && !v_out) || (uintptr_t)k_out % al || (uintptr_t)v_out % al) return fail(G4H_ERR_ARG, "%s: null or misaligned outputs", fn);
+    a.k_out = k_out;
+    a.v_out = v_out;
+    a.f16 = out_type == F16;
+    G4_NEED_INIT();
+    G4_HIP(launch_paged_read(a, (hipStream_t)stream));
+    return G4H_OK;
+}
+
+static int check_paged_heads(const char *fn, const PagedPool &p, const PagedBatch &b, int n_head) {
+    if (n_head < 1 || n_head % p.n_kv) return fail(G4H_ERR_SHAPE, "%s: n_head=%d not a multiple of n_kv=%d", fn, n_head, p.n_kv);
+    if ((int64_t)b.n_tok * n_head > 1 << 24) return fail(G4H_ERR_ARG, "%s: n_tok * n_head = %lld (up to 2^24)", fn, (long long)b.n_tok * n_head);
+    return G4H_OK;
+}
+extern "C" size_t g4h_paged_attn_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head) {
+    const char *fn = "g4h_paged_attn_workspace_bytes";
+    PagedPool p;
+    PagedBatch b;
+    if (paged_args(fn, kv, batch, p, b, true) || check_paged_heads(fn, p, b, n_head)) return 0;
+    return paged_attn_workspace(p, b, n_head);
+}
+extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head, const float *q, size_t q_stride, float scale,
+                              float softcap, int window, float *out, size_t out_stride, void *ws, size_t ws_bytes, void *stream) {
+    const char *fn = "g4h_paged_attn";
+    PagedAttn a;
+    if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
+    if (int rc = check_paged_heads(fn, a.p, a.b, n_head)) return rc;
+    const size_t row = (size_t)n_head * a.p.hd;
+    if (int rc = paged_rows(fn, "q", q, q_stride, row, a.b.n_tok)) return rc;
+    if (int rc = paged_rows(fn, "out", out, out_stride, row, a.b.n_tok)) return rc;
+    if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f || window < 0)
+        return fail(G4H_ERR_ARG, "%s: scale=%g softcap=%g window=%d", fn, scale, softcap, window);
+    if (a.b.n_prefix && !a.b.prefix) return fail(G4H_ERR_ARG, "%s: a prefix of %d positions needs its pages", fn, a.b.n_prefix);
+    if (a.b.n_tok) {
+        const size_t n = a.b.n_tok - 1;
+        if (q < out + n * out_stride + row && out < q + n * q_stride + row) return fail(G4H_ERR_ARG, "%s: q and out overlap", fn);
+    }
+    const size_t need = paged_attn_workspace(a.p, a.b, n_head);
+    if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
+        return fail(G4H_ERR_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, ws ? ws_bytes : (size_t)0);
+    a.n_head = n_head;
+    a.grp = n_head / a.p.n_kv;
+    a.q = q;
+    a.out = out;
+    a.qs = q_stride;
+    a.os = out_stride;
+    a.scale = scale;
+    a.cap = softcap;
+    a.window = window;
+    a.ws = (uint8_t *)ws;
+    G4_NEED_INIT();
+    G4_HIP(launch_paged_attn(a, (hipStream_t)stream));
     return G4H_OK;
 }

@@ -269,6 +269,104 @@ size_t g4h_attn_prefill_workspace_bytes(int n_head, int hd, int pos0, int nb);
 int g4h_kv_store(int kv_type, const float *src_dev, void *dst_dev, int hd, int rows,
                  size_t dst_stride, void *stream);
 
+/* ------------------------------------------------------ paged KV cache ---- */
+/* A batch of sequences over one pool of pages (no counterpart in the
+ * reference, whose cache holds one sequence, model.c:437-449): rows are rotated
+ * and appended for all sequences in one call, and one attention call serves
+ * single tokens, prompt chunks and mixtures of both.
+ *
+ * The pools hold n_pages pages of `page` slots for n_kv heads of hd elements,
+ * g4h_paged_pool_bytes() each for keys and for values, 16-byte aligned:
+ *   G4H_F16         a page is [n_kv][page][hd] halves;
+ *   G4H_Q8_0, Q4_0  the quants of its [n_kv][page] rows, then their fp16 scales
+ *                   [n_kv][page][hd / 32].  Key element e = 32 s + 8 g + j: q8_0
+ *                   byte g hd/4 + 8 s + j, q4_0 nibble (j >> 1) + 4 (j & 1) of
+ *                   dword g hd/32 + s; value element e = 16 m + c: q8_0 byte
+ *                   c hd/16 + m, q4_0 nibble m of those starting at byte
+ *                   c hd/32.  A q8_0 byte holds quant + 128, a nibble quant + 8.
+ * Limits: page a multiple of 16 up to 4096; hd 64, 128, 256 or 512; a page
+ * below 2 GiB; any n_pages >= 1 (offsets are 64-bit). */
+typedef struct {
+    int kv_type;           /* G4H_F16, G4H_Q8_0 or G4H_Q4_0 */
+    int n_kv, hd, page;
+    int64_t n_pages;
+    void *k_dev, *v_dev;
+    int *status_dev;       /* one device word that calls OR G4H_PAGED_* into, or NULL */
+} g4h_paged_kv;
+/* What a call found in the batch's device arrays: a page id outside
+ * [0, n_pages) where a position is stored or read; a length outside [0,
+ * max_len] or past the table's table_stride pages, offsets that descend or
+ * leave [0, n_tok].  Such rows are not appended, and read as NaN by the
+ * attention; nothing outside the pools and the given arrays is touched. */
+enum { G4H_PAGED_BAD_PAGE = 1, G4H_PAGED_BAD_BATCH = 2 };
+/* The batch.  Its arrays live on the device, so that a captured graph is
+ * replayed with other lengths and pages; the host values bound them.  Sequence
+ * s has q_off[s+1] - q_off[s] new tokens, rows q_off[s] .. of the activations
+ * (q_off_dev NULL: one each, row s), and len[s] positions in its own pages, the
+ * new tokens last: token i of n sits at len - n + i.  A token before position 0
+ * (a slot of a padded batch with len 0) has no position: it is not appended and
+ * attends nothing.  Rows behind the last sequence's are left as they were.
+ * With n_prefix, every sequence continues a prefix of n_prefix positions whose
+ * rows are in the pages prefix_dev[0 .. ceil(n_prefix / page)), shared by all:
+ * own position p is position n_prefix + p. */
+typedef struct {
+    int n_seq, n_tok;          /* sequences; rows of the activations (any counts >= 0) */
+    const int *q_off_dev;      /* n_seq + 1 ascending offsets, or NULL */
+    const int *len_dev;        /* n_seq lengths, 0 .. max_len */
+    const int *table_dev;      /* n_seq rows of table_stride page ids, position p in entry p / page */
+    int table_stride;
+    int max_len;               /* most own positions of a sequence, up to 2^26 */
+    int n_prefix;              /* 0 .. 2^26 */
+    const int *prefix_dev;     /* the prefix's page ids (append and read do not use them) */
+} g4h_paged_batch;
+/* RoPE of the first n_rot (a multiple of 8 up to hd; 0: none) elements of a
+ * head: pair i turns by position * base^(-2 i / n_rot) / factor[i], the angle
+ * taken in 64 bits; pairs are (i, i + n_rot / 2), or (2 i, 2 i + 1) with
+ * interleaved. */
+typedef struct {
+    int n_rot, interleaved;
+    double base;
+    const float *factor_dev;   /* n_rot / 2 divisors (rope_freqs), or NULL */
+} g4h_rope;
+
+/* bytes of one pool; 0 for a bad type or shape */
+size_t g4h_paged_pool_bytes(int kv_type, int n_kv, int hd, int page, int64_t n_pages);
+/* Appends the batch's new rows: k (rotated by `rope`, NULL: as it is) and v,
+ * fp32 [n_tok][n_kv][hd] at k_stride / v_stride floats per token (0: packed),
+ * rounded to the cache's type as g4h_kv_store does; and, with n_head > 0, the
+ * queries q [n_tok][n_head][hd] rotated into q_out (q itself, at the same
+ * stride, or another array).  Strides let all three be parts of one fused
+ * projection's rows.  Two tokens of one batch must not share a slot.
+ * Asynchronous, capturable, needs no workspace. */
+int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_rope *rope, int n_head, const float *q_dev,
+                     size_t q_stride, float *q_out_dev, size_t q_out_stride, const float *k_dev, size_t k_stride,
+                     const float *v_dev, size_t v_stride, void *stream);
+/* The cached rows of the batch's new tokens as values: k_out / v_out (either
+ * may be NULL) packed [n_tok][n_kv][hd] of out_type G4H_F32 (exact) or G4H_F16
+ * (rounded).  With q_off spanning whole sequences this reads them out.
+ * Tokens without a position or with a bad page are left as they were. */
+int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out_type, void *k_out_dev, void *v_out_dev,
+                   void *stream);
+/* Attention of the batch's new tokens, their own rows already appended.  A
+ * token at position p (prefix included) attends positions max(0, p + 1 -
+ * window) .. p (window 0: 0 .. p):
+ *   s_j = scale * q . k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);
+ *   out = sum_j softmax(s)_j v_j, zeros for a token without a position.
+ * q / out: fp32 [n_tok][n_head][hd], at q_stride / out_stride floats per token
+ * (0: packed); query head h reads KV head h / (n_head / n_kv).  All in fp32
+ * precision (queries and weights enter the matrix cores as two halves each),
+ * unlike g4h_attn_decode, which rounds as the reference does.  The prefix's
+ * rows are read once for the whole batch.  A non-finite cached value reaches
+ * the rows that attend it and no others.  ws: g4h_paged_attn_workspace_bytes()
+ * of caller-owned scratch, 16-byte aligned; it needs no initial contents and
+ * keeps nothing from call to call, but calls that overlap must not share it.
+ * Asynchronous, capturable.  A row's bits depend on the batch it runs in (on
+ * how the positions are split), not on the run. */
+size_t g4h_paged_attn_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head);
+int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head, const float *q_dev, size_t q_stride,
+                   float scale, float softcap, int window, float *out_dev, size_t out_stride, void *ws_dev, size_t ws_bytes,
+                   void *stream);
+
 /* -------------------------------------------------------- decode step ---- */
 /* A gemma-style decoder resident on the device (the model behind
  * g4_ctx_init / g4_forward, g4run.h:303-311): layer order of model.c:647-736
