@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a) {
         }
         if (own < 0) continue;
         const int ent = paged_entry(p, own >> 4), slot = own - ent * p.page;
-        const int id = a.b.table[(size_t)seq * a.b.table_stride + ent];
+        const int id = paged_ld(a.b.table, (int64_t)seq * a.b.table_stride + ent);
         const bool stored = (uint64_t)(int64_t)id < (uint64_t)p.n_pages;
         if (!stored && threadIdx.x == 0) paged_flag(p, PAGED_BAD_PAGE);
         if (half) {
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedRead a) {
     }
     if (own < 0) return;
     const int ent = paged_entry(p, own >> 4), slot = own - ent * p.page;
-    const int id = a.b.table[(size_t)seq * a.b.table_stride + ent];
+    const int id = paged_ld(a.b.table, (int64_t)seq * a.b.table_stride + ent);
     if ((uint64_t)(int64_t)id >= (uint64_t)p.n_pages) {
         if (threadIdx.x == 0) paged_flag(p, PAGED_BAD_PAGE);
         return;

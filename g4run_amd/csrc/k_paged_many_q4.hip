@@ -1,0 +1,8 @@
+// k_paged_many_q4.hip -- k_paged_many (paged_many.h) over Q4_0 pages
+#include "paged_many.h"
+
+namespace g4 {
+
+hipError_t pa_many_q4(const PagedAttn &a, const PagedPlan &pl, unsigned blocks, hipStream_t s) { return pa_many<Q4_0>(a, pl, blocks, s); }
+
+}  // namespace g4

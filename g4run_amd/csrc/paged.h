@@ -45,6 +45,13 @@ __device__ __forceinline__ void paged_flag(const PagedPool &p, int bits) {
     if (p.status) atomicOr(p.status, bits);
 }
 
+// The batch's arrays do not change while a call runs: read through the constant
+// address space, a wave-uniform index takes a scalar load, which does not wait
+// behind the vector loads in flight.
+__device__ __forceinline__ int paged_ld(const int *p, int64_t i) {
+    return ((const __attribute__((address_space(4))) int *)p)[i];
+}
+
 // A sequence as a call may use it: its tokens [t0, t0 + nq) within n_tok, its
 // length; bad lengths and offsets are flagged by the caller.
 struct PagedSeq {
@@ -53,10 +60,10 @@ struct PagedSeq {
 };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedPool &p, const PagedBatch &b, int s) {
     PagedSeq r;
-    r.len = b.len[s];
+    r.len = paged_ld(b.len, s);
     r.bad = r.len < 0 || r.len > b.max_len || (int64_t)r.len > (int64_t)b.table_stride * p.page;
     if (b.q_off) {
-        const int a = b.q_off[s], e = b.q_off[s + 1];
+        const int a = paged_ld(b.q_off, s), e = paged_ld(b.q_off, s + 1);
         r.t0 = min(max(a, 0), b.n_tok);
         r.nq = min(max(e, r.t0), b.n_tok) - r.t0;
         if (r.t0 != a || r.t0 + r.nq != e) r.bad = true;
@@ -75,7 +82,7 @@ __device__ __forceinline__ int paged_find(const PagedBatch &b, int t) {
     int n = 0;
     for (int s0 = 1; s0 <= b.n_seq; s0 += 64) {
         const int s = s0 + lane;
-        n += __popcll(__ballot(s <= b.n_seq && b.q_off[s] <= t));
+        n += __popcll(__ballot(s <= b.n_seq && paged_ld(b.q_off, s) <= t));
     }
     return n;
 }

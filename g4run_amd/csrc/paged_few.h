@@ -1,0 +1,516 @@
+// paged_few.h -- attention of a few rows over the paged KV cache (paged_attn.h):
+// single tokens of many sequences, short drafts, the prefix of a small batch.
+//
+// Bound by the cache's bytes.  The call's positions are one list of steps (one
+// KV head of one sequence: few_unit positions each), cut into equal shares for
+// workgroups that all fit on the device at once, so ragged lengths leave no
+// workgroup idle.  A piece (a share's part of one sequence and head) that is
+// the whole sequence is written out; the first and last piece of a share
+// go through the workspace.
+//
+// A workgroup's 4 waves take 32 positions each of a step of 128, on
+// v_mfma_f32_16x16x32_f16 with the rows as columns.  Up to 8 rows (ST) sit as
+// high halves in columns 0..7 and low halves in 8..15: the second half costs no
+// matrix instruction.  K and V go from the pages to registers, each lane's loads
+// being the operand's runs of bytes (the layout of the quantized rows is made for
+// it); f16 value rows are turned (8 positions x 2 elements) with v_perm_b32.  A
+// step's K registers are loaded again as soon as its scores are taken, its V
+// registers after the sums.  Heads of 256 and 512: two and four waves share 32
+// positions, each with 128 of the elements, their scores added through LDS (whole
+// heads of 256 in one wave's registers spilled: 32 sequences of up to 8192
+// positions, 8 q / 4 kv heads, 188 us).
+#pragma once
+
+#include "paged_attn.h"
+
+namespace g4 {
+
+// Operands of 32 positions and HE elements of the head (one wave's): raw bytes.
+template <int HE, int KVT>
+struct PaTile {
+    static constexpr int KW = KVT == Q4_0 ? HE / 32 : HE / 16;                           // dwords of a lane's key run (f16: of four)
+    static constexpr int VW = KVT == F16 ? HE / 32 : KVT == Q8_0 ? HE / 64 : (HE >= 128 ? HE / 128 : 1);
+    static constexpr int DW = HE / 64;                                                   // dwords of a row's scales
+    uint32_t k[2][KVT == F16 ? HE / 8 : KW];   // [unit][dwords]
+    uint32_t v[8][VW];                         // [position 4 t + i][dwords]
+    uint32_t dk[KVT == F16 ? 1 : 8][DW], dv[KVT == F16 ? 1 : 8][DW];
+};
+
+template <int HD, int HE, int KVT>
+__device__ __forceinline__ void pa_load_k(PaTile<HE, KVT> &t, const PagedPool &p, const PaUnit u[2], int c, int g, int ew) {
+    using T = PaTile<HE, KVT>;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint8_t *row = p.k + u[h].row + c * paged_row_bytes(KVT, HD);
+        if constexpr (KVT == F16) {
+#pragma unroll
+            for (int s = 0; s < HE / 32; s++) pa_load<4>(t.k[h] + 4 * s, row + 2 * HE * ew + 64 * s + 16 * g);
+        } else {
+            pa_load<T::KW>(t.k[h], row + 4 * T::KW * ((HD / HE) * g + ew));
+#pragma unroll
+            for (int i = 0; i < 4; i++) pa_load<T::DW>(t.dk[4 * h + i], p.k + u[h].sc + (4 * g + i) * (HD / 16) + (HE / 16) * ew);
+        }
+    }
+}
+template <int HD, int HE, int KVT>
+__device__ __forceinline__ void pa_load_v(PaTile<HE, KVT> &t, const PagedPool &p, const PaUnit u[2], int c, int g, int ew) {
+    using T = PaTile<HE, KVT>;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int i = 4 * g + (j & 3);
+        const uint8_t *row = p.v + u[j >> 2].row + i * paged_row_bytes(KVT, HD);
+        if constexpr (KVT == F16 && HE == 64) {
+            pa_load<2>(t.v[j], row + 8 * c);
+        } else if constexpr (KVT == F16) {
+#pragma unroll
+            for (int n = 0; n < HE / 128; n++) pa_load<4>(t.v[j] + 4 * n, row + 2 * HE * ew + 256 * n + 16 * c);
+        } else if constexpr (KVT == Q4_0 && HE == 64) {
+            t.v[j][0] = *(const uint16_t *)(row + 2 * c);
+        } else {
+            pa_load<T::VW>(t.v[j], row + 4 * T::VW * ((HD / HE) * c + ew));
+        }
+        if constexpr (KVT != F16) pa_load<T::DW>(t.dv[j], p.v + u[j >> 2].sc + i * (HD / 16) + (HE / 16) * ew);
+    }
+}
+
+// key operand of unit h, 32 elements s
+template <int HE, int KVT>
+__device__ __forceinline__ pa_v8h pa_key(const PaTile<HE, KVT> &t, int h, int s) {
+    if constexpr (KVT == F16) return pa_op(t.k[h][4 * s], t.k[h][4 * s + 1], t.k[h][4 * s + 2], t.k[h][4 * s + 3]);
+    else if constexpr (KVT == Q8_0) {
+        const uint32_t a = t.k[h][2 * s], b = t.k[h][2 * s + 1];
+        return pa_op(pa_q8(__builtin_amdgcn_perm(0, a, 0x0c010c00u)), pa_q8(__builtin_amdgcn_perm(0, a, 0x0c030c02u)),
+                     pa_q8(__builtin_amdgcn_perm(0, b, 0x0c010c00u)), pa_q8(__builtin_amdgcn_perm(0, b, 0x0c030c02u)));
+    } else {
+        const uint32_t w = t.k[h][s];
+        return pa_op(pa_q4(pa_nib(w, 0)), pa_q4(pa_nib(w, 1)), pa_q4(pa_nib(w, 2)), pa_q4(pa_nib(w, 3)));
+    }
+}
+// value operand of the 16 elements m (pa_elem) over the 32 positions
+template <int HE, int KVT>
+__device__ __forceinline__ pa_v8h pa_value(const PaTile<HE, KVT> &t, int m) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (KVT == F16) {
+            const int d = HE == 64 ? m >> 1 : 4 * (m >> 3) + ((m & 7) >> 1);
+            w[k] = __builtin_amdgcn_perm(t.v[2 * k + 1][d], t.v[2 * k][d], (m & 1) ? 0x07060302u : 0x05040100u);
+        } else if constexpr (KVT == Q8_0) {
+            const uint32_t b = m & 3;
+            w[k] = pa_q8(__builtin_amdgcn_perm(t.v[2 * k + 1][m >> 2], t.v[2 * k][m >> 2], 0x0c000c00u | b | ((4 + b) << 16)));
+        } else {
+            const int d = m >> 3, n = m & 3;
+            w[k] = pa_q4(__builtin_amdgcn_perm(pa_nib(t.v[2 * k + 1][d], n), pa_nib(t.v[2 * k][d], n), (m & 4) ? 0x07060302u : 0x05040100u));
+        }
+    }
+    return pa_op(w[0], w[1], w[2], w[3]);
+}
+// element (of the wave's HE) that value tile m holds in its operand row x (0..15)
+template <int HE, int KVT>
+__device__ __forceinline__ int pa_elem(int m, int x) {
+    return KVT != F16 ? 16 * m + x : HE == 64 ? 4 * x + m : 128 * (m >> 3) + 8 * x + (m & 7);
+}
+
+template <int HD, int KVT, bool ST>
+__global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl) {
+    constexpr int R = ST ? 8 : 16, HE = HD > 128 ? 128 : HD, ES = HD / HE, PW = 4 / ES, NS = HE / 32, NM = HE / 16;
+    constexpr int QP = HD + 8;                               // padded query row
+    constexpr size_t QB = 2 * R * QP * 2, OB = (size_t)PW * 8 * (HD + 4) * 4;
+    __shared__ __align__(16) uint8_t lds[QB > OB ? QB : OB]; // the queries' halves [2][R][QP]; then sums [PW][8][HD + 4]
+    __shared__ float qsc[R];
+    __shared__ float2 wml[4][R];                             // two waves of one tile may differ in m (by their elements' scales)
+    __shared__ __align__(16) float xs[ES > 1 ? 2 : 1][ES > 1 ? 4 : 1][ES > 1 ? 64 : 1][8];   // partial scores of the waves of one tile
+    _Float16 *const qh = (_Float16 *)lds;
+    float *const buf = (float *)lds;
+    const int lane = threadIdx.x & 63, wave = pa_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, pw = wave / ES;
+    const PagedPool &p = a.p;
+    const PagedBatch &b = a.b;
+    const int G = a.grp, rc = ST ? c & 7 : c;
+
+    int mine;
+    const int total = pa_total(a, pl, mine), share = pa_share(total);
+    const int first = blockIdx.x * share, stop = min(first + share, total);
+    for (int u = first; u < stop;) {
+        // the piece: steps [step, step + n) of `all` of one KV head
+        const bool pre = u < pl.few_pre * p.n_kv;
+        PagedSeq sq;
+        int kvh, step, all, seglen, hi0, hi1, lo0, lo1, base0;
+        const int *table;
+        bool bad = false;
+        if (pre) {
+            sq.t0 = 0;
+            sq.nq = pa_tokens(b);
+            sq.bad = false;
+            all = pl.few_pre;
+            kvh = u / all;
+            step = u - kvh * all;
+            seglen = b.n_prefix;
+            table = b.prefix;
+            hi0 = hi1 = seglen - 1;
+            lo0 = 0;
+            lo1 = a.window ? 0x7fffffff : 0;                 // row by row
+            base0 = 0;
+            sq.len = seglen;
+        } else {
+            int seq, before;
+            const int v = u - pl.few_pre * p.n_kv;
+            pa_find_step(a, pl, mine, v, seq, before);
+            sq = paged_seq(p, b, seq);
+            const int low = pa_low(sq.len - sq.nq, a.window);
+            all = pa_seq_steps(a, pl, sq);
+            kvh = (v - before) / all;
+            step = v - before - kvh * all;
+            seglen = sq.bad ? 0 : sq.len;
+            bad = sq.bad;
+            table = b.table + (size_t)seq * b.table_stride;
+            hi0 = sq.len - sq.nq;
+            hi1 = sq.len - 1;
+            lo0 = a.window ? max(0, hi0 + 1 - a.window) : 0;
+            lo1 = a.window ? max(0, hi1 + 1 - a.window) : 0;
+            base0 = low;
+            if (bad && threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
+        }
+        const int n = min(all - step, stop - u), rows = sq.nq * G;
+        const bool whole = n == all;
+        const int slot = 2 * blockIdx.x + (u != first);
+        u += n;
+        const int start = base0 + (step << pl.few_shift), end = min(start + (n << pl.few_shift), min(hi1 + 1, seglen));
+        const bool mixed = hi0 != hi1 || lo0 != lo1;         // whether the rows differ in what they attend
+        const int last = (seglen - 1) >> 4, iters = end > start ? (end - start + 32 * PW - 1) / (32 * PW) : 0;
+
+        // queries: loaded first, ahead of the stream
+        constexpr int LPR = 256 / R, QN = HD / (4 * LPR) > 0 ? HD / (4 * LPR) : 1;
+        const int qr = threadIdx.x / LPR, ql = threadIdx.x % LPR;
+        pa_v4f qv[QN];
+        {
+            const int i = (int)(qr * pl.grp_inv >> 16), h = qr - i * G;
+            const float *src = a.q + (size_t)(sq.t0 + i) * a.qs + (size_t)(kvh * G + h) * HD;
+            const bool al = ((uintptr_t)src & 15) == 0;
+#pragma unroll
+            for (int k = 0; k < QN; k++) {
+                const int e = 4 * (ql + LPR * k);
+                qv[k] = pa_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                if (qr < rows && e < HD) {
+                    if (al) qv[k] = *(const pa_v4f *)(src + e);
+                    else qv[k] = pa_v4f{src[e], src[e + 1], src[e + 2], src[e + 3]};
+                }
+            }
+        }
+        // the lane's row: positions [rlo, rhi]
+        int rlo = lo0, rhi = hi0;
+        if (rc < rows) {
+            const int i = (int)(rc * pl.grp_inv >> 16);
+            if (!pre) {
+                rhi = hi0 + i;
+                rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
+            } else if (a.window) {
+                rlo = max(0, pa_token_pos(p, b, sq.t0 + i) + 1 - a.window);
+            }
+        }
+
+        PaTile<HE, KVT> kv;
+        PaUnit un[2], nx[2];
+        PaUnits us, more_us;                                 // of 32 steps, and of the next 32
+        int base = start + 32 * pw;
+        if (iters) {
+            us = pa_units<KVT>(p, table, base >> 4, 2 * PW, last, kvh, bad);
+            nx[0] = pa_unit<HD, KVT>(p, us, 0);
+            nx[1] = pa_unit<HD, KVT>(p, us, 1);
+            pa_load_k<HD, HE, KVT>(kv, p, nx, c, g, ew);
+            pa_load_v<HD, HE, KVT>(kv, p, nx, c, g, ew);
+        }
+        lds_barrier();                                       // the previous piece's sums are read
+        {
+            float am = 0.0f;
+#pragma unroll
+            for (int k = 0; k < QN; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) am = fmaxf(am, fabsf(qv[k][i]));
+            am = group_max<LPR>(am);
+            const int sh = pa_shift(am);
+            if (ql == 0) qsc[qr] = pa_score_scale<KVT>(a, sh);
+#pragma unroll
+            for (int k = 0; k < QN; k++) {
+                const int e = 4 * (ql + LPR * k);
+                uint2 hi, lo;
+                pa_split(__builtin_ldexpf(qv[k][0], sh), __builtin_ldexpf(qv[k][1], sh), hi.x, lo.x);
+                pa_split(__builtin_ldexpf(qv[k][2], sh), __builtin_ldexpf(qv[k][3], sh), hi.y, lo.y);
+                if (e < HD) {
+                    *(uint2 *)(qh + qr * QP + e) = hi;
+                    *(uint2 *)(qh + (R + qr) * QP + e) = lo;
+                }
+            }
+        }
+        lds_barrier();
+        const _Float16 *const q0 = qh + ((ST && c >= 8 ? R : 0) + rc) * QP + HE * ew + 8 * g, *const q1 = qh + (R + rc) * QP + HE * ew + 8 * g;
+        pa_v8h x0[NS], x1[ST ? 1 : NS];
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            x0[s] = *(const pa_v8h *)(q0 + 32 * s);
+            if constexpr (!ST) x1[s] = *(const pa_v8h *)(q1 + 32 * s);
+        }
+        const float qs = qsc[rc], capl = a.cap * 1.4426950408889634f;
+
+        pa_v4f o[NM];
+        float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (int e = 0; e < NM; e++) o[e] = pa_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+        for (int it = 0; it < iters; it++, base += 32 * PW) {
+            const bool more = it + 1 < iters;
+            un[0] = nx[0];
+            un[1] = nx[1];
+            if ((it & 31) == 31) us = more_us;
+            if (more) {
+                nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
+                nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
+            }
+            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units<KVT>(p, table, (base >> 4) + 64 * PW, 2 * PW, last, kvh, bad);
+            const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
+            // scores at positions base + 16 h + 4 g + i
+            pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const pa_v8h ko = pa_key<HE, KVT>(kv, h, s);
+                    if constexpr (KVT == F16) {
+                        sc[h] = pa_mma(ko, x0[s], sc[h]);
+                        if constexpr (!ST) sc[h] = pa_mma(ko, x1[s], sc[h]);
+                    } else {
+                        pa_v4f d = pa_mma(ko, x0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f});
+                        if constexpr (!ST) d = pa_mma(ko, x1[s], d);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sc[h][i] = __builtin_fmaf(pa_scale(kv.dk[4 * h + i], s), d[i], sc[h][i]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);               // the next keys go where these were
+            if (more) pa_load_k<HD, HE, KVT>(kv, p, nx, c, g, ew);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (ES > 1) {
+                *(pa_v4f *)xs[it & 1][wave][lane] = sc[0];
+                *(pa_v4f *)(xs[it & 1][wave][lane] + 4) = sc[1];
+                lds_barrier();
+                const int w0 = wave & ~(ES - 1);
+                sc[0] = *(const pa_v4f *)xs[it & 1][w0][lane];
+                sc[1] = *(const pa_v4f *)(xs[it & 1][w0][lane] + 4);
+#pragma unroll
+                for (int x = 1; x < ES; x++) {
+                    sc[0] += *(const pa_v4f *)xs[it & 1][w0 + x][lane];
+                    sc[1] += *(const pa_v4f *)(xs[it & 1][w0 + x][lane] + 4);
+                }
+            }
+            float w[8], mt = -__builtin_inff();
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float x = sc[j >> 2][j & 3];
+                if constexpr (ST) x += xor8(x);
+                w[j] = x * qs;
+            }
+            if (a.cap > 0.0f) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) w[j] = capl * pa_tanh(w[j]);
+            }
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int pos = base + 16 * (j >> 2) + 4 * g + (j & 3);
+                    w[j] = pos >= rlo && pos <= rhi && pos < end ? w[j] : -__builtin_inff();
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float x = w[j];
+                if constexpr (KVT != F16) {                  // + the exponent of the position's largest value scale
+                    uint32_t dm = 1;                         // all zero: the smallest scale there is
+#pragma unroll
+                    for (int d = 0; d < HE / 64; d++) dm = max(dm, max(kv.dv[j][d] & 0x7fffu, (kv.dv[j][d] >> 16) & 0x7fffu));
+                    x += (float)__builtin_amdgcn_frexp_expf(h2f((uint16_t)dm));
+                }
+                mt = fmaxf(mt, x);
+            }
+            mt = fmaxf(mt, partner<16>(mt));
+            mt = fmaxf(mt, partner<32>(mt));
+            const float mn = fmaxf(m, mt);
+            if (__any(mn > m)) {
+                const float cr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+                l *= cr;
+#pragma unroll
+                for (int e = 0; e < NM; e++) o[e] *= cr;
+                m = mn;
+            }
+            const float mr = m == -__builtin_inff() ? 0.0f : m - PA_SHIFT;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                w[j] = __builtin_amdgcn_exp2f(w[j] - mr);
+                l += w[j];
+            }
+            // positions that no row of the tile attends may hold anything: zeros
+            // for them; non-finite values that some rows attend and some do not
+            // are taken out and added to those that do (rare, one by one)
+            bool odd = false;
+            if constexpr (KVT == F16) {
+                if (edge) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int pos = base + 16 * (j >> 2) + 4 * g + (j & 3);
+                        const uint32_t live = pos < lo0 || pos >= end ? 0u : ~0u;
+#pragma unroll
+                        for (int d = 0; d < PaTile<HE, KVT>::VW; d++) kv.v[j][d] &= live;
+                    }
+                    if (mixed) {
+                        uint32_t nf = 0;                     // bit 15 or 31 where an exponent is all ones
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+#pragma unroll
+                            for (int d = 0; d < PaTile<HE, KVT>::VW; d++) nf |= (kv.v[j][d] & 0x7c007c00u) + 0x04000400u;
+                        odd = __any(nf & 0x80008000u);
+                        if (odd) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+#pragma unroll
+                                for (int d = 0; d < PaTile<HE, KVT>::VW; d++) kv.v[j][d] = pa_finite(kv.v[j][d]);
+                        }
+                    }
+                }
+                uint32_t ph[4], pq[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    pa_split(w[2 * k], w[2 * k + 1], ph[k], pq[k]);
+                    if constexpr (ST) ph[k] = c < 8 ? ph[k] : pq[k];
+                }
+                const pa_v8h b0 = pa_op(ph[0], ph[1], ph[2], ph[3]), b1 = pa_op(pq[0], pq[1], pq[2], pq[3]);
+#pragma unroll
+                for (int e = 0; e < NM; e++) {
+                    const pa_v8h va = pa_value<HE, KVT>(kv, e);
+                    o[e] = pa_mma(va, b0, o[e]);
+                    if constexpr (!ST) o[e] = pa_mma(va, b1, o[e]);
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < NS; s++) {               // blocks of 32 elements: value tiles 2 s, 2 s + 1
+                    uint32_t ph[4], pq[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float w0 = w[2 * k], w1 = w[2 * k + 1];
+                        pa_split(w0 == 0.0f ? 0.0f : w0 * pa_scale(kv.dv[2 * k], s), w1 == 0.0f ? 0.0f : w1 * pa_scale(kv.dv[2 * k + 1], s), ph[k], pq[k]);
+                        if constexpr (ST) ph[k] = c < 8 ? ph[k] : pq[k];
+                    }
+                    const pa_v8h b0 = pa_op(ph[0], ph[1], ph[2], ph[3]), b1 = pa_op(pq[0], pq[1], pq[2], pq[3]);
+#pragma unroll
+                    for (int e = 2 * s; e < 2 * s + 2; e++) {
+                        const pa_v8h va = pa_value<HE, KVT>(kv, e);
+                        o[e] = pa_mma(va, b0, o[e]);
+                        if constexpr (!ST) o[e] = pa_mma(va, b1, o[e]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) pa_load_v<HD, HE, KVT>(kv, p, nx, c, g, ew);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (KVT == F16) {
+                if (odd) {
+                    for (int x = 0; x < 32; x++) {
+                        const int pos = base + x;
+                        if (pos < lo0 || pos >= end) continue;
+                        const uint16_t *row = (const uint16_t *)(p.v + (x < 16 ? un[0].row : un[1].row)) + (x & 15) * HD + HE * ew;
+                        float wx = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float v = __shfl(w[j], 16 * ((x & 15) >> 2) + c, 64);
+                            if (j == 4 * (x >> 4) + (x & 3)) wx = v;
+                        }
+                        const bool sees = pos >= rlo && pos <= rhi && !(ST && c >= 8);
+#pragma unroll
+                        for (int e = 0; e < NM; e++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const uint16_t hv = row[pa_elem<HE, KVT>(e, 4 * g + i)];
+                                if (sees && (hv & 0x7c00) == 0x7c00) o[e][i] += wx * h2f(hv);
+                            }
+                    }
+                }
+            }
+        }
+        if (__any(bad)) {
+            if (lane == 0 && !sq.bad) paged_flag(p, PAGED_BAD_PAGE);
+            l = __builtin_nanf("");
+        }
+
+        // the position waves' results joined in order, 8 rows at a time
+        l += partner<16>(l);
+        l += partner<32>(l);
+        if (lane < R) wml[wave][lane] = make_float2(m, l);
+        if constexpr (ST) {
+#pragma unroll
+            for (int e = 0; e < NM; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[e][i] += xor8(o[e][i]);
+        }
+        constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
+#pragma unroll
+        for (int k = 0; k < R / 8; k++) {
+            lds_barrier();                                   // the queries (the previous rows' sums) are read
+            if ((c >> 3) == k) {
+#pragma unroll
+                for (int e = 0; e < NM; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) buf[(pw * 8 + (c & 7)) * (HD + 4) + HE * ew + pa_elem<HE, KVT>(e, 4 * g + i)] = o[e][i];
+            }
+            lds_barrier();
+            for (int x = threadIdx.x; x < 8 * (HD / 4); x += 256) {
+                const int r8 = x / (HD / 4), e4 = x % (HD / 4) * 4, r = 8 * k + r8;
+                if (r >= rows) continue;
+                float mm = -__builtin_inff();
+#pragma unroll
+                for (int w = 0; w < 4; w++) mm = fmaxf(mm, wml[w][r].x);
+                float ls = 0.0f;
+                pa_v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < PW; w++) {
+                    const float2 ml = wml[w * ES][r];
+                    const float f = ml.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mm);
+                    ls += ml.y == ml.y ? f * ml.y : ml.y;    // a bad page's NaN stays
+                    const float mo = wml[w * ES + (ES > 1 ? e4 / HE : 0)][r].x;
+                    s += *(const pa_v4f *)&buf[(w * 8 + r8) * (HD + 4) + e4] * (mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mm));
+                }
+                s *= VS;
+                const int i = (int)(r * pl.grp_inv >> 16), tok = sq.t0 + i, head = kvh * G + (r - i * G);
+                const size_t row = (size_t)tok * a.n_head + head;
+                if (!pre && whole && b.n_prefix == 0) {
+                    s = !sq.bad && hi0 + i < 0 ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / ls);
+                    pa_store4(a.out + (size_t)tok * a.os + (size_t)head * HD + e4, s);
+                } else if (!pre && whole) {
+                    const size_t at = row * pl.nown;
+                    *(pa_v4f *)(pl.oo + at * HD + e4) = s;
+                    if (e4 == 0) pl.oml[at] = make_float2(mm, ls);
+                } else {
+                    const size_t at = (size_t)slot * R + r;
+                    *(pa_v4f *)(pl.fo + at * HD + e4) = s;
+                    if (e4 == 0) pl.fml[at] = make_float2(mm, ls);
+                }
+            }
+        }
+    }
+}
+
+template <int KVT, int HD>
+hipError_t pa_few_hd(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
+    const dim3 grid(pl.few_wgs), wg(256);
+    if (pl.few_rows <= 8) hipLaunchKernelGGL((k_paged_few<HD, KVT, true>), grid, wg, 0, s, a, pl);
+    else hipLaunchKernelGGL((k_paged_few<HD, KVT, false>), grid, wg, 0, s, a, pl);
+    return hipGetLastError();
+}
+template <int KVT>
+hipError_t pa_few(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
+    switch (a.p.hd) {
+    case 64: return pa_few_hd<KVT, 64>(a, pl, s);
+    case 128: return pa_few_hd<KVT, 128>(a, pl, s);
+    case 256: return pa_few_hd<KVT, 256>(a, pl, s);
+    case 512: return pa_few_hd<KVT, 512>(a, pl, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace g4
