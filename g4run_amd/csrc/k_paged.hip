@@ -10,82 +10,77 @@ namespace {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Workgroups the many-row kernel's splits aim at, and positions of a split at
-// least: a split of 128 rows writes and reads back as many bytes as it reads for
-// 256 positions.
-constexpr int MANY_WGS = 256, MANY_CHUNK = 256;
-
-int many_splits(int64_t items, int span) {
-    return std::max(1, std::min<int>((int)(MANY_WGS / std::max<int64_t>(items, 1)), ceil_div(span, MANY_CHUNK)));
-}
-void many_chunk(int64_t items, int span, int &n, int &chunk) {
-    chunk = std::max(MANY_CHUNK, ceil_div(ceil_div(span, many_splits(items, span)), 32) * 32);
-    n = std::max(1, ceil_div(span, chunk));
-}
-
 struct Layout {
     PagedPlan pl;
-    bool few, many, join;
-    size_t fo, oo, po, fml, oml, pml, total;
+    bool join;
+    size_t fo, fml, mo, mml, own, pre, wo, wml, total;
 };
 // window 0 gives the most workspace
-Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window, bool bound) {
+Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     Layout y;
     PagedPlan &pl = y.pl;
+    PagedList &few = pl.few, &many = pl.many;
     const int64_t rows = (int64_t)b.n_tok * grp;             // of one KV head
-    // Sequences of at most few_rows rows are the few-row kernel's: 8 (one matrix
-    // instruction per operand) where no sequence can have more, else 16.
-    pl.few_rows = grp > 16 ? 0 : (b.q_off ? rows : grp) <= 8 ? 8 : 16;
-    if (b.n_prefix && pl.few_rows == 8 && rows > 8 && rows <= 16) pl.few_rows = 16;
-    y.few = pl.few_rows > 0;
-    const bool few_pre = b.n_prefix && y.few && rows <= pl.few_rows;
-    const bool many_own = b.q_off ? b.n_tok > (y.few ? pl.few_rows / grp : 0) : !y.few;
-    const bool many_pre = b.n_prefix && !few_pre;
-    y.many = many_own || many_pre;
-    // few: the most own positions of a sequence it takes (few_rows tokens at most)
     pl.grp_inv = 65536 / grp + 1;
-    // a step is at least what a workgroup takes at once; up to 256 positions stay
-    // one step, so that no join is launched for them
-    pl.few_shift = b.max_len <= 256 && !b.n_prefix ? 8 : 7;
-    const int64_t fspan = window ? std::min<int64_t>(b.max_len, (int64_t)window + 32 + 16) : b.max_len;
+    // Sequences of at most few.rows rows are the few-row kernel's: 8 (one matrix
+    // instruction per operand) where no sequence can have more, else 16.
+    few.rows = grp > 16 ? 0 : (b.q_off ? rows : grp) <= 8 ? 8 : 16;
+    if (b.n_prefix && few.rows == 8 && rows > 8 && rows <= 16) few.rows = 16;
+    const bool few_pre = b.n_prefix && few.rows && rows <= few.rows;
+    const bool many_own = b.q_off ? b.n_tok > (few.rows ? few.rows / grp : 0) : !few.rows;
+    const bool many_pre = b.n_prefix && !few_pre;
+    few.least = 1;
+    few.pre_tiles = few_pre ? 1 : 0;
+    many.least = 2;
+    // positions a tile attends at most: its first token's window rounded down to
+    // 32, and its later tokens
+    auto span = [&](int tokens) { return window ? std::min<int64_t>(b.max_len, (int64_t)window + 32 + tokens) : (int64_t)b.max_len; };
+    const int64_t fspan = span(16);
+    // A step is at least what a workgroup takes at once; up to 256 positions stay
+    // one step, so that no join is launched for them.
     int64_t steps;
-    for (;; pl.few_shift++) {                                // counted in 32 bits on the device
-        pl.few_unit = 1 << pl.few_shift;
-        pl.few_pre = few_pre ? ceil_div(b.n_prefix, pl.few_unit) : 0;
-        steps = ((int64_t)b.n_seq * std::max(1, ceil_div(fspan, pl.few_unit)) + pl.few_pre) * p.n_kv;
+    for (few.shift = b.max_len <= 256 && !b.n_prefix ? 8 : 7;; few.shift++) {       // counted in 32 bits on the device
+        few.unit = 1 << few.shift;
+        few.pre_steps = few_pre ? ceil_div(b.n_prefix, few.unit) : 0;
+        steps = ((int64_t)b.n_seq * std::max(1, ceil_div(fspan, few.unit)) + few.pre_steps) * p.n_kv;
         if (steps < (1 << 30)) break;
     }
-    pl.few_wgs = (int)std::min<int64_t>(PA_FEW_WGS, steps);
-    // many: tiles of up to 128 rows (64 of heads of 512), evenly filled
-    const int most = p.hd > 256 ? 64 : 128;
-    const int64_t tiles = std::max<int64_t>(1, ceil_div(b.q_off || many_pre ? rows : grp, most));
-    pl.many_rows = (int)std::min<int64_t>(most, ceil_div(ceil_div(b.q_off || many_pre ? rows : grp, tiles), 32) * 32);
-    pl.own_slots = pl.pre_slots = pl.own_chunk = pl.pre_chunk = pl.npre = 0;
-    pl.nown = 1;
-    int64_t slots = 0;
-    if (many_own) {
-        const int least = b.q_off && y.few ? pl.few_rows / grp + 1 : 1;      // tokens of a sequence it takes
-        slots = b.q_off ? ceil_div(rows, pl.many_rows) + std::min(b.n_seq, b.n_tok / least) : (int64_t)b.n_seq * ceil_div(grp, pl.many_rows);
-        pl.own_slots = (int)slots;
-        const int64_t span = window ? std::min<int64_t>(b.max_len, (int64_t)window + 32 + pl.many_rows / grp + 1) : b.max_len;
-        many_chunk(slots * p.n_kv, (int)span, pl.nown, pl.own_chunk);
-        if (bound) pl.nown = many_splits(slots * p.n_kv, b.max_len);
+    few.wgs = (int)std::min<int64_t>(PA_FEW_WGS, steps);
+    y.join = b.n_prefix || (few.rows && fspan > few.unit);
+    // Many rows: tiles of up to 128 (64 of heads of 512), evenly filled; as many
+    // workgroups as fit on the device at once.
+    many.rows = 0;
+    many.pre_tiles = 0;
+    if (many_own || many_pre) {
+        const int most = p.hd > 256 ? 64 : 128;
+        const int64_t shared = b.q_off || many_pre ? rows : grp, tiles = ceil_div(shared, most);
+        many.rows = (int)std::min<int64_t>(most, ceil_div(ceil_div(shared, tiles), 32) * 32);
+        many.pre_tiles = many_pre ? ceil_div(rows, many.rows) : 0;
+        const int least = b.q_off && few.rows ? few.rows / grp + 1 : 1;      // tokens of a sequence it takes
+        const int64_t own = !many_own ? 0 : b.q_off ? ceil_div(rows, many.rows) + std::min(b.n_seq, b.n_tok / least)
+                                                    : (int64_t)b.n_seq * ceil_div(grp, many.rows);
+        const int64_t mspan = span(many.rows / grp + 1);
+        for (many.shift = 6;; many.shift++) {
+            many.unit = 1 << many.shift;
+            many.pre_steps = many_pre ? ceil_div(b.n_prefix, many.unit) : 0;
+            steps = (own * std::max(1, ceil_div(mspan, many.unit)) + (int64_t)many.pre_tiles * many.pre_steps) * p.n_kv;
+            if (steps < (1 << 30)) break;
+        }
+        many.wgs = (int)std::min<int64_t>(p.hd >= 256 ? 256 : 512, ceil_div(steps, many.least));
+        y.join |= mspan > many.unit;
     }
-    if (many_pre) {
-        pl.pre_slots = ceil_div(rows, pl.many_rows);
-        many_chunk((int64_t)pl.pre_slots * p.n_kv, b.n_prefix, pl.npre, pl.pre_chunk);
-    }
-    y.join = b.n_prefix || pl.nown > 1 || (y.few && fspan > pl.few_unit);
-    const size_t all = (size_t)b.n_tok * p.n_kv * grp, few = y.few && y.join ? (size_t)pl.few_wgs * 2 * pl.few_rows : 0;
-    const size_t own = b.n_prefix || pl.nown > 1 ? all * pl.nown : 0, pre = all * pl.npre;
+    const size_t all = y.join ? (size_t)b.n_tok * p.n_kv * grp : 0, whole = b.n_prefix ? all : 0;
+    const size_t f = y.join && few.rows ? (size_t)few.wgs * 2 * few.rows : 0, m = y.join && many.rows ? (size_t)many.wgs * 2 * many.rows : 0;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
-    y.fo = take(few * p.hd * 4);
-    y.fml = take(few * sizeof(float2));
-    y.oo = take(own * p.hd * 4);
-    y.oml = take(own * sizeof(float2));
-    y.po = take(pre * p.hd * 4);
-    y.pml = take(pre * sizeof(float2));
+    y.fo = take(f * p.hd * 4);
+    y.fml = take(f * sizeof(float2));
+    y.mo = take(m * p.hd * 4);
+    y.mml = take(m * sizeof(float2));
+    y.own = take(all * sizeof(uint2));
+    y.pre = take(whole * sizeof(uint2));
+    y.wo = take(whole * p.hd * 4);
+    y.wml = take(whole * sizeof(float2));
     y.total = at;
     return y;
 }
@@ -98,61 +93,31 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
     __shared__ float lg[16];                                 // at most 16 groups: hd >= 64
     __shared__ pa_v4f part[256];
     const int hd = a.p.hd, hd4 = hd / 4, groups = 256 / hd4, gi = threadIdx.x / hd4, e4 = threadIdx.x % hd4 * 4;
-    const int tok = blockIdx.x / a.n_head, head = blockIdx.x - tok * a.n_head, kvh = head / a.grp;
+    const int tok = blockIdx.x / a.n_head, head = blockIdx.x - tok * a.n_head;
+    const size_t row = blockIdx.x;
+    const bool prefix = a.b.n_prefix > 0;
+    const uint2 own = pl.own[row], pre = prefix ? pl.pre[row] : make_uint2(0, 0);      // of a row without a sequence: not used
     const int seq = paged_find(a.b, tok);
     if (seq >= a.b.n_seq) return;                            // behind the last sequence
     const PagedSeq sq = paged_seq(a.p, a.b, seq);
     const int i = tok - sq.t0;
     if (i < 0 || i >= sq.nq) return;
-    const size_t row = (size_t)tok * a.n_head + head;
-    const bool few = sq.nq * a.grp <= pl.few_rows;
-    int mine, share = 1, fb = 0, fi0 = 0, nf = 0, nw = 0;    // own few pieces: first workgroup, their number; whole ones
-    if (few || pl.few_pre) share = pa_share(pa_total(a, pl, mine));
-    if (few) {
-        const int all = pa_seq_steps(a, pl, sq);
-        fb = pl.few_pre * a.p.n_kv + pa_before(a, pl, mine, seq) + kvh * all;
-        fi0 = fb / share;
-        nf = (fb + all - 1) / share - fi0 + 1;
-        if (nf == 1) {
-            if (a.b.n_prefix == 0) return;                   // written by the kernel
-            nf = 0;
-            nw = 1;
-        }
-    } else {
-        int lo, hi;
-        pa_tile_span(sq, a.grp, pl.many_rows, (i * a.grp + head % a.grp) / pl.many_rows, a.window, lo, hi);
-        nw = pa_tile_chunks(sq, pl, lo, hi);
-        if (pl.nown == 1 && a.b.n_prefix == 0) return;
-    }
-    int pb = 0, pi0 = 0, np = 0;
-    if (pl.few_pre) {
-        pb = kvh * pl.few_pre;
-        pi0 = pb / share;
-        np = (pb + pl.few_pre - 1) / share - pi0 + 1;
-    }
-    // partial result k: prefix pieces or chunks, then own pieces or chunks
-    const int R = pl.few_rows, nq0 = np ? np : pl.npre, total = nq0 + nf + nw;
+    const int n_pre = pre.x >> 1, n_own = own.x >> 1, total = n_pre + n_own;
+    if (n_own == 0) return;                                  // written out
+    // partial result k: the prefix's pieces, then the own ones
     auto at = [&](int k, const float *&o, const float2 *&ml) {
-        if (k < nq0) {
-            if (np) {
-                const size_t s = (size_t)(2 * (pi0 + k) + (k == 0 && pb != pi0 * share)) * R + (size_t)tok * a.grp + head % a.grp;
-                o = pl.fo + s * hd;
-                ml = pl.fml + s;
-            } else {
-                const size_t s = row * pl.npre + k;
-                o = pl.po + s * hd;
-                ml = pl.pml + s;
-            }
-        } else if (nf) {
-            const int n = k - nq0;
-            const size_t s = (size_t)(2 * (fi0 + n) + (n == 0 && fb != fi0 * share)) * R + (size_t)i * a.grp + head % a.grp;
-            o = pl.fo + s * hd;
-            ml = pl.fml + s;
-        } else {
-            const size_t s = row * pl.nown + (k - nq0);
-            o = pl.oo + s * hd;
-            ml = pl.oml + s;
+        const uint2 d = k < n_pre ? pre : own;
+        if (k >= n_pre) k -= n_pre;
+        if (d.y == ~0u) {
+            o = pl.wo + row * hd;
+            ml = pl.wml + row;
+            return;
         }
+        const bool many = d.x & 1;
+        const int w = (int)(d.y >> 9) + k, wgs = many ? pl.many.wgs : pl.few.wgs, rows = many ? pl.many.rows : pl.few.rows;
+        const size_t s = (size_t)(2 * min(w, wgs - 1) + (k == 0 ? d.y >> 8 & 1 : 0)) * rows + (d.y & 255);
+        o = (many ? pl.many.o : pl.few.o) + s * hd;
+        ml = (many ? pl.many.ml : pl.few.ml) + s;
     };
     float mm = -__builtin_inff();
     for (int k = threadIdx.x; k < total; k += 256) {
@@ -192,30 +157,25 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
 
 }  // namespace
 
-size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head) {
-    return layout(p, b, n_head / p.n_kv, 0, true).total;
-}
+size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head) { return layout(p, b, n_head / p.n_kv, 0).total; }
 
 hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s) {
     const PagedPool &p = a.p;
     const PagedBatch &b = a.b;
     if (b.n_tok == 0 || b.n_seq == 0) return hipSuccess;
-    Layout y = layout(p, b, a.grp, a.window, false);
+    Layout y = layout(p, b, a.grp, a.window);
     PagedPlan &pl = y.pl;
-    pl.fo = (float *)(a.ws + y.fo);
-    pl.oo = (float *)(a.ws + y.oo);
-    pl.po = (float *)(a.ws + y.po);
-    pl.fml = (float2 *)(a.ws + y.fml);
-    pl.oml = (float2 *)(a.ws + y.oml);
-    pl.pml = (float2 *)(a.ws + y.pml);
-    if (y.many) {
-        const int64_t blocks = ((int64_t)pl.own_slots * pl.nown + (int64_t)pl.pre_slots * pl.npre) * p.n_kv;
-        if (blocks > 0xffffff) return hipErrorInvalidValue;
-        if (hipError_t e = p.type == F16 ? pa_many_f16(a, pl, (unsigned)blocks, s)
-                         : p.type == Q8_0 ? pa_many_q8(a, pl, (unsigned)blocks, s) : pa_many_q4(a, pl, (unsigned)blocks, s))
-            return e;
-    }
-    if (y.few)
+    pl.few.o = (float *)(a.ws + y.fo);
+    pl.few.ml = (float2 *)(a.ws + y.fml);
+    pl.many.o = (float *)(a.ws + y.mo);
+    pl.many.ml = (float2 *)(a.ws + y.mml);
+    pl.own = y.join ? (uint2 *)(a.ws + y.own) : nullptr;
+    pl.pre = (uint2 *)(a.ws + y.pre);
+    pl.wo = (float *)(a.ws + y.wo);
+    pl.wml = (float2 *)(a.ws + y.wml);
+    if (pl.many.rows)
+        if (hipError_t e = p.type == F16 ? pa_many_f16(a, pl, s) : p.type == Q8_0 ? pa_many_q8(a, pl, s) : pa_many_q4(a, pl, s)) return e;
+    if (pl.few.rows)
         if (hipError_t e = p.type == F16 ? pa_few_f16(a, pl, s) : p.type == Q8_0 ? pa_few_q8(a, pl, s) : pa_few_q4(a, pl, s)) return e;
     if (y.join) {
         hipLaunchKernelGGL(k_paged_join, dim3((unsigned)(b.n_tok * a.n_head)), dim3(256), 0, s, a, pl);

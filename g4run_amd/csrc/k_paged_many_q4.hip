@@ -3,6 +3,6 @@
 
 namespace g4 {
 
-hipError_t pa_many_q4(const PagedAttn &a, const PagedPlan &pl, unsigned blocks, hipStream_t s) { return pa_many<Q4_0>(a, pl, blocks, s); }
+hipError_t pa_many_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) { return pa_many<Q4_0>(a, pl, s); }
 
 }  // namespace g4

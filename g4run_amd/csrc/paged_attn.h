@@ -11,19 +11,17 @@
 // Precision: fp32.  K and V enter exactly (halves, or the integers of the block
 // formats, their scales applied in fp32 to the scores and to the weights).  A
 // query row is scaled by a power of two to [2^14, 2^15) and split into two
-// halves (22 bits), a weight likewise.  Weights are exp2(s - m + 12), for
+// halves (22 bits), a weight likewise.  Weights are exp2(s - m + 6), for
 // quantized values with m over s + the exponent of the position's largest
 // scale, so weight x scale neither overflows nor falls among the halves'
 // subnormals while it matters.
 //
 // Two kernels share a call:
 //   k_paged_few   row tiles of up to 16 rows (single tokens; the prefix of a small
-//                 batch): bound by the cache's bytes.  The batch's positions are
-//                 one list of steps, dealt evenly to the workgroups.
+//                 batch): bound by the cache's bytes.
 //   k_paged_many  sequences of more rows (prompt chunks; the prefix of a large
 //                 batch): bound by the matrix cores.  K and V pass through LDS
 //                 once for up to 128 rows.
-// Partial results go through the workspace to k_paged_join.
 #pragma once
 
 #include "paged.h"
@@ -36,22 +34,38 @@ typedef float pa_v4f __attribute__((ext_vector_type(4)));
 typedef float pa_v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t pa_v4u __attribute__((ext_vector_type(4)));
 
-// The split of a call.  Partial results: the few-row kernel's [wgs][2][R] (a
-// workgroup's first and last piece), and per row [nown] own chunks (a whole few-row
-// sequence beside a prefix: chunk 0) and [npre] prefix chunks.
+// The split of a call.  Each kernel's work is one list of steps (`unit` positions
+// of one row tile of one KV head: the prefix's tiles, then the sequences' in
+// order), cut into equal shares for its workgroups.  A piece -- the part of a
+// share that lies in one tile of one head -- is written out where it is the whole
+// tile and there is no prefix; else its sums go to the workspace: slot 2 w for
+// workgroup w's first piece, 2 w + 1 for another (only the first and the last of a
+// share, and whole tiles beside a prefix, are partial).  The tile's first piece
+// tells k_paged_join where its rows' pieces lie.
+struct PagedList {
+    int rows;                        // rows of a tile; the few-row kernel: most rows of a sequence it takes
+    int wgs, least;                  // workgroups; steps of a share at least
+    int unit, shift;                 // positions of a step, and their log2
+    int pre_tiles, pre_steps;        // the prefix's tiles (0: not this kernel's), and steps of each
+    float *o;                        // [2 wgs][rows][hd] unnormalised sums
+    float2 *ml;                      // [2 wgs][rows] maximum (log2), sum
+};
 struct PagedPlan {
-    int few_rows;                    // sequences of up to this many rows are the few-row kernel's
-    int few_wgs, few_unit, few_shift;    // its workgroups; positions of a step, and their log2
+    PagedList few, many;             // rows 0: the kernel does not run
     uint32_t grp_inv;                // rows to tokens: r / grp == r * grp_inv >> 16 for r < 16
-    int few_pre;                     // whether the prefix is its too: steps of the prefix (0: no)
-    int many_rows;                   // rows of a workgroup of the many-row kernel
-    int own_slots, nown, own_chunk;  // its tiles of the sequences' own positions, and chunks
-    int pre_slots, npre, pre_chunk;  // and of the prefix's
-    float *fo, *oo, *po;             // unnormalised sums: few, own, prefix
-    float2 *fml, *oml, *pml;         // maximum (log2), sum
+    // where a (token, head) row's partial results lie, own positions and prefix:
+    // count << 1 | kernel (0 few), slot << 8 | row of the tile; [0] count 0 where
+    // the row is written out
+    uint2 *own, *pre;
+    float *wo;                       // [token][head][hd] whole tiles' sums beside a prefix
+    float2 *wml;
 };
 
-constexpr float PA_SHIFT = 12.0f;    // weights are scaled by 2^12: their low halves stay normal
+// Weights are scaled by 2^6 over a maximum that may lag by 2^8: their low halves
+// stay normal and the largest, 2^14 (times a scale below 1), finite.  Without the
+// lag some row of a tile raises its maximum, and all sums are rescaled, in most of
+// the first steps.
+constexpr float PA_SHIFT = 6.0f, PA_LAG = 8.0f;
 
 __device__ __forceinline__ int pa_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ uint32_t pa_pk(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
@@ -174,33 +188,68 @@ __device__ __forceinline__ int pa_scan(int v) {
     return v;
 }
 
-// ---- the few-row kernel's list of steps ----
-__device__ __forceinline__ int pa_seq_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q) {
-    return q.bad ? 1 : max(1, (q.len - pa_low(q.len - q.nq, a.window) + pl.few_unit - 1) >> pl.few_shift);
+// ---- the lists of steps ----
+// Which sequences are a kernel's (MANY: more rows than the few-row kernel takes),
+// their tiles, and a tile's positions [lo, hi] (own; lo a multiple of 32).
+template <bool MANY>
+__device__ __forceinline__ const PagedList &pa_list(const PagedPlan &pl) {
+    if constexpr (MANY) return pl.many;
+    else return pl.few;
 }
-// steps of sequence s for one KV head: 0 when it is not this kernel's
+template <bool MANY>
+__device__ __forceinline__ int pa_tiles(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q) {
+    const bool few = q.nq * a.grp <= pl.few.rows;
+    if constexpr (MANY) return few ? 0 : (q.nq * a.grp + pl.many.rows - 1) / pl.many.rows;
+    else return few && q.nq > 0;
+}
+template <bool MANY>
+__device__ __forceinline__ void pa_tile_span(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile, int &lo, int &hi) {
+    const int p0 = q.len - q.nq;
+    if constexpr (MANY) {
+        lo = pa_low(p0 + tile * pl.many.rows / a.grp, a.window);
+        hi = p0 + min(q.nq - 1, ((tile + 1) * pl.many.rows - 1) / a.grp);
+    } else {
+        lo = pa_low(p0, a.window);
+        hi = q.len - 1;
+    }
+}
+template <bool MANY>
+__device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile) {
+    if (q.bad) return 1;
+    const PagedList &y = pa_list<MANY>(pl);
+    int lo, hi;
+    pa_tile_span<MANY>(a, pl, q, tile, lo, hi);
+    return max(1, (hi - lo + y.unit) >> y.shift);
+}
+// steps of sequence s for one KV head
+template <bool MANY>
 __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, int s) {
     const PagedSeq q = paged_seq(a.p, a.b, s);
-    if (q.nq == 0 || q.nq * a.grp > pl.few_rows) return 0;
-    return pa_seq_steps(a, pl, q);
+    const int tiles = pa_tiles<MANY>(a, pl, q);
+    int n = 0;
+    for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY>(a, pl, q, t);
+    return n;
 }
-// All steps of the call (wave-uniform; the whole wave calls it), 64 sequences
-// at a time; the first 64 sequences' own in `mine`.
+// All steps of the list (wave-uniform; the whole wave calls it), 64 sequences at a
+// time; the lane's own of the first 64 in `mine`.
+template <bool MANY>
 __device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl, int &mine) {
+    const PagedList &y = pa_list<MANY>(pl);
     const int lane = threadIdx.x & 63;
-    mine = lane < a.b.n_seq ? pa_steps(a, pl, lane) : 0;
+    mine = lane < a.b.n_seq ? pa_steps<MANY>(a, pl, lane) : 0;
     int n = mine;
-    for (int s = 64 + lane; s < a.b.n_seq; s += 64) n += pa_steps(a, pl, s);
+    for (int s = 64 + lane; s < a.b.n_seq; s += 64) n += pa_steps<MANY>(a, pl, s);
     n = pa_uniform(group_isum<64>(n));
-    return (n + pl.few_pre) * a.p.n_kv;
+    return (n + y.pre_tiles * y.pre_steps) * a.p.n_kv;
 }
 // the sequence whose steps hold step u (counted without the prefix's) and the
 // number of steps before it
+template <bool MANY>
 __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan &pl, int mine, int u, int &seq, int &before) {
     const int lane = threadIdx.x & 63;
     before = 0;
     for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
-        const int n = (s0 == 0 ? mine : s0 + lane < a.b.n_seq ? pa_steps(a, pl, s0 + lane) : 0) * a.p.n_kv;
+        const int n = (s0 == 0 ? mine : s0 + lane < a.b.n_seq ? pa_steps<MANY>(a, pl, s0 + lane) : 0) * a.p.n_kv;
         const int incl = pa_scan(n);
         const uint64_t past = __ballot(before + incl > u);
         if (past) {
@@ -213,59 +262,108 @@ __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan
     }
     seq = a.b.n_seq;
 }
-// the steps before sequence `seq` (wave-uniform)
-__device__ __forceinline__ int pa_before(const PagedAttn &a, const PagedPlan &pl, int mine, int seq) {
-    const int lane = threadIdx.x & 63;
-    int n = lane < seq ? mine : 0;
-    for (int s = 64 + lane; s < seq; s += 64) n += pa_steps(a, pl, s);
-    return pa_uniform(group_isum<64>(n)) * a.p.n_kv;
-}
-// steps of a workgroup: fewer than PA_FEW_WGS workgroups are launched only where
-// each step has one
 constexpr int PA_FEW_WGS = 512;
-__device__ __forceinline__ int pa_share(int total) { return max(1, (total + PA_FEW_WGS - 1) / PA_FEW_WGS); }
+__device__ __forceinline__ int pa_share(const PagedList &y, int total) { return max(y.least, (total + y.wgs - 1) / y.wgs); }
 
-// ---- the many-row kernel's tiles ----
-// The slot-th row tile (wave-uniform): sequences' tiles one after another.
-// seq = n_seq when there are fewer.
-__device__ __forceinline__ void pa_find_tile(const PagedAttn &a, const PagedPlan &pl, int slot, int &seq, int &tile) {
+// A piece: steps [step, step + n) of the `all` of one tile of one KV head.
+struct PaPiece {
+    PagedSeq sq;                     // the prefix: all tokens of the batch
+    int kvh, tile, step, n, all;
+    int seglen, start, end;          // positions of the segment; the piece's [start, end)
+    int hi0, hi1, lo0, lo1;          // the first and the last row's last and first positions
+    int slot;                        // of its sums
+    const int *table;
+    bool pre;
+};
+// the piece at step u of a share [first, stop)
+template <bool MANY>
+__device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, int wg, int u, int first, int stop) {
+    const PagedList &y = pa_list<MANY>(pl);
     const PagedBatch &b = a.b;
-    const int R = pl.many_rows;
-    if (!b.q_off) {
-        const int per = (a.grp + R - 1) / R;
-        seq = slot / per;
-        tile = slot - seq * per;
-        return;
-    }
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
-        const int s = s0 + lane;
-        int n = 0;
-        if (s < b.n_seq) {
-            const int nq = paged_seq(a.p, b, s).nq;
-            if (nq > pl.few_rows / a.grp) n = (nq * a.grp + R - 1) / R;
+    PaPiece x;
+    const int pre_all = y.pre_tiles * y.pre_steps * a.p.n_kv;
+    x.pre = u < pre_all;
+    int base;
+    if (x.pre) {
+        x.sq.t0 = 0;
+        x.sq.nq = pa_tokens(b);
+        x.sq.len = x.seglen = b.n_prefix;
+        x.sq.bad = false;
+        x.all = y.pre_steps;
+        const int t = u / x.all;
+        x.step = u - t * x.all;
+        x.kvh = y.pre_tiles == 1 ? t : t / y.pre_tiles;
+        x.tile = t - x.kvh * y.pre_tiles;
+        x.table = b.prefix;
+        x.hi0 = x.hi1 = x.seglen - 1;
+        x.lo0 = base = 0;
+        x.lo1 = a.window ? 0x7fffffff : 0;                   // row by row
+    } else {
+        int seq, before;
+        pa_find_step<MANY>(a, pl, mine, u - pre_all, seq, before);
+        x.sq = paged_seq(a.p, b, seq);
+        int v = u - pre_all - before;
+        if constexpr (MANY) {
+            const int tiles = pa_tiles<MANY>(a, pl, x.sq);
+            int head = 0;                                    // steps of one KV head
+            for (int t = 0; t < tiles; t++) head += pa_tile_steps<MANY>(a, pl, x.sq, t);
+            x.kvh = v / head;
+            v -= x.kvh * head;
+            x.tile = 0;
+            for (x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0); v >= x.all; x.all = pa_tile_steps<MANY>(a, pl, x.sq, ++x.tile)) v -= x.all;
+        } else {
+            x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0);
+            x.tile = 0;
+            x.kvh = v / x.all;
+            v -= x.kvh * x.all;
         }
-        const int incl = pa_scan(n);
-        const uint64_t past = __ballot(before + incl > slot);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            seq = s0 + l;
-            tile = slot - before - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l));
-            return;
-        }
-        before += __builtin_amdgcn_readlane(incl, 63);
+        x.step = v;
+        pa_tile_span<MANY>(a, pl, x.sq, x.tile, base, x.hi1);
+        x.hi0 = x.sq.len - x.sq.nq + (MANY ? x.tile * pl.many.rows / a.grp : 0);
+        x.lo0 = a.window ? max(0, x.hi0 + 1 - a.window) : 0;
+        x.lo1 = a.window ? max(0, x.hi1 + 1 - a.window) : 0;
+        x.seglen = x.sq.bad ? 0 : x.sq.len;
+        x.table = b.table + (size_t)seq * b.table_stride;
     }
-    seq = b.n_seq;
-    tile = 0;
+    x.n = min(x.all - x.step, stop - u);
+    x.start = base + (x.step << y.shift);
+    x.end = min(x.start + (x.n << y.shift), min(x.hi1 + 1, x.seglen));
+    x.slot = 2 * wg + (u != first);
+    return x;
 }
-// own positions of a row tile: [lo, hi], lo a multiple of 32; and its chunks
-__device__ __forceinline__ void pa_tile_span(const PagedSeq &q, int grp, int R, int tile, int window, int &lo, int &hi) {
-    lo = pa_low(q.len - q.nq + tile * R / grp, window);
-    hi = q.len - q.nq + min(q.nq - 1, ((tile + 1) * R - 1) / grp);
-}
-__device__ __forceinline__ int pa_tile_chunks(const PagedSeq &q, const PagedPlan &pl, int lo, int hi) {
-    return q.bad ? 1 : min(pl.nown, max(1, (hi + pl.own_chunk - lo) / pl.own_chunk));
+// Where row r (of its tile) of a piece puts its sums: out (normalised), or `o` and
+// `ml`; and, from a tile's first piece, where k_paged_join finds them.
+struct PaSink {
+    float *o;
+    float2 *ml;
+    bool out;
+};
+template <bool MANY>
+__device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &pl, const PaPiece &x, int share, int r, int tok, int head, bool note) {
+    const PagedList &y = pa_list<MANY>(pl);
+    const size_t row = (size_t)tok * a.n_head + head;
+    const bool whole = x.n == x.all;
+    PaSink s;
+    s.out = !x.pre && whole && a.b.n_prefix == 0;
+    if (s.out) {
+        s.o = a.out + (size_t)tok * a.os + (size_t)head * a.p.hd;
+        s.ml = nullptr;
+        if (note && pl.own) pl.own[row] = make_uint2(0, 0);
+    } else if (!x.pre && whole) {
+        s.o = pl.wo + row * a.p.hd;
+        s.ml = pl.wml + row;
+        if (note) pl.own[row] = make_uint2(2 | MANY, ~0u);
+    } else {
+        const size_t at = (size_t)x.slot * y.rows + r;
+        s.o = y.o + at * a.p.hd;
+        s.ml = y.ml + at;
+        if (note && x.step == 0) {
+            // later pieces start the next workgroups' shares
+            const int rest = x.all - x.n, count = 1 + (rest + share - 1) / share;
+            (x.pre ? pl.pre : pl.own)[row] = make_uint2((uint32_t)count << 1 | MANY, (uint32_t)x.slot << 8 | (uint32_t)r);
+        }
+    }
+    return s;
 }
 
 // two halves, those that are not finite as 0
@@ -296,8 +394,8 @@ __device__ __forceinline__ void pa_store4(float *d, pa_v4f s) {
 hipError_t pa_few_f16(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
 hipError_t pa_few_q8(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
 hipError_t pa_few_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
-hipError_t pa_many_f16(const PagedAttn &a, const PagedPlan &pl, unsigned blocks, hipStream_t s);
-hipError_t pa_many_q8(const PagedAttn &a, const PagedPlan &pl, unsigned blocks, hipStream_t s);
-hipError_t pa_many_q4(const PagedAttn &a, const PagedPlan &pl, unsigned blocks, hipStream_t s);
+hipError_t pa_many_f16(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+hipError_t pa_many_q8(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+hipError_t pa_many_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
 
 }  // namespace g4

@@ -1,12 +1,8 @@
 // paged_few.h -- attention of a few rows over the paged KV cache (paged_attn.h):
 // single tokens of many sequences, short drafts, the prefix of a small batch.
 //
-// Bound by the cache's bytes.  The call's positions are one list of steps (one
-// KV head of one sequence: few_unit positions each), cut into equal shares for
-// workgroups that all fit on the device at once, so ragged lengths leave no
-// workgroup idle.  A piece (a share's part of one sequence and head) that is
-// the whole sequence is written out; the first and last piece of a share
-// go through the workspace.
+// Bound by the cache's bytes.  The workgroups all fit on the device at once, and
+// their shares of the list of steps are equal, so ragged lengths leave none idle.
 //
 // A workgroup's 4 waves take 32 positions each of a step of 128, on
 // v_mfma_f32_16x16x32_f16 with the rows as columns.  Up to 8 rows (ST) sit as
@@ -128,55 +124,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
     const int G = a.grp, rc = ST ? c & 7 : c;
 
     int mine;
-    const int total = pa_total(a, pl, mine), share = pa_share(total);
+    const int total = pa_total<false>(a, pl, mine), share = pa_share(pl.few, total);
     const int first = blockIdx.x * share, stop = min(first + share, total);
     for (int u = first; u < stop;) {
-        // the piece: steps [step, step + n) of `all` of one KV head
-        const bool pre = u < pl.few_pre * p.n_kv;
-        PagedSeq sq;
-        int kvh, step, all, seglen, hi0, hi1, lo0, lo1, base0;
-        const int *table;
-        bool bad = false;
-        if (pre) {
-            sq.t0 = 0;
-            sq.nq = pa_tokens(b);
-            sq.bad = false;
-            all = pl.few_pre;
-            kvh = u / all;
-            step = u - kvh * all;
-            seglen = b.n_prefix;
-            table = b.prefix;
-            hi0 = hi1 = seglen - 1;
-            lo0 = 0;
-            lo1 = a.window ? 0x7fffffff : 0;                 // row by row
-            base0 = 0;
-            sq.len = seglen;
-        } else {
-            int seq, before;
-            const int v = u - pl.few_pre * p.n_kv;
-            pa_find_step(a, pl, mine, v, seq, before);
-            sq = paged_seq(p, b, seq);
-            const int low = pa_low(sq.len - sq.nq, a.window);
-            all = pa_seq_steps(a, pl, sq);
-            kvh = (v - before) / all;
-            step = v - before - kvh * all;
-            seglen = sq.bad ? 0 : sq.len;
-            bad = sq.bad;
-            table = b.table + (size_t)seq * b.table_stride;
-            hi0 = sq.len - sq.nq;
-            hi1 = sq.len - 1;
-            lo0 = a.window ? max(0, hi0 + 1 - a.window) : 0;
-            lo1 = a.window ? max(0, hi1 + 1 - a.window) : 0;
-            base0 = low;
-            if (bad && threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
-        }
-        const int n = min(all - step, stop - u), rows = sq.nq * G;
-        const bool whole = n == all;
-        const int slot = 2 * blockIdx.x + (u != first);
-        u += n;
-        const int start = base0 + (step << pl.few_shift), end = min(start + (n << pl.few_shift), min(hi1 + 1, seglen));
-        const bool mixed = hi0 != hi1 || lo0 != lo1;         // whether the rows differ in what they attend
-        const int last = (seglen - 1) >> 4, iters = end > start ? (end - start + 32 * PW - 1) / (32 * PW) : 0;
+        const PaPiece x = pa_piece<false>(a, pl, mine, blockIdx.x, u, first, stop);
+        u += x.n;
+        const PagedSeq &sq = x.sq;
+        const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = sq.nq * G;
+        bool bad = sq.bad;
+        if (bad && threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
+        const bool mixed = hi0 != x.hi1 || lo0 != lo1;       // whether the rows differ in what they attend
+        const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 32 * PW - 1) / (32 * PW) : 0;
 
         // queries: loaded first, ahead of the stream
         constexpr int LPR = 256 / R, QN = HD / (4 * LPR) > 0 ? HD / (4 * LPR) : 1;
@@ -200,7 +158,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
         int rlo = lo0, rhi = hi0;
         if (rc < rows) {
             const int i = (int)(rc * pl.grp_inv >> 16);
-            if (!pre) {
+            if (!x.pre) {
                 rhi = hi0 + i;
                 rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
             } else if (a.window) {
@@ -213,7 +171,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
         PaUnits us, more_us;                                 // of 32 steps, and of the next 32
         int base = start + 32 * pw;
         if (iters) {
-            us = pa_units<KVT>(p, table, base >> 4, 2 * PW, last, kvh, bad);
+            us = pa_units<KVT>(p, x.table, base >> 4, 2 * PW, last, kvh, bad);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             pa_load_k<HD, HE, KVT>(kv, p, nx, c, g, ew);
@@ -243,11 +201,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
         }
         lds_barrier();
         const _Float16 *const q0 = qh + ((ST && c >= 8 ? R : 0) + rc) * QP + HE * ew + 8 * g, *const q1 = qh + (R + rc) * QP + HE * ew + 8 * g;
-        pa_v8h x0[NS], x1[ST ? 1 : NS];
+        pa_v8h qa[NS], qb[ST ? 1 : NS];
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            x0[s] = *(const pa_v8h *)(q0 + 32 * s);
-            if constexpr (!ST) x1[s] = *(const pa_v8h *)(q1 + 32 * s);
+            qa[s] = *(const pa_v8h *)(q0 + 32 * s);
+            if constexpr (!ST) qb[s] = *(const pa_v8h *)(q1 + 32 * s);
         }
         const float qs = qsc[rc], capl = a.cap * 1.4426950408889634f;
 
@@ -265,7 +223,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
                 nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
             }
-            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units<KVT>(p, table, (base >> 4) + 64 * PW, 2 * PW, last, kvh, bad);
+            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units<KVT>(p, x.table, (base >> 4) + 64 * PW, 2 * PW, last, kvh, bad);
             const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
             // scores at positions base + 16 h + 4 g + i
             pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -275,11 +233,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                 for (int h = 0; h < 2; h++) {
                     const pa_v8h ko = pa_key<HE, KVT>(kv, h, s);
                     if constexpr (KVT == F16) {
-                        sc[h] = pa_mma(ko, x0[s], sc[h]);
-                        if constexpr (!ST) sc[h] = pa_mma(ko, x1[s], sc[h]);
+                        sc[h] = pa_mma(ko, qa[s], sc[h]);
+                        if constexpr (!ST) sc[h] = pa_mma(ko, qb[s], sc[h]);
                     } else {
-                        pa_v4f d = pa_mma(ko, x0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f});
-                        if constexpr (!ST) d = pa_mma(ko, x1[s], d);
+                        pa_v4f d = pa_mma(ko, qa[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f});
+                        if constexpr (!ST) d = pa_mma(ko, qb[s], d);
 #pragma unroll
                         for (int i = 0; i < 4; i++) sc[h][i] = __builtin_fmaf(pa_scale(kv.dk[4 * h + i], s), d[i], sc[h][i]);
                     }
@@ -296,17 +254,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                 sc[0] = *(const pa_v4f *)xs[it & 1][w0][lane];
                 sc[1] = *(const pa_v4f *)(xs[it & 1][w0][lane] + 4);
 #pragma unroll
-                for (int x = 1; x < ES; x++) {
-                    sc[0] += *(const pa_v4f *)xs[it & 1][w0 + x][lane];
-                    sc[1] += *(const pa_v4f *)(xs[it & 1][w0 + x][lane] + 4);
+                for (int k = 1; k < ES; k++) {
+                    sc[0] += *(const pa_v4f *)xs[it & 1][w0 + k][lane];
+                    sc[1] += *(const pa_v4f *)(xs[it & 1][w0 + k][lane] + 4);
                 }
             }
             float w[8], mt = -__builtin_inff();
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                float x = sc[j >> 2][j & 3];
-                if constexpr (ST) x += xor8(x);
-                w[j] = x * qs;
+                float y = sc[j >> 2][j & 3];
+                if constexpr (ST) y += xor8(y);
+                w[j] = y * qs;
             }
             if (a.cap > 0.0f) {
 #pragma unroll
@@ -321,20 +279,19 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                float x = w[j];
+                float y = w[j];
                 if constexpr (KVT != F16) {                  // + the exponent of the position's largest value scale
                     uint32_t dm = 1;                         // all zero: the smallest scale there is
 #pragma unroll
                     for (int d = 0; d < HE / 64; d++) dm = max(dm, max(kv.dv[j][d] & 0x7fffu, (kv.dv[j][d] >> 16) & 0x7fffu));
-                    x += (float)__builtin_amdgcn_frexp_expf(h2f((uint16_t)dm));
+                    y += (float)__builtin_amdgcn_frexp_expf(h2f((uint16_t)dm));
                 }
-                mt = fmaxf(mt, x);
+                mt = fmaxf(mt, y);
             }
             mt = fmaxf(mt, partner<16>(mt));
             mt = fmaxf(mt, partner<32>(mt));
-            const float mn = fmaxf(m, mt);
-            if (__any(mn > m)) {
-                const float cr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+            if (__any(mt > m + PA_LAG)) {
+                const float mn = fmaxf(m, mt), cr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
                 l *= cr;
 #pragma unroll
                 for (int e = 0; e < NM; e++) o[e] *= cr;
@@ -411,15 +368,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (KVT == F16) {
                 if (odd) {
-                    for (int x = 0; x < 32; x++) {
-                        const int pos = base + x;
+                    for (int k = 0; k < 32; k++) {
+                        const int pos = base + k;
                         if (pos < lo0 || pos >= end) continue;
-                        const uint16_t *row = (const uint16_t *)(p.v + (x < 16 ? un[0].row : un[1].row)) + (x & 15) * HD + HE * ew;
+                        const uint16_t *row = (const uint16_t *)(p.v + (k < 16 ? un[0].row : un[1].row)) + (k & 15) * HD + HE * ew;
                         float wx = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            const float v = __shfl(w[j], 16 * ((x & 15) >> 2) + c, 64);
-                            if (j == 4 * (x >> 4) + (x & 3)) wx = v;
+                            const float v = __shfl(w[j], 16 * ((k & 15) >> 2) + c, 64);
+                            if (j == 4 * (k >> 4) + (k & 3)) wx = v;
                         }
                         const bool sees = pos >= rlo && pos <= rhi && !(ST && c >= 8);
 #pragma unroll
@@ -459,8 +416,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                     for (int i = 0; i < 4; i++) buf[(pw * 8 + (c & 7)) * (HD + 4) + HE * ew + pa_elem<HE, KVT>(e, 4 * g + i)] = o[e][i];
             }
             lds_barrier();
-            for (int x = threadIdx.x; x < 8 * (HD / 4); x += 256) {
-                const int r8 = x / (HD / 4), e4 = x % (HD / 4) * 4, r = 8 * k + r8;
+            for (int y = threadIdx.x; y < 8 * (HD / 4); y += 256) {
+                const int r8 = y / (HD / 4), e4 = y % (HD / 4) * 4, r = 8 * k + r8;
                 if (r >= rows) continue;
                 float mm = -__builtin_inff();
 #pragma unroll
@@ -477,18 +434,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                 }
                 s *= VS;
                 const int i = (int)(r * pl.grp_inv >> 16), tok = sq.t0 + i, head = kvh * G + (r - i * G);
-                const size_t row = (size_t)tok * a.n_head + head;
-                if (!pre && whole && b.n_prefix == 0) {
+                const PaSink to = pa_sink<false>(a, pl, x, share, r, tok, head, e4 == 0);
+                if (to.out) {
                     s = !sq.bad && hi0 + i < 0 ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / ls);
-                    pa_store4(a.out + (size_t)tok * a.os + (size_t)head * HD + e4, s);
-                } else if (!pre && whole) {
-                    const size_t at = row * pl.nown;
-                    *(pa_v4f *)(pl.oo + at * HD + e4) = s;
-                    if (e4 == 0) pl.oml[at] = make_float2(mm, ls);
+                    pa_store4(to.o + e4, s);
                 } else {
-                    const size_t at = (size_t)slot * R + r;
-                    *(pa_v4f *)(pl.fo + at * HD + e4) = s;
-                    if (e4 == 0) pl.fml[at] = make_float2(mm, ls);
+                    *(pa_v4f *)(to.o + e4) = s;
+                    if (e4 == 0) *to.ml = make_float2(mm, ls);
                 }
             }
         }
@@ -497,8 +449,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
 
 template <int KVT, int HD>
 hipError_t pa_few_hd(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
-    const dim3 grid(pl.few_wgs), wg(256);
-    if (pl.few_rows <= 8) hipLaunchKernelGGL((k_paged_few<HD, KVT, true>), grid, wg, 0, s, a, pl);
+    const dim3 grid(pl.few.wgs), wg(256);
+    if (pl.few.rows <= 8) hipLaunchKernelGGL((k_paged_few<HD, KVT, true>), grid, wg, 0, s, a, pl);
     else hipLaunchKernelGGL((k_paged_few<HD, KVT, false>), grid, wg, 0, s, a, pl);
     return hipGetLastError();
 }

@@ -39,11 +39,11 @@ struct PmStage {
     static constexpr int KRUNS = KVT == F16 ? 32 * HD / 8 : KVT == Q8_0 ? 32 * HD / 16 : 32 * HD / 8;
     static constexpr int KT = (KRUNS + 255) / 256;
     static constexpr int KD = KVT == Q4_0 ? 1 : 4;           // dwords of a run
-    // V: 8 positions of one (ks, g) x (f16: 8 elements of 16 bytes; q8_0: 4 bytes, q4_0: 2 bytes = 4 elements 16 apart)
-    static constexpr int VE = KVT == F16 ? 8 : 4;
+    // V: 8 positions of one (ks, g) x (f16: 4 elements, 8 bytes; q8_0: 4 bytes, q4_0: 2 bytes = 4 elements 16 apart)
+    static constexpr int VE = 4;
     static constexpr int VTASKS = 4 * HD / VE;
     static constexpr int VT = (VTASKS + 255) / 256;
-    static constexpr int VD = KVT == F16 ? 4 : 1;
+    static constexpr int VD = KVT == F16 ? 2 : 1;
     static constexpr int STASKS = KVT == F16 ? 0 : 2 * 32 * HD / 64;     // dwords of scales, K then V
     static constexpr int SCT = (STASKS + 255) / 256;
     uint32_t k[KT][KD], v[VT][8][VD], s[SCT ? SCT : 1];
@@ -139,7 +139,7 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
                     const int pos = pm_pos(ks, g, j);
                     const bool dead = pos < lo || pos >= hi;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < T::VD; i++) {
                         uint32_t y = dead ? 0u : v[j][i];
                         const bool a0 = (y & 0x7c00u) == 0x7c00u, a1 = (y & 0x7c000000u) == 0x7c000000u;
                         odd |= a0 | a1;
@@ -149,8 +149,8 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int e = 8 * at + i;
+            for (int i = 0; i < 4; i++) {
+                const int e = 4 * at + i;
                 pa_v4u w;
 #pragma unroll
                 for (int k = 0; k < 4; k++) w[k] = __builtin_amdgcn_perm(v[2 * k + 1][i >> 1], v[2 * k][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
@@ -192,329 +192,298 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
 
 template <int HD, int KVT>
 __global__ __launch_bounds__(256, HD >= 256 ? 1 : 2) void k_paged_many(PagedAttn a, PagedPlan pl) {
-    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 16, NE = HE / 32;
-    __shared__ __align__(16) PmTile<HD, KVT> tiles[HD > 256 ? 1 : 2];
+    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 16, NE = HE / 32, NB = HD > 256 ? 1 : 2;   // NB: buffers
+    __shared__ __align__(16) PmTile<HD, KVT> tiles[NB];
     __shared__ __align__(16) float xs[ES > 1 ? 4 : 1][ES > 1 ? 64 : 1][16];
     __shared__ int odds[3];                                  // by iteration: whether the tile held a non-finite value
-    constexpr int NB = HD > 256 ? 1 : 2;                     // buffers
     const int lane = threadIdx.x & 63, wave = pa_uniform(threadIdx.x >> 6), c = lane & 31, g = lane >> 5, ew = wave % ES, rw = wave / ES;
     const PagedPool &p = a.p;
     const PagedBatch &b = a.b;
-    const int G = a.grp, R = pl.many_rows;
+    const int G = a.grp, R = pl.many.rows;
 
-    // the item: prefix items first
-    int item = blockIdx.x;
-    const int npre_items = pl.pre_slots * p.n_kv * pl.npre;
-    const bool pre = item < npre_items;
-    if (!pre) item -= npre_items;
-    const int slots = pre ? pl.pre_slots : pl.own_slots;
-    int tile = item % slots;
-    item /= slots;
-    const int kvh = item % p.n_kv, chunk = item / p.n_kv;
-    PagedSeq sq;
-    int seglen, start, end, hi0, hi1, lo0, lo1;              // the first and last row's last and first positions
-    const int *table;
-    bool bad = false;
-    if (pre) {
-        sq.t0 = 0;
-        sq.nq = pa_tokens(b);
-        sq.bad = false;
-        if (tile * R >= sq.nq * G) return;
-        seglen = b.n_prefix;
-        table = b.prefix;
-        start = chunk * pl.pre_chunk;
-        end = min(start + pl.pre_chunk, seglen);
-        sq.len = seglen;
-        hi0 = hi1 = seglen - 1;
-        lo0 = 0;
-        lo1 = a.window ? 0x7fffffff : 0;                     // row by row
-    } else {
-        int seq;
-        pa_find_tile(a, pl, tile, seq, tile);
-        seq = pa_uniform(seq);
-        tile = pa_uniform(tile);
-        if (seq >= b.n_seq) return;
-        sq = paged_seq(p, b, seq);
-        if (tile * R >= sq.nq * G) return;
-        bad = sq.bad;
-        int lo;
-        pa_tile_span(sq, G, R, tile, a.window, lo, hi1);
-        if (chunk >= pa_tile_chunks(sq, pl, lo, hi1)) return;
+    // Workgroups of one XCD (every eighth) take neighbouring shares: row tiles
+    // that read the same K and V find them in its L2.
+    const int per = (pl.many.wgs + 7) >> 3, w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    int mine;
+    const int total = pa_total<true>(a, pl, mine), share = pa_share(pl.many, total);
+    const int first = w * share, stop = w < pl.many.wgs ? min(first + share, total) : 0;
+    for (int u = first; u < stop;) {
+        const PaPiece x = pa_piece<true>(a, pl, mine, w, u, first, stop);
+        u += x.n;
+        const PagedSeq &sq = x.sq;
+        const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end;
+        bool bad = sq.bad;
         if (bad && threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
-        seglen = sq.bad ? 0 : sq.len;
-        table = b.table + (size_t)seq * b.table_stride;
-        start = lo + chunk * pl.own_chunk;
-        end = min(min(start + pl.own_chunk, hi1 + 1), seglen);
-        hi0 = sq.len - sq.nq + tile * R / G;
-        lo0 = a.window ? max(0, hi0 + 1 - a.window) : 0;
-        lo1 = a.window ? max(0, hi1 + 1 - a.window) : 0;
-    }
-    const int last = (seglen - 1) >> 4, iters = end > start ? (end - start + 31) / 32 : 0;
+        const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 31) / 32 : 0;
 
-    // the lane's row, its positions [rlo, rhi], and its query in two halves
-    const int r = tile * R + 32 * rw + c;
-    const bool ok = 32 * rw < R && r < sq.nq * G;
-    const bool busy = 32 * rw < R && tile * R + 32 * rw < sq.nq * G;     // whether the wave has rows
-    const int ri = ok ? r / G : 0, head = kvh * G + (ok ? r - ri * G : 0), tok = sq.t0 + ri;
-    int rlo = lo0, rhi = hi0;
-    if (ok) {
-        if (!pre) {
-            rhi = sq.len - sq.nq + ri;
-            rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
-        } else if (a.window) {
-            rlo = max(0, pa_token_pos(p, b, tok) + 1 - a.window);
-        }
-    }
-    PmStage<HD, KVT> st;
-    PaUnits us, more_us;                                     // of 32 steps, and of the next 32
-    PaUnit un[2], nx[2];
-    if (iters) {
-        us = pa_units<KVT>(p, table, start >> 4, 2, last, kvh, bad);
-        nx[0] = pa_unit<HD, KVT>(p, us, 0);
-        nx[1] = pa_unit<HD, KVT>(p, us, 1);
-        pm_load<HD, KVT>(st, p, nx);
-    }
-    pa_v8h q0[NS], q1[NS];
-    float qs;
-    {
-        const float *src = a.q + (size_t)tok * a.qs + (size_t)head * HD + HE * ew + 8 * g;
-        const bool al = ((uintptr_t)src & 15) == 0;
-        float am = 0.0f;
-        pa_v4f x[NS][2];
-#pragma unroll
-        for (int s = 0; s < NS; s++)
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const float *d = src + 16 * s + 4 * k;
-                x[s][k] = !ok ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : al ? *(const pa_v4f *)d : pa_v4f{d[0], d[1], d[2], d[3]};
-#pragma unroll
-                for (int i = 0; i < 4; i++) am = fmaxf(am, fabsf(x[s][k][i]));
+        // the lane's row, its positions [rlo, rhi], and its query in two halves
+        const int r = x.tile * R + 32 * rw + c;
+        const bool ok = 32 * rw < R && r < sq.nq * G;
+        const bool busy = 32 * rw < R && x.tile * R + 32 * rw < sq.nq * G;   // whether the wave has rows
+        const int ri = ok ? r / G : 0, head = kvh * G + (ok ? r - ri * G : 0), tok = sq.t0 + ri;
+        int rlo = lo0, rhi = hi0;
+        if (ok) {
+            if (!x.pre) {
+                rhi = sq.len - sq.nq + ri;
+                rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
+            } else if (a.window) {
+                rlo = max(0, pa_token_pos(p, b, tok) + 1 - a.window);
             }
-        am = fmaxf(am, partner<32>(am));
-        if constexpr (ES > 1) {                              // over both halves of the elements
-            xs[wave][lane][0] = am;
-            __syncthreads();
-            am = fmaxf(am, xs[wave ^ 1][lane][0]);
-            __syncthreads();
         }
-        const int sh = pa_shift(am);
-        qs = pa_score_scale<KVT>(a, sh);
-#pragma unroll
-        for (int s = 0; s < NS; s++) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                pa_split(__builtin_ldexpf(x[s][k >> 1][2 * (k & 1)], sh), __builtin_ldexpf(x[s][k >> 1][2 * (k & 1) + 1], sh), hi[k], lo[k]);
-            q0[s] = pa_op(hi[0], hi[1], hi[2], hi[3]);
-            q1[s] = pa_op(lo[0], lo[1], lo[2], lo[3]);
-        }
-    }
-    const float capl = a.cap * 1.4426950408889634f;
-    pa_v16f o[NE];
-    float m = -__builtin_inff(), l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < NE; e++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[e][i] = 0.0f;
-    if (threadIdx.x < 3) odds[threadIdx.x] = 0;
-    __syncthreads();
-
-    for (int it = 0, turn = 0; it < iters; it++, turn = turn == 2 ? 0 : turn + 1) {
-        const int base = start + 32 * it;
-        const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
-        PmTile<HD, KVT> &d = tiles[NB == 2 ? it & 1 : 0];
-        if (NB == 1 && it) __syncthreads();                  // one buffer: the previous positions are used
-        if (pm_store<HD, KVT>(d, st, edge, lo0 - base, end - base)) odds[turn] = 1;
-        un[0] = nx[0];
-        un[1] = nx[1];
-        if ((it & 31) == 31) us = more_us;
-        if (it + 1 < iters) {
-            nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
-            nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
+        PmStage<HD, KVT> st;
+        PaUnits us, more_us;                                     // of 32 steps, and of the next 32
+        PaUnit un[2], nx[2];
+        if (iters) {
+            us = pa_units<KVT>(p, x.table, start >> 4, 2, last, kvh, bad);
+            nx[0] = pa_unit<HD, KVT>(p, us, 0);
+            nx[1] = pa_unit<HD, KVT>(p, us, 1);
             pm_load<HD, KVT>(st, p, nx);
         }
-        if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units<KVT>(p, table, (base >> 4) + 64, 2, last, kvh, bad);
-        lds_barrier();
-        const int odd = odds[turn];
-        if (threadIdx.x == 0) odds[turn == 0 ? 2 : turn - 1] = 0;        // the iteration after the next's: written behind the next barrier
-        if (!busy && ES == 1) continue;
-        // scores at positions base + 8 (i / 4) + 4 g + i % 4
-        pa_v16f sc;
+        pa_v8h q0[NS], q1[NS];
+        float qs;
+        {
+            // twice over the row: the largest magnitude, then the halves
+            const float *src = a.q + (size_t)tok * a.qs + (size_t)head * HD + HE * ew + 8 * g;
+            const bool al = ((uintptr_t)src & 15) == 0;
+            auto ld = [&](int s, int k) {
+                const float *d = src + 16 * s + 4 * k;
+                return !ok ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : al ? *(const pa_v4f *)d : pa_v4f{d[0], d[1], d[2], d[3]};
+            };
+            float am = 0.0f;
+#pragma unroll 8
+            for (int s = 0; s < NS; s++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) sc[i] = 0.0f;
-        const _Float16 *kr = &d.k[c][HE * ew + 8 * g];
-        if constexpr (KVT == F16) {
+                for (int k = 0; k < 2; k++) {
+                    const pa_v4f y = ld(s, k);
+                    am = fmaxf(fmaxf(am, fmaxf(fabsf(y[0]), fabsf(y[1]))), fmaxf(fabsf(y[2]), fabsf(y[3])));
+                }
+            am = fmaxf(am, partner<32>(am));
+            if constexpr (ES > 1) {                              // over both halves of the elements
+                __syncthreads();
+                xs[wave][lane][0] = am;
+                __syncthreads();
+                am = fmaxf(am, xs[wave ^ 1][lane][0]);
+                __syncthreads();
+            }
+            const int sh = pa_shift(am);
+            qs = pa_score_scale<KVT>(a, sh);
 #pragma unroll
             for (int s = 0; s < NS; s++) {
-                const pa_v8h ko = *(const pa_v8h *)(kr + 16 * s);
-                sc = pa_mma32(ko, q0[s], sc);
-                sc = pa_mma32(ko, q1[s], sc);
+                const pa_v4f y = ld(s, 0), z = ld(s, 1);
+                uint32_t hi[4], lo[4];
+                pa_split(__builtin_ldexpf(y[0], sh), __builtin_ldexpf(y[1], sh), hi[0], lo[0]);
+                pa_split(__builtin_ldexpf(y[2], sh), __builtin_ldexpf(y[3], sh), hi[1], lo[1]);
+                pa_split(__builtin_ldexpf(z[0], sh), __builtin_ldexpf(z[1], sh), hi[2], lo[2]);
+                pa_split(__builtin_ldexpf(z[2], sh), __builtin_ldexpf(z[3], sh), hi[3], lo[3]);
+                q0[s] = pa_op(hi[0], hi[1], hi[2], hi[3]);
+                q1[s] = pa_op(lo[0], lo[1], lo[2], lo[3]);
+                if (s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
-        } else {
+        }
+        const float capl = a.cap * 1.4426950408889634f;
+        pa_v16f o[NE];
+        float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
-            for (int s = 0; s < NE; s++) {
-                pa_v16f x;
+        for (int e = 0; e < NE; e++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = 0.0f;
+            for (int i = 0; i < 16; i++) o[e][i] = 0.0f;
+        __syncthreads();                                         // the previous piece's tiles are used
+        if (threadIdx.x < 3) odds[threadIdx.x] = 0;
+        __syncthreads();
+
+        for (int it = 0, turn = 0; it < iters; it++, turn = turn == 2 ? 0 : turn + 1) {
+            const int base = start + 32 * it;
+            const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
+            PmTile<HD, KVT> &d = tiles[NB == 2 ? it & 1 : 0];
+            if (NB == 1 && it) __syncthreads();                  // one buffer: the previous positions are used
+            if (pm_store<HD, KVT>(d, st, edge, lo0 - base, end - base)) odds[turn] = 1;
+            un[0] = nx[0];
+            un[1] = nx[1];
+            if ((it & 31) == 31) us = more_us;
+            if (it + 1 < iters) {
+                nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
+                nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
+                pm_load<HD, KVT>(st, p, nx);
+            }
+            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units<KVT>(p, x.table, (base >> 4) + 64, 2, last, kvh, bad);
+            lds_barrier();
+            const int odd = odds[turn];
+            if (threadIdx.x == 0) odds[turn == 0 ? 2 : turn - 1] = 0;        // the iteration after the next's: written behind the next barrier
+            if (!busy && ES == 1) continue;
+            // scores at positions base + 8 (i / 4) + 4 g + i % 4
+            pa_v16f sc;
 #pragma unroll
-                for (int k = 2 * s; k < 2 * s + 2; k++) {
-                    const pa_v8h ko = *(const pa_v8h *)(kr + 16 * k);
-                    x = pa_mma32(ko, q0[k], x);
-                    x = pa_mma32(ko, q1[k], x);
+            for (int i = 0; i < 16; i++) sc[i] = 0.0f;
+            const _Float16 *kr = &d.k[c][HE * ew + 8 * g];
+            if constexpr (KVT == F16) {
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const pa_v8h ko = *(const pa_v8h *)(kr + 16 * s);
+                    sc = pa_mma32(ko, q0[s], sc);
+                    sc = pa_mma32(ko, q1[s], sc);
                 }
+            } else {
+#pragma unroll
+                for (int s = 0; s < NE; s++) {
+                    pa_v16f y;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) y[i] = 0.0f;
+#pragma unroll
+                    for (int k = 2 * s; k < 2 * s + 2; k++) {
+                        const pa_v8h ko = *(const pa_v8h *)(kr + 16 * k);
+                        y = pa_mma32(ko, q0[k], y);
+                        y = pa_mma32(ko, q1[k], y);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint2 dd = *(const uint2 *)&d.dk[NE * ew + s][8 * k + 4 * g];
+                        sc[4 * k] = __builtin_fmaf(pa_lo(dd.x), y[4 * k], sc[4 * k]);
+                        sc[4 * k + 1] = __builtin_fmaf(pa_hi(dd.x), y[4 * k + 1], sc[4 * k + 1]);
+                        sc[4 * k + 2] = __builtin_fmaf(pa_lo(dd.y), y[4 * k + 2], sc[4 * k + 2]);
+                        sc[4 * k + 3] = __builtin_fmaf(pa_hi(dd.y), y[4 * k + 3], sc[4 * k + 3]);
+                    }
+                }
+            }
+            if constexpr (ES > 1) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) *(pa_v4f *)&xs[wave][lane][4 * k] = pa_v4f{sc[4 * k], sc[4 * k + 1], sc[4 * k + 2], sc[4 * k + 3]};
+                lds_barrier();
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const uint2 dd = *(const uint2 *)&d.dk[NE * ew + s][8 * k + 4 * g];
-                    sc[4 * k] = __builtin_fmaf(pa_lo(dd.x), x[4 * k], sc[4 * k]);
-                    sc[4 * k + 1] = __builtin_fmaf(pa_hi(dd.x), x[4 * k + 1], sc[4 * k + 1]);
-                    sc[4 * k + 2] = __builtin_fmaf(pa_lo(dd.y), x[4 * k + 2], sc[4 * k + 2]);
-                    sc[4 * k + 3] = __builtin_fmaf(pa_hi(dd.y), x[4 * k + 3], sc[4 * k + 3]);
+                    const pa_v4f y = *(const pa_v4f *)&xs[wave ^ 1][lane][4 * k];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[4 * k + i] += y[i];
                 }
             }
-        }
-        if constexpr (ES > 1) {
+            float mt = -__builtin_inff();
 #pragma unroll
-            for (int k = 0; k < 4; k++) *(pa_v4f *)&xs[wave][lane][4 * k] = pa_v4f{sc[4 * k], sc[4 * k + 1], sc[4 * k + 2], sc[4 * k + 3]};
-            lds_barrier();
+            for (int i = 0; i < 16; i++) sc[i] *= qs;
+            if (a.cap > 0.0f) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const pa_v4f x = *(const pa_v4f *)&xs[wave ^ 1][lane][4 * k];
-#pragma unroll
-                for (int i = 0; i < 4; i++) sc[4 * k + i] += x[i];
+                for (int i = 0; i < 16; i++) sc[i] = capl * pa_tanh(sc[i]);
             }
-        }
-        float mt = -__builtin_inff();
+            if (edge) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) sc[i] *= qs;
-        if (a.cap > 0.0f) {
+                for (int i = 0; i < 16; i++) {
+                    const int pos = base + 8 * (i >> 2) + 4 * g + (i & 3);
+                    sc[i] = pos >= rlo && pos <= rhi && pos < end ? sc[i] : -__builtin_inff();
+                }
+            }
+            if constexpr (KVT == F16) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[i] = capl * pa_tanh(sc[i]);
-        }
-        if (edge) {
+                for (int i = 0; i < 16; i++) mt = fmaxf(mt, sc[i]);
+            } else {
+                // + the exponent of the position's largest value scale
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint2 y = make_uint2(0x00010001u, 0x00010001u);      // all zero: the smallest scale there is
+#pragma unroll
+                    for (int s = 0; s < HD / 32; s++) {
+                        const uint2 z = *(const uint2 *)&d.dv[s][8 * k + 4 * g];
+                        y.x = max(y.x & 0xffffu, z.x & 0x7fffu) | max(y.x & 0xffff0000u, z.x & 0x7fff0000u);
+                        y.y = max(y.y & 0xffffu, z.y & 0x7fffu) | max(y.y & 0xffff0000u, z.y & 0x7fff0000u);
+                    }
+                    mt = fmaxf(mt, sc[4 * k] + (float)__builtin_amdgcn_frexp_expf(pa_lo(y.x)));
+                    mt = fmaxf(mt, sc[4 * k + 1] + (float)__builtin_amdgcn_frexp_expf(pa_hi(y.x)));
+                    mt = fmaxf(mt, sc[4 * k + 2] + (float)__builtin_amdgcn_frexp_expf(pa_lo(y.y)));
+                    mt = fmaxf(mt, sc[4 * k + 3] + (float)__builtin_amdgcn_frexp_expf(pa_hi(y.y)));
+                }
+            }
+            mt = fmaxf(mt, partner<32>(mt));
+            if (__any(mt > m + PA_LAG)) {
+                const float mn = fmaxf(m, mt), cr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+                l *= cr;
+#pragma unroll
+                for (int e = 0; e < NE; e++) o[e] *= cr;
+                m = mn;
+            }
+            const float mr = m == -__builtin_inff() ? 0.0f : m - PA_SHIFT;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const int pos = base + 8 * (i >> 2) + 4 * g + (i & 3);
-                sc[i] = pos >= rlo && pos <= rhi && pos < end ? sc[i] : -__builtin_inff();
+                sc[i] = __builtin_amdgcn_exp2f(sc[i] - mr);
+                l += sc[i];
             }
-        }
-        if constexpr (KVT == F16) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) mt = fmaxf(mt, sc[i]);
-        } else {
-            // + the exponent of the position's largest value scale
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                uint2 x = make_uint2(0x00010001u, 0x00010001u);      // all zero: the smallest scale there is
-#pragma unroll
-                for (int s = 0; s < HD / 32; s++) {
-                    const uint2 y = *(const uint2 *)&d.dv[s][8 * k + 4 * g];
-                    x.x = max(x.x & 0xffffu, y.x & 0x7fffu) | max(x.x & 0xffff0000u, y.x & 0x7fff0000u);
-                    x.y = max(x.y & 0xffffu, y.y & 0x7fffu) | max(x.y & 0xffff0000u, y.y & 0x7fff0000u);
-                }
-                mt = fmaxf(mt, sc[4 * k] + (float)__builtin_amdgcn_frexp_expf(pa_lo(x.x)));
-                mt = fmaxf(mt, sc[4 * k + 1] + (float)__builtin_amdgcn_frexp_expf(pa_hi(x.x)));
-                mt = fmaxf(mt, sc[4 * k + 2] + (float)__builtin_amdgcn_frexp_expf(pa_lo(x.y)));
-                mt = fmaxf(mt, sc[4 * k + 3] + (float)__builtin_amdgcn_frexp_expf(pa_hi(x.y)));
-            }
-        }
-        mt = fmaxf(mt, partner<32>(mt));
-        const float mn = fmaxf(m, mt);
-        if (__any(mn > m)) {
-            const float cr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-            l *= cr;
-#pragma unroll
-            for (int e = 0; e < NE; e++) o[e] *= cr;
-            m = mn;
-        }
-        const float mr = m == -__builtin_inff() ? 0.0f : m - PA_SHIFT;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            sc[i] = __builtin_amdgcn_exp2f(sc[i] - mr);
-            l += sc[i];
-        }
-        if constexpr (KVT == F16) {
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) pa_split(sc[8 * ks + 2 * k], sc[8 * ks + 2 * k + 1], hi[k], lo[k]);
-                const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-                for (int e = 0; e < NE; e++) {
-                    const pa_v8h va = *(const pa_v8h *)d.v[ks][NE * ew + e][lane];
-                    o[e] = pa_mma32(va, b0, o[e]);
-                    o[e] = pa_mma32(va, b1, o[e]);
-                }
-            }
-            if (odd) {
-                // non-finite values, zero in LDS, added to the rows that attend them
-                for (int x = 0; x < 32; x++) {
-                    const int pos = base + x;
-                    if (pos < lo0 || pos >= end) continue;
-                    const uint16_t *row = (const uint16_t *)(p.v + (x < 16 ? un[0].row : un[1].row)) + (x & 15) * HD + HE * ew;
-                    float wx = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float v = __shfl(sc[i], 32 * ((x >> 2) & 1) + c, 64);
-                        if (i == 4 * (x >> 3) + (x & 3)) wx = v;
-                    }
-                    const bool sees = pos >= rlo && pos <= rhi;
-#pragma unroll
-                    for (int e = 0; e < NE; e++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const uint16_t hv = row[32 * e + 8 * (i >> 2) + 4 * g + (i & 3)];
-                            if (sees && (hv & 0x7c00) == 0x7c00) o[e][i] += wx * h2f(hv);
-                        }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < NE; e++) {
+            if constexpr (KVT == F16) {
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
                     uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const uint2 dd = *(const uint2 *)&d.dv[NE * ew + e][16 * ks + 8 * k + 4 * g];
-                        const float w0 = sc[8 * ks + 4 * k], w1 = sc[8 * ks + 4 * k + 1], w2 = sc[8 * ks + 4 * k + 2], w3 = sc[8 * ks + 4 * k + 3];
-                        pa_split(w0 == 0.0f ? 0.0f : w0 * pa_lo(dd.x), w1 == 0.0f ? 0.0f : w1 * pa_hi(dd.x), hi[2 * k], lo[2 * k]);
-                        pa_split(w2 == 0.0f ? 0.0f : w2 * pa_lo(dd.y), w3 == 0.0f ? 0.0f : w3 * pa_hi(dd.y), hi[2 * k + 1], lo[2 * k + 1]);
+                    for (int k = 0; k < 4; k++) pa_split(sc[8 * ks + 2 * k], sc[8 * ks + 2 * k + 1], hi[k], lo[k]);
+                    const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+                    for (int e = 0; e < NE; e++) {
+                        const pa_v8h va = *(const pa_v8h *)d.v[ks][NE * ew + e][lane];
+                        o[e] = pa_mma32(va, b0, o[e]);
+                        o[e] = pa_mma32(va, b1, o[e]);
                     }
-                    const pa_v8h va = *(const pa_v8h *)d.v[ks][NE * ew + e][lane];
-                    o[e] = pa_mma32(va, pa_op(hi[0], hi[1], hi[2], hi[3]), o[e]);
-                    o[e] = pa_mma32(va, pa_op(lo[0], lo[1], lo[2], lo[3]), o[e]);
+                }
+                if (odd) {
+                    // non-finite values, zero in LDS, added to the rows that attend them
+                    for (int k = 0; k < 32; k++) {
+                        const int pos = base + k;
+                        if (pos < lo0 || pos >= end) continue;
+                        const uint16_t *row = (const uint16_t *)(p.v + (k < 16 ? un[0].row : un[1].row)) + (k & 15) * HD + HE * ew;
+                        float wx = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float v = __shfl(sc[i], 32 * ((k >> 2) & 1) + c, 64);
+                            if (i == 4 * (k >> 3) + (k & 3)) wx = v;
+                        }
+                        const bool sees = pos >= rlo && pos <= rhi;
+#pragma unroll
+                        for (int e = 0; e < NE; e++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const uint16_t hv = row[32 * e + 8 * (i >> 2) + 4 * g + (i & 3)];
+                                if (sees && (hv & 0x7c00) == 0x7c00) o[e][i] += wx * h2f(hv);
+                            }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < NE; e++) {
+#pragma unroll
+                    for (int ks = 0; ks < 2; ks++) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const uint2 dd = *(const uint2 *)&d.dv[NE * ew + e][16 * ks + 8 * k + 4 * g];
+                            const float w0 = sc[8 * ks + 4 * k], w1 = sc[8 * ks + 4 * k + 1], w2 = sc[8 * ks + 4 * k + 2], w3 = sc[8 * ks + 4 * k + 3];
+                            pa_split(w0 == 0.0f ? 0.0f : w0 * pa_lo(dd.x), w1 == 0.0f ? 0.0f : w1 * pa_hi(dd.x), hi[2 * k], lo[2 * k]);
+                            pa_split(w2 == 0.0f ? 0.0f : w2 * pa_lo(dd.y), w3 == 0.0f ? 0.0f : w3 * pa_hi(dd.y), hi[2 * k + 1], lo[2 * k + 1]);
+                        }
+                        const pa_v8h va = *(const pa_v8h *)d.v[ks][NE * ew + e][lane];
+                        o[e] = pa_mma32(va, pa_op(hi[0], hi[1], hi[2], hi[3]), o[e]);
+                        o[e] = pa_mma32(va, pa_op(lo[0], lo[1], lo[2], lo[3]), o[e]);
+                    }
                 }
             }
         }
-    }
-    if (!busy) return;
-    if (__any(bad)) {
-        if (lane == 0 && !sq.bad) paged_flag(p, PAGED_BAD_PAGE);
-        l = __builtin_nanf("");
-    }
-    l += partner<32>(l);
-    if (!ok) return;
-    constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
-    const size_t row = (size_t)tok * a.n_head + head;
-    const bool direct = !pre && pl.nown == 1 && b.n_prefix == 0;
-    const size_t at = pre ? row * pl.npre + chunk : row * pl.nown + chunk;
-    float *to = direct ? a.out + (size_t)tok * a.os + (size_t)head * HD : (pre ? pl.po : pl.oo) + at * HD;
-    const float f = direct ? VS / l : VS;
-    const bool none = direct && !sq.bad && sq.len - sq.nq + ri < 0;
-#pragma unroll
-    for (int e = 0; e < NE; e++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const pa_v4f x = {o[e][4 * k], o[e][4 * k + 1], o[e][4 * k + 2], o[e][4 * k + 3]};
-            pa_store4(to + HE * ew + 32 * e + 8 * k + 4 * g, none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : x * f);
+        if (__any(bad)) {
+            if (lane == 0 && !sq.bad) paged_flag(p, PAGED_BAD_PAGE);
+            l = __builtin_nanf("");
         }
-    if (!direct && g == 0 && ew == 0) (pre ? pl.pml : pl.oml)[at] = make_float2(m, l);
+        l += partner<32>(l);
+        if (ok) {
+            constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
+            const PaSink to = pa_sink<true>(a, pl, x, share, r - x.tile * R, tok, head, g == 0 && ew == 0);
+            const float f = to.out ? VS / l : VS;
+            const bool none = to.out && !sq.bad && sq.len - sq.nq + ri < 0;
+#pragma unroll
+            for (int e = 0; e < NE; e++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const pa_v4f y = {o[e][4 * k], o[e][4 * k + 1], o[e][4 * k + 2], o[e][4 * k + 3]};
+                    pa_store4(to.o + HE * ew + 32 * e + 8 * k + 4 * g, none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : y * f);
+                }
+            if (!to.out && g == 0 && ew == 0) *to.ml = make_float2(m, l);
+        }
+    }
 }
 
 template <int KVT>
-hipError_t pa_many(const PagedAttn &a, const PagedPlan &pl, unsigned blocks, hipStream_t s) {
-    const dim3 grid(blocks), wg(256);
+hipError_t pa_many(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
+    const dim3 grid((pl.many.wgs + 7) / 8 * 8), wg(256);
     switch (a.p.hd) {
     case 64: hipLaunchKernelGGL((k_paged_many<64, KVT>), grid, wg, 0, s, a, pl); break;
     case 128: hipLaunchKernelGGL((k_paged_many<128, KVT>), grid, wg, 0, s, a, pl); break;
