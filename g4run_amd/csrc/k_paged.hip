@@ -85,19 +85,36 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     return y;
 }
 
-// One (token, head) row per workgroup: out = sum of exp2(m_k - M) O_k / sum of
-// exp2(m_k - M) l_k over the row's partial results in a fixed order.  Groups of
-// hd / 4 threads take every so-many-th of them.
+// One (token, head) row: out = sum of exp2(m_k - M) O_k / sum of exp2(m_k - M) l_k
+// over the row's partial results in a fixed order, by groups of hd / 4 threads.
+// SPLIT: a workgroup per row, each group every so-many-th of its results (few rows
+// of many pieces); else a group per row (many rows of few: a workgroup's one active
+// group left the chip empty, 9000 rows of 256 took 18 us).
+template <bool SPLIT>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
     __shared__ float red[4];
     __shared__ float lg[16];                                 // at most 16 groups: hd >= 64
-    __shared__ pa_v4f part[256];
+    __shared__ pa_v4f part[SPLIT ? 256 : 1];
     const int hd = a.p.hd, hd4 = hd / 4, groups = 256 / hd4, gi = threadIdx.x / hd4, e4 = threadIdx.x % hd4 * 4;
-    const int tok = blockIdx.x / a.n_head, head = blockIdx.x - tok * a.n_head;
-    const size_t row = blockIdx.x;
+    const int64_t row = SPLIT ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * groups + gi;
+    if (row >= (int64_t)a.b.n_tok * a.n_head) return;
+    const int tok = (int)(row / a.n_head), head = (int)(row - (int64_t)tok * a.n_head);
     const bool prefix = a.b.n_prefix > 0;
     const uint2 own = pl.own[row], pre = prefix ? pl.pre[row] : make_uint2(0, 0);      // of a row without a sequence: not used
-    const int seq = paged_find(a.b, tok);
+    int seq;
+    if constexpr (SPLIT) seq = paged_find(a.b, tok);
+    else {
+        seq = tok < a.b.n_seq ? tok : a.b.n_seq;
+        if (a.b.q_off) {                                     // a group's own: the last sequence that starts at or before the token
+            int x = 0, y = a.b.n_seq + 1;
+            while (y - x > 1) {
+                const int z = (x + y) >> 1;
+                if (paged_ld(a.b.q_off, z) <= tok) x = z;
+                else y = z;
+            }
+            seq = x;
+        }
+    }
     if (seq >= a.b.n_seq) return;                            // behind the last sequence
     const PagedSeq sq = paged_seq(a.p, a.b, seq);
     const int i = tok - sq.t0;
@@ -119,21 +136,24 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
         o = (many ? pl.many.o : pl.few.o) + s * hd;
         ml = (many ? pl.many.ml : pl.few.ml) + s;
     };
+    const int k0 = SPLIT ? gi : 0, step = SPLIT ? groups : 1;
     float mm = -__builtin_inff();
-    for (int k = threadIdx.x; k < total; k += 256) {
+    for (int k = SPLIT ? threadIdx.x : 0; k < total; k += SPLIT ? 256 : 1) {
         const float *o;
         const float2 *ml;
         at(k, o, ml);
         mm = fmaxf(mm, ml->x);
     }
-    mm = group_max<64>(mm);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mm;
-    __syncthreads();
-    mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if constexpr (SPLIT) {
+        mm = group_max<64>(mm);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mm;
+        __syncthreads();
+        mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
     pa_v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
 #pragma unroll 4
-    for (int k = gi; k < total; k += groups) {
+    for (int k = k0; k < total; k += step) {
         const float *o;
         const float2 *ml;
         at(k, o, ml);
@@ -143,13 +163,15 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
         l += x.y == x.y ? f * x.y : x.y;                     // a bad page's NaN stays
         s += v * f;
     }
-    part[threadIdx.x] = s;
-    if (e4 == 0) lg[gi] = l;
-    __syncthreads();
-    if (gi) return;
-    for (int k = 1; k < groups; k++) {
-        s += part[k * hd4 + threadIdx.x];
-        l += lg[k];
+    if constexpr (SPLIT) {
+        part[threadIdx.x] = s;
+        if (e4 == 0) lg[gi] = l;
+        __syncthreads();
+        if (gi) return;
+        for (int k = 1; k < groups; k++) {
+            s += part[k * hd4 + threadIdx.x];
+            l += lg[k];
+        }
     }
     const bool none = !sq.bad && sq.len - sq.nq + i < 0;
     pa_store4(a.out + (size_t)tok * a.os + (size_t)head * hd + e4, none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / l));
@@ -178,7 +200,9 @@ hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s) {
     if (pl.few.rows)
         if (hipError_t e = p.type == F16 ? pa_few_f16(a, pl, s) : p.type == Q8_0 ? pa_few_q8(a, pl, s) : pa_few_q4(a, pl, s)) return e;
     if (y.join) {
-        hipLaunchKernelGGL(k_paged_join, dim3((unsigned)(b.n_tok * a.n_head)), dim3(256), 0, s, a, pl);
+        const int64_t rows = (int64_t)b.n_tok * a.n_head;
+        if (rows <= 2048) hipLaunchKernelGGL(k_paged_join<true>, dim3((unsigned)rows), dim3(256), 0, s, a, pl);
+        else hipLaunchKernelGGL(k_paged_join<false>, dim3(ceil_div(rows, 256 / (p.hd / 4))), dim3(256), 0, s, a, pl);
         return hipGetLastError();
     }
     return hipSuccess;

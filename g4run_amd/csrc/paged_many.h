@@ -190,10 +190,18 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
     return odd;
 }
 
+// between a wave's own LDS writes and reads of what its other lanes wrote
+__device__ __forceinline__ void pm_wave() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// rows of 32 floats on their way between memory and operands, padded
+constexpr int PM_COLS = 36, PM_TR = 32 * PM_COLS;
+
 template <int HD, int KVT>
 __global__ __launch_bounds__(256, HD >= 256 ? 1 : 2) void k_paged_many(PagedAttn a, PagedPlan pl) {
     constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 16, NE = HE / 32, NB = HD > 256 ? 1 : 2;   // NB: buffers
-    __shared__ __align__(16) PmTile<HD, KVT> tiles[NB];
+    constexpr size_t TB = sizeof(PmTile<HD, KVT>) * NB, RB = (size_t)4 * PM_TR * 4;
+    __shared__ __align__(16) uint8_t lds[TB > RB ? TB : RB];  // the tiles; before and after them rows on their way (4 waves' PM_TR floats)
+    PmTile<HD, KVT> *const tiles = (PmTile<HD, KVT> *)lds;
     __shared__ __align__(16) float xs[ES > 1 ? 4 : 1][ES > 1 ? 64 : 1][16];
     __shared__ int odds[3];                                  // by iteration: whether the tile held a non-finite value
     const int lane = threadIdx.x & 63, wave = pa_uniform(threadIdx.x >> 6), c = lane & 31, g = lane >> 5, ew = wave % ES, rw = wave / ES;
@@ -239,45 +247,66 @@ __global__ __launch_bounds__(256, HD >= 256 ? 1 : 2) void k_paged_many(PagedAttn
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             pm_load<HD, KVT>(st, p, nx);
         }
+        // The wave's 32 query rows, 32 elements at a time through its part of LDS:
+        // whole lines from memory, then the operand's 8 elements of one row.
         pa_v8h q0[NS], q1[NS];
         float qs;
         {
-            // twice over the row: the largest magnitude, then the halves
-            const float *src = a.q + (size_t)tok * a.qs + (size_t)head * HD + HE * ew + 8 * g;
-            const bool al = ((uintptr_t)src & 15) == 0;
-            auto ld = [&](int s, int k) {
-                const float *d = src + 16 * s + 4 * k;
-                return !ok ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : al ? *(const pa_v4f *)d : pa_v4f{d[0], d[1], d[2], d[3]};
-            };
-            float am = 0.0f;
-#pragma unroll 8
-            for (int s = 0; s < NS; s++)
+            pa_v4f y[NE][4];                                     // rows 8 k + lane / 8, elements 32 e + 4 (lane % 8) ..
+            float am[4];
+            const float *src[4];
+            const bool al = (((uintptr_t)a.q & 15) | (a.qs & 3)) == 0;
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const pa_v4f y = ld(s, k);
-                    am = fmaxf(fmaxf(am, fmaxf(fabsf(y[0]), fabsf(y[1]))), fmaxf(fabsf(y[2]), fabsf(y[3])));
+            for (int k = 0; k < 4; k++) {
+                const int rr = x.tile * R + 32 * rw + 8 * k + (lane >> 3), i = rr / G;
+                src[k] = 32 * rw < R && rr < sq.nq * G ? a.q + (size_t)(sq.t0 + i) * a.qs + (size_t)(kvh * G + rr - i * G) * HD + HE * ew + 4 * (lane & 7) : nullptr;
+                am[k] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < NE; e++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float *d = src[k] + 32 * e;
+                    y[e][k] = !src[k] ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : al ? *(const pa_v4f *)d : pa_v4f{d[0], d[1], d[2], d[3]};
                 }
-            am = fmaxf(am, partner<32>(am));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+#pragma unroll
+                for (int e = 0; e < NE; e++)
+                    am[k] = fmaxf(fmaxf(am[k], fmaxf(fabsf(y[e][k][0]), fabsf(y[e][k][1]))), fmaxf(fabsf(y[e][k][2]), fabsf(y[e][k][3])));
+                am[k] = group_max<8>(am[k]);
+            }
+            float *const tr = (float *)lds + wave * PM_TR;
+            __syncthreads();                                     // the previous piece's tiles and rows are used
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if ((lane & 7) == 0) tr[(8 * k + (lane >> 3)) * PM_COLS] = am[k];
+            pm_wave();
+            float mx = tr[c * PM_COLS];                          // the lane's row
             if constexpr (ES > 1) {                              // over both halves of the elements
                 __syncthreads();
-                xs[wave][lane][0] = am;
-                __syncthreads();
-                am = fmaxf(am, xs[wave ^ 1][lane][0]);
+                mx = fmaxf(mx, ((float *)lds + (wave ^ 1) * PM_TR)[c * PM_COLS]);
                 __syncthreads();
             }
-            const int sh = pa_shift(am);
+            const int sh = pa_shift(mx);
             qs = pa_score_scale<KVT>(a, sh);
 #pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const pa_v4f y = ld(s, 0), z = ld(s, 1);
-                uint32_t hi[4], lo[4];
-                pa_split(__builtin_ldexpf(y[0], sh), __builtin_ldexpf(y[1], sh), hi[0], lo[0]);
-                pa_split(__builtin_ldexpf(y[2], sh), __builtin_ldexpf(y[3], sh), hi[1], lo[1]);
-                pa_split(__builtin_ldexpf(z[0], sh), __builtin_ldexpf(z[1], sh), hi[2], lo[2]);
-                pa_split(__builtin_ldexpf(z[2], sh), __builtin_ldexpf(z[3], sh), hi[3], lo[3]);
-                q0[s] = pa_op(hi[0], hi[1], hi[2], hi[3]);
-                q1[s] = pa_op(lo[0], lo[1], lo[2], lo[3]);
-                if (s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            for (int e = 0; e < NE; e++) {
+                pm_wave();
+#pragma unroll
+                for (int k = 0; k < 4; k++) *(pa_v4f *)(tr + (8 * k + (lane >> 3)) * PM_COLS + 4 * (lane & 7)) = y[e][k];
+                pm_wave();
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const pa_v4f u0 = *(const pa_v4f *)(tr + c * PM_COLS + 16 * s + 8 * g), u1 = *(const pa_v4f *)(tr + c * PM_COLS + 16 * s + 8 * g + 4);
+                    uint32_t hi[4], lo[4];
+                    pa_split(__builtin_ldexpf(u0[0], sh), __builtin_ldexpf(u0[1], sh), hi[0], lo[0]);
+                    pa_split(__builtin_ldexpf(u0[2], sh), __builtin_ldexpf(u0[3], sh), hi[1], lo[1]);
+                    pa_split(__builtin_ldexpf(u1[0], sh), __builtin_ldexpf(u1[1], sh), hi[2], lo[2]);
+                    pa_split(__builtin_ldexpf(u1[2], sh), __builtin_ldexpf(u1[3], sh), hi[3], lo[3]);
+                    q0[2 * e + s] = pa_op(hi[0], hi[1], hi[2], hi[3]);
+                    q1[2 * e + s] = pa_op(lo[0], lo[1], lo[2], lo[3]);
+                }
             }
         }
         const float capl = a.cap * 1.4426950408889634f;
@@ -287,7 +316,7 @@ __global__ __launch_bounds__(256, HD >= 256 ? 1 : 2) void k_paged_many(PagedAttn
         for (int e = 0; e < NE; e++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[e][i] = 0.0f;
-        __syncthreads();                                         // the previous piece's tiles are used
+        __syncthreads();
         if (threadIdx.x < 3) odds[threadIdx.x] = 0;
         __syncthreads();
 
@@ -464,19 +493,39 @@ __global__ __launch_bounds__(256, HD >= 256 ? 1 : 2) void k_paged_many(PagedAttn
             l = __builtin_nanf("");
         }
         l += partner<32>(l);
-        if (ok) {
-            constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
-            const PaSink to = pa_sink<true>(a, pl, x, share, r - x.tile * R, tok, head, g == 0 && ew == 0);
-            const float f = to.out ? VS / l : VS;
-            const bool none = to.out && !sq.bad && sq.len - sq.nq + ri < 0;
+        // out through LDS as the queries came in
+        float *const tr = (float *)lds + wave * PM_TR;
+        __syncthreads();                                         // the tiles are used
+        constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
+        float *to[4];
+        bool out = false;
+        if (g == 0) {
+            PaSink k = {nullptr, nullptr, false};
+            if (ok) {
+                k = pa_sink<true>(a, pl, x, share, r - x.tile * R, tok, head, ew == 0);
+                if (!k.out && ew == 0) *k.ml = make_float2(m, l);
+            }
+            out = k.out;
+            *(float **)(tr + c * PM_COLS) = k.o;
+        }
+        out = __any(out);
+        pm_wave();
 #pragma unroll
-            for (int e = 0; e < NE; e++)
+        for (int k = 0; k < 4; k++) to[k] = *(float **)(tr + (8 * k + (lane >> 3)) * PM_COLS);
+        const bool none = out && !sq.bad && sq.len - sq.nq + ri < 0;
+        const float f = none ? 0.0f : out ? VS / l : VS;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const pa_v4f y = {o[e][4 * k], o[e][4 * k + 1], o[e][4 * k + 2], o[e][4 * k + 3]};
-                    pa_store4(to.o + HE * ew + 32 * e + 8 * k + 4 * g, none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : y * f);
-                }
-            if (!to.out && g == 0 && ew == 0) *to.ml = make_float2(m, l);
+        for (int e = 0; e < NE; e++) {
+            pm_wave();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const pa_v4f y = {o[e][4 * k], o[e][4 * k + 1], o[e][4 * k + 2], o[e][4 * k + 3]};
+                *(pa_v4f *)(tr + c * PM_COLS + 8 * k + 4 * g) = none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : y * f;
+            }
+            pm_wave();
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (to[k]) pa_store4(to[k] + HE * ew + 32 * e + 4 * (lane & 7), *(const pa_v4f *)(tr + (8 * k + (lane >> 3)) * PM_COLS + 4 * (lane & 7)));
         }
     }
 }
