@@ -54,7 +54,7 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     if (many_own || many_pre) {
         const int most = p.hd > 256 ? 64 : 128;
         const int64_t shared = b.q_off || many_pre ? rows : grp, tiles = ceil_div(shared, most);
-        many.rows = (int)std::min<int64_t>(most, ceil_div(ceil_div(shared, tiles), 32) * 32);
+        many.rows = (int)std::min<int64_t>(most, ceil_div(ceil_div(shared, tiles), 16) * 16);
         many.pre_tiles = many_pre ? ceil_div(rows, many.rows) : 0;
         const int least = b.q_off && few.rows ? few.rows / grp + 1 : 1;      // tokens of a sequence it takes
         const int64_t own = !many_own ? 0 : b.q_off ? ceil_div(rows, many.rows) + std::min(b.n_seq, b.n_tok / least)

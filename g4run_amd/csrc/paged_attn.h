@@ -366,6 +366,22 @@ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &p
     return s;
 }
 
+// max of unsigned halves; the biased exponent of a (positive) half as a float
+typedef unsigned short pa_v2s __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pa_pkmax(uint32_t x, uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pa_v2s, x), __builtin_bit_cast(pa_v2s, y)));
+}
+__device__ __forceinline__ float pa_exponent(uint32_t h, int which) { return (float)((h >> (which ? 26 : 10)) & 31u); }
+// A weight's offset from the running maximum: for quantized values that maximum is
+// over s + the biased exponent (15 more than the exponent).
+template <int KVT>
+__device__ __forceinline__ constexpr float pa_shift_of() { return KVT == F16 ? PA_SHIFT : PA_SHIFT + 14.0f; }
+// two weights times two halves' scales, split
+__device__ __forceinline__ void pa_split_scaled(float u, float v, uint32_t d, uint32_t &hi, uint32_t &lo) {
+    const float x = __builtin_fmaf(pa_lo(d), u, 0.0f), y = __builtin_fmaf(pa_hi(d), v, 0.0f);
+    hi = pa_pk(x, y);
+    lo = pa_pk(__builtin_fmaf(pa_lo(hi), -1.0f, x), __builtin_fmaf(pa_hi(hi), -1.0f, y));
+}
 // two halves, those that are not finite as 0
 __device__ __forceinline__ uint32_t pa_finite(uint32_t x) {
     x = (x & 0x7c00u) == 0x7c00u ? x & 0xffff0000u : x;
@@ -378,7 +394,7 @@ __device__ __forceinline__ int pa_shift(float am) {
 }
 __device__ __forceinline__ void pa_split(float u, float v, uint32_t &hi, uint32_t &lo) {
     hi = pa_pk(u, v);
-    lo = pa_pk(u - pa_lo(hi), v - pa_hi(hi));
+    lo = pa_pk(__builtin_fmaf(pa_lo(hi), -1.0f, u), __builtin_fmaf(pa_hi(hi), -1.0f, v));
 }
 // factor from a raw score product to log2 units (before a cap: to tanh's argument)
 template <int KVT>

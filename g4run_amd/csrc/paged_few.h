@@ -277,16 +277,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                     w[j] = pos >= rlo && pos <= rhi && pos < end ? w[j] : -__builtin_inff();
                 }
             }
+            if constexpr (KVT == F16) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float y = w[j];
-                if constexpr (KVT != F16) {                  // + the exponent of the position's largest value scale
-                    uint32_t dm = 1;                         // all zero: the smallest scale there is
+                for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j]);
+            } else {
+                // + the exponent of the position's largest value scale
 #pragma unroll
-                    for (int d = 0; d < HE / 64; d++) dm = max(dm, max(kv.dv[j][d] & 0x7fffu, (kv.dv[j][d] >> 16) & 0x7fffu));
-                    y += (float)__builtin_amdgcn_frexp_expf(h2f((uint16_t)dm));
+                for (int j = 0; j < 8; j++) {
+                    uint32_t dm = kv.dv[j][0] & 0x7fff7fffu;
+#pragma unroll
+                    for (int d = 1; d < HE / 64; d++) dm = pa_pkmax(dm, kv.dv[j][d] & 0x7fff7fffu);
+                    mt = fmaxf(mt, w[j] + pa_exponent(max(dm << 16, dm), 1));
                 }
-                mt = fmaxf(mt, y);
             }
             mt = fmaxf(mt, partner<16>(mt));
             mt = fmaxf(mt, partner<32>(mt));
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                 for (int e = 0; e < NM; e++) o[e] *= cr;
                 m = mn;
             }
-            const float mr = m == -__builtin_inff() ? 0.0f : m - PA_SHIFT;
+            const float mr = m == -__builtin_inff() ? 0.0f : m - pa_shift_of<KVT>();
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 w[j] = __builtin_amdgcn_exp2f(w[j] - mr);
@@ -345,13 +347,22 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                     if constexpr (!ST) o[e] = pa_mma(va, b1, o[e]);
                 }
             } else {
+                // a scale of a position that the row does not attend may be anything
+                if (edge) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const uint32_t live = w[j] == 0.0f ? 0u : ~0u;
+#pragma unroll
+                        for (int d = 0; d < HE / 64; d++) kv.dv[j][d] &= live;
+                    }
+                }
 #pragma unroll
                 for (int s = 0; s < NS; s++) {               // blocks of 32 elements: value tiles 2 s, 2 s + 1
                     uint32_t ph[4], pq[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const float w0 = w[2 * k], w1 = w[2 * k + 1];
-                        pa_split(w0 == 0.0f ? 0.0f : w0 * pa_scale(kv.dv[2 * k], s), w1 == 0.0f ? 0.0f : w1 * pa_scale(kv.dv[2 * k + 1], s), ph[k], pq[k]);
+                        const float y = __builtin_fmaf(pa_scale(kv.dv[2 * k], s), w[2 * k], 0.0f), z = __builtin_fmaf(pa_scale(kv.dv[2 * k + 1], s), w[2 * k + 1], 0.0f);
+                        pa_split(y, z, ph[k], pq[k]);
                         if constexpr (ST) ph[k] = c < 8 ? ph[k] : pq[k];
                     }
                     const pa_v8h b0 = pa_op(ph[0], ph[1], ph[2], ph[3]), b1 = pa_op(pq[0], pq[1], pq[2], pq[3]);
