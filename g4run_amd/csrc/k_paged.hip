@@ -22,12 +22,15 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     PagedList &few = pl.few, &many = pl.many;
     const int64_t rows = (int64_t)b.n_tok * grp;             // of one KV head
     pl.grp_inv = 65536 / grp + 1;
+    many.toks = 1;
+    many.toks_inv = 0;
     // Sequences of at most few.rows rows are the few-row kernel's: 8 (one matrix
     // instruction per operand) where no sequence can have more, else 16.
     few.rows = grp > 16 ? 0 : (b.q_off ? rows : grp) <= 8 ? 8 : 16;
     if (b.n_prefix && few.rows == 8 && rows > 8 && rows <= 16) few.rows = 16;
+    few.toks = few.rows / grp;
     const bool few_pre = b.n_prefix && few.rows && rows <= few.rows;
-    const bool many_own = b.q_off ? b.n_tok > (few.rows ? few.rows / grp : 0) : !few.rows;
+    const bool many_own = b.q_off ? b.n_tok > few.toks : !few.rows;
     const bool many_pre = b.n_prefix && !few_pre;
     few.least = 1;
     few.pre_tiles = few_pre ? 1 : 0;
@@ -47,26 +50,25 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     }
     few.wgs = (int)std::min<int64_t>(PA_FEW_WGS, steps);
     y.join = b.n_prefix || (few.rows && fspan > few.unit);
-    // Many rows: tiles of up to 128 (64 of heads of 512), evenly filled; as many
-    // workgroups as fit on the device at once.
+    // Many rows: tiles of whole tokens, up to 128 rows (64 of heads of 512), evenly
+    // filled; as many workgroups as fit on the device at once.
     many.rows = 0;
     many.pre_tiles = 0;
     if (many_own || many_pre) {
-        const int most = p.hd > 256 ? 64 : 128;
-        const int64_t shared = b.q_off || many_pre ? rows : grp, tiles = ceil_div(shared, most);
-        many.rows = (int)std::min<int64_t>(most, ceil_div(ceil_div(shared, tiles), 16) * 16);
-        many.pre_tiles = many_pre ? ceil_div(rows, many.rows) : 0;
-        const int least = b.q_off && few.rows ? few.rows / grp + 1 : 1;      // tokens of a sequence it takes
-        const int64_t own = !many_own ? 0 : b.q_off ? ceil_div(rows, many.rows) + std::min(b.n_seq, b.n_tok / least)
-                                                    : (int64_t)b.n_seq * ceil_div(grp, many.rows);
-        const int64_t mspan = span(many.rows / grp + 1);
+        const int most = paged_most_group(p.hd) / grp, toks = b.q_off || many_pre ? b.n_tok : 1;
+        many.toks = ceil_div(toks, ceil_div(toks, most));
+        many.toks_inv = many.toks == 1 ? 0 : (uint32_t)(0x100000000ull / many.toks + 1);
+        many.rows = many.toks * grp;
+        many.pre_tiles = many_pre ? ceil_div(b.n_tok, many.toks) : 0;
+        const int64_t own = !many_own ? 0 : b.q_off ? ceil_div(b.n_tok, many.toks) + std::min(b.n_seq, b.n_tok / (few.toks + 1)) : b.n_seq;
+        const int64_t mspan = span(many.toks);
         for (many.shift = 6;; many.shift++) {
             many.unit = 1 << many.shift;
             many.pre_steps = many_pre ? ceil_div(b.n_prefix, many.unit) : 0;
             steps = (own * std::max(1, ceil_div(mspan, many.unit)) + (int64_t)many.pre_tiles * many.pre_steps) * p.n_kv;
             if (steps < (1 << 30)) break;
         }
-        many.wgs = (int)std::min<int64_t>(p.hd >= 256 ? 256 : 512, ceil_div(steps, many.least));
+        many.wgs = (int)std::min<int64_t>(p.hd >= 128 ? 256 : 512, ceil_div(steps, many.least));
         y.join |= mspan > many.unit;
     }
     const size_t all = y.join ? (size_t)b.n_tok * p.n_kv * grp : 0, whole = b.n_prefix ? all : 0;

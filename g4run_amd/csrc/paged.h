@@ -38,6 +38,9 @@ struct PagedRope {
 
 __host__ __device__ constexpr int paged_row_bytes(int type, int hd) { return type == F16 ? hd * 2 : type == Q8_0 ? hd : hd / 2; }
 
+// query heads of a KV head at most: a token's rows share a tile
+__host__ __device__ constexpr int paged_most_group(int hd) { return hd > 256 ? 64 : 128; }
+
 // page entry and slot of unit u
 __device__ __forceinline__ int paged_entry(const PagedPool &p, int u) { return p.inv ? (int)__umulhi((uint32_t)u, p.inv) : u; }
 

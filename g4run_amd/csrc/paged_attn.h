@@ -44,6 +44,8 @@ typedef uint32_t pa_v4u __attribute__((ext_vector_type(4)));
 // tells k_paged_join where its rows' pieces lie.
 struct PagedList {
     int rows;                        // rows of a tile; the few-row kernel: most rows of a sequence it takes
+    int toks;                        // many: tokens of a tile, rows / grp; few: most tokens of a sequence
+    uint32_t toks_inv;               // many: n / toks == umulhi(n, toks_inv) for n <= 2^24 (0: toks is 1)
     int wgs, least;                  // workgroups; steps of a share at least
     int unit, shift;                 // positions of a step, and their log2
     int pre_tiles, pre_steps;        // the prefix's tiles (0: not this kernel's), and steps of each
@@ -113,14 +115,16 @@ __device__ __forceinline__ void pa_load(uint32_t *d, const uint8_t *p) {
 struct PaUnits {
     int id, row;
 };
-template <int KVT>
-__device__ __forceinline__ PaUnits pa_units(const PagedPool &p, const int *table, int first, int stride, int last, int kvh, bool &bad) {
+__device__ __forceinline__ PaUnits pa_units(const PagedPool &p, const int *table, int first, int stride, int last, int kvh) {
     const int lane = threadIdx.x & 63, u = min(first + stride * (lane >> 1) + (lane & 1), last), ent = paged_entry(p, u);
     PaUnits x;
     x.id = paged_ld(table, ent);
     x.row = kvh * p.page + (u - ent * p.units) * 16;
-    if ((uint64_t)(int64_t)x.id >= (uint64_t)p.n_pages) { bad = true; x.id = 0; }
     return x;
+}
+// before their first use (not with the load, which would be waited for there)
+__device__ __forceinline__ void pa_check(const PagedPool &p, PaUnits &x, bool &bad) {
+    if ((uint64_t)(int64_t)x.id >= (uint64_t)p.n_pages) { bad = true; x.id = 0; }
 }
 // the offset of a unit's rows in the pools and, quantized, of their scales
 struct PaUnit {
@@ -197,21 +201,17 @@ __device__ __forceinline__ const PagedList &pa_list(const PagedPlan &pl) {
     else return pl.few;
 }
 template <bool MANY>
-__device__ __forceinline__ int pa_tiles(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q) {
-    const bool few = q.nq * a.grp <= pl.few.rows;
-    if constexpr (MANY) return few ? 0 : (q.nq * a.grp + pl.many.rows - 1) / pl.many.rows;
-    else return few && q.nq > 0;
+__device__ __forceinline__ int pa_tiles(const PagedPlan &pl, const PagedSeq &q) {
+    if (q.nq <= pl.few.toks) return !MANY && q.nq > 0;
+    if constexpr (!MANY) return 0;
+    const uint32_t n = q.nq + pl.many.toks - 1;
+    return pl.many.toks_inv ? (int)__umulhi(n, pl.many.toks_inv) : (int)n;
 }
 template <bool MANY>
 __device__ __forceinline__ void pa_tile_span(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile, int &lo, int &hi) {
-    const int p0 = q.len - q.nq;
-    if constexpr (MANY) {
-        lo = pa_low(p0 + tile * pl.many.rows / a.grp, a.window);
-        hi = p0 + min(q.nq - 1, ((tile + 1) * pl.many.rows - 1) / a.grp);
-    } else {
-        lo = pa_low(p0, a.window);
-        hi = q.len - 1;
-    }
+    const int first = q.len - q.nq + (MANY ? tile * pl.many.toks : 0);
+    lo = pa_low(first, a.window);
+    hi = MANY ? min(q.len, first + pl.many.toks) - 1 : q.len - 1;
 }
 template <bool MANY>
 __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile) {
@@ -225,7 +225,7 @@ __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const PagedPlan
 template <bool MANY>
 __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, int s) {
     const PagedSeq q = paged_seq(a.p, a.b, s);
-    const int tiles = pa_tiles<MANY>(a, pl, q);
+    const int tiles = pa_tiles<MANY>(pl, q);
     int n = 0;
     for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY>(a, pl, q, t);
     return n;
@@ -304,22 +304,20 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
         x.sq = paged_seq(a.p, b, seq);
         int v = u - pre_all - before;
         if constexpr (MANY) {
-            const int tiles = pa_tiles<MANY>(a, pl, x.sq);
+            const int tiles = pa_tiles<MANY>(pl, x.sq);
             int head = 0;                                    // steps of one KV head
             for (int t = 0; t < tiles; t++) head += pa_tile_steps<MANY>(a, pl, x.sq, t);
-            x.kvh = v / head;
-            v -= x.kvh * head;
+            for (x.kvh = 0; v >= head; x.kvh++) v -= head;
             x.tile = 0;
             for (x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0); v >= x.all; x.all = pa_tile_steps<MANY>(a, pl, x.sq, ++x.tile)) v -= x.all;
         } else {
             x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0);
             x.tile = 0;
-            x.kvh = v / x.all;
-            v -= x.kvh * x.all;
+            for (x.kvh = 0; v >= x.all; x.kvh++) v -= x.all;
         }
         x.step = v;
         pa_tile_span<MANY>(a, pl, x.sq, x.tile, base, x.hi1);
-        x.hi0 = x.sq.len - x.sq.nq + (MANY ? x.tile * pl.many.rows / a.grp : 0);
+        x.hi0 = x.sq.len - x.sq.nq + (MANY ? x.tile * pl.many.toks : 0);
         x.lo0 = a.window ? max(0, x.hi0 + 1 - a.window) : 0;
         x.lo1 = a.window ? max(0, x.hi1 + 1 - a.window) : 0;
         x.seglen = x.sq.bad ? 0 : x.sq.len;

@@ -171,7 +171,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
         PaUnits us, more_us;                                 // of 32 steps, and of the next 32
         int base = start + 32 * pw;
         if (iters) {
-            us = pa_units<KVT>(p, x.table, base >> 4, 2 * PW, last, kvh, bad);
+            us = pa_units(p, x.table, base >> 4, 2 * PW, last, kvh);
+            pa_check(p, us, bad);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             pa_load_k<HD, HE, KVT>(kv, p, nx, c, g, ew);
@@ -218,12 +219,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
             const bool more = it + 1 < iters;
             un[0] = nx[0];
             un[1] = nx[1];
-            if ((it & 31) == 31) us = more_us;
+            if ((it & 31) == 31 && it + 1 < iters) {
+                us = more_us;
+                pa_check(p, us, bad);
+            }
             if (more) {
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
                 nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
             }
-            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units<KVT>(p, x.table, (base >> 4) + 64 * PW, 2 * PW, last, kvh, bad);
+            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units(p, x.table, (base >> 4) + 64 * PW, 2 * PW, last, kvh);
             const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
             // scores at positions base + 16 h + 4 g + i
             pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};

@@ -187,6 +187,24 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
     return odd;
 }
 
+// read(i) brings operand i of N from LDS, use(i, operand) multiplies with it: reads
+// run AHEAD of their use.  (Left to itself the compiler reads, waits and multiplies
+// one by one: 130 cycles of LDS latency for 32 of matrix instructions.)
+template <int N, int AHEAD, typename R, typename U>
+__device__ __forceinline__ void pm_pipeline(R read, U use) {
+    pa_v8h x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD && i < N; i++) x[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        __builtin_amdgcn_sched_barrier(0);
+        const pa_v8h y = x[i % AHEAD];
+        use(i, y);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + AHEAD < N) x[i % AHEAD] = read(i + AHEAD);
+    }
+}
+
 // between a wave's own LDS writes and reads of what its other lanes wrote
 __device__ __forceinline__ void pm_wave() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
@@ -194,7 +212,7 @@ __device__ __forceinline__ void pm_wave() { asm volatile("s_waitcnt lgkmcnt(0)" 
 constexpr int PM_COLS = 36, PM_TR = 16 * PM_COLS;
 
 template <int HD, int KVT>
-__global__ __launch_bounds__(PM_THREADS, HD >= 256 ? 2 : 4) void k_paged_many(PagedAttn a, PagedPlan pl) {
+__global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(PagedAttn a, PagedPlan pl) {
     constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2;   // NB: buffers
     constexpr size_t TB = sizeof(PmTile<HD, KVT>) * NB, RB = (size_t)8 * PM_TR * 4;
     __shared__ __align__(16) uint8_t lds[TB > RB ? TB : RB]; // the tiles; before and after them rows on their way
@@ -218,7 +236,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 256 ? 2 : 4) void k_paged_many(Pa
         const PaPiece x = pa_piece<true>(a, pl, mine, wg, u, first, stop);
         u += x.n;
         const PagedSeq &sq = x.sq;
-        const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = sq.nq * G, r0 = x.tile * R + 16 * rw;
+        const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = min(sq.nq * G, (x.tile + 1) * R), r0 = x.tile * R + 16 * rw;     // the tile's rows end at `rows`
         bool bad = sq.bad;
         if (bad && threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
         const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 31) / 32 : 0;
@@ -227,13 +245,14 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 256 ? 2 : 4) void k_paged_many(Pa
         PaUnits us, more_us;                                 // of 32 steps, and of the next 32
         PaUnit un[2], nx[2];
         if (iters) {
-            us = pa_units<KVT>(p, x.table, start >> 4, 2, last, kvh, bad);
+            us = pa_units(p, x.table, start >> 4, 2, last, kvh);
+            pa_check(p, us, bad);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             pm_load<HD, KVT>(st, p, nx);
         }
         // The wave's rows: 16 rw ..; busy: it has some.  The lane's: r0 + c.
-        const bool busy = 16 * rw < R && r0 < rows, ok = busy && r0 + c < rows;
+        const bool busy = r0 < rows, ok = r0 + c < rows;
         const int ri = ok ? (r0 + c) / G : 0, head = kvh * G + (ok ? r0 + c - ri * G : 0), tok = sq.t0 + ri;
         int rlo = lo0, rhi = hi0;                            // the lane's row attends [rlo, rhi]
         if (ok) {
@@ -255,7 +274,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 256 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const int r = r0 + 8 * k + (lane >> 3), i = r / G;
-                const bool in = busy && r < rows;
+                const bool in = r < rows;
                 const float *src = a.q + (size_t)(sq.t0 + (in ? i : 0)) * a.qs + (size_t)(kvh * G + (in ? r - i * G : 0)) * HD + HE * ew + 4 * (lane & 7);
                 float am = 0.0f;
 #pragma unroll
@@ -309,36 +328,37 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 256 ? 2 : 4) void k_paged_many(Pa
             if (pm_store<HD, KVT>(d, st, edge, lo0 - base, end - base)) odds[turn] = 1;
             un[0] = nx[0];
             un[1] = nx[1];
-            if ((it & 31) == 31) us = more_us;
+            if ((it & 31) == 31 && it + 1 < iters) {
+                us = more_us;
+                pa_check(p, us, bad);
+            }
             if (it + 1 < iters) {
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
                 nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
                 pm_load<HD, KVT>(st, p, nx);
             }
-            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units<KVT>(p, x.table, (base >> 4) + 64, 2, last, kvh, bad);
+            if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units(p, x.table, (base >> 4) + 64, 2, last, kvh);
             lds_barrier();
             const int odd = odds[turn];
             if (threadIdx.x == 0) odds[turn == 0 ? 2 : turn - 1] = 0;    // the iteration after the next's: written behind the next barrier
             if (!busy && ES == 1) continue;
             // scores of row c at positions base + pm_pos(g, j)
             pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const pa_v8h ko = *(const pa_v8h *)&d.k[16 * h + c][HE * ew + 32 * s + 8 * g];
-                    if constexpr (KVT == F16) {
-                        sc[h] = pa_mma(ko, q0[s], sc[h]);
-                        sc[h] = pa_mma(ko, q1[s], sc[h]);
-                    } else {
-                        const pa_v4f y = pa_mma(ko, q1[s], pa_mma(ko, q0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f}));
-                        const uint2 dd = *(const uint2 *)&d.dk[NS * ew + s][16 * h + 4 * g];
-                        sc[h][0] = __builtin_fmaf(pa_lo(dd.x), y[0], sc[h][0]);
-                        sc[h][1] = __builtin_fmaf(pa_hi(dd.x), y[1], sc[h][1]);
-                        sc[h][2] = __builtin_fmaf(pa_lo(dd.y), y[2], sc[h][2]);
-                        sc[h][3] = __builtin_fmaf(pa_hi(dd.y), y[3], sc[h][3]);
-                    }
+            pm_pipeline<2 * NS, 4>([&](int i) { return *(const pa_v8h *)&d.k[16 * (i & 1) + c][HE * ew + 32 * (i >> 1) + 8 * g]; },
+                                   [&](int i, pa_v8h ko) {
+                const int s = i >> 1, h = i & 1;
+                if constexpr (KVT == F16) {
+                    sc[h] = pa_mma(ko, q0[s], sc[h]);
+                    sc[h] = pa_mma(ko, q1[s], sc[h]);
+                } else {
+                    const pa_v4f y = pa_mma(ko, q1[s], pa_mma(ko, q0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f}));
+                    const uint2 dd = *(const uint2 *)&d.dk[NS * ew + s][16 * h + 4 * g];
+                    sc[h][0] = __builtin_fmaf(pa_lo(dd.x), y[0], sc[h][0]);
+                    sc[h][1] = __builtin_fmaf(pa_hi(dd.x), y[1], sc[h][1]);
+                    sc[h][2] = __builtin_fmaf(pa_lo(dd.y), y[2], sc[h][2]);
+                    sc[h][3] = __builtin_fmaf(pa_hi(dd.y), y[3], sc[h][3]);
                 }
+            });
             if constexpr (ES > 1) {
                 *(pa_v4f *)xs[wave][lane] = sc[0];
                 *(pa_v4f *)(xs[wave][lane] + 4) = sc[1];
@@ -398,12 +418,10 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 256 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
                 for (int k = 0; k < 4; k++) pa_split(w[2 * k], w[2 * k + 1], hi[k], lo[k]);
                 const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-                for (int e = 0; e < NM; e++) {
-                    const pa_v8h va = *(const pa_v8h *)d.v[NM * ew + e][lane];
+                pm_pipeline<NM, 4>([&](int e) { return *(const pa_v8h *)d.v[NM * ew + e][lane]; }, [&](int e, pa_v8h va) {
                     o[e] = pa_mma(va, b0, o[e]);
                     o[e] = pa_mma(va, b1, o[e]);
-                }
+                });
                 if (odd) {
                     // non-finite values, zero in LDS, added to the rows that attend them
                     for (int k = 0; k < 32; k++) {

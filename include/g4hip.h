@@ -353,7 +353,8 @@ int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out
  *   s_j = scale * q . k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);
  *   out = sum_j softmax(s)_j v_j, zeros for a token without a position.
  * q / out: fp32 [n_tok][n_head][hd], at q_stride / out_stride floats per token
- * (0: packed); query head h reads KV head h / (n_head / n_kv).  All in fp32
+ * (0: packed); query head h reads KV head h / (n_head / n_kv), up to 128 heads a
+ * KV head (64 of hd 512).  All in fp32
  * precision (queries and weights enter the matrix cores as two halves each),
  * unlike g4h_attn_decode, which rounds as the reference does.  The prefix's
  * rows are read once for the whole batch.  A non-finite cached value reaches
