@@ -48,7 +48,7 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
         steps = ((int64_t)b.n_seq * std::max(1, ceil_div(fspan, few.unit)) + few.pre_steps) * p.n_kv;
         if (steps < (1 << 30)) break;
     }
-    few.wgs = (int)std::min<int64_t>(PA_FEW_WGS, steps);
+    few.wgs = (int)std::min<int64_t>(256 * pa_few_per_cu(p.type, p.hd, few.rows <= 8), steps);
     y.join = b.n_prefix || (few.rows && fspan > few.unit);
     // Many rows: tiles of whole tokens, up to 128 rows (64 of heads of 512), evenly
     // filled; as many workgroups as fit on the device at once.

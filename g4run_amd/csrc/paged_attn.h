@@ -69,6 +69,50 @@ struct PagedPlan {
 // the first steps.
 constexpr float PA_SHIFT = 6.0f, PA_LAG = 8.0f;
 
+// A kernel's arguments, and a copy of them read again where it is asked for: what
+// the outer loop over the pieces needs between two of them then stays in memory,
+// not in registers (with all of it held, 40 vector registers more).
+struct PagedCall {
+    PagedAttn a;
+    PagedPlan pl;
+};
+template <typename T>
+__device__ __forceinline__ void pa_global(T *&p) {
+    auto *g = (__attribute__((address_space(1))) T *)p;
+    asm("" : "+s"(g));
+    p = (T *)g;
+}
+__device__ __forceinline__ PagedCall pa_fresh() {
+    static_assert(sizeof(PagedCall) % 4 == 0, "read by dwords");
+    auto *p = (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    uint32_t w[sizeof(PagedCall) / 4];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof w / 4); i++) w[i] = p[i];
+    PagedCall k = __builtin_bit_cast(PagedCall, w);
+    // pointers to global memory, which arguments are known to be and loaded ones are
+    // not: flat accesses would count as LDS accesses too
+    pa_global(k.a.p.k);
+    pa_global(k.a.p.v);
+    pa_global(k.a.p.status);
+    pa_global(k.a.q);
+    pa_global(k.a.out);
+    pa_global(k.pl.few.o);
+    pa_global(k.pl.few.ml);
+    pa_global(k.pl.many.o);
+    pa_global(k.pl.many.ml);
+    pa_global(k.pl.own);
+    pa_global(k.pl.pre);
+    pa_global(k.pl.wo);
+    pa_global(k.pl.wml);
+    return k;
+}
+__device__ __forceinline__ int pa_thread() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 __device__ __forceinline__ int pa_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ uint32_t pa_pk(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 __device__ __forceinline__ float pa_lo(uint32_t h) { return (float)__builtin_bit_cast(pa_v2h, h)[0]; }
@@ -139,22 +183,30 @@ __device__ __forceinline__ PaUnit pa_unit(const PagedPool &p, const PaUnits &us,
     return x;
 }
 
-// log2(e) cap tanh(x): an odd polynomial below 0.3 (next term 9e-3 x^11, below
-// 6e-8 x there), where 1 - exp would lose the small value
-__device__ __forceinline__ float pa_tanh(float x) {
-    const float x2 = x * x;
-    float p = __builtin_fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f);
-    p = __builtin_fmaf(x2, p, 2.0f / 15.0f);
-    p = __builtin_fmaf(x2, p, -1.0f / 3.0f);
-    p = __builtin_fmaf(x * x2, p, x);
-    const float ax = fabsf(x);
-    if (__any(ax > 0.3f)) {
-        const float t = __builtin_amdgcn_exp2f(-2.885390081777927f * ax);
-        const float r = (1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t);
-        p = ax > 0.3f ? copysignf(r, x) : p;
-        p = x == x ? p : x;
+// x = tanh(x) of a lane's 8 scores: an odd polynomial below 0.3 (next term 9e-3
+// x^11, below 6e-8 x there), where 1 - exp would lose the small value
+__device__ __forceinline__ void pa_tanh8(float x[8]) {
+    float most = 0.0f;
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float x2 = x[j] * x[j];
+        float y = __builtin_fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f);
+        y = __builtin_fmaf(x2, y, 2.0f / 15.0f);
+        y = __builtin_fmaf(x2, y, -1.0f / 3.0f);
+        p[j] = __builtin_fmaf(x[j] * x2, y, x[j]);
+        most = fmaxf(most, fabsf(x[j]));
     }
-    return p;
+    if (__any(most > 0.3f)) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float ax = fabsf(x[j]), t = __builtin_amdgcn_exp2f(-2.885390081777927f * ax);
+            const float r = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x[j]);
+            p[j] = ax > 0.3f ? r : p[j];                     // NaN: the polynomial's
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = p[j];
 }
 
 // the batch's rows that attend the prefix
@@ -262,7 +314,6 @@ __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan
     }
     seq = a.b.n_seq;
 }
-constexpr int PA_FEW_WGS = 512;
 __device__ __forceinline__ int pa_share(const PagedList &y, int total) { return max(y.least, (total + y.wgs - 1) / y.wgs); }
 
 // A piece: steps [step, step + n) of the `all` of one tile of one KV head.
@@ -399,9 +450,16 @@ template <int KVT>
 __device__ __forceinline__ float pa_score_scale(const PagedAttn &a, int sh) {
     return __builtin_ldexpf(a.scale * (KVT == Q8_0 ? 512.0f : 1.0f) * (a.cap > 0.0f ? 1.0f / a.cap : 1.4426950408889634f), -sh);
 }
-__device__ __forceinline__ void pa_store4(float *d, pa_v4f s) {
-    if (((uintptr_t)d & 15) == 0) *(pa_v4f *)d = s;
+__device__ __forceinline__ void pa_store4(float *to, pa_v4f s) {
+    auto *d = (__attribute__((address_space(1))) float *)to;
+    if (((uintptr_t)to & 15) == 0) *(__attribute__((address_space(1))) pa_v4f *)d = s;
     else { d[0] = s[0]; d[1] = s[1]; d[2] = s[2]; d[3] = s[3]; }
+}
+
+// the few-row kernel's workgroups per CU: what its registers allow (quantized
+// pages' scales and conversions take more)
+__host__ __device__ constexpr int pa_few_per_cu(int type, int hd, bool st) {
+    return hd == 64 ? (type == F16 ? 4 : 3) : type == F16 && hd == 128 && st ? 3 : 2;
 }
 
 // launches of one cache type; the few-row variants hold 8 or 16 rows

@@ -108,7 +108,7 @@ __device__ __forceinline__ int pa_elem(int m, int x) {
 }
 
 template <int HD, int KVT, bool ST>
-__global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl) {
+__global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(PagedCall call) {
     constexpr int R = ST ? 8 : 16, HE = HD > 128 ? 128 : HD, ES = HD / HE, PW = 4 / ES, NS = HE / 32, NM = HE / 16;
     constexpr int QP = HD + 8;                               // padded query row
     constexpr size_t QB = 2 * R * QP * 2, OB = (size_t)PW * 8 * (HD + 4) * 4;
@@ -118,27 +118,30 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
     __shared__ __align__(16) float xs[ES > 1 ? 2 : 1][ES > 1 ? 4 : 1][ES > 1 ? 64 : 1][8];   // partial scores of the waves of one tile
     _Float16 *const qh = (_Float16 *)lds;
     float *const buf = (float *)lds;
-    const int lane = threadIdx.x & 63, wave = pa_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, pw = wave / ES;
-    const PagedPool &p = a.p;
-    const PagedBatch &b = a.b;
-    const int G = a.grp, rc = ST ? c & 7 : c;
 
     int mine;
-    const int total = pa_total<false>(a, pl, mine), share = pa_share(pl.few, total);
+    const int total = pa_total<false>(call.a, call.pl, mine), share = pa_share(call.pl.few, total);
     const int first = blockIdx.x * share, stop = min(first + share, total);
     for (int u = first; u < stop;) {
+        const PagedCall call = pa_fresh();
+        const PagedAttn &a = call.a;
+        const PagedPlan &pl = call.pl;
+        const PagedPool &p = a.p;
+        const PagedBatch &b = a.b;
+        const int tid = pa_thread(), lane = tid & 63, wave = pa_uniform(tid >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, pw = wave / ES;
+        const int G = a.grp, rc = ST ? c & 7 : c;
         const PaPiece x = pa_piece<false>(a, pl, mine, blockIdx.x, u, first, stop);
         u += x.n;
         const PagedSeq &sq = x.sq;
         const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = sq.nq * G;
         bool bad = sq.bad;
-        if (bad && threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
+        if (bad && tid == 0) paged_flag(p, PAGED_BAD_BATCH);
         const bool mixed = hi0 != x.hi1 || lo0 != lo1;       // whether the rows differ in what they attend
         const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 32 * PW - 1) / (32 * PW) : 0;
 
         // queries: loaded first, ahead of the stream
         constexpr int LPR = 256 / R, QN = HD / (4 * LPR) > 0 ? HD / (4 * LPR) : 1;
-        const int qr = threadIdx.x / LPR, ql = threadIdx.x % LPR;
+        const int qr = tid / LPR, ql = tid % LPR;
         pa_v4f qv[QN];
         {
             const int i = (int)(qr * pl.grp_inv >> 16), h = qr - i * G;
@@ -271,8 +274,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                 w[j] = y * qs;
             }
             if (a.cap > 0.0f) {
+                pa_tanh8(w);
 #pragma unroll
-                for (int j = 0; j < 8; j++) w[j] = capl * pa_tanh(w[j]);
+                for (int j = 0; j < 8; j++) w[j] *= capl;
             }
             if (edge) {
 #pragma unroll
@@ -400,6 +404,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                             for (int i = 0; i < 4; i++) {
                                 const uint16_t hv = row[pa_elem<HE, KVT>(e, 4 * g + i)];
                                 if (sees && (hv & 0x7c00) == 0x7c00) o[e][i] += wx * h2f(hv);
+                                __builtin_amdgcn_sched_barrier(0);
                             }
                     }
                 }
@@ -431,7 +436,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
                     for (int i = 0; i < 4; i++) buf[(pw * 8 + (c & 7)) * (HD + 4) + HE * ew + pa_elem<HE, KVT>(e, 4 * g + i)] = o[e][i];
             }
             lds_barrier();
-            for (int y = threadIdx.x; y < 8 * (HD / 4); y += 256) {
+            for (int y = tid; y < 8 * (HD / 4); y += 256) {
                 const int r8 = y / (HD / 4), e4 = y % (HD / 4) * 4, r = 8 * k + r8;
                 if (r >= rows) continue;
                 float mm = -__builtin_inff();
@@ -465,8 +470,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_few(PagedAttn a, PagedPlan pl)
 template <int KVT, int HD>
 hipError_t pa_few_hd(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
     const dim3 grid(pl.few.wgs), wg(256);
-    if (pl.few.rows <= 8) hipLaunchKernelGGL((k_paged_few<HD, KVT, true>), grid, wg, 0, s, a, pl);
-    else hipLaunchKernelGGL((k_paged_few<HD, KVT, false>), grid, wg, 0, s, a, pl);
+    if (pl.few.rows <= 8) hipLaunchKernelGGL((k_paged_few<HD, KVT, true>), grid, wg, 0, s, PagedCall{a, pl});
+    else hipLaunchKernelGGL((k_paged_few<HD, KVT, false>), grid, wg, 0, s, PagedCall{a, pl});
     return hipGetLastError();
 }
 template <int KVT>

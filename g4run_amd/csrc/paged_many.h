@@ -52,34 +52,37 @@ struct PmStage {
 };
 
 template <int HD, int KVT>
-__device__ __forceinline__ void pm_load(PmStage<HD, KVT> &t, const PagedPool &p, const PaUnit u[2]) {
+__device__ __forceinline__ void pm_load(PmStage<HD, KVT> &t, const PagedPool &p, const PaUnit u[2], int tid) {
     using T = PmStage<HD, KVT>;
     constexpr int RB = paged_row_bytes(KVT, HD);
 #pragma unroll
     for (int n = 0; n < T::KT; n++) {
-        const int x = threadIdx.x + PM_THREADS * n;
+        const int x = tid + PM_THREADS * n;
         if (T::KRUNS % PM_THREADS && x >= T::KRUNS) break;
-        constexpr int per = RB / (4 * T::KD);
+        constexpr int per = RB / (4 * T::KD), step = PM_THREADS / per;       // positions of one n
         const int pos = x / per, at = x % per;
-        pa_load<T::KD>(t.k[n], p.k + (pos < 16 ? u[0].row : u[1].row) + (pos & 15) * RB + at * 4 * T::KD);
+        const uint32_t off = (pos & 15) * RB + at * 4 * T::KD;
+        if constexpr (step <= 16) pa_load<T::KD>(t.k[n], p.k + (n * step < 16 ? u[0].row : u[1].row) + off);
+        else pa_load<T::KD>(t.k[n], p.k + (pos < 16 ? u[0].row : u[1].row) + off);
     }
 #pragma unroll
     for (int n = 0; n < T::VT; n++) {
-        const int x = threadIdx.x + PM_THREADS * n;
+        const int x = tid + PM_THREADS * n;
         if (T::VTASKS % PM_THREADS && x >= T::VTASKS) break;
         constexpr int per = HD / T::VE;
-        const int g = x / per, at = x % per;
+        const int g = per % 64 == 0 ? pa_uniform(x / per) : x / per;
+        const uint32_t off = x % per * (KVT == Q4_0 ? 2 : 4);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const uint8_t *row = p.v + u[j >> 2].row + (4 * g + (j & 3)) * RB;
-            if constexpr (KVT == Q4_0) t.v[n][j] = *(const uint16_t *)(row + 2 * at);
-            else t.v[n][j] = *(const uint32_t *)(row + 4 * at);
+            const uint8_t *row = p.v + u[j >> 2].row + (uint32_t)(4 * g + (j & 3)) * RB;
+            if constexpr (KVT == Q4_0) t.v[n][j] = *(const uint16_t *)(row + off);
+            else t.v[n][j] = *(const uint32_t *)(row + off);
         }
     }
     if constexpr (T::SCT > 0) {
 #pragma unroll
         for (int n = 0; n < T::SCT; n++) {
-            const int x = threadIdx.x + PM_THREADS * n;
+            const int x = tid + PM_THREADS * n;
             if (T::STASKS % PM_THREADS && x >= T::STASKS) break;
             constexpr int per = HD / 64;
             const int pos = x / per % 32, at = x % per;
@@ -93,13 +96,13 @@ __device__ __forceinline__ void pm_load(PmStage<HD, KVT> &t, const PagedPool &p,
 // [lo, hi) counted from the tile's first) become 0, and so do non-finite ones;
 // returns whether there was one of the latter.
 template <int HD, int KVT>
-__device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, KVT> &t, bool edge, int lo, int hi) {
+__device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, KVT> &t, bool edge, int lo, int hi, int tid) {
     using T = PmStage<HD, KVT>;
     constexpr int RB = paged_row_bytes(KVT, HD);
     bool odd = false;
 #pragma unroll
     for (int n = 0; n < T::KT; n++) {
-        const int x = threadIdx.x + PM_THREADS * n;
+        const int x = tid + PM_THREADS * n;
         if (T::KRUNS % PM_THREADS && x >= T::KRUNS) break;
         constexpr int per = RB / (4 * T::KD);
         const int pos = x / per, at = x % per;
@@ -124,10 +127,10 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
     }
 #pragma unroll
     for (int n = 0; n < T::VT; n++) {
-        const int x = threadIdx.x + PM_THREADS * n;
+        const int x = tid + PM_THREADS * n;
         if (T::VTASKS % PM_THREADS && x >= T::VTASKS) break;
         constexpr int per = HD / T::VE;
-        const int g = x / per, at = x % per;
+        const int g = per % 64 == 0 ? pa_uniform(x / per) : x / per, at = x % per;
         uint32_t v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = t.v[n][j];
@@ -175,7 +178,7 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
     if constexpr (T::SCT > 0) {
 #pragma unroll
         for (int n = 0; n < T::SCT; n++) {
-            const int x = threadIdx.x + PM_THREADS * n;
+            const int x = tid + PM_THREADS * n;
             if (T::STASKS % PM_THREADS && x >= T::STASKS) break;
             constexpr int per = HD / 64;
             const int pos = x / per % 32, at = x % per;
@@ -212,33 +215,36 @@ __device__ __forceinline__ void pm_wave() { asm volatile("s_waitcnt lgkmcnt(0)" 
 constexpr int PM_COLS = 36, PM_TR = 16 * PM_COLS;
 
 template <int HD, int KVT>
-__global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(PagedAttn a, PagedPlan pl) {
-    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2;   // NB: buffers
+__global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(PagedCall call) {
+    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2, AHEAD = HD > 64 ? 4 : 2;   // NB: buffers
     constexpr size_t TB = sizeof(PmTile<HD, KVT>) * NB, RB = (size_t)8 * PM_TR * 4;
     __shared__ __align__(16) uint8_t lds[TB > RB ? TB : RB]; // the tiles; before and after them rows on their way
     __shared__ __align__(16) float xs[ES > 1 ? 8 : 1][ES > 1 ? 64 : 1][8];   // partial scores of wave pairs
     __shared__ int odds[3];                                  // by iteration: whether the tile held a non-finite value
     PmTile<HD, KVT> *const tiles = (PmTile<HD, KVT> *)lds;
-    const int lane = threadIdx.x & 63, wave = pa_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, rw = wave / ES;
-    const PagedPool &p = a.p;
-    const PagedBatch &b = a.b;
-    const int G = a.grp, R = pl.many.rows;
-    float *const tr = (float *)lds + wave * PM_TR;
-    const float capl = a.cap * 1.4426950408889634f;
 
     // Workgroups of one XCD (every eighth) take neighbouring shares: row tiles
     // that read the same K and V find them in its L2.
-    const int per = (pl.many.wgs + 7) >> 3, wg = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    const int per = (call.pl.many.wgs + 7) >> 3, wg = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     int mine;
-    const int total = pa_total<true>(a, pl, mine), share = pa_share(pl.many, total);
-    const int first = wg * share, stop = wg < pl.many.wgs ? min(first + share, total) : 0;
+    const int total = pa_total<true>(call.a, call.pl, mine), share = pa_share(call.pl.many, total);
+    const int first = wg * share, stop = wg < call.pl.many.wgs ? min(first + share, total) : 0;
     for (int u = first; u < stop;) {
+        const PagedCall call = pa_fresh();
+        const PagedAttn &a = call.a;
+        const PagedPlan &pl = call.pl;
+        const PagedPool &p = a.p;
+        const PagedBatch &b = a.b;
+        const int tid = pa_thread(), lane = tid & 63, wave = pa_uniform(tid >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, rw = wave / ES;
+        const int G = a.grp, R = pl.many.rows;
+        float *const tr = (float *)lds + wave * PM_TR;
+        const float capl = a.cap * 1.4426950408889634f;
         const PaPiece x = pa_piece<true>(a, pl, mine, wg, u, first, stop);
         u += x.n;
         const PagedSeq &sq = x.sq;
         const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = min(sq.nq * G, (x.tile + 1) * R), r0 = x.tile * R + 16 * rw;     // the tile's rows end at `rows`
         bool bad = sq.bad;
-        if (bad && threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
+        if (bad && tid == 0) paged_flag(p, PAGED_BAD_BATCH);
         const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 31) / 32 : 0;
 
         PmStage<HD, KVT> st;
@@ -249,7 +255,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             pa_check(p, us, bad);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
-            pm_load<HD, KVT>(st, p, nx);
+            pm_load<HD, KVT>(st, p, nx, tid);
         }
         // The wave's rows: 16 rw ..; busy: it has some.  The lane's: r0 + c.
         const bool busy = r0 < rows, ok = r0 + c < rows;
@@ -317,7 +323,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
         for (int e = 0; e < NM; e++) o[e] = pa_v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        if (threadIdx.x < 3) odds[threadIdx.x] = 0;
+        if (tid < 3) odds[tid] = 0;
         __syncthreads();
 
         for (int it = 0, turn = 0; it < iters; it++, turn = turn == 2 ? 0 : turn + 1) {
@@ -325,7 +331,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
             PmTile<HD, KVT> &d = tiles[NB == 2 ? it & 1 : 0];
             if (NB == 1 && it) __syncthreads();              // one buffer: the previous positions are used
-            if (pm_store<HD, KVT>(d, st, edge, lo0 - base, end - base)) odds[turn] = 1;
+            if (pm_store<HD, KVT>(d, st, edge, lo0 - base, end - base, tid)) odds[turn] = 1;
             un[0] = nx[0];
             un[1] = nx[1];
             if ((it & 31) == 31 && it + 1 < iters) {
@@ -335,30 +341,43 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             if (it + 1 < iters) {
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
                 nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
-                pm_load<HD, KVT>(st, p, nx);
+                pm_load<HD, KVT>(st, p, nx, tid);
             }
             if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units(p, x.table, (base >> 4) + 64, 2, last, kvh);
             lds_barrier();
             const int odd = odds[turn];
-            if (threadIdx.x == 0) odds[turn == 0 ? 2 : turn - 1] = 0;    // the iteration after the next's: written behind the next barrier
+            if (tid == 0) odds[turn == 0 ? 2 : turn - 1] = 0;    // the iteration after the next's: written behind the next barrier
             if (!busy && ES == 1) continue;
-            // scores of row c at positions base + pm_pos(g, j)
-            pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-            pm_pipeline<2 * NS, 4>([&](int i) { return *(const pa_v8h *)&d.k[16 * (i & 1) + c][HE * ew + 32 * (i >> 1) + 8 * g]; },
+            // scores of row c at positions base + pm_pos(g, j): high and low halves apart,
+            // so that no instruction waits for the one before it
+            pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}, s2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            auto scaled = [&](int n, pa_v4f y) {
+                const int h = n & 1;
+                const uint2 dd = *(const uint2 *)&d.dk[NS * ew + (n >> 1)][16 * h + 4 * g];
+                sc[h][0] = __builtin_fmaf(pa_lo(dd.x), y[0], sc[h][0]);
+                sc[h][1] = __builtin_fmaf(pa_hi(dd.x), y[1], sc[h][1]);
+                sc[h][2] = __builtin_fmaf(pa_lo(dd.y), y[2], sc[h][2]);
+                sc[h][3] = __builtin_fmaf(pa_hi(dd.y), y[3], sc[h][3]);
+            };
+            pm_pipeline<2 * NS, AHEAD>([&](int i) { return *(const pa_v8h *)&d.k[16 * (i & 1) + c][HE * ew + 32 * (i >> 1) + 8 * g]; },
                                    [&](int i, pa_v8h ko) {
                 const int s = i >> 1, h = i & 1;
                 if constexpr (KVT == F16) {
                     sc[h] = pa_mma(ko, q0[s], sc[h]);
-                    sc[h] = pa_mma(ko, q1[s], sc[h]);
+                    s2[h] = pa_mma(ko, q1[s], s2[h]);
                 } else {
+                    // scaled one operand later, when the products are there
                     const pa_v4f y = pa_mma(ko, q1[s], pa_mma(ko, q0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f}));
-                    const uint2 dd = *(const uint2 *)&d.dk[NS * ew + s][16 * h + 4 * g];
-                    sc[h][0] = __builtin_fmaf(pa_lo(dd.x), y[0], sc[h][0]);
-                    sc[h][1] = __builtin_fmaf(pa_hi(dd.x), y[1], sc[h][1]);
-                    sc[h][2] = __builtin_fmaf(pa_lo(dd.y), y[2], sc[h][2]);
-                    sc[h][3] = __builtin_fmaf(pa_hi(dd.y), y[3], sc[h][3]);
+                    if (i) scaled(i - 1, s2[0]);
+                    s2[0] = y;
                 }
             });
+            if constexpr (KVT == F16) {
+                sc[0] += s2[0];
+                sc[1] += s2[1];
+            } else {
+                scaled(2 * NS - 1, s2[0]);
+            }
             if constexpr (ES > 1) {
                 *(pa_v4f *)xs[wave][lane] = sc[0];
                 *(pa_v4f *)(xs[wave][lane] + 4) = sc[1];
@@ -370,8 +389,9 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j] = sc[j >> 2][j & 3] * qs;
             if (a.cap > 0.0f) {
+                pa_tanh8(w);
 #pragma unroll
-                for (int j = 0; j < 8; j++) w[j] = capl * pa_tanh(w[j]);
+                for (int j = 0; j < 8; j++) w[j] *= capl;
             }
             if (edge) {
 #pragma unroll
@@ -418,10 +438,13 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
                 for (int k = 0; k < 4; k++) pa_split(w[2 * k], w[2 * k + 1], hi[k], lo[k]);
                 const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
-                pm_pipeline<NM, 4>([&](int e) { return *(const pa_v8h *)d.v[NM * ew + e][lane]; }, [&](int e, pa_v8h va) {
+                pa_v8h before;                               // low halves one operand later
+                pm_pipeline<NM, AHEAD>([&](int e) { return *(const pa_v8h *)d.v[NM * ew + e][lane]; }, [&](int e, pa_v8h va) {
                     o[e] = pa_mma(va, b0, o[e]);
-                    o[e] = pa_mma(va, b1, o[e]);
+                    if (e) o[e - 1] = pa_mma(before, b1, o[e - 1]);
+                    before = va;
                 });
+                o[NM - 1] = pa_mma(before, b1, o[NM - 1]);
                 if (odd) {
                     // non-finite values, zero in LDS, added to the rows that attend them
                     for (int k = 0; k < 32; k++) {
@@ -436,12 +459,15 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                         }
                         const bool sees = pos >= rlo && pos <= rhi;
 #pragma unroll
-                        for (int e = 0; e < NM; e++)
+                        for (int e = 0; e < NM; e++) {
+                            const uint2 hv = *(const uint2 *)(row + 16 * e + 4 * g);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                const uint16_t hv = row[16 * e + 4 * g + i];
-                                if (sees && (hv & 0x7c00) == 0x7c00) o[e][i] += wx * h2f(hv);
+                                const uint32_t v = (i < 2 ? hv.x : hv.y) >> (16 * (i & 1)) & 0xffffu;
+                                if (sees && (v & 0x7c00) == 0x7c00) o[e][i] += wx * h2f((uint16_t)v);
                             }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
                 }
             } else {
@@ -461,12 +487,11 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                         pa_split_scaled(w[4 * h + 2], w[4 * h + 3], dd.y & live[2 * h + 1], hi[2 * h + 1], lo[2 * h + 1]);
                     }
                     const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-                    for (int e = 2 * s; e < 2 * s + 2; e++) {
-                        const pa_v8h va = *(const pa_v8h *)d.v[NM * ew + e][lane];
-                        o[e] = pa_mma(va, b0, o[e]);
-                        o[e] = pa_mma(va, b1, o[e]);
-                    }
+                    const pa_v8h v0 = *(const pa_v8h *)d.v[NM * ew + 2 * s][lane], v1 = *(const pa_v8h *)d.v[NM * ew + 2 * s + 1][lane];
+                    o[2 * s] = pa_mma(v0, b0, o[2 * s]);
+                    o[2 * s + 1] = pa_mma(v1, b0, o[2 * s + 1]);
+                    o[2 * s] = pa_mma(v0, b1, o[2 * s]);
+                    o[2 * s + 1] = pa_mma(v1, b1, o[2 * s + 1]);
                 }
             }
         }
@@ -514,10 +539,10 @@ template <int KVT>
 hipError_t pa_many(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
     const dim3 grid((pl.many.wgs + 7) / 8 * 8), wg(PM_THREADS);
     switch (a.p.hd) {
-    case 64: hipLaunchKernelGGL((k_paged_many<64, KVT>), grid, wg, 0, s, a, pl); break;
-    case 128: hipLaunchKernelGGL((k_paged_many<128, KVT>), grid, wg, 0, s, a, pl); break;
-    case 256: hipLaunchKernelGGL((k_paged_many<256, KVT>), grid, wg, 0, s, a, pl); break;
-    case 512: hipLaunchKernelGGL((k_paged_many<512, KVT>), grid, wg, 0, s, a, pl); break;
+    case 64: hipLaunchKernelGGL((k_paged_many<64, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
+    case 128: hipLaunchKernelGGL((k_paged_many<128, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
+    case 256: hipLaunchKernelGGL((k_paged_many<256, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
+    case 512: hipLaunchKernelGGL((k_paged_many<512, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
