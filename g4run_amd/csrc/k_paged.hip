@@ -40,20 +40,27 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     auto span = [&](int tokens) { return window ? std::min<int64_t>(b.max_len, (int64_t)window + 32 + tokens) : (int64_t)b.max_len; };
     const int64_t fspan = span(16);
     // A step is at least what a workgroup takes at once; up to 256 positions stay
-    // one step, so that no join is launched for them.
+    // one step, so that no join is launched for them.  A sequence's tile counts as
+    // `lead` steps more, for its queries, first loads and results: 64 sequences of
+    // 2000 of 4096 positions, 8 KV heads of 128, 8 bits, take 75 us with a lead of 1, 73
+    // with 2, 93 without; a lead of 2 is slower where steps are few (the shares' last
+    // step rounded up).  None where every step has its workgroup.
     int64_t steps;
     for (few.shift = b.max_len <= 256 && !b.n_prefix ? 8 : 7;; few.shift++) {       // counted in 32 bits on the device
         few.unit = 1 << few.shift;
         few.pre_steps = few_pre ? ceil_div(b.n_prefix, few.unit) : 0;
         steps = ((int64_t)b.n_seq * std::max(1, ceil_div(fspan, few.unit)) + few.pre_steps) * p.n_kv;
-        if (steps < (1 << 30)) break;
+        if (steps < (1 << 27)) break;
     }
     few.wgs = (int)std::min<int64_t>(256 * pa_few_per_cu(p.type, p.hd, few.rows <= 8), steps);
+    few.lead = steps > few.wgs ? 1 : 0;
     y.join = b.n_prefix || (few.rows && fspan > few.unit);
     // Many rows: tiles of whole tokens, up to 128 rows (64 of heads of 512), evenly
-    // filled; as many workgroups as fit on the device at once.
+    // filled; as many workgroups as fit on the device at once.  Steps of 32 positions,
+    // a lead of 5 (four prompts of 509 behind 3800, 4 KV heads of 256: 91 us with 2,
+    // 83 with 4, 80 with 6; the same order for heads of 64).
     many.rows = 0;
-    many.pre_tiles = 0;
+    many.pre_tiles = many.lead = 0;
     if (many_own || many_pre) {
         const int most = paged_most_group(p.hd) / grp, toks = b.q_off || many_pre ? b.n_tok : 1;
         many.toks = ceil_div(toks, ceil_div(toks, most));
@@ -62,13 +69,14 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
         many.pre_tiles = many_pre ? ceil_div(b.n_tok, many.toks) : 0;
         const int64_t own = !many_own ? 0 : b.q_off ? ceil_div(b.n_tok, many.toks) + std::min(b.n_seq, b.n_tok / (few.toks + 1)) : b.n_seq;
         const int64_t mspan = span(many.toks);
-        for (many.shift = 6;; many.shift++) {
+        for (many.shift = 5;; many.shift++) {
             many.unit = 1 << many.shift;
             many.pre_steps = many_pre ? ceil_div(b.n_prefix, many.unit) : 0;
             steps = (own * std::max(1, ceil_div(mspan, many.unit)) + (int64_t)many.pre_tiles * many.pre_steps) * p.n_kv;
-            if (steps < (1 << 30)) break;
+            if (steps < (1 << 27)) break;
         }
         many.wgs = (int)std::min<int64_t>(p.hd >= 128 ? 256 : 512, ceil_div(steps, many.least));
+        many.lead = ceil_div(steps, many.least) > many.wgs ? 5 : 0;
         y.join |= mspan > many.unit;
     }
     const size_t all = y.join ? (size_t)b.n_tok * p.n_kv * grp : 0, whole = b.n_prefix ? all : 0;
@@ -91,33 +99,27 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
 // over the row's partial results in a fixed order, by groups of hd / 4 threads.
 // SPLIT: a workgroup per row, each group every so-many-th of its results (few rows
 // of many pieces); else a group per row (many rows of few: a workgroup's one active
-// group left the chip empty, 9000 rows of 256 took 18 us).
+// group left the chip empty, 9000 rows of 256 took 18 us).  Bound by the latency of
+// reads that depend on each other, so: the row's sequence by one load of the whole
+// wave, four results' maxima and sums at once under a running maximum.
 template <bool SPLIT>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
-    __shared__ float red[4];
-    __shared__ float lg[16];                                 // at most 16 groups: hd >= 64
+    __shared__ float2 ml_of[SPLIT ? 16 : 1];                 // at most 16 groups: hd >= 64
     __shared__ pa_v4f part[SPLIT ? 256 : 1];
     const int hd = a.p.hd, hd4 = hd / 4, groups = 256 / hd4, gi = threadIdx.x / hd4, e4 = threadIdx.x % hd4 * 4;
-    const int64_t row = SPLIT ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * groups + gi;
-    if (row >= (int64_t)a.b.n_tok * a.n_head) return;
-    const int tok = (int)(row / a.n_head), head = (int)(row - (int64_t)tok * a.n_head);
-    const bool prefix = a.b.n_prefix > 0;
-    const uint2 own = pl.own[row], pre = prefix ? pl.pre[row] : make_uint2(0, 0);      // of a row without a sequence: not used
-    int seq;
+    const int all = a.b.n_tok * a.n_head, mine = SPLIT ? (int)blockIdx.x : (int)blockIdx.x * groups + gi, row = min(mine, all - 1);   // up to 2^24
+    const int tok = row / a.n_head, head = row - tok * a.n_head;
+    const uint2 own = pl.own[row], pre = a.b.n_prefix > 0 ? pl.pre[row] : make_uint2(0, 0);      // of a row without a sequence: not used
+    int seq = 0;
     if constexpr (SPLIT) seq = paged_find(a.b, tok);
     else {
-        seq = tok < a.b.n_seq ? tok : a.b.n_seq;
-        if (a.b.q_off) {                                     // a group's own: the last sequence that starts at or before the token
-            int x = 0, y = a.b.n_seq + 1;
-            while (y - x > 1) {
-                const int z = (x + y) >> 1;
-                if (paged_ld(a.b.q_off, z) <= tok) x = z;
-                else y = z;
-            }
-            seq = x;
+        const int t1 = __builtin_amdgcn_readlane(tok, 63);   // a wave's rows lie in up to 4 tokens
+        for (int t = pa_uniform(tok); t <= t1; t++) {
+            const int s = paged_find(a.b, t);
+            if (t == tok) seq = s;
         }
     }
-    if (seq >= a.b.n_seq) return;                            // behind the last sequence
+    if (mine >= all || seq >= a.b.n_seq) return;             // behind the last row or sequence
     const PagedSeq sq = paged_seq(a.p, a.b, seq);
     const int i = tok - sq.t0;
     if (i < 0 || i >= sq.nq) return;
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
         const uint2 d = k < n_pre ? pre : own;
         if (k >= n_pre) k -= n_pre;
         if (d.y == ~0u) {
-            o = pl.wo + row * hd;
+            o = pl.wo + (size_t)row * hd;
             ml = pl.wml + row;
             return;
         }
@@ -138,42 +140,46 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
         o = (many ? pl.many.o : pl.few.o) + s * hd;
         ml = (many ? pl.many.ml : pl.few.ml) + s;
     };
-    const int k0 = SPLIT ? gi : 0, step = SPLIT ? groups : 1;
-    float mm = -__builtin_inff();
-    for (int k = SPLIT ? threadIdx.x : 0; k < total; k += SPLIT ? 256 : 1) {
-        const float *o;
-        const float2 *ml;
-        at(k, o, ml);
-        mm = fmaxf(mm, ml->x);
-    }
-    if constexpr (SPLIT) {
-        mm = group_max<64>(mm);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mm;
-        __syncthreads();
-        mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    }
     pa_v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-#pragma unroll 4
-    for (int k = k0; k < total; k += step) {
-        const float *o;
-        const float2 *ml;
-        at(k, o, ml);
-        const float2 x = *ml;
-        const pa_v4f v = *(const pa_v4f *)(o + e4);
-        const float f = x.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x.x - mm);
+    float m = -__builtin_inff(), l = 0.0f;
+    auto add = [&](float2 x, pa_v4f v, float mn) {
+        const float f = x.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x.x - mn);
         l += x.y == x.y ? f * x.y : x.y;                     // a bad page's NaN stays
         s += v * f;
+    };
+    constexpr int N = 4;
+    const int step = SPLIT ? groups : 1;
+    for (int k = SPLIT ? gi : 0; k < total; k += N * step) {
+        float2 x[N];
+        pa_v4f v[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const float *o;
+            const float2 *ml;
+            at(min(k + j * step, total - 1), o, ml);
+            x[j] = *ml;
+            v[j] = *(const pa_v4f *)(o + e4);
+        }
+        float mn = m;
+#pragma unroll
+        for (int j = 0; j < N; j++) mn = fmaxf(mn, x[j].x);
+        const float f = m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+        s *= f;
+        m = mn;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (k + j * step < total) add(x[j], v[j], mn);
     }
     if constexpr (SPLIT) {
         part[threadIdx.x] = s;
-        if (e4 == 0) lg[gi] = l;
+        if (e4 == 0) ml_of[gi] = make_float2(m, l);
         __syncthreads();
         if (gi) return;
-        for (int k = 1; k < groups; k++) {
-            s += part[k * hd4 + threadIdx.x];
-            l += lg[k];
-        }
+        for (int k = 0; k < groups; k++) m = fmaxf(m, ml_of[k].x);
+        s = pa_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        l = 0.0f;
+        for (int k = 0; k < groups; k++) add(ml_of[k], part[k * hd4 + threadIdx.x], m);
     }
     const bool none = !sq.bad && sq.len - sq.nq + i < 0;
     pa_store4(a.out + (size_t)tok * a.os + (size_t)head * hd + e4, none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / l));

@@ -48,6 +48,7 @@ struct PagedList {
     uint32_t toks_inv;               // many: n / toks == umulhi(n, toks_inv) for n <= 2^24 (0: toks is 1)
     int wgs, least;                  // workgroups; steps of a share at least
     int unit, shift;                 // positions of a step, and their log2
+    int lead;                        // steps that the start of a sequence's tile counts as
     int pre_tiles, pre_steps;        // the prefix's tiles (0: not this kernel's), and steps of each
     float *o;                        // [2 wgs][rows][hd] unnormalised sums
     float2 *ml;                      // [2 wgs][rows] maximum (log2), sum
@@ -280,7 +281,7 @@ __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl,
     const int tiles = pa_tiles<MANY>(pl, q);
     int n = 0;
     for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY>(a, pl, q, t);
-    return n;
+    return n + tiles * pa_list<MANY>(pl).lead;
 }
 // All steps of the list (wave-uniform; the whole wave calls it), 64 sequences at a
 // time; the lane's own of the first 64 in `mine`.
@@ -316,10 +317,12 @@ __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan
 }
 __device__ __forceinline__ int pa_share(const PagedList &y, int total) { return max(y.least, (total + y.wgs - 1) / y.wgs); }
 
-// A piece: steps [step, step + n) of the `all` of one tile of one KV head.
+// A piece: steps [step, step + n) of the `all` of one tile of one KV head.  (The
+// lead comes before step 0, so the shares of the list stay contiguous.)
 struct PaPiece {
     PagedSeq sq;                     // the prefix: all tokens of the batch
     int kvh, tile, step, n, all;
+    int took;                        // of the share: n and what it holds of the lead; n is 0 where it ends in that
     int seglen, start, end;          // positions of the segment; the piece's [start, end)
     int hi0, hi1, lo0, lo1;          // the first and the last row's last and first positions
     int slot;                        // of its sums
@@ -334,7 +337,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
     PaPiece x;
     const int pre_all = y.pre_tiles * y.pre_steps * a.p.n_kv;
     x.pre = u < pre_all;
-    int base;
+    int base, v, lead = 0;                                   // v: the step of the tile, its lead counted
     if (x.pre) {
         x.sq.t0 = 0;
         x.sq.nq = pa_tokens(b);
@@ -342,7 +345,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
         x.sq.bad = false;
         x.all = y.pre_steps;
         const int t = u / x.all;
-        x.step = u - t * x.all;
+        v = u - t * x.all;
         x.kvh = y.pre_tiles == 1 ? t : t / y.pre_tiles;
         x.tile = t - x.kvh * y.pre_tiles;
         x.table = b.prefix;
@@ -350,23 +353,23 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
         x.lo0 = base = 0;
         x.lo1 = a.window ? 0x7fffffff : 0;                   // row by row
     } else {
+        lead = y.lead;
         int seq, before;
         pa_find_step<MANY>(a, pl, mine, u - pre_all, seq, before);
         x.sq = paged_seq(a.p, b, seq);
-        int v = u - pre_all - before;
+        v = u - pre_all - before;
         if constexpr (MANY) {
             const int tiles = pa_tiles<MANY>(pl, x.sq);
-            int head = 0;                                    // steps of one KV head
+            int head = tiles * y.lead;                       // steps of one KV head
             for (int t = 0; t < tiles; t++) head += pa_tile_steps<MANY>(a, pl, x.sq, t);
             for (x.kvh = 0; v >= head; x.kvh++) v -= head;
             x.tile = 0;
-            for (x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0); v >= x.all; x.all = pa_tile_steps<MANY>(a, pl, x.sq, ++x.tile)) v -= x.all;
+            for (x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0); v >= y.lead + x.all; x.all = pa_tile_steps<MANY>(a, pl, x.sq, ++x.tile)) v -= y.lead + x.all;
         } else {
             x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0);
             x.tile = 0;
-            for (x.kvh = 0; v >= x.all; x.kvh++) v -= x.all;
+            for (x.kvh = 0; v >= y.lead + x.all; x.kvh++) v -= y.lead + x.all;
         }
-        x.step = v;
         pa_tile_span<MANY>(a, pl, x.sq, x.tile, base, x.hi1);
         x.hi0 = x.sq.len - x.sq.nq + (MANY ? x.tile * pl.many.toks : 0);
         x.lo0 = a.window ? max(0, x.hi0 + 1 - a.window) : 0;
@@ -374,7 +377,9 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
         x.seglen = x.sq.bad ? 0 : x.sq.len;
         x.table = b.table + (size_t)seq * b.table_stride;
     }
-    x.n = min(x.all - x.step, stop - u);
+    x.step = max(0, v - lead);
+    x.took = min(lead + x.all - v, stop - u);
+    x.n = max(0, v + x.took - lead) - x.step;
     x.start = base + (x.step << y.shift);
     x.end = min(x.start + (x.n << y.shift), min(x.hi1 + 1, x.seglen));
     x.slot = 2 * wg + (u != first);

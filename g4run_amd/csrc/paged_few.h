@@ -131,7 +131,8 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         const int tid = pa_thread(), lane = tid & 63, wave = pa_uniform(tid >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, pw = wave / ES;
         const int G = a.grp, rc = ST ? c & 7 : c;
         const PaPiece x = pa_piece<false>(a, pl, mine, blockIdx.x, u, first, stop);
-        u += x.n;
+        u += x.took;
+        if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;
         const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = sq.nq * G;
         bool bad = sq.bad;

@@ -240,7 +240,8 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         float *const tr = (float *)lds + wave * PM_TR;
         const float capl = a.cap * 1.4426950408889634f;
         const PaPiece x = pa_piece<true>(a, pl, mine, wg, u, first, stop);
-        u += x.n;
+        u += x.took;
+        if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;
         const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = min(sq.nq * G, (x.tile + 1) * R), r0 = x.tile * R + 16 * rw;     // the tile's rows end at `rows`
         bool bad = sq.bad;
