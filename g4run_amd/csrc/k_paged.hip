@@ -39,14 +39,15 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     // 32, and its later tokens
     auto span = [&](int tokens) { return window ? std::min<int64_t>(b.max_len, (int64_t)window + 32 + tokens) : (int64_t)b.max_len; };
     const int64_t fspan = span(16);
-    // A step is at least what a workgroup takes at once; up to 256 positions stay
+    // A step is what a workgroup takes at once (of heads of 512 its four waves share
+    // 32 positions; with steps of 128, 16 windows of 1024 took 23.3 us, now 21.7); up to 256 positions stay
     // one step, so that no join is launched for them.  A sequence's tile counts as
     // `lead` steps more, for its queries, first loads and results: 64 sequences of
     // 2000 of 4096 positions, 8 KV heads of 128, 8 bits, take 75 us with a lead of 1, 73
     // with 2, 93 without; a lead of 2 is slower where steps are few (the shares' last
     // step rounded up).  None where every step has its workgroup.
     int64_t steps;
-    for (few.shift = b.max_len <= 256 && !b.n_prefix ? 8 : 7;; few.shift++) {       // counted in 32 bits on the device
+    for (few.shift = b.max_len <= 256 && !b.n_prefix ? 8 : p.hd == 512 ? 5 : p.hd == 256 ? 6 : 7;; few.shift++) {       // counted in 32 bits on the device
         few.unit = 1 << few.shift;
         few.pre_steps = few_pre ? ceil_div(b.n_prefix, few.unit) : 0;
         steps = ((int64_t)b.n_seq * std::max(1, ceil_div(fspan, few.unit)) + few.pre_steps) * p.n_kv;

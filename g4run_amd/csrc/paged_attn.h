@@ -450,6 +450,11 @@ __device__ __forceinline__ void pa_split(float u, float v, uint32_t &hi, uint32_
     hi = pa_pk(u, v);
     lo = pa_pk(__builtin_fmaf(pa_lo(hi), -1.0f, u), __builtin_fmaf(pa_hi(hi), -1.0f, v));
 }
+// the high half of both where part is 0, the low half where it is -1
+__device__ __forceinline__ uint32_t pa_half(float u, float v, float part) {
+    const uint32_t hi = pa_pk(u, v);
+    return pa_pk(__builtin_fmaf(pa_lo(hi), part, u), __builtin_fmaf(pa_hi(hi), part, v));
+}
 // factor from a raw score product to log2 units (before a cap: to tanh's argument)
 template <int KVT>
 __device__ __forceinline__ float pa_score_scale(const PagedAttn &a, int sh) {

@@ -214,6 +214,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         }
         const float qs = qsc[rc], capl = a.cap * 1.4426950408889634f;
 
+        const float part = c < 8 ? 0.0f : -1.0f;             // ST: the lane's half of a weight
         pa_v4f o[NM];
         float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
@@ -345,8 +346,8 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                 uint32_t ph[4], pq[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    pa_split(w[2 * k], w[2 * k + 1], ph[k], pq[k]);
-                    if constexpr (ST) ph[k] = c < 8 ? ph[k] : pq[k];
+                    if constexpr (ST) ph[k] = pa_half(w[2 * k], w[2 * k + 1], part);
+                    else pa_split(w[2 * k], w[2 * k + 1], ph[k], pq[k]);
                 }
                 const pa_v8h b0 = pa_op(ph[0], ph[1], ph[2], ph[3]), b1 = pa_op(pq[0], pq[1], pq[2], pq[3]);
 #pragma unroll
@@ -371,8 +372,8 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const float y = __builtin_fmaf(pa_scale(kv.dv[2 * k], s), w[2 * k], 0.0f), z = __builtin_fmaf(pa_scale(kv.dv[2 * k + 1], s), w[2 * k + 1], 0.0f);
-                        pa_split(y, z, ph[k], pq[k]);
-                        if constexpr (ST) ph[k] = c < 8 ? ph[k] : pq[k];
+                        if constexpr (ST) ph[k] = pa_half(y, z, part);
+                        else pa_split(y, z, ph[k], pq[k]);
                     }
                     const pa_v8h b0 = pa_op(ph[0], ph[1], ph[2], ph[3]), b1 = pa_op(pq[0], pq[1], pq[2], pq[3]);
 #pragma unroll
