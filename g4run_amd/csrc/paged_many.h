@@ -27,12 +27,14 @@ constexpr int PM_THREADS = 512;
 __device__ __forceinline__ int pm_pos(int g, int j) { return 16 * (j >> 2) + 4 * g + (j & 3); }
 
 // LDS of 32 positions: K [32][HD + 8] halves; V [HD / 16][64 lanes][8] as operands;
-// the scales [HD / 32][32] of K and of V (quantized)
+// the scales [HD / 32][32] of K and of V, and each position's pa_exponent of its
+// largest V scale (quantized)
 template <int HD, int KVT>
 struct PmTile {
     _Float16 k[32][HD + 8];
     _Float16 v[HD / 16][64][8];
     uint16_t dk[KVT == F16 ? 1 : HD / 32][32], dv[KVT == F16 ? 1 : HD / 32][32];
+    float ev[KVT == F16 ? 4 : 32];
 };
 
 // What a thread carries of the next 32 positions.
@@ -185,23 +187,37 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
             uint16_t(*to)[32] = x < T::STASKS / 2 ? d.dk : d.dv;
             to[2 * at][pos] = (uint16_t)t.s[n];
             to[2 * at + 1][pos] = (uint16_t)(t.s[n] >> 16);
+            if (x >= T::STASKS / 2) {
+                const uint32_t y = t.s[n] & 0x7fff7fffu;
+                const float e = group_max<per>(pa_exponent(max(y << 16, y), 1));
+                if (at == 0) d.ev[pos] = e;
+            }
         }
     }
     return odd;
 }
+
+struct PmKey {
+    pa_v8h x;
+    uint2 d;
+};
+struct PmValue {
+    pa_v8h x[2];
+    uint2 d[2];
+};
 
 // read(i) brings operand i of N from LDS, use(i, operand) multiplies with it: reads
 // run AHEAD of their use.  (Left to itself the compiler reads, waits and multiplies
 // one by one: 130 cycles of LDS latency for 32 of matrix instructions.)
 template <int N, int AHEAD, typename R, typename U>
 __device__ __forceinline__ void pm_pipeline(R read, U use) {
-    pa_v8h x[AHEAD];
+    decltype(read(0)) x[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD && i < N; i++) x[i] = read(i);
 #pragma unroll
     for (int i = 0; i < N; i++) {
         __builtin_amdgcn_sched_barrier(0);
-        const pa_v8h y = x[i % AHEAD];
+        const auto y = x[i % AHEAD];
         use(i, y);
         __builtin_amdgcn_sched_barrier(0);
         if (i + AHEAD < N) x[i % AHEAD] = read(i + AHEAD);
@@ -216,7 +232,7 @@ constexpr int PM_COLS = 36, PM_TR = 16 * PM_COLS;
 
 template <int HD, int KVT>
 __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(PagedCall call) {
-    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2, AHEAD = HD > 64 ? 4 : 2;   // NB: buffers
+    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2, AHEAD = HD > 64 ? 4 : 2, BLOCKS = HD > 64 ? 2 : 1;    // NB: buffers
     constexpr size_t TB = sizeof(PmTile<HD, KVT>) * NB, RB = (size_t)8 * PM_TR * 4;
     __shared__ __align__(16) uint8_t lds[TB > RB ? TB : RB]; // the tiles; before and after them rows on their way
     __shared__ __align__(16) float xs[ES > 1 ? 8 : 1][ES > 1 ? 64 : 1][8];   // partial scores of wave pairs
@@ -352,32 +368,30 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             // scores of row c at positions base + pm_pos(g, j): high and low halves apart,
             // so that no instruction waits for the one before it
             pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}, s2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-            auto scaled = [&](int n, pa_v4f y) {
-                const int h = n & 1;
-                const uint2 dd = *(const uint2 *)&d.dk[NS * ew + (n >> 1)][16 * h + 4 * g];
-                sc[h][0] = __builtin_fmaf(pa_lo(dd.x), y[0], sc[h][0]);
-                sc[h][1] = __builtin_fmaf(pa_hi(dd.x), y[1], sc[h][1]);
-                sc[h][2] = __builtin_fmaf(pa_lo(dd.y), y[2], sc[h][2]);
-                sc[h][3] = __builtin_fmaf(pa_hi(dd.y), y[3], sc[h][3]);
-            };
-            pm_pipeline<2 * NS, AHEAD>([&](int i) { return *(const pa_v8h *)&d.k[16 * (i & 1) + c][HE * ew + 32 * (i >> 1) + 8 * g]; },
-                                   [&](int i, pa_v8h ko) {
-                const int s = i >> 1, h = i & 1;
-                if constexpr (KVT == F16) {
-                    sc[h] = pa_mma(ko, q0[s], sc[h]);
-                    s2[h] = pa_mma(ko, q1[s], s2[h]);
-                } else {
-                    // scaled one operand later, when the products are there
-                    const pa_v4f y = pa_mma(ko, q1[s], pa_mma(ko, q0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f}));
-                    if (i) scaled(i - 1, s2[0]);
-                    s2[0] = y;
-                }
-            });
+            auto key = [&](int i) { return *(const pa_v8h *)&d.k[16 * (i & 1) + c][HE * ew + 32 * (i >> 1) + 8 * g]; };
             if constexpr (KVT == F16) {
+                pm_pipeline<2 * NS, AHEAD>(key, [&](int i, pa_v8h ko) {
+                    sc[i & 1] = pa_mma(ko, q0[i >> 1], sc[i & 1]);
+                    s2[i & 1] = pa_mma(ko, q1[i >> 1], s2[i & 1]);
+                });
                 sc[0] += s2[0];
                 sc[1] += s2[1];
             } else {
-                scaled(2 * NS - 1, s2[0]);
+                // scaled one operand later, when the products are there
+                uint2 before;
+                auto scaled = [&](int h) {
+                    sc[h][0] = __builtin_fmaf(pa_lo(before.x), s2[0][0], sc[h][0]);
+                    sc[h][1] = __builtin_fmaf(pa_hi(before.x), s2[0][1], sc[h][1]);
+                    sc[h][2] = __builtin_fmaf(pa_lo(before.y), s2[0][2], sc[h][2]);
+                    sc[h][3] = __builtin_fmaf(pa_hi(before.y), s2[0][3], sc[h][3]);
+                };
+                pm_pipeline<2 * NS, AHEAD>([&](int i) { return PmKey{key(i), *(const uint2 *)&d.dk[NS * ew + (i >> 1)][16 * (i & 1) + 4 * g]}; }, [&](int i, PmKey k) {
+                    const pa_v4f y = pa_mma(k.x, q1[i >> 1], pa_mma(k.x, q0[i >> 1], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f}));
+                    if (i) scaled(1 - (i & 1));
+                    s2[0] = y;
+                    before = k.d;
+                });
+                scaled(1);
             }
             if constexpr (ES > 1) {
                 *(pa_v4f *)xs[wave][lane] = sc[0];
@@ -407,17 +421,9 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                 for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j]);
             } else {
                 // + the exponent of the position's largest value scale
-                uint32_t dm[4] = {0, 0, 0, 0};
+                const pa_v4f e[2] = {*(const pa_v4f *)&d.ev[4 * g], *(const pa_v4f *)&d.ev[16 + 4 * g]};
 #pragma unroll
-                for (int s = 0; s < HD / 32; s++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint2 dd = *(const uint2 *)&d.dv[s][16 * h + 4 * g];
-                        dm[2 * h] = pa_pkmax(dm[2 * h], dd.x & 0x7fff7fffu);
-                        dm[2 * h + 1] = pa_pkmax(dm[2 * h + 1], dd.y & 0x7fff7fffu);
-                    }
-#pragma unroll
-                for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j] + pa_exponent(dm[j >> 1], j & 1));
+                for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j] + e[j >> 2][j & 3]);
             }
             mt = fmaxf(mt, partner<16>(mt));
             mt = fmaxf(mt, partner<32>(mt));
@@ -478,22 +484,24 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
                     for (int k = 0; k < 4; k++) live[k] = (w[2 * k] == 0.0f ? 0u : 0xffffu) | (w[2 * k + 1] == 0.0f ? 0u : 0xffff0000u);
                 }
-#pragma unroll
-                for (int s = 0; s < NS; s++) {               // blocks of 32 elements: value tiles 2 s, 2 s + 1
+                // blocks of 32 elements: value tiles 2 s, 2 s + 1
+                pm_pipeline<NS, BLOCKS>([&](int s) {
+                    const uint16_t *dv = d.dv[NS * ew + s];
+                    const pa_v8h(*v)[64] = (const pa_v8h(*)[64])d.v[NM * ew + 2 * s];
+                    return PmValue{{v[0][lane], v[1][lane]}, {*(const uint2 *)&dv[4 * g], *(const uint2 *)&dv[16 + 4 * g]}};
+                }, [&](int s, PmValue x) {
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const uint2 dd = *(const uint2 *)&d.dv[NS * ew + s][16 * h + 4 * g];
-                        pa_split_scaled(w[4 * h], w[4 * h + 1], dd.x & live[2 * h], hi[2 * h], lo[2 * h]);
-                        pa_split_scaled(w[4 * h + 2], w[4 * h + 3], dd.y & live[2 * h + 1], hi[2 * h + 1], lo[2 * h + 1]);
+                        pa_split_scaled(w[4 * h], w[4 * h + 1], x.d[h].x & live[2 * h], hi[2 * h], lo[2 * h]);
+                        pa_split_scaled(w[4 * h + 2], w[4 * h + 3], x.d[h].y & live[2 * h + 1], hi[2 * h + 1], lo[2 * h + 1]);
                     }
                     const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
-                    const pa_v8h v0 = *(const pa_v8h *)d.v[NM * ew + 2 * s][lane], v1 = *(const pa_v8h *)d.v[NM * ew + 2 * s + 1][lane];
-                    o[2 * s] = pa_mma(v0, b0, o[2 * s]);
-                    o[2 * s + 1] = pa_mma(v1, b0, o[2 * s + 1]);
-                    o[2 * s] = pa_mma(v0, b1, o[2 * s]);
-                    o[2 * s + 1] = pa_mma(v1, b1, o[2 * s + 1]);
-                }
+                    o[2 * s] = pa_mma(x.x[0], b0, o[2 * s]);
+                    o[2 * s + 1] = pa_mma(x.x[1], b0, o[2 * s + 1]);
+                    o[2 * s] = pa_mma(x.x[0], b1, o[2 * s]);
+                    o[2 * s + 1] = pa_mma(x.x[1], b1, o[2 * s + 1]);
+                });
             }
         }
         if (__any(bad)) {
