@@ -184,13 +184,14 @@ __device__ __forceinline__ PaUnit pa_unit(const PagedPool &p, const PaUnits &us,
     return x;
 }
 
-// x = tanh(x) of a lane's 8 scores: an odd polynomial below 0.3 (next term 9e-3
+// x = tanh(x) of a lane's N scores: an odd polynomial below 0.3 (next term 9e-3
 // x^11, below 6e-8 x there), where 1 - exp would lose the small value
-__device__ __forceinline__ void pa_tanh8(float x[8]) {
+template <int N>
+__device__ __forceinline__ void pa_tanh(float (&x)[N]) {
     float most = 0.0f;
-    float p[8];
+    float p[N];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
+    for (int j = 0; j < N; j++) {
         const float x2 = x[j] * x[j];
         float y = __builtin_fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f);
         y = __builtin_fmaf(x2, y, 2.0f / 15.0f);
@@ -200,14 +201,14 @@ __device__ __forceinline__ void pa_tanh8(float x[8]) {
     }
     if (__any(most > 0.3f)) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < N; j++) {
             const float ax = fabsf(x[j]), t = __builtin_amdgcn_exp2f(-2.885390081777927f * ax);
             const float r = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x[j]);
             p[j] = ax > 0.3f ? r : p[j];                     // NaN: the polynomial's
         }
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = p[j];
+    for (int j = 0; j < N; j++) x[j] = p[j];
 }
 
 // the batch's rows that attend the prefix
@@ -420,6 +421,11 @@ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &p
     return s;
 }
 
+// lane N of the lane's 16
+template <int N>
+__device__ __forceinline__ float pa_lane16(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + N, 0xF, 0xF, false));    // row_newbcast
+}
 // max of unsigned halves; the biased exponent of a (positive) half as a float
 typedef unsigned short pa_v2s __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pa_pkmax(uint32_t x, uint32_t y) {

@@ -30,6 +30,7 @@ struct PaTile {
     uint32_t k[2][KVT == F16 ? HE / 8 : KW];   // [unit][dwords]
     uint32_t v[8][VW];                         // [position 4 t + i][dwords]
     uint32_t dk[KVT == F16 ? 1 : 8][DW], dv[KVT == F16 ? 1 : 8][DW];
+    uint32_t de[KVT == F16 ? 1 : DW];          // value scales of position j = c % 8 of the lane group's 8
 };
 
 template <int HD, int HE, int KVT>
@@ -67,6 +68,7 @@ __device__ __forceinline__ void pa_load_v(PaTile<HE, KVT> &t, const PagedPool &p
         }
         if constexpr (KVT != F16) pa_load<T::DW>(t.dv[j], p.v + u[j >> 2].sc + i * (HD / 16) + (HE / 16) * ew);
     }
+    if constexpr (KVT != F16) pa_load<T::DW>(t.de, p.v + ((c & 4) ? u[1].sc : u[0].sc) + (4 * g + (c & 3)) * (HD / 16) + (HE / 16) * ew);
 }
 
 // key operand of unit h, 32 elements s
@@ -276,9 +278,22 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                 w[j] = y * qs;
             }
             if (a.cap > 0.0f) {
-                pa_tanh8(w);
+                if constexpr (ST) {                          // columns c and c ^ 8 hold the same scores: half of them each
+                    float y[4];
 #pragma unroll
-                for (int j = 0; j < 8; j++) w[j] *= capl;
+                    for (int j = 0; j < 4; j++) y[j] = c < 8 ? w[j] : w[4 + j];
+                    pa_tanh(y);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float z = y[j] * capl, other = xor8(z);
+                        w[j] = c < 8 ? z : other;
+                        w[4 + j] = c < 8 ? other : z;
+                    }
+                } else {
+                    pa_tanh(w);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) w[j] *= capl;
+                }
             }
             if (edge) {
 #pragma unroll
@@ -291,14 +306,14 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
 #pragma unroll
                 for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j]);
             } else {
-                // + the exponent of the position's largest value scale
+                // + the exponent of the position's largest value scale, found by one
+                // lane of eight for each position
+                uint32_t dm = kv.de[0] & 0x7fff7fffu;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    uint32_t dm = kv.dv[j][0] & 0x7fff7fffu;
-#pragma unroll
-                    for (int d = 1; d < HE / 64; d++) dm = pa_pkmax(dm, kv.dv[j][d] & 0x7fff7fffu);
-                    mt = fmaxf(mt, w[j] + pa_exponent(max(dm << 16, dm), 1));
-                }
+                for (int d = 1; d < HE / 64; d++) dm = pa_pkmax(dm, kv.de[d] & 0x7fff7fffu);
+                const float e = pa_exponent(max(dm << 16, dm), 1);
+                mt = fmaxf(fmaxf(fmaxf(w[0] + pa_lane16<0>(e), w[1] + pa_lane16<1>(e)), fmaxf(w[2] + pa_lane16<2>(e), w[3] + pa_lane16<3>(e))),
+                           fmaxf(fmaxf(w[4] + pa_lane16<4>(e), w[5] + pa_lane16<5>(e)), fmaxf(w[6] + pa_lane16<6>(e), w[7] + pa_lane16<7>(e))));
             }
             mt = fmaxf(mt, partner<16>(mt));
             mt = fmaxf(mt, partner<32>(mt));

@@ -404,7 +404,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j] = sc[j >> 2][j & 3] * qs;
             if (a.cap > 0.0f) {
-                pa_tanh8(w);
+                pa_tanh(w);
 #pragma unroll
                 for (int j = 0; j < 8; j++) w[j] *= capl;
             }
