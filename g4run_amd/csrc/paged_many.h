@@ -26,13 +26,14 @@ constexpr int PM_THREADS = 512;
 // of a wave's scores and of the second product's operand.
 __device__ __forceinline__ int pm_pos(int g, int j) { return 16 * (j >> 2) + 4 * g + (j & 3); }
 
-// LDS of 32 positions: K [32][HD + 8] halves; V [HD / 16][64 lanes][8] as operands;
+// LDS of 32 positions: K [32][HD + 8] halves; V [32][HD + 16] halves, read
+// transposed (ds_read_b64_tr_b16), quantized V [HD / 16][64 lanes][8] as operands;
 // the scales [HD / 32][32] of K and of V, and each position's pa_exponent of its
 // largest V scale (quantized)
 template <int HD, int KVT>
 struct PmTile {
     _Float16 k[32][HD + 8];
-    _Float16 v[HD / 16][64][8];
+    _Float16 v[KVT == F16 ? 32 * (HD + 16) / 512 : HD / 16][64][8];
     uint16_t dk[KVT == F16 ? 1 : HD / 32][32], dv[KVT == F16 ? 1 : HD / 32][32];
     float ev[KVT == F16 ? 4 : 32];
 };
@@ -44,13 +45,12 @@ struct PmStage {
     static constexpr int KRUNS = KVT == F16 ? 32 * HD / 8 : KVT == Q8_0 ? 32 * HD / 16 : 32 * HD / 8;
     static constexpr int KT = (KRUNS + PM_THREADS - 1) / PM_THREADS;
     static constexpr int KD = KVT == Q4_0 ? 1 : 4;           // dwords of a run
-    // V: 8 positions of one g x VE elements (f16: 2 adjacent, 4 bytes; q8_0 4 bytes, q4_0 2 bytes: 4, 16 apart)
-    static constexpr int VE = KVT == F16 ? 2 : 4;
-    static constexpr int VTASKS = 4 * HD / VE;
+    // V: f16 runs as K's; else 8 positions of one g x 4 elements, 16 apart (q8_0 4 bytes, q4_0 2 bytes)
+    static constexpr int VTASKS = KVT == F16 ? KRUNS : HD;
     static constexpr int VT = (VTASKS + PM_THREADS - 1) / PM_THREADS;
     static constexpr int STASKS = KVT == F16 ? 0 : 2 * 32 * HD / 64;     // dwords of scales, K then V
     static constexpr int SCT = (STASKS + PM_THREADS - 1) / PM_THREADS;
-    uint32_t k[KT][KD], v[VT][8], s[SCT ? SCT : 1];
+    uint32_t k[KT][KD], v[VT][KVT == F16 ? 4 : 8], s[SCT ? SCT : 1];
 };
 
 template <int HD, int KVT>
@@ -69,16 +69,22 @@ __device__ __forceinline__ void pm_load(PmStage<HD, KVT> &t, const PagedPool &p,
     }
 #pragma unroll
     for (int n = 0; n < T::VT; n++) {
-        const int x = tid + PM_THREADS * n;
+        const int x = (KVT == F16 ? tid ^ 256 : tid) + PM_THREADS * n;   // heads of 64: half of the waves K, half V
         if (T::VTASKS % PM_THREADS && x >= T::VTASKS) break;
-        constexpr int per = HD / T::VE;
-        const int g = per % 64 == 0 ? pa_uniform(x / per) : x / per;
-        const uint32_t off = x % per * (KVT == Q4_0 ? 2 : 4);
+        if constexpr (KVT == F16) {
+            constexpr int per = RB / 16;
+            const int pos = x / per;
+            pa_load<4>(t.v[n], p.v + (pos < 16 ? u[0].row : u[1].row) + (uint32_t)((pos & 15) * RB + x % per * 16));
+        } else {
+            constexpr int per = HD / 4;
+            const int g = per % 64 == 0 ? pa_uniform(x / per) : x / per;
+            const uint32_t off = x % per * (KVT == Q4_0 ? 2 : 4);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint8_t *row = p.v + u[j >> 2].row + (uint32_t)(4 * g + (j & 3)) * RB;
-            if constexpr (KVT == Q4_0) t.v[n][j] = *(const uint16_t *)(row + off);
-            else t.v[n][j] = *(const uint32_t *)(row + off);
+            for (int j = 0; j < 8; j++) {
+                const uint8_t *row = p.v + u[j >> 2].row + (uint32_t)(4 * g + (j & 3)) * RB;
+                if constexpr (KVT == Q4_0) t.v[n][j] = *(const uint16_t *)(row + off);
+                else t.v[n][j] = *(const uint32_t *)(row + off);
+            }
         }
     }
     if constexpr (T::SCT > 0) {
@@ -129,40 +135,29 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
     }
 #pragma unroll
     for (int n = 0; n < T::VT; n++) {
-        const int x = tid + PM_THREADS * n;
+        const int x = (KVT == F16 ? tid ^ 256 : tid) + PM_THREADS * n;
         if (T::VTASKS % PM_THREADS && x >= T::VTASKS) break;
-        constexpr int per = HD / T::VE;
-        const int g = per % 64 == 0 ? pa_uniform(x / per) : x / per, at = x % per;
-        uint32_t v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = t.v[n][j];
         if constexpr (KVT == F16) {
+            constexpr int per = RB / 16;
+            const int pos = x / per, at = x % per;
+            pa_v4u w = {t.v[n][0], t.v[n][1], t.v[n][2], t.v[n][3]};
             if (edge) {
                 uint32_t nf = 0;                             // bit 15 or 31 where an exponent is all ones
+                if (pos < lo || pos >= hi) w = pa_v4u{0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int pos = pm_pos(g, j);
-                    v[j] = pos < lo || pos >= hi ? 0u : v[j];
-                    nf |= (v[j] & 0x7c007c00u) + 0x04000400u;
-                }
+                for (int k = 0; k < 4; k++) nf |= (w[k] & 0x7c007c00u) + 0x04000400u;
                 if (nf & 0x80008000u) {
                     odd = true;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = pa_finite(v[j]);
+                    for (int k = 0; k < 4; k++) w[k] = pa_finite(w[k]);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int e = 2 * at + i;
-                pa_v4u w;
-#pragma unroll
-                for (int k = 0; k < 4; k++) w[k] = __builtin_amdgcn_perm(v[2 * k + 1], v[2 * k], i ? 0x07060302u : 0x05040100u);
-                *(pa_v4u *)d.v[e >> 4][16 * g + (e & 15)] = w;
-            }
+            *(pa_v4u *)(&d.v[0][0][0] + pos * (HD + 16) + 8 * at) = w;
         } else {
             // q8_0 bytes 4 at .. / q4_0 nibbles 4 at ..: c = 4 at / (HD / 16), tiles m0 .. m0 + 3, elements 16 m + c
-            constexpr int per16 = HD / 64;
-            const int c = at / per16, m0 = at % per16 * 4;
+            constexpr int per = HD / 4, per16 = HD / 64;
+            const int g = per % 64 == 0 ? pa_uniform(x / per) : x / per, at = x % per, c = at / per16, m0 = at % per16 * 4;
+            const uint32_t *v = t.v[n];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 pa_v4u w;
@@ -197,6 +192,13 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
     return odd;
 }
 
+typedef short pa_v4s __attribute__((ext_vector_type(4)));
+typedef short pa_v8s __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) pa_v4s *pa_lds4;
+__device__ __forceinline__ pa_v8h pm_turned(const _Float16 *a, const _Float16 *b) {
+    const pa_v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds4)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds4)b);
+    return __builtin_bit_cast(pa_v8h, pa_v8s{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w});
+}
 struct PmKey {
     pa_v8h x;
     uint2 d;
@@ -446,7 +448,9 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                 for (int k = 0; k < 4; k++) pa_split(w[2 * k], w[2 * k + 1], hi[k], lo[k]);
                 const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
                 pa_v8h before;                               // low halves one operand later
-                pm_pipeline<NM, AHEAD>([&](int e) { return *(const pa_v8h *)d.v[NM * ew + e][lane]; }, [&](int e, pa_v8h va) {
+                // 16 lanes give 4 positions of 16 elements and get 4 positions of their own
+                const _Float16 *const vt = &d.v[0][0][0] + (4 * g + (c >> 2)) * (HD + 16) + HE * ew + 4 * (c & 3);
+                pm_pipeline<NM, AHEAD>([&](int e) { return pm_turned(vt + 16 * e, vt + 16 * (HD + 16) + 16 * e); }, [&](int e, pa_v8h va) {
                     o[e] = pa_mma(va, b0, o[e]);
                     if (e) o[e - 1] = pa_mma(before, b1, o[e - 1]);
                     before = va;
