@@ -130,12 +130,20 @@ __device__ __forceinline__ uint32_t pa_q8(uint32_t x) {
     const pa_v2h k = {(_Float16)32768.0f, (_Float16)32768.0f}, c = {(_Float16)-0.25f, (_Float16)-0.25f};
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(pa_v2h, x), k, c));
 }
-// halves 1024 + (quant + 8) to quant, exactly
-__device__ __forceinline__ uint32_t pa_q4(uint32_t x) {
-    const pa_v2h c = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(pa_v2h, x) + c);
+// nibbles K (of 4) of both halves, quant + 8, to quant, exactly: bits 0..3 under the
+// exponent of 1024 are 1024 + x, bits 4..7 are 1024 + 16 x
+template <int K>
+__device__ __forceinline__ uint32_t pa_q4(uint32_t w) {
+    const uint32_t y = K < 2 ? w : w >> 8;
+    if constexpr (K % 2 == 0) {
+        const pa_v2h c = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(pa_v2h, (y & 0x000f000fu) | 0x64006400u) + c);
+    } else {
+        const pa_v2h k = {(_Float16)0.0625f, (_Float16)0.0625f}, c = {(_Float16)-72.0f, (_Float16)-72.0f};
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(pa_v2h, (y & 0x00f000f0u) | 0x64006400u), k, c));
+    }
 }
-__device__ __forceinline__ uint32_t pa_nib(uint32_t w, int k) { return ((w >> (4 * k)) & 0x000f000fu) | 0x64006400u; }
+__device__ __forceinline__ uint32_t pa_q4(uint32_t w, int k) { return k == 0 ? pa_q4<0>(w) : k == 1 ? pa_q4<1>(w) : k == 2 ? pa_q4<2>(w) : pa_q4<3>(w); }
 
 template <int N>
 __device__ __forceinline__ void pa_load(uint32_t *d, const uint8_t *p) {

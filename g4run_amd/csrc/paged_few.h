@@ -81,7 +81,7 @@ __device__ __forceinline__ pa_v8h pa_key(const PaTile<HE, KVT> &t, int h, int s)
                      pa_q8(__builtin_amdgcn_perm(0, b, 0x0c010c00u)), pa_q8(__builtin_amdgcn_perm(0, b, 0x0c030c02u)));
     } else {
         const uint32_t w = t.k[h][s];
-        return pa_op(pa_q4(pa_nib(w, 0)), pa_q4(pa_nib(w, 1)), pa_q4(pa_nib(w, 2)), pa_q4(pa_nib(w, 3)));
+        return pa_op(pa_q4<0>(w), pa_q4<1>(w), pa_q4<2>(w), pa_q4<3>(w));
     }
 }
 // value operand of the 16 elements m (pa_elem) over the 32 positions
@@ -97,8 +97,8 @@ __device__ __forceinline__ pa_v8h pa_value(const PaTile<HE, KVT> &t, int m) {
             const uint32_t b = m & 3;
             w[k] = pa_q8(__builtin_amdgcn_perm(t.v[2 * k + 1][m >> 2], t.v[2 * k][m >> 2], 0x0c000c00u | b | ((4 + b) << 16)));
         } else {
-            const int d = m >> 3, n = m & 3;
-            w[k] = pa_q4(__builtin_amdgcn_perm(pa_nib(t.v[2 * k + 1][d], n), pa_nib(t.v[2 * k][d], n), (m & 4) ? 0x07060302u : 0x05040100u));
+            const int d = m >> 3;
+            w[k] = pa_q4(__builtin_amdgcn_perm(t.v[2 * k + 1][d], t.v[2 * k][d], (m & 4) ? 0x07060302u : 0x05040100u), m & 3);
         }
     }
     return pa_op(w[0], w[1], w[2], w[3]);

@@ -130,7 +130,7 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
         } else {
             const int g4 = at / (HD / 32), s = at % (HD / 32);
             const uint32_t w = t.k[n][0];
-            *(pa_v4u *)&d.k[pos][32 * s + 8 * g4] = pa_v4u{pa_q4(pa_nib(w, 0)), pa_q4(pa_nib(w, 1)), pa_q4(pa_nib(w, 2)), pa_q4(pa_nib(w, 3))};
+            *(pa_v4u *)&d.k[pos][32 * s + 8 * g4] = pa_v4u{pa_q4<0>(w), pa_q4<1>(w), pa_q4<2>(w), pa_q4<3>(w)};
         }
     }
 #pragma unroll
@@ -166,7 +166,7 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
                     if constexpr (KVT == Q8_0)
                         w[k] = pa_q8(__builtin_amdgcn_perm(v[2 * k + 1], v[2 * k], 0x0c000c00u | i | ((4 + i) << 16)));
                     else
-                        w[k] = pa_q4(__builtin_amdgcn_perm(pa_nib(v[2 * k + 1], i), pa_nib(v[2 * k], i), 0x05040100u));
+                        w[k] = pa_q4(__builtin_amdgcn_perm(v[2 * k + 1], v[2 * k], 0x05040100u), i);
                 }
                 *(pa_v4u *)d.v[m0 + i][16 * g + c] = w;
             }
