@@ -429,11 +429,6 @@ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &p
     return s;
 }
 
-// lane N of the lane's 16
-template <int N>
-__device__ __forceinline__ float pa_lane16(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + N, 0xF, 0xF, false));    // row_newbcast
-}
 // max of unsigned halves; the biased exponent of a (positive) half as a float
 typedef unsigned short pa_v2s __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pa_pkmax(uint32_t x, uint32_t y) {
@@ -480,10 +475,10 @@ __device__ __forceinline__ void pa_store4(float *to, pa_v4f s) {
     else { d[0] = s[0]; d[1] = s[1]; d[2] = s[2]; d[3] = s[3]; }
 }
 
-// the few-row kernel's workgroups per CU: what its registers allow (quantized
-// pages' scales and conversions take more)
+// the few-row kernel's workgroups per CU: what its registers allow (3 of 8-bit
+// heads of 128 fit with 32 bytes of spills: 73 us for 70, more results to join)
 __host__ __device__ constexpr int pa_few_per_cu(int type, int hd, bool st) {
-    return hd == 64 ? (type == F16 ? 4 : 3) : type == F16 && hd == 128 && st ? 3 : 2;
+    return hd == 64 ? 4 : type == F16 && hd == 128 && st ? 3 : 2;
 }
 
 // launches of one cache type; the few-row variants hold 8 or 16 rows

@@ -29,9 +29,25 @@ struct PaTile {
     static constexpr int DW = HE / 64;                                                   // dwords of a row's scales
     uint32_t k[2][KVT == F16 ? HE / 8 : KW];   // [unit][dwords]
     uint32_t v[8][VW];                         // [position 4 t + i][dwords]
-    uint32_t dk[KVT == F16 ? 1 : 8][DW], dv[KVT == F16 ? 1 : 8][DW];
-    uint32_t de[KVT == F16 ? 1 : DW];          // value scales of position j = c % 8 of the lane group's 8
+    uint32_t sc[KVT == F16 ? 1 : DW];          // of position lane % 32, K's in lanes 0..31, V's in the others
 };
+// The scales through LDS: one load of the wave brings all 64 rows', where a lane
+// loading the 16 that it multiplies with took 17 of a step's 27 load instructions
+// (64 sequences of up to 4096 positions, 8 KV heads of 128, 8 bits: 73 us, now 70).
+template <int HE>
+struct PaScales {
+    uint32_t d[2][32][HE / 64];
+    float e[32];                               // pa_exponent of V's largest
+};
+
+template <int N>
+__device__ __forceinline__ void pa_read(uint32_t *d, const void *lds) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const pa_v4u x = ((const pa_v4u *)lds)[i / 4];
+        d[i] = x[0]; d[i + 1] = x[1]; d[i + 2] = x[2]; d[i + 3] = x[3];
+    }
+}
 
 template <int HD, int HE, int KVT>
 __device__ __forceinline__ void pa_load_k(PaTile<HE, KVT> &t, const PagedPool &p, const PaUnit u[2], int c, int g, int ew) {
@@ -44,10 +60,13 @@ __device__ __forceinline__ void pa_load_k(PaTile<HE, KVT> &t, const PagedPool &p
             for (int s = 0; s < HE / 32; s++) pa_load<4>(t.k[h] + 4 * s, row + 2 * HE * ew + 64 * s + 16 * g);
         } else {
             pa_load<T::KW>(t.k[h], row + 4 * T::KW * ((HD / HE) * g + ew));
-#pragma unroll
-            for (int i = 0; i < 4; i++) pa_load<T::DW>(t.dk[4 * h + i], p.k + u[h].sc + (4 * g + i) * (HD / 16) + (HE / 16) * ew);
         }
     }
+}
+template <int HD, int HE, int KVT>
+__device__ __forceinline__ void pa_load_scales(PaTile<HE, KVT> &t, const PagedPool &p, const PaUnit u[2], int lane, int ew) {
+    const uint8_t *pool = lane < 32 ? p.k : p.v;
+    pa_load<PaTile<HE, KVT>::DW>(t.sc, pool + ((lane & 16) ? u[1].sc : u[0].sc) + ((lane & 15) * (HD / 16) + (HE / 16) * ew));
 }
 template <int HD, int HE, int KVT>
 __device__ __forceinline__ void pa_load_v(PaTile<HE, KVT> &t, const PagedPool &p, const PaUnit u[2], int c, int g, int ew) {
@@ -66,9 +85,7 @@ __device__ __forceinline__ void pa_load_v(PaTile<HE, KVT> &t, const PagedPool &p
         } else {
             pa_load<T::VW>(t.v[j], row + 4 * T::VW * ((HD / HE) * c + ew));
         }
-        if constexpr (KVT != F16) pa_load<T::DW>(t.dv[j], p.v + u[j >> 2].sc + i * (HD / 16) + (HE / 16) * ew);
     }
-    if constexpr (KVT != F16) pa_load<T::DW>(t.de, p.v + ((c & 4) ? u[1].sc : u[0].sc) + (4 * g + (c & 3)) * (HD / 16) + (HE / 16) * ew);
 }
 
 // key operand of unit h, 32 elements s
@@ -118,6 +135,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
     __shared__ float qsc[R];
     __shared__ float2 wml[4][R];                             // two waves of one tile may differ in m (by their elements' scales)
     __shared__ __align__(16) float xs[ES > 1 ? 2 : 1][ES > 1 ? 4 : 1][ES > 1 ? 64 : 1][8];   // partial scores of the waves of one tile
+    __shared__ __align__(16) PaScales<HE> scl[KVT == F16 ? 1 : 4];           // of a wave
     _Float16 *const qh = (_Float16 *)lds;
     float *const buf = (float *)lds;
 
@@ -181,6 +199,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
             pa_check(p, us, bad);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
+            if constexpr (KVT != F16) pa_load_scales<HD, HE, KVT>(kv, p, nx, lane, ew);
             pa_load_k<HD, HE, KVT>(kv, p, nx, c, g, ew);
             pa_load_v<HD, HE, KVT>(kv, p, nx, c, g, ew);
         }
@@ -236,6 +255,22 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
             }
             if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units(p, x.table, (base >> 4) + 64 * PW, 2 * PW, last, kvh);
             const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
+            constexpr int DW = PaTile<HE, KVT>::DW;
+            uint32_t dk[8][DW], dv[8][DW];                   // of the lane's 8 positions
+            PaScales<HE> &sl = scl[KVT == F16 ? 0 : wave];
+            if constexpr (KVT != F16) {
+                // a wave's LDS accesses complete in order
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int d = 0; d < DW; d++) sl.d[lane >> 5][lane & 31][d] = kv.sc[d];
+                uint32_t dm = kv.sc[0] & 0x7fff7fffu;
+#pragma unroll
+                for (int d = 1; d < DW; d++) dm = pa_pkmax(dm, kv.sc[d] & 0x7fff7fffu);
+                if (lane >= 32) sl.e[lane & 31] = pa_exponent(max(dm << 16, dm), 1);
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int h = 0; h < 2; h++) pa_read<4 * DW>(dk[4 * h], sl.d[0][16 * h + 4 * g]);
+            }
             // scores at positions base + 16 h + 4 g + i
             pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -250,12 +285,15 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                         pa_v4f d = pa_mma(ko, qa[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f});
                         if constexpr (!ST) d = pa_mma(ko, qb[s], d);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) sc[h][i] = __builtin_fmaf(pa_scale(kv.dk[4 * h + i], s), d[i], sc[h][i]);
+                        for (int i = 0; i < 4; i++) sc[h][i] = __builtin_fmaf(pa_scale(dk[4 * h + i], s), d[i], sc[h][i]);
                     }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);               // the next keys go where these were
-            if (more) pa_load_k<HD, HE, KVT>(kv, p, nx, c, g, ew);
+            if (more) {
+                if constexpr (KVT != F16) pa_load_scales<HD, HE, KVT>(kv, p, nx, lane, ew);
+                pa_load_k<HD, HE, KVT>(kv, p, nx, c, g, ew);
+            }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (ES > 1) {
                 *(pa_v4f *)xs[it & 1][wave][lane] = sc[0];
@@ -306,14 +344,12 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
 #pragma unroll
                 for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j]);
             } else {
-                // + the exponent of the position's largest value scale, found by one
-                // lane of eight for each position
-                uint32_t dm = kv.de[0] & 0x7fff7fffu;
+                // + the exponent of the position's largest value scale
+                const pa_v4f e[2] = {*(const pa_v4f *)&sl.e[4 * g], *(const pa_v4f *)&sl.e[16 + 4 * g]};
 #pragma unroll
-                for (int d = 1; d < HE / 64; d++) dm = pa_pkmax(dm, kv.de[d] & 0x7fff7fffu);
-                const float e = pa_exponent(max(dm << 16, dm), 1);
-                mt = fmaxf(fmaxf(fmaxf(w[0] + pa_lane16<0>(e), w[1] + pa_lane16<1>(e)), fmaxf(w[2] + pa_lane16<2>(e), w[3] + pa_lane16<3>(e))),
-                           fmaxf(fmaxf(w[4] + pa_lane16<4>(e), w[5] + pa_lane16<5>(e)), fmaxf(w[6] + pa_lane16<6>(e), w[7] + pa_lane16<7>(e))));
+                for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j] + e[j >> 2][j & 3]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) pa_read<4 * DW>(dv[4 * h], sl.d[1][16 * h + 4 * g]);
             }
             mt = fmaxf(mt, partner<16>(mt));
             mt = fmaxf(mt, partner<32>(mt));
@@ -378,7 +414,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                     for (int j = 0; j < 8; j++) {
                         const uint32_t live = w[j] == 0.0f ? 0u : ~0u;
 #pragma unroll
-                        for (int d = 0; d < HE / 64; d++) kv.dv[j][d] &= live;
+                        for (int d = 0; d < DW; d++) dv[j][d] &= live;
                     }
                 }
 #pragma unroll
@@ -386,7 +422,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                     uint32_t ph[4], pq[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const float y = __builtin_fmaf(pa_scale(kv.dv[2 * k], s), w[2 * k], 0.0f), z = __builtin_fmaf(pa_scale(kv.dv[2 * k + 1], s), w[2 * k + 1], 0.0f);
+                        const float y = __builtin_fmaf(pa_scale(dv[2 * k], s), w[2 * k], 0.0f), z = __builtin_fmaf(pa_scale(dv[2 * k + 1], s), w[2 * k + 1], 0.0f);
                         if constexpr (ST) ph[k] = pa_half(y, z, part);
                         else pa_split(y, z, ph[k], pq[k]);
                     }
