@@ -26,13 +26,18 @@ constexpr int PM_THREADS = 512;
 // of a wave's scores and of the second product's operand.
 __device__ __forceinline__ int pm_pos(int g, int j) { return 16 * (j >> 2) + 4 * g + (j & 3); }
 
-// LDS of 32 positions: K [32][HD + 8] halves; V [32][HD + 16] halves, read
+// Where 8 elements of a K row lie in LDS: unit g of elements 32 s, row c of 16.  Rows
+// are moved about by (s, g), so that neither the 16 lanes that write one row's units
+// nor those that read 16 rows' meet in a bank.
+__device__ __forceinline__ int pm_key(int c, int g, int s) { return 16 * g + (c ^ g ^ (4 * (s & 3))); }
+
+// LDS of 32 positions: K as operands [2 s + half][64 units of 8 halves] (pm_key); V [32][HD + 16] halves, read
 // transposed (ds_read_b64_tr_b16), quantized V [HD / 16][64 lanes][8] as operands;
 // the scales [HD / 32][32] of K and of V, and each position's pa_exponent of its
 // largest V scale (quantized)
 template <int HD, int KVT>
 struct PmTile {
-    _Float16 k[32][HD + 8];
+    _Float16 k[HD / 16][64][8];
     _Float16 v[KVT == F16 ? 32 * (HD + 16) / 512 : HD / 16][64][8];
     uint16_t dk[KVT == F16 ? 1 : HD / 32][32], dv[KVT == F16 ? 1 : HD / 32][32];
     float ev[KVT == F16 ? 4 : 32];
@@ -115,7 +120,7 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
         constexpr int per = RB / (4 * T::KD);
         const int pos = x / per, at = x % per;
         if constexpr (KVT == F16) {
-            *(pa_v4u *)&d.k[pos][8 * at] = pa_v4u{t.k[n][0], t.k[n][1], t.k[n][2], t.k[n][3]};
+            *(pa_v4u *)d.k[2 * (at >> 2) + (pos >> 4)][pm_key(pos & 15, at & 3, at >> 2)] = pa_v4u{t.k[n][0], t.k[n][1], t.k[n][2], t.k[n][3]};
         } else if constexpr (KVT == Q8_0) {
             // bytes 16 at ..: group g4 = 16 at / (HD / 4), elements 32 s + 8 g4 + j of two s
             constexpr int G4 = HD / 64;                      // runs of a group
@@ -123,14 +128,14 @@ __device__ __forceinline__ bool pm_store(PmTile<HD, KVT> &d, const PmStage<HD, K
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 const uint32_t a = t.k[n][2 * s], b = t.k[n][2 * s + 1];
-                *(pa_v4u *)&d.k[pos][32 * (s0 + s) + 8 * g4] =
+                *(pa_v4u *)d.k[2 * (s0 + s) + (pos >> 4)][pm_key(pos & 15, g4, s0 + s)] =
                     pa_v4u{pa_q8(__builtin_amdgcn_perm(0, a, 0x0c010c00u)), pa_q8(__builtin_amdgcn_perm(0, a, 0x0c030c02u)),
                            pa_q8(__builtin_amdgcn_perm(0, b, 0x0c010c00u)), pa_q8(__builtin_amdgcn_perm(0, b, 0x0c030c02u))};
             }
         } else {
             const int g4 = at / (HD / 32), s = at % (HD / 32);
             const uint32_t w = t.k[n][0];
-            *(pa_v4u *)&d.k[pos][32 * s + 8 * g4] = pa_v4u{pa_q4<0>(w), pa_q4<1>(w), pa_q4<2>(w), pa_q4<3>(w)};
+            *(pa_v4u *)d.k[2 * s + (pos >> 4)][pm_key(pos & 15, g4, s)] = pa_v4u{pa_q4<0>(w), pa_q4<1>(w), pa_q4<2>(w), pa_q4<3>(w)};
         }
     }
 #pragma unroll
@@ -370,7 +375,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             // scores of row c at positions base + pm_pos(g, j): high and low halves apart,
             // so that no instruction waits for the one before it
             pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}, s2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-            auto key = [&](int i) { return *(const pa_v8h *)&d.k[16 * (i & 1) + c][HE * ew + 32 * (i >> 1) + 8 * g]; };
+            auto key = [&](int i) { return *(const pa_v8h *)d.k[2 * NS * ew + i][pm_key(c, g, i >> 1)]; };
             if constexpr (KVT == F16) {
                 pm_pipeline<2 * NS, AHEAD>(key, [&](int i, pa_v8h ko) {
                     sc[i & 1] = pa_mma(ko, q0[i >> 1], sc[i & 1]);
