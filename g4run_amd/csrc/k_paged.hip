@@ -26,7 +26,9 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     many.toks_inv = 0;
     // Sequences of at most few.rows rows are the few-row kernel's: 8 (one matrix
     // instruction per operand) where no sequence can have more, else 16.
-    few.rows = grp > 16 ? 0 : (b.q_off ? rows : grp) <= 8 ? 8 : 16;
+    // None where sequences have 64 tokens on average: the other kernel then takes the
+    // short ones among them too, and a launch is saved (four prompts: 82 -> 77 us).
+    few.rows = grp > 16 || (b.q_off && b.n_tok >= 64 * (int64_t)b.n_seq) ? 0 : (b.q_off ? rows : grp) <= 8 ? 8 : 16;
     if (b.n_prefix && few.rows == 8 && rows > 8 && rows <= 16) few.rows = 16;
     few.toks = few.rows / grp;
     const bool few_pre = b.n_prefix && few.rows && rows <= few.rows;

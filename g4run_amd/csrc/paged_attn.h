@@ -439,12 +439,6 @@ __device__ __forceinline__ float pa_exponent(uint32_t h, int which) { return (fl
 // over s + the biased exponent (15 more than the exponent).
 template <int KVT>
 __device__ __forceinline__ constexpr float pa_shift_of() { return KVT == F16 ? PA_SHIFT : PA_SHIFT + 14.0f; }
-// two weights times two halves' scales, split
-__device__ __forceinline__ void pa_split_scaled(float u, float v, uint32_t d, uint32_t &hi, uint32_t &lo) {
-    const float x = __builtin_fmaf(pa_lo(d), u, 0.0f), y = __builtin_fmaf(pa_hi(d), v, 0.0f);
-    hi = pa_pk(x, y);
-    lo = pa_pk(__builtin_fmaf(pa_lo(hi), -1.0f, x), __builtin_fmaf(pa_hi(hi), -1.0f, y));
-}
 // two halves, those that are not finite as 0
 __device__ __forceinline__ uint32_t pa_finite(uint32_t x) {
     x = (x & 0x7c00u) == 0x7c00u ? x & 0xffff0000u : x;
@@ -456,8 +450,15 @@ __device__ __forceinline__ int pa_shift(float am) {
     return am > 0.0f && am < __builtin_inff() ? min(max(15 - __builtin_amdgcn_frexp_expf(am), -126), 126) : 0;
 }
 __device__ __forceinline__ void pa_split(float u, float v, uint32_t &hi, uint32_t &lo) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));                                   // or a conversion and a subtraction each
     hi = pa_pk(u, v);
-    lo = pa_pk(__builtin_fmaf(pa_lo(hi), -1.0f, u), __builtin_fmaf(pa_hi(hi), -1.0f, v));
+    lo = pa_pk(__builtin_fmaf(pa_lo(hi), minus, u), __builtin_fmaf(pa_hi(hi), minus, v));
+}
+// two weights times two halves' scales, split
+__device__ __forceinline__ void pa_split_scaled(float u, float v, uint32_t d, uint32_t &hi, uint32_t &lo) {
+    const float x = __builtin_fmaf(pa_lo(d), u, 0.0f), y = __builtin_fmaf(pa_hi(d), v, 0.0f);
+    pa_split(x, y, hi, lo);
 }
 // the high half of both where part is 0, the low half where it is -1
 __device__ __forceinline__ uint32_t pa_half(float u, float v, float part) {

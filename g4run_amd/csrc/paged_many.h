@@ -239,7 +239,7 @@ constexpr int PM_COLS = 36, PM_TR = 16 * PM_COLS;
 
 template <int HD, int KVT>
 __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(PagedCall call) {
-    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2, AHEAD = HD > 64 ? 4 : 2, BLOCKS = HD > 64 ? 2 : 1;    // NB: buffers
+    constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2, AHEAD = HD == 64 || HD == 512 ? 2 : 4, BLOCKS = HD > 64 ? 2 : 1;    // NB: buffers
     constexpr size_t TB = sizeof(PmTile<HD, KVT>) * NB, RB = (size_t)8 * PM_TR * 4;
     __shared__ __align__(16) uint8_t lds[TB > RB ? TB : RB]; // the tiles; before and after them rows on their way
     __shared__ __align__(16) float xs[ES > 1 ? 8 : 1][ES > 1 ? 64 : 1][8];   // partial scores of wave pairs
