@@ -1040,9 +1040,9 @@ extern "C" int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *bat
 
 static int check_paged_heads(const char *fn, const PagedPool &p, const PagedBatch &b, int n_head) {
     if (n_head < 1 || n_head % p.n_kv) return fail(G4H_ERR_SHAPE, "%s: n_head=%d not a multiple of n_kv=%d", fn, n_head, p.n_kv);
+    if ((int64_t)b.n_tok * n_head > 1 << 24) return fail(G4H_ERR_ARG, "%s: n_tok * n_head = %lld (up to 2^24)", fn, (long long)b.n_tok * n_head);
     if (n_head / p.n_kv > paged_most_group(p.hd))
         return fail(G4H_ERR_SHAPE, "%s: %d query heads per KV head (up to %d)", fn, n_head / p.n_kv, paged_most_group(p.hd));
-    if ((int64_t)b.n_tok * n_head > 1 << 24) return fail(G4H_ERR_ARG, "%s: n_tok * n_head = %lld (up to 2^24)", fn, (long long)b.n_tok * n_head);
     return G4H_OK;
 }
 extern "C" size_t g4h_paged_attn_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head) {

@@ -412,7 +412,8 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                 if (edge) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const uint32_t live = w[j] == 0.0f ? 0u : ~0u;
+                        const int pos = base + 16 * (j >> 2) + 4 * g + (j & 3);
+                        const uint32_t live = pos >= rlo && pos <= rhi && pos < end ? ~0u : 0u;
 #pragma unroll
                         for (int d = 0; d < DW; d++) dv[j][d] &= live;
                     }

@@ -491,7 +491,10 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                 uint32_t live[4] = {~0u, ~0u, ~0u, ~0u};
                 if (edge) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) live[k] = (w[2 * k] == 0.0f ? 0u : 0xffffu) | (w[2 * k + 1] == 0.0f ? 0u : 0xffff0000u);
+                    for (int j = 0; j < 8; j++) {
+                        const int pos = base + pm_pos(g, j);
+                        if (!(pos >= rlo && pos <= rhi && pos < end)) live[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
+                    }
                 }
                 // blocks of 32 elements: value tiles 2 s, 2 s + 1
                 pm_pipeline<NS, BLOCKS>([&](int s) {

@@ -115,7 +115,11 @@ def attend(q, keys, vals, pos, scale, cap=0.0, window=0):
     exponential (2^-22 of the score and 2^-22), tanh (cap 2^-21), the weighted
     sum over n positions (n 2^-24 at worst, here 2^-18, far above what n random
     roundings give) -- a score off by d moves a weight by d (1 + d), numerator
-    and denominator both."""
+    and denominator both.  A weight's low half has steps of 2^-24, of 2^6 for the
+    row's largest weight (quantized: of weight times scale, against the largest
+    such product and its scale's power of two, so at most 2 more): what lies
+    below 2^-30 of the largest is cut, 2^-29 of it from each of n positions, times
+    a value of at most the largest."""
     lo = max(0, pos + 1 - window) if window else 0
     if pos < 0:
         return np.zeros_like(q, dtype=np.float64), np.zeros(len(q))
@@ -129,7 +133,8 @@ def attend(q, keys, vals, pos, scale, cap=0.0, window=0):
         w = np.exp(s - s.max())
         out = (w[:, None] * v).sum(0) / w.sum()
         mag = (w[:, None] * np.abs(v)).sum(0) / w.sum()
-    return out, (2 * d + 2.0 ** -18) * mag + 1e-30
+        cut = 2.0 ** -29 * len(v) * np.abs(v).max() * w.max() / w.sum()
+    return out, (2 * d + 2.0 ** -18) * mag + cut + 1e-30
 
 
 class Case:

@@ -32,6 +32,63 @@ def test_prompts(gpu, t, hd, n_head, n_kv, new, lens):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("n_prefix,window", [(0, 0), (0, 50), (70, 0), (70, 90)])
+def test_prompts_of_64_tokens_on_average(gpu, t, hd, n_prefix, window):
+    # one kernel takes them all, single tokens and empty sequences too
+    Case(gpu, t, 2, 1, hd, 16, [230, 300, 0, 60], new=[200, 1, 0, 60], pad=1, n_prefix=n_prefix, seed=hd).check(window=window, cap=30.0 if window else 0.0)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd,heads", [(64, 128), (64, 127), (128, 128), (256, 128), (512, 64), (512, 33)])
+@pytest.mark.parametrize("n_prefix", [0, 40])
+def test_most_heads_of_one_kv_head(gpu, t, hd, heads, n_prefix):
+    Case(gpu, t, heads, 1, hd, 16, [70, 1, 300], n_prefix=n_prefix, seed=heads).check()
+    Case(gpu, t, heads, 1, hd, 16, [40, 3], new=[3, 1], n_prefix=n_prefix, seed=heads).check()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd,n_kv,n_seq,longest", [(64, 4, 300, 500), (128, 2, 200, 900), (256, 2, 150, 600), (512, 1, 150, 400)])
+def test_more_steps_than_workgroups(gpu, t, hd, n_kv, n_seq, longest):
+    # shares that hold several short tiles, begin inside one, or end where one begins
+    lens = np.random.default_rng(n_seq).integers(0, longest, n_seq)
+    lens[::7] = np.arange(len(lens[::7])) % 40
+    Case(gpu, t, n_kv, n_kv, hd, 16, [int(n) for n in lens], seed=hd).check()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_more_steps_of_prompts_than_workgroups(gpu, t, hd):
+    rng = np.random.default_rng(hd)
+    new = [int(n) for n in rng.integers(0, 90, 24)]
+    lens = [n + int(m) for n, m in zip(new, rng.integers(0, 500, 24))]
+    Case(gpu, t, 6 if hd < 512 else 4, 2, hd, 16, lens, new=new, seed=hd).check()
+
+
+@pytest.mark.parametrize("t", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("new", [[1, 1], [40, 30]])
+def test_bad_scales_reach_only_their_readers(gpu, t, new):
+    # an infinite scale of a value far below the row's largest weight: 0 x inf, as in the formula
+    c = Case(gpu, t, 2, 1, 64, 16, [80, 37], new=new, spread=30.0, seed=41)
+    clean, tol = c.expect(1.0, window=24)
+    n = U.row_bytes(t, 64)
+    where = ((0, 60), (1, 20))
+    for seq, pos in where:
+        at = c.page * n + (pos % 16) * 4
+        c.pool.v[c.table[seq, pos // 16], at:at + 2] = np.asarray([np.inf], np.float16).view(np.uint8)
+    c.kv.v.upload(c.pool.v)
+    got = c.attn(1.0, window=24).astype(np.float64)
+    for seq, pos in where:
+        for i in range(c.new[seq]):
+            own, r = c.lens[seq] - c.new[seq] + i, c.off[seq] + i
+            if own - 24 < pos <= own:
+                assert not np.isfinite(got[r, :, :32]).any(), (seq, i)
+                assert np.all(np.abs(got[r, :, 32:] - clean[r, :, 32:]) <= tol[r, :, 32:])
+            else:
+                assert np.all(np.abs(got[r] - clean[r]) <= tol[r]), (seq, i)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
 @pytest.mark.parametrize("window", [1, 5, 31, 32, 100, 1000])
 @pytest.mark.parametrize("new", [[1, 1, 1], [20, 7, 33]])
 def test_window(gpu, t, window, new):
@@ -234,6 +291,26 @@ def test_graph_replays_with_other_lengths(gpu, t, n_prefix):
         eager = c.attn(0.125)
         assert np.array_equal(eager, got), step
     assert c.kv.status() == 0
+
+
+def test_two_graphs_over_one_workspace(gpu):
+    """A decode call and a call of prompts, captured apart over one workspace,
+    replayed one after the other; what the other left in it changes nothing."""
+    G = gpu
+    a = Case(G, F16, 8, 2, 128, 16, [400, 33, 0, 250], n_prefix=100, seed=18)
+    b = Case(G, Q8_0, 8, 2, 64, 16, [300, 290, 7], new=[150, 30, 7], pad=2, seed=19)
+    s = G.Stream()
+    ws = G.Buffer(max(G.paged_attn_workspace_bytes(c.kv, c.batch, 8) for c in (a, b)))
+    ws.upload(np.full(ws.nbytes, 0xff, np.uint8))
+    outs = [G.Buffer.from_array(np.full((c.n_tok, 8, c.hd), 7.5, np.float32)) for c in (a, b)]
+    gs = [G.Graph(s.ptr, lambda c=c, o=o: G.paged_attn(c.kv, c.batch, c.d["q"], 8, o, scale=0.1, ws=ws, stream=s.ptr)) for c, o in zip((a, b), outs)]
+    want = [c.expect(0.1) for c in (a, b)]
+    for turn in range(4):
+        for k in ((0, 1), (1, 0))[turn & 1]:
+            gs[k].launch(s.ptr)
+            s.synchronize()
+            got = outs[k].download(np.float32, want[k][0].shape)
+            assert np.all(np.abs(got - want[k][0]) <= want[k][1]), (turn, k)
 
 
 def test_streams_run_side_by_side(gpu):

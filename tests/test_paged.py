@@ -126,6 +126,16 @@ def test_refused_attention(abi):
     _expect(G, _attn(L, kv, _batch(G, n_prefix=5)), "ERR_ARG")
 
 
+@pytest.mark.parametrize("hd,most", [(64, 128), (128, 128), (256, 128), (512, 64)])
+def test_refused_head_groups(abi, hd, most):
+    G, L = abi
+    kv, b = _kv(G, hd=hd, n_kv=1), _batch(G)
+    assert L.g4h_paged_attn_workspace_bytes(C.byref(kv), C.byref(b), most + 1) == 0
+    _expect(G, _attn(L, kv, b, n_head=most + 1), "ERR_SHAPE")
+    if not G._inited:
+        assert _attn(L, kv, b, n_head=most) == G.ERR_DEVICE
+
+
 def test_workspace_bytes(abi):
     G, L = abi
     size = lambda kv, b, h: L.g4h_paged_attn_workspace_bytes(C.byref(kv), C.byref(b), h)  # noqa: E731
