@@ -1061,7 +1061,9 @@ extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *bat
     const size_t row = (size_t)n_head * a.p.hd;
     if (int rc = paged_rows(fn, "q", q, q_stride, row, a.b.n_tok)) return rc;
     if (int rc = paged_rows(fn, "out", out, out_stride, row, a.b.n_tok)) return rc;
-    if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f || window < 0)
+    // scores are taken in log2 units and for 8-bit pages by 512 times the scale
+    const bool cap_ok = softcap == 0.0f || (softcap >= 0x1p-100f && softcap <= 0x1p100f);
+    if (!cap_ok || !std::isfinite(scale * 1024.0f) || (softcap && !std::isfinite(scale * 1024.0f / softcap)) || window < 0)
         return fail(G4H_ERR_ARG, "%s: scale=%g softcap=%g window=%d", fn, scale, softcap, window);
     if (a.b.n_prefix && !a.b.prefix) return fail(G4H_ERR_ARG, "%s: a prefix of %d positions needs its pages", fn, a.b.n_prefix);
     if (a.b.n_tok) {

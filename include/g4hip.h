@@ -352,6 +352,8 @@ int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out
  * window) .. p (window 0: 0 .. p):
  *   s_j = scale * q . k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);
  *   out = sum_j softmax(s)_j v_j, zeros for a token without a position.
+ * softcap is 0 or within 2^-100 .. 2^100, and 1024 scale (1024 scale / softcap)
+ * finite.
  * q / out: fp32 [n_tok][n_head][hd], at q_stride / out_stride floats per token
  * (0: packed); query head h reads KV head h / (n_head / n_kv), up to 128 heads a
  * KV head (64 of hd 512).  All in fp32

@@ -126,6 +126,16 @@ def test_refused_attention(abi):
     _expect(G, _attn(L, kv, _batch(G, n_prefix=5)), "ERR_ARG")
 
 
+def test_refused_scales(abi):
+    G, L = abi
+    kv, b = _kv(G), _batch(G)
+    for kw in [dict(cap=2.0 ** -101), dict(cap=2.0 ** 101), dict(scale=2.0 ** 120), dict(scale=-2.0 ** 30, cap=2.0 ** -99), dict(cap=float("nan"))]:
+        _expect(G, _attn(L, kv, b, **kw), "ERR_ARG")
+    if not G._inited:
+        for kw in [dict(cap=2.0 ** -100), dict(cap=2.0 ** 100), dict(scale=-2.0 ** 110), dict(scale=0.0)]:
+            assert _attn(L, kv, b, **kw) == G.ERR_DEVICE
+
+
 @pytest.mark.parametrize("hd,most", [(64, 128), (128, 128), (256, 128), (512, 64)])
 def test_refused_head_groups(abi, hd, most):
     G, L = abi
