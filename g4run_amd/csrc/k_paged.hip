@@ -102,7 +102,7 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
 // over the row's partial results in a fixed order, by groups of hd / 4 threads.
 // SPLIT: a workgroup per row, each group every so-many-th of its results (few rows
 // of many pieces); else a group per row (many rows of few: a workgroup's one active
-// group left the chip empty, 9000 rows of 256 took 18 us).  Bound by the latency of
+// group left the chip empty, 9000 rows of 256 took 18 us, now 11.4).  Bound by the latency of
 // reads that depend on each other, so: the row's sequence by one load of the whole
 // wave, four results' maxima and sums at once under a running maximum.
 template <bool SPLIT>
