@@ -78,16 +78,19 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedPool &p, const PagedBat
 }
 
 // The sequence of token t, found by one wave together: the last s with
-// q_off[s] <= t, 64 offsets at a time; n_seq when t is behind all of them.
+// q_off[s] <= t, by 64 offsets at a time (4096 sequences: two reads); n_seq when t
+// is behind all of them.
 __device__ __forceinline__ int paged_find(const PagedBatch &b, int t) {
     if (!b.q_off) return t < b.n_seq ? t : b.n_seq;
     const int lane = threadIdx.x & 63;
-    int n = 0;
-    for (int s0 = 1; s0 <= b.n_seq; s0 += 64) {
-        const int s = s0 + lane;
-        n += __popcll(__ballot(s <= b.n_seq && paged_ld(b.q_off, s) <= t));
+    int lo = 0, hi = b.n_seq;                                // it is one of lo .. hi
+    while (hi - lo > 64) {
+        const int step = (hi - lo + 63) >> 6, s = lo + (lane + 1) * step;
+        lo += step * __popcll(__ballot(s <= hi && paged_ld(b.q_off, min(s, hi)) <= t));
+        hi = min(hi, lo + step - 1);
     }
-    return n;
+    const int s = lo + 1 + lane;
+    return lo + __popcll(__ballot(s <= hi && paged_ld(b.q_off, min(s, hi)) <= t));
 }
 
 struct PagedAppend {

@@ -304,25 +304,29 @@ __device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl,
     n = pa_uniform(group_isum<64>(n));
     return (n + y.pre_tiles * y.pre_steps) * a.p.n_kv;
 }
-// the sequence whose steps hold step u (counted without the prefix's) and the
-// number of steps before it
+// The sequence whose steps hold step u (counted without the prefix's) and the
+// number of steps before it.  A workgroup asks for ascending u: the search goes on
+// from the 64 sequences where the last one ended.
+struct PaFind {
+    int s0 = 0, before = 0;
+};
 template <bool MANY>
-__device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan &pl, int mine, int u, int &seq, int &before) {
+__device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan &pl, int mine, int u, PaFind &from, int &seq, int &before) {
     const int lane = threadIdx.x & 63;
-    before = 0;
-    for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
-        const int n = (s0 == 0 ? mine : s0 + lane < a.b.n_seq ? pa_steps<MANY>(a, pl, s0 + lane) : 0) * a.p.n_kv;
+    for (; from.s0 < a.b.n_seq; from.s0 += 64) {
+        const int n = (from.s0 == 0 ? mine : from.s0 + lane < a.b.n_seq ? pa_steps<MANY>(a, pl, from.s0 + lane) : 0) * a.p.n_kv;
         const int incl = pa_scan(n);
-        const uint64_t past = __ballot(before + incl > u);
+        const uint64_t past = __ballot(from.before + incl > u);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
-            seq = s0 + l;
-            before += __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l);
+            seq = from.s0 + l;
+            before = from.before + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l);
             return;
         }
-        before += __builtin_amdgcn_readlane(incl, 63);
+        from.before += __builtin_amdgcn_readlane(incl, 63);
     }
     seq = a.b.n_seq;
+    before = from.before;
 }
 __device__ __forceinline__ int pa_share(const PagedList &y, int total) { return max(y.least, (total + y.wgs - 1) / y.wgs); }
 
@@ -340,7 +344,7 @@ struct PaPiece {
 };
 // the piece at step u of a share [first, stop)
 template <bool MANY>
-__device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, int wg, int u, int first, int stop) {
+__device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, PaFind &from, int wg, int u, int first, int stop) {
     const PagedList &y = pa_list<MANY>(pl);
     const PagedBatch &b = a.b;
     PaPiece x;
@@ -364,7 +368,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
     } else {
         lead = y.lead;
         int seq, before;
-        pa_find_step<MANY>(a, pl, mine, u - pre_all, seq, before);
+        pa_find_step<MANY>(a, pl, mine, u - pre_all, from, seq, before);
         x.sq = paged_seq(a.p, b, seq);
         v = u - pre_all - before;
         if constexpr (MANY) {

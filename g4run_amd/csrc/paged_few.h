@@ -147,6 +147,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
     int mine;
     const int total = pa_total<false>(call.a, call.pl, mine), share = pa_share(call.pl.few, total);
     const int first = blockIdx.x * share, stop = min(first + share, total);
+    PaFind from;
     for (int u = first; u < stop;) {
         const PagedCall call = pa_fresh();
         const PagedAttn &a = call.a;
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         const PagedBatch &b = a.b;
         const int tid = pa_thread(), lane = tid & 63, wave = pa_uniform(tid >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, pw = wave / ES;
         const int G = a.grp, rc = ST ? c & 7 : c;
-        const PaPiece x = pa_piece<false>(a, pl, mine, blockIdx.x, u, first, stop);
+        const PaPiece x = pa_piece<false>(a, pl, mine, from, blockIdx.x, u, first, stop);
         u += x.took;
         if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;

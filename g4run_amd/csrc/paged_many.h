@@ -262,6 +262,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
     int mine;
     const int total = pa_total<true>(call.a, call.pl, mine), share = pa_share(call.pl.many, total);
     const int first = wg * share, stop = wg < call.pl.many.wgs ? min(first + share, total) : 0;
+    PaFind from;
     for (int u = first; u < stop;) {
         const PagedCall call = pa_fresh();
         const PagedAttn &a = call.a;
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         const int G = a.grp, R = pl.many.rows;
         float *const tr = (float *)lds + wave * PM_TR;
         const float capl = a.cap * 1.4426950408889634f;
-        const PaPiece x = pa_piece<true>(a, pl, mine, wg, u, first, stop);
+        const PaPiece x = pa_piece<true>(a, pl, mine, from, wg, u, first, stop);
         u += x.took;
         if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;

@@ -135,6 +135,26 @@ def test_many_sequences(gpu):
     Case(gpu, F16, 2, 1, 64, 16, [v + i % 9 for i, v in enumerate(new)], new=new, pad=5, seed=6).check()
 
 
+@pytest.mark.parametrize("n", [65, 4097, 4700])
+def test_thousands_of_sequences(gpu, n):
+    # offsets searched in two and three levels, workgroups that pass many sequences
+    new = [(i * 5) % 3 for i in range(n)]
+    c = Case(gpu, F16, 1, 1, 64, 16, [v + i % 17 for i, v in enumerate(new)], new=new, pad=3, seed=n)
+    c.check()
+    k, v, q = _append(c, gpu, 64)
+    _check_append(c, gpu, k, v, q, 64)
+    Case(gpu, F16, 1, 1, 64, 16, [i % 19 for i in range(n)], n_prefix=20, seed=n).check()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+@pytest.mark.parametrize("new", [None, [40, 30, 1]])
+def test_scales_of_any_sign(gpu, t, scale, new):
+    c = Case(gpu, t, 4, 2, 64, 16, [70, 33, 5], new=new, seed=42)
+    c.check(scale=scale)
+    c.check(scale=scale, cap=4.0, window=20)
+
+
 @pytest.mark.parametrize("spread", [1e-4, 300.0])
 def test_magnitudes(gpu, spread):
     # queries and keys far from 1; one key takes all the weight at 300
