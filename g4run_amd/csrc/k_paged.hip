@@ -99,17 +99,19 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
 }
 
 // One (token, head) row: out = sum of exp2(m_k - M) O_k / sum of exp2(m_k - M) l_k
-// over the row's partial results in a fixed order, by groups of hd / 4 threads.
-// SPLIT: a workgroup per row, each group every so-many-th of its results (few rows
-// of many pieces); else a group per row (many rows of few: a workgroup's one active
-// group left the chip empty, 9000 rows of 256 took 18 us, now 11.4).  Bound by the latency of
-// reads that depend on each other, so: the row's sequence by one load of the whole
-// wave, four results' maxima and sums at once under a running maximum.
+// over the row's partial results in a fixed order.  SPLIT: a workgroup per row, or
+// per row and 64 elements where those are few (36 rows of 512 from 250 pieces: 36 us,
+// 9.6 so; 512 rows of 512 from a few: 7.0 us, 11.5 so), its groups of threads every
+// so-many-th result; else a group of hd / 4 threads per row (many rows of few: a
+// workgroup's one active group left the chip empty, 9000 rows of 256 took 18 us, now
+// 11.4).  Bound by the latency of reads that depend on each other, so: the row's
+// sequence by one load of the whole wave, four results' maxima and sums at once
+// under a running maximum.
 template <bool SPLIT>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
-    __shared__ float2 ml_of[SPLIT ? 16 : 1];                 // at most 16 groups: hd >= 64
+    __shared__ float2 ml_of[SPLIT ? 16 : 1];                 // groups: of 16 threads at least
     __shared__ pa_v4f part[SPLIT ? 256 : 1];
-    const int hd = a.p.hd, hd4 = hd / 4, groups = 256 / hd4, gi = threadIdx.x / hd4, e4 = threadIdx.x % hd4 * 4;
+    const int hd = a.p.hd, hd4 = hd / 4 / (SPLIT ? gridDim.y : 1), groups = 256 / hd4, gi = threadIdx.x / hd4, e4 = 4 * (threadIdx.x % hd4 + (SPLIT ? hd4 * blockIdx.y : 0));
     const int all = a.b.n_tok * a.n_head, mine = SPLIT ? (int)blockIdx.x : (int)blockIdx.x * groups + gi, row = min(mine, all - 1);   // up to 2^24
     const int tok = row / a.n_head, head = row - tok * a.n_head;
     const uint2 own = pl.own[row], pre = a.b.n_prefix > 0 ? pl.pre[row] : make_uint2(0, 0);      // of a row without a sequence: not used
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
     }
     if constexpr (SPLIT) {
         part[threadIdx.x] = s;
-        if (e4 == 0) ml_of[gi] = make_float2(m, l);
+        if (threadIdx.x % hd4 == 0) ml_of[gi] = make_float2(m, l);
         __syncthreads();
         if (gi) return;
         for (int k = 0; k < groups; k++) m = fmaxf(m, ml_of[k].x);
@@ -212,7 +214,7 @@ hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s) {
         if (hipError_t e = p.type == F16 ? pa_few_f16(a, pl, s) : p.type == Q8_0 ? pa_few_q8(a, pl, s) : pa_few_q4(a, pl, s)) return e;
     if (y.join) {
         const int64_t rows = (int64_t)b.n_tok * a.n_head;
-        if (rows <= 2048) hipLaunchKernelGGL(k_paged_join<true>, dim3((unsigned)rows), dim3(256), 0, s, a, pl);
+        if (rows <= 2048) hipLaunchKernelGGL(k_paged_join<true>, dim3((unsigned)rows, rows * (p.hd / 64) <= 1024 ? p.hd / 64 : 1), dim3(256), 0, s, a, pl);
         else hipLaunchKernelGGL(k_paged_join<false>, dim3(ceil_div(rows, 256 / (p.hd / 4))), dim3(256), 0, s, a, pl);
         return hipGetLastError();
     }

@@ -277,11 +277,30 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         u += x.took;
         if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;
-        const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = min(sq.nq * G, (x.tile + 1) * R), r0 = x.tile * R + 16 * rw;     // the tile's rows end at `rows`
+        const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = min(sq.nq * G, (x.tile + 1) * R);     // the tile's rows end at `rows`
         bool bad = sq.bad;
         if (bad && tid == 0) paged_flag(p, PAGED_BAD_BATCH);
         const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 31) / 32 : 0;
 
+        // The queries first (rows 8 k + lane / 8 of the wave's, elements 32 s + 4 (lane %
+        // 8) ..): they are back with the page ids, and used while the first keys and values come.
+        const int r0 = x.tile * R + 16 * rw;                 // the wave's rows: r0 ..
+        pa_v4f y[NS][2];
+        {
+            const bool al = (((uintptr_t)a.q & 15) | (a.qs & 3)) == 0;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int r = r0 + 8 * k + (lane >> 3), i = r / G;
+                const bool in = r < rows;
+                const float *src = a.q + (size_t)(sq.t0 + (in ? i : 0)) * a.qs + (size_t)(kvh * G + (in ? r - i * G : 0)) * HD + HE * ew + 4 * (lane & 7);
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const float *d = src + 32 * s;
+                    y[s][k] = !in ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : al ? *(const pa_v4f *)d : pa_v4f{d[0], d[1], d[2], d[3]};
+                }
+            }
+        }
+        asm volatile("" ::: "memory");
         PmStage<HD, KVT> st;
         PaUnits us, more_us;                                 // of 32 steps, and of the next 32
         PaUnit un[2], nx[2];
@@ -292,7 +311,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             pm_load<HD, KVT>(st, p, nx, tid);
         }
-        // The wave's rows: 16 rw ..; busy: it has some.  The lane's: r0 + c.
+        // busy: the wave has rows; the lane's: r0 + c
         const bool busy = r0 < rows, ok = r0 + c < rows;
         const int ri = ok ? (r0 + c) / G : 0, head = kvh * G + (ok ? r0 + c - ri * G : 0), tok = sq.t0 + ri;
         int rlo = lo0, rhi = hi0;                            // the lane's row attends [rlo, rhi]
@@ -310,19 +329,9 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         pa_v8h q0[NS], q1[NS];
         float qs;
         {
-            pa_v4f y[NS][2];                                 // rows 8 k + lane / 8, elements 32 s + 4 (lane % 8) ..
-            const bool al = (((uintptr_t)a.q & 15) | (a.qs & 3)) == 0;
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const int r = r0 + 8 * k + (lane >> 3), i = r / G;
-                const bool in = r < rows;
-                const float *src = a.q + (size_t)(sq.t0 + (in ? i : 0)) * a.qs + (size_t)(kvh * G + (in ? r - i * G : 0)) * HD + HE * ew + 4 * (lane & 7);
                 float am = 0.0f;
-#pragma unroll
-                for (int s = 0; s < NS; s++) {
-                    const float *d = src + 32 * s;
-                    y[s][k] = !in ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : al ? *(const pa_v4f *)d : pa_v4f{d[0], d[1], d[2], d[3]};
-                }
 #pragma unroll
                 for (int s = 0; s < NS; s++)
                     am = fmaxf(fmaxf(am, fmaxf(fabsf(y[s][k][0]), fabsf(y[s][k][1]))), fmaxf(fabsf(y[s][k][2]), fabsf(y[s][k][3])));
