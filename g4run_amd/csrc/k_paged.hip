@@ -34,9 +34,7 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     const bool few_pre = b.n_prefix && few.rows && rows <= few.rows;
     const bool many_own = b.q_off ? b.n_tok > few.toks : !few.rows;
     const bool many_pre = b.n_prefix && !few_pre;
-    few.least = 1;
     few.pre_tiles = few_pre ? 1 : 0;
-    many.least = 2;
     // positions a tile attends at most: its first token's window rounded down to
     // 32, and its later tokens
     auto span = [&](int tokens) { return window ? std::min<int64_t>(b.max_len, (int64_t)window + 32 + tokens) : (int64_t)b.max_len; };
@@ -60,8 +58,9 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     y.join = b.n_prefix || (few.rows && fspan > few.unit);
     // Many rows: tiles of whole tokens, up to 128 rows (64 of heads of 512), evenly
     // filled; as many workgroups as fit on the device at once.  Steps of 32 positions,
-    // a lead of 5 (four prompts of 509 behind 3800, 4 KV heads of 256: 91 us with 2,
-    // 83 with 4, 80 with 6; the same order for heads of 64).
+    // each its workgroup where they are few (24 rows of 256 over 76 positions: 22 us,
+    // with shares of 2 at least 29.6), a lead of 5 (four prompts of 509 behind 3800, 4
+    // KV heads of 256: 91 us with 2, 83 with 4, 80 with 6; the same order for heads of 64).
     many.rows = 0;
     many.pre_tiles = many.lead = 0;
     if (many_own || many_pre) {
@@ -78,8 +77,8 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
             steps = (own * std::max(1, ceil_div(mspan, many.unit)) + (int64_t)many.pre_tiles * many.pre_steps) * p.n_kv;
             if (steps < (1 << 27)) break;
         }
-        many.wgs = (int)std::min<int64_t>(p.hd >= 128 ? 256 : 512, ceil_div(steps, many.least));
-        many.lead = ceil_div(steps, many.least) > many.wgs ? 5 : 0;
+        many.wgs = (int)std::min<int64_t>(p.hd >= 128 ? 256 : 512, steps);
+        many.lead = steps > many.wgs ? 5 : 0;
         y.join |= mspan > many.unit;
     }
     const size_t all = y.join ? (size_t)b.n_tok * p.n_kv * grp : 0, whole = b.n_prefix ? all : 0;

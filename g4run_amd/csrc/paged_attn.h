@@ -46,7 +46,7 @@ struct PagedList {
     int rows;                        // rows of a tile; the few-row kernel: most rows of a sequence it takes
     int toks;                        // many: tokens of a tile, rows / grp; few: most tokens of a sequence
     uint32_t toks_inv;               // many: n / toks == umulhi(n, toks_inv) for n <= 2^24 (0: toks is 1)
-    int wgs, least;                  // workgroups; steps of a share at least
+    int wgs;                         // workgroups
     int unit, shift;                 // positions of a step, and their log2
     int lead;                        // steps that the start of a sequence's tile counts as
     int pre_tiles, pre_steps;        // the prefix's tiles (0: not this kernel's), and steps of each
@@ -328,7 +328,7 @@ __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan
     seq = a.b.n_seq;
     before = from.before;
 }
-__device__ __forceinline__ int pa_share(const PagedList &y, int total) { return max(y.least, (total + y.wgs - 1) / y.wgs); }
+__device__ __forceinline__ int pa_share(const PagedList &y, int total) { return (total + y.wgs - 1) / y.wgs; }
 
 // A piece: steps [step, step + n) of the `all` of one tile of one KV head.  (The
 // lead comes before step 0, so the shares of the list stay contiguous.)
