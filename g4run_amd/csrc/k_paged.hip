@@ -100,7 +100,7 @@ Layout layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
 // One (token, head) row: out = sum of exp2(m_k - M) O_k / sum of exp2(m_k - M) l_k
 // over the row's partial results in a fixed order.  SPLIT: a workgroup per row, or
 // per row and 64 elements where those are few (36 rows of 512 from 250 pieces: 36 us,
-// 9.6 so; 512 rows of 512 from a few: 7.0 us, 11.5 so), its groups of threads every
+// 9.6 so; 256 rows of 256 from a few: 5.0 us, 5.5 so), its groups of threads every
 // so-many-th result; else a group of hd / 4 threads per row (many rows of few: a
 // workgroup's one active group left the chip empty, 9000 rows of 256 took 18 us, now
 // 11.4).  Bound by the latency of reads that depend on each other, so: the row's
@@ -213,7 +213,7 @@ hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s) {
         if (hipError_t e = p.type == F16 ? pa_few_f16(a, pl, s) : p.type == Q8_0 ? pa_few_q8(a, pl, s) : pa_few_q4(a, pl, s)) return e;
     if (y.join) {
         const int64_t rows = (int64_t)b.n_tok * a.n_head;
-        if (rows <= 2048) hipLaunchKernelGGL(k_paged_join<true>, dim3((unsigned)rows, rows * (p.hd / 64) <= 1024 ? p.hd / 64 : 1), dim3(256), 0, s, a, pl);
+        if (rows <= 2048) hipLaunchKernelGGL(k_paged_join<true>, dim3((unsigned)rows, rows * (p.hd / 64) <= 512 ? p.hd / 64 : 1), dim3(256), 0, s, a, pl);
         else hipLaunchKernelGGL(k_paged_join<false>, dim3(ceil_div(rows, 256 / (p.hd / 4))), dim3(256), 0, s, a, pl);
         return hipGetLastError();
     }
