@@ -50,9 +50,13 @@ __device__ __forceinline__ void paged_flag(const PagedPool &p, int bits) {
 
 // The batch's arrays do not change while a call runs: read through the constant
 // address space, a wave-uniform index takes a scalar load, which does not wait
-// behind the vector loads in flight.
-__device__ __forceinline__ int paged_ld(const int *p, int64_t i) {
+// behind the vector loads in flight.  (The host's twin of the split reads its own.)
+__host__ __device__ __forceinline__ int paged_ld(const int *p, int64_t i) {
+#ifdef __HIP_DEVICE_COMPILE__
     return ((const __attribute__((address_space(4))) int *)p)[i];
+#else
+    return p[i];
+#endif
 }
 
 // A sequence as a call may use it: its tokens [t0, t0 + nq) within n_tok, its
@@ -61,7 +65,7 @@ struct PagedSeq {
     int t0, nq, len;
     bool bad;
 };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedPool &p, const PagedBatch &b, int s) {
+__host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedPool &p, const PagedBatch &b, int s) {
     PagedSeq r;
     r.len = paged_ld(b.len, s);
     r.bad = r.len < 0 || r.len > b.max_len || (int64_t)r.len > (int64_t)b.table_stride * p.page;
@@ -124,8 +128,8 @@ struct PagedAttn {
     int window;
     uint8_t *ws;
 };
-// workspace of a call: partial results of every (token, head) row and position
-// split, 0 where a call writes its outputs directly
+// workspace of a call: the workgroups' partial results and where each (token, head)
+// row's lie, 0 where a call writes its outputs directly
 size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head);
 hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s);
 

@@ -38,10 +38,12 @@ typedef uint32_t pa_v4u __attribute__((ext_vector_type(4)));
 // of one row tile of one KV head: the prefix's tiles, then the sequences' in
 // order), cut into equal shares for its workgroups.  A piece -- the part of a
 // share that lies in one tile of one head -- is written out where it is the whole
-// tile and there is no prefix; else its sums go to the workspace: slot 2 w for
-// workgroup w's first piece, 2 w + 1 for another (only the first and the last of a
-// share, and whole tiles beside a prefix, are partial).  The tile's first piece
-// tells k_paged_join where its rows' pieces lie.
+// tile and there is no prefix; else its sums go to the workspace.  A whole tile's
+// have a place by row, one for the prefix's tile and one for the row's own.  Of the
+// other pieces a share holds two at most, its first and its last: slot 2 w for
+// workgroup w's first piece, 2 w + 1 for its last.  The tile's first piece tells
+// k_paged_join where its rows' pieces lie.  The functions of the split run on the
+// host too, where a test follows every piece of a call.
 struct PagedList {
     int rows;                        // rows of a tile; the few-row kernel: most rows of a sequence it takes
     int toks;                        // many: tokens of a tile, rows / grp; few: most tokens of a sequence
@@ -60,7 +62,7 @@ struct PagedPlan {
     // count << 1 | kernel (0 few), slot << 8 | row of the tile; [0] count 0 where
     // the row is written out
     uint2 *own, *pre;
-    float *wo;                       // [token][head][hd] whole tiles' sums beside a prefix
+    float *wo;                       // [2][token][head][hd] whole tiles' sums beside a prefix: own positions, the prefix
     float2 *wml;
 };
 
@@ -220,11 +222,11 @@ __device__ __forceinline__ void pa_tanh(float (&x)[N]) {
 }
 
 // the batch's rows that attend the prefix
-__device__ __forceinline__ int pa_tokens(const PagedBatch &b) {
+__host__ __device__ __forceinline__ int pa_tokens(const PagedBatch &b) {
     return b.q_off ? min(max(paged_ld(b.q_off, b.n_seq), 0), b.n_tok) : min(b.n_seq, b.n_tok);
 }
 // first own position that tokens from `first` on attend, rounded down to 32
-__device__ __forceinline__ int pa_low(int first, int window) { return window ? max(0, first + 1 - window) & ~31 : 0; }
+__host__ __device__ __forceinline__ int pa_low(int first, int window) { return window ? max(0, first + 1 - window) & ~31 : 0; }
 
 // position of global token tok (prefix included), its sequence looked up
 __device__ __forceinline__ int pa_token_pos(const PagedPool &p, const PagedBatch &b, int tok) {
@@ -258,25 +260,25 @@ __device__ __forceinline__ int pa_scan(int v) {
 // Which sequences are a kernel's (MANY: more rows than the few-row kernel takes),
 // their tiles, and a tile's positions [lo, hi] (own; lo a multiple of 32).
 template <bool MANY>
-__device__ __forceinline__ const PagedList &pa_list(const PagedPlan &pl) {
+__host__ __device__ __forceinline__ const PagedList &pa_list(const PagedPlan &pl) {
     if constexpr (MANY) return pl.many;
     else return pl.few;
 }
 template <bool MANY>
-__device__ __forceinline__ int pa_tiles(const PagedPlan &pl, const PagedSeq &q) {
+__host__ __device__ __forceinline__ int pa_tiles(const PagedPlan &pl, const PagedSeq &q) {
     if (q.nq <= pl.few.toks) return !MANY && q.nq > 0;
     if constexpr (!MANY) return 0;
     const uint32_t n = q.nq + pl.many.toks - 1;
-    return pl.many.toks_inv ? (int)__umulhi(n, pl.many.toks_inv) : (int)n;
+    return pl.many.toks_inv ? (int)((uint64_t)n * pl.many.toks_inv >> 32) : (int)n;
 }
 template <bool MANY>
-__device__ __forceinline__ void pa_tile_span(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile, int &lo, int &hi) {
+__host__ __device__ __forceinline__ void pa_tile_span(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile, int &lo, int &hi) {
     const int first = q.len - q.nq + (MANY ? tile * pl.many.toks : 0);
     lo = pa_low(first, a.window);
     hi = MANY ? min(q.len, first + pl.many.toks) - 1 : q.len - 1;
 }
 template <bool MANY>
-__device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile) {
+__host__ __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile) {
     if (q.bad) return 1;
     const PagedList &y = pa_list<MANY>(pl);
     int lo, hi;
@@ -285,7 +287,7 @@ __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const PagedPlan
 }
 // steps of sequence s for one KV head
 template <bool MANY>
-__device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, int s) {
+__host__ __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, int s) {
     const PagedSeq q = paged_seq(a.p, a.b, s);
     const int tiles = pa_tiles<MANY>(pl, q);
     int n = 0;
@@ -328,7 +330,7 @@ __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan
     seq = a.b.n_seq;
     before = from.before;
 }
-__device__ __forceinline__ int pa_share(const PagedList &y, int total) { return (total + y.wgs - 1) / y.wgs; }
+__host__ __device__ __forceinline__ int pa_share(const PagedList &y, int total) { return (total + y.wgs - 1) / y.wgs; }
 
 // A piece: steps [step, step + n) of the `all` of one tile of one KV head.  (The
 // lead comes before step 0, so the shares of the list stay contiguous.)
@@ -342,9 +344,9 @@ struct PaPiece {
     const int *table;
     bool pre;
 };
-// the piece at step u of a share [first, stop)
-template <bool MANY>
-__device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, PaFind &from, int wg, int u, int first, int stop) {
+// the piece at step u of a share [first, stop); find(u, seq, before) as pa_find_step
+template <bool MANY, typename F>
+__host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, const PagedPlan &pl, int wg, int u, int first, int stop, F find) {
     const PagedList &y = pa_list<MANY>(pl);
     const PagedBatch &b = a.b;
     PaPiece x;
@@ -368,7 +370,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
     } else {
         lead = y.lead;
         int seq, before;
-        pa_find_step<MANY>(a, pl, mine, u - pre_all, from, seq, before);
+        find(u - pre_all, seq, before);
         x.sq = paged_seq(a.p, b, seq);
         v = u - pre_all - before;
         if constexpr (MANY) {
@@ -398,6 +400,10 @@ __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan 
     x.slot = 2 * wg + (u != first);
     return x;
 }
+template <bool MANY>
+__device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, PaFind &from, int wg, int u, int first, int stop) {
+    return pa_piece_by<MANY>(a, pl, wg, u, first, stop, [&](int v, int &seq, int &before) { pa_find_step<MANY>(a, pl, mine, v, from, seq, before); });
+}
 // Where row r (of its tile) of a piece puts its sums: out (normalised), or `o` and
 // `ml`; and, from a tile's first piece, where k_paged_join finds them.
 struct PaSink {
@@ -406,7 +412,7 @@ struct PaSink {
     bool out;
 };
 template <bool MANY>
-__device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &pl, const PaPiece &x, int share, int r, int tok, int head, bool note) {
+__host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &pl, const PaPiece &x, int share, int r, int tok, int head, bool note) {
     const PagedList &y = pa_list<MANY>(pl);
     const size_t row = (size_t)tok * a.n_head + head;
     const bool whole = x.n == x.all;
@@ -416,10 +422,11 @@ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &p
         s.o = a.out + (size_t)tok * a.os + (size_t)head * a.p.hd;
         s.ml = nullptr;
         if (note && pl.own) pl.own[row] = make_uint2(0, 0);
-    } else if (!x.pre && whole) {
-        s.o = pl.wo + row * a.p.hd;
-        s.ml = pl.wml + row;
-        if (note) pl.own[row] = make_uint2(2 | MANY, ~0u);
+    } else if (whole) {
+        const size_t at = row + (x.pre ? (size_t)a.b.n_tok * a.n_head : 0);
+        s.o = pl.wo + at * a.p.hd;
+        s.ml = pl.wml + at;
+        if (note) (x.pre ? pl.pre : pl.own)[row] = make_uint2(2 | MANY, ~0u);
     } else {
         const size_t at = (size_t)x.slot * y.rows + r;
         s.o = y.o + at * a.p.hd;
@@ -431,6 +438,26 @@ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &p
         }
     }
     return s;
+}
+
+// where partial result k of a row lies: the prefix's pieces, then the own ones
+struct PaPart {
+    const float *o;
+    const float2 *ml;
+};
+__host__ __device__ __forceinline__ PaPart pa_part(const PagedAttn &a, const PagedPlan &pl, size_t row, uint2 pre, uint2 own, int k) {
+    const int n_pre = pre.x >> 1;
+    const bool in_pre = k < n_pre;
+    const uint2 d = in_pre ? pre : own;
+    if (!in_pre) k -= n_pre;
+    if (d.y == ~0u) {
+        const size_t at = row + (in_pre ? (size_t)a.b.n_tok * a.n_head : 0);
+        return PaPart{pl.wo + at * a.p.hd, pl.wml + at};
+    }
+    const bool many = d.x & 1;
+    const int w = (int)(d.y >> 9) + k, wgs = many ? pl.many.wgs : pl.few.wgs, rows = many ? pl.many.rows : pl.few.rows;
+    const size_t s = (size_t)(2 * min(w, wgs - 1) + (k == 0 ? d.y >> 8 & 1 : 0)) * rows + (d.y & 255);
+    return PaPart{(many ? pl.many.o : pl.few.o) + s * a.p.hd, (many ? pl.many.ml : pl.few.ml) + s};
 }
 
 // max of unsigned halves; the biased exponent of a (positive) half as a float

@@ -212,3 +212,61 @@ class Case:
         assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {worst:.3g} tolerances, first {tuple(np.argwhere(bad)[0])}"
         assert self.kv.status() == 0
         return worst
+
+
+class LongCase(Case):
+    """A Case of many rows: the same batch, filled and attended array by array."""
+
+    def _fill(self, pages, n, spread):
+        out = []
+        for value in (False, True):
+            x = (self.rng.standard_normal((n, self.n_kv, self.hd), np.float32) * np.float32(spread)).astype(np.float32)
+            raw, pos, hd = self.pool.v if value else self.pool.k, np.arange(n), self.hd
+            size = row_bytes(self.t, hd)
+            rows = raw[:, :self.n_kv * self.page * size].reshape(len(raw), self.n_kv, self.page, size)
+            at = (pages[pos // self.page][:, None], np.arange(self.n_kv), (pos % self.page)[:, None])
+            if self.t == F16:
+                rows[at] = x.astype(np.float16).view(np.uint8)
+            else:
+                q, d = quantize(self.t, x)
+                q = q.reshape(x.shape)
+                if self.t == Q8_0:
+                    b = np.zeros(x.shape, np.uint8)
+                    b[..., self.pool.v8 if value else self.pool.k8] = q + 128
+                else:
+                    b = np.zeros(x.shape, np.uint8)
+                    b[..., self.pool.v4 if value else self.pool.k4] = q + 8
+                    b = b[..., 0::2] | (b[..., 1::2] << 4)
+                rows[at] = b
+                raw[:, self.n_kv * self.page * size:].reshape(len(raw), self.n_kv, self.page, hd // 16)[at] = d.view(np.uint8)
+            out.append(values(self.t, x))
+        return out
+
+    def expect(self, scale, cap=0.0, window=0):
+        """As Case.expect; a row's tolerance takes the largest value up to its position."""
+        grp, hd = self.n_head // self.n_kv, self.hd
+        out, tol = np.full((self.n_tok, self.n_head, hd), 7.5), np.zeros((self.n_tok, self.n_head, hd))
+        for s, (n, size) in enumerate(zip(self.new, self.lens)):
+            own = size - n + np.arange(n)
+            pos = np.where(own >= 0, self.n_prefix + own, -1)
+            for kv in range(self.n_kv if n else 0):
+                k, v = (np.concatenate([self.shared[w][:, kv], self.rows[s][w][:, kv]]) for w in (0, 1))
+                key = np.arange(len(k))
+                seen = key <= pos[:, None]
+                if window:
+                    seen &= key > pos[:, None] - window
+                top = np.concatenate([np.maximum.accumulate(np.abs(v).max(1)), [0.0]])[pos]
+                for h in range(kv * grp, (kv + 1) * grp):
+                    q = self.q[self.off[s]:self.off[s] + n, h].astype(np.float64)
+                    x = q @ k.T * scale
+                    mag = np.where(seen, np.abs(q) @ np.abs(k).T * abs(scale), 0.0).max(1, initial=0.0)
+                    if cap:
+                        x = cap * np.tanh(x / cap)
+                    x = np.where(seen, x, -np.inf)
+                    d = mag * (2.0 ** -21 + hd * 2.0 ** -24) + np.where(seen, np.abs(x), 0.0).max(1, initial=0.0) * 2.0 ** -22 + cap * 2.0 ** -21 + 2.0 ** -22
+                    w = np.exp(x - x.max(1, initial=-1e300)[:, None])
+                    total = np.maximum(w.sum(1), 1e-300)[:, None]
+                    t = slice(self.off[s], self.off[s] + n)
+                    out[t, h] = w @ v / total
+                    tol[t, h] = (2 * d[:, None] + 2.0 ** -18) * (w @ np.abs(v)) / total + 2.0 ** -29 * (seen.sum(1) * top)[:, None] / total + 1e-30
+        return out, tol
