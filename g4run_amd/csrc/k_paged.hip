@@ -12,8 +12,8 @@ namespace {
 // 9.6 so; 256 rows of 256 from a few: 5.0 us, 5.5 so), its groups of threads every
 // so-many-th result; else a group of hd / 4 threads per row (many rows of few: a
 // workgroup's one active group left the chip empty, 9000 rows of 256 took 18 us, now
-// 11.4).  Bound by the latency of reads that depend on each other, so: the row's
-// sequence by one load of the whole wave, four results' maxima and sums at once
+// 11.4).  Bound by the latency of reads that depend on each other, so: what the
+// kernels noted of the row and nothing else, four results' maxima and sums at once
 // under a running maximum.
 template <bool SPLIT>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
@@ -22,22 +22,9 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
     const int hd = a.p.hd, hd4 = hd / 4 / (SPLIT ? gridDim.y : 1), groups = 256 / hd4, gi = threadIdx.x / hd4, e4 = 4 * (threadIdx.x % hd4 + (SPLIT ? hd4 * blockIdx.y : 0));
     const int all = a.b.n_tok * a.n_head, mine = SPLIT ? (int)blockIdx.x : (int)blockIdx.x * groups + gi, row = min(mine, all - 1);   // up to 2^24
     const int tok = row / a.n_head, head = row - tok * a.n_head;
-    const uint2 own = pl.own[row], pre = a.b.n_prefix > 0 ? pl.pre[row] : make_uint2(0, 0);      // of a row without a sequence: not used
-    int seq = 0;
-    if constexpr (SPLIT) seq = paged_find(a.b, tok);
-    else {
-        const int t1 = __builtin_amdgcn_readlane(tok, 63);   // a wave's rows lie in up to 4 tokens
-        for (int t = pa_uniform(tok); t <= t1; t++) {
-            const int s = paged_find(a.b, t);
-            if (t == tok) seq = s;
-        }
-    }
-    if (mine >= all || seq >= a.b.n_seq) return;             // behind the last row or sequence
-    const PagedSeq sq = paged_seq(a.p, a.b, seq);
-    const int i = tok - sq.t0;
-    if (i < 0 || i >= sq.nq) return;
-    const int n_pre = pre.x >> 1, n_own = own.x >> 1, total = n_pre + n_own;
-    if (n_own == 0) return;                                  // written out
+    const uint2 own = pl.own[row], pre = a.b.n_prefix > 0 ? pl.pre[row] : make_uint2(0, 0);
+    const int n_pre = pre.x >> 2, n_own = own.x >> 2, total = n_pre + n_own;
+    if (mine >= all || n_own == 0) return;
     pa_v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
     float m = -__builtin_inff(), l = 0.0f;
     auto add = [&](float2 x, pa_v4f v, float mn) {
@@ -77,7 +64,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
         l = 0.0f;
         for (int k = 0; k < groups; k++) add(ml_of[k], part[k * hd4 + threadIdx.x], m);
     }
-    const bool none = !sq.bad && sq.len - sq.nq + i < 0;
+    const bool none = own.x & 2;
     pa_store4(a.out + (size_t)tok * a.os + (size_t)head * hd + e4, none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / l));
 }
 

@@ -63,17 +63,19 @@ __host__ __device__ __forceinline__ int paged_ld(const int *p, int64_t i) {
 // length; bad lengths and offsets are flagged by the caller.
 struct PagedSeq {
     int t0, nq, len;
-    bool bad;
+    bool bad, torn;                  // torn: by its offsets
 };
 __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedPool &p, const PagedBatch &b, int s) {
     PagedSeq r;
     r.len = paged_ld(b.len, s);
+    r.torn = false;
     r.bad = r.len < 0 || r.len > b.max_len || (int64_t)r.len > (int64_t)b.table_stride * p.page;
     if (b.q_off) {
         const int a = paged_ld(b.q_off, s), e = paged_ld(b.q_off, s + 1);
         r.t0 = min(max(a, 0), b.n_tok);
         r.nq = min(max(e, r.t0), b.n_tok) - r.t0;
-        if (r.t0 != a || r.t0 + r.nq != e) r.bad = true;
+        r.torn = r.t0 != a || r.t0 + r.nq != e;
+        r.bad |= r.torn;
     } else {
         r.t0 = s;
         r.nq = s < b.n_tok ? 1 : 0;

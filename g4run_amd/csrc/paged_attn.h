@@ -59,8 +59,9 @@ struct PagedPlan {
     PagedList few, many;             // rows 0: the kernel does not run
     uint32_t grp_inv;                // rows to tokens: r / grp == r * grp_inv >> 16 for r < 16
     // where a (token, head) row's partial results lie, own positions and prefix:
-    // count << 1 | kernel (0 few), slot << 8 | row of the tile; [0] count 0 where
-    // the row is written out
+    // count << 2 | whether it has no position << 1 | kernel (0 few), slot << 8 | row of
+    // the tile; [0] count 0 where there is nothing to join: the row is written out,
+    // or no sequence's
     uint2 *own, *pre;
     float *wo;                       // [2][token][head][hd] whole tiles' sums beside a prefix: own positions, the prefix
     float2 *wml;
@@ -221,18 +222,19 @@ __device__ __forceinline__ void pa_tanh(float (&x)[N]) {
     for (int j = 0; j < N; j++) x[j] = p[j];
 }
 
-// the batch's rows that attend the prefix
-__host__ __device__ __forceinline__ int pa_tokens(const PagedBatch &b) {
-    return b.q_off ? min(max(paged_ld(b.q_off, b.n_seq), 0), b.n_tok) : min(b.n_seq, b.n_tok);
+// the end of the batch's tokens; n_seq: its sequences before the first torn one
+__host__ __device__ __forceinline__ int pa_tokens(const PagedBatch &b, int n_seq) {
+    if (n_seq == 0) return 0;
+    return b.q_off ? paged_ld(b.q_off, n_seq) : min(n_seq, b.n_tok);
 }
 // first own position that tokens from `first` on attend, rounded down to 32
 __host__ __device__ __forceinline__ int pa_low(int first, int window) { return window ? max(0, first + 1 - window) & ~31 : 0; }
 
 // position of global token tok (prefix included), its sequence looked up
-__device__ __forceinline__ int pa_token_pos(const PagedPool &p, const PagedBatch &b, int tok) {
+__device__ __forceinline__ int pa_token_pos(const PagedPool &p, const PagedBatch &b, int n_seq, int tok) {
     int s = tok;
     if (b.q_off) {
-        int x = 0, y = b.n_seq;                              // last s with q_off[s] <= tok
+        int x = 0, y = n_seq;                                // last s with q_off[s] <= tok
         while (y - x > 1) {
             const int z = (x + y) >> 1;
             if (paged_ld(b.q_off, z) <= tok) x = z;
@@ -285,24 +287,39 @@ __host__ __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const 
     pa_tile_span<MANY>(a, pl, q, tile, lo, hi);
     return max(1, (hi - lo + y.unit) >> y.shift);
 }
-// steps of sequence s for one KV head
+// steps of a sequence for one KV head
 template <bool MANY>
-__host__ __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, int s) {
-    const PagedSeq q = paged_seq(a.p, a.b, s);
+__host__ __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q) {
     const int tiles = pa_tiles<MANY>(pl, q);
     int n = 0;
     for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY>(a, pl, q, t);
     return n + tiles * pa_list<MANY>(pl).lead;
 }
 // All steps of the list (wave-uniform; the whole wave calls it), 64 sequences at a
-// time; the lane's own of the first 64 in `mine`.
+// time; the lane's own of the first 64 in `mine`.  The batch ends at the first torn
+// sequence, n_seq: offsets that descend would give tokens to several sequences, and
+// more steps than the host counted.
 template <bool MANY>
-__device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl, int &mine) {
+__device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl, int &mine, int &n_seq) {
     const PagedList &y = pa_list<MANY>(pl);
     const int lane = threadIdx.x & 63;
-    mine = lane < a.b.n_seq ? pa_steps<MANY>(a, pl, lane) : 0;
+    auto at = [&](int s0) {
+        PagedSeq q = {0, 0, 0, false, false};
+        if (s0 + lane < n_seq) q = paged_seq(a.p, a.b, s0 + lane);
+        if (a.b.q_off) {
+            const uint64_t torn = __ballot(q.torn);
+            if (torn) {
+                n_seq = s0 + __ffsll((unsigned long long)torn) - 1;
+                if (s0 + lane >= n_seq) q.nq = 0;
+            }
+        }
+        return pa_steps<MANY>(a, pl, q);
+    };
+    n_seq = a.b.n_seq;
+    mine = at(0);
     int n = mine;
-    for (int s = 64 + lane; s < a.b.n_seq; s += 64) n += pa_steps<MANY>(a, pl, s);
+    for (int s0 = 64; s0 < n_seq; s0 += 64) n += at(s0);
+    n_seq = pa_uniform(n_seq);
     n = pa_uniform(group_isum<64>(n));
     return (n + y.pre_tiles * y.pre_steps) * a.p.n_kv;
 }
@@ -316,7 +333,7 @@ template <bool MANY>
 __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan &pl, int mine, int u, PaFind &from, int &seq, int &before) {
     const int lane = threadIdx.x & 63;
     for (; from.s0 < a.b.n_seq; from.s0 += 64) {
-        const int n = (from.s0 == 0 ? mine : from.s0 + lane < a.b.n_seq ? pa_steps<MANY>(a, pl, from.s0 + lane) : 0) * a.p.n_kv;
+        const int n = (from.s0 == 0 ? mine : from.s0 + lane < a.b.n_seq ? pa_steps<MANY>(a, pl, paged_seq(a.p, a.b, from.s0 + lane)) : 0) * a.p.n_kv;
         const int incl = pa_scan(n);
         const uint64_t past = __ballot(from.before + incl > u);
         if (past) {
@@ -346,7 +363,7 @@ struct PaPiece {
 };
 // the piece at step u of a share [first, stop); find(u, seq, before) as pa_find_step
 template <bool MANY, typename F>
-__host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, const PagedPlan &pl, int wg, int u, int first, int stop, F find) {
+__host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, const PagedPlan &pl, int n_seq, int wg, int u, int first, int stop, F find) {
     const PagedList &y = pa_list<MANY>(pl);
     const PagedBatch &b = a.b;
     PaPiece x;
@@ -355,7 +372,7 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
     int base, v, lead = 0;                                   // v: the step of the tile, its lead counted
     if (x.pre) {
         x.sq.t0 = 0;
-        x.sq.nq = pa_tokens(b);
+        x.sq.nq = pa_tokens(b, n_seq);
         x.sq.len = x.seglen = b.n_prefix;
         x.sq.bad = false;
         x.all = y.pre_steps;
@@ -401,8 +418,8 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
     return x;
 }
 template <bool MANY>
-__device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, PaFind &from, int wg, int u, int first, int stop) {
-    return pa_piece_by<MANY>(a, pl, wg, u, first, stop, [&](int v, int &seq, int &before) { pa_find_step<MANY>(a, pl, mine, v, from, seq, before); });
+__device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, int n_seq, PaFind &from, int wg, int u, int first, int stop) {
+    return pa_piece_by<MANY>(a, pl, n_seq, wg, u, first, stop, [&](int v, int &seq, int &before) { pa_find_step<MANY>(a, pl, mine, v, from, seq, before); });
 }
 // Where row r (of its tile) of a piece puts its sums: out (normalised), or `o` and
 // `ml`; and, from a tile's first piece, where k_paged_join finds them.
@@ -412,7 +429,7 @@ struct PaSink {
     bool out;
 };
 template <bool MANY>
-__host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &pl, const PaPiece &x, int share, int r, int tok, int head, bool note) {
+__host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &pl, const PaPiece &x, int share, int r, int tok, int head, uint32_t none, bool note) {
     const PagedList &y = pa_list<MANY>(pl);
     const size_t row = (size_t)tok * a.n_head + head;
     const bool whole = x.n == x.all;
@@ -426,7 +443,7 @@ __host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const Pag
         const size_t at = row + (x.pre ? (size_t)a.b.n_tok * a.n_head : 0);
         s.o = pl.wo + at * a.p.hd;
         s.ml = pl.wml + at;
-        if (note) (x.pre ? pl.pre : pl.own)[row] = make_uint2(2 | MANY, ~0u);
+        if (note) (x.pre ? pl.pre : pl.own)[row] = make_uint2(4 | none << 1 | MANY, ~0u);
     } else {
         const size_t at = (size_t)x.slot * y.rows + r;
         s.o = y.o + at * a.p.hd;
@@ -434,30 +451,52 @@ __host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const Pag
         if (note && x.step == 0) {
             // later pieces start the next workgroups' shares
             const int rest = x.all - x.n, count = 1 + (rest + share - 1) / share;
-            (x.pre ? pl.pre : pl.own)[row] = make_uint2((uint32_t)count << 1 | MANY, (uint32_t)x.slot << 8 | (uint32_t)r);
+            (x.pre ? pl.pre : pl.own)[row] = make_uint2((uint32_t)count << 2 | none << 1 | MANY, (uint32_t)x.slot << 8 | (uint32_t)r);
         }
     }
     return s;
 }
 
+// Rows of tokens that are no sequence's are noted too, so that k_paged_join goes by
+// the notes alone; those from a torn sequence on become NaN.
+__host__ __device__ __forceinline__ void pa_outside(const PagedAttn &a, const PagedPlan &pl, int n_seq, int thread, int threads) {
+    const int before = n_seq && a.b.q_off ? paged_ld(a.b.q_off, 0) : 0, end = pa_tokens(a.b, n_seq);
+    if (pl.own) {
+        const int n = (before + a.b.n_tok - end) * a.n_head;             // up to 2^24
+        for (int i = thread; i < n; i += threads) pl.own[i < before * a.n_head ? i : i + (end - before) * a.n_head] = make_uint2(0, 0);
+    }
+    if (n_seq < a.b.n_seq) {
+        const int row = a.n_head * a.p.hd;
+        for (int t = end; t < a.b.n_tok; t++)
+            for (int e = thread; e < row; e += threads) a.out[(size_t)t * a.os + e] = __builtin_nanf("");
+    }
+}
 // where partial result k of a row lies: the prefix's pieces, then the own ones
 struct PaPart {
     const float *o;
     const float2 *ml;
 };
 __host__ __device__ __forceinline__ PaPart pa_part(const PagedAttn &a, const PagedPlan &pl, size_t row, uint2 pre, uint2 own, int k) {
-    const int n_pre = pre.x >> 1;
+    // both kernels' lists first: loaded where they are chosen, they are loads by lane
+    const PagedList few = pl.few, many = pl.many;
+    const float *const wo = pl.wo;
+    const float2 *const wml = pl.wml;
+    const int n_pre = pre.x >> 2, hd = a.p.hd;
     const bool in_pre = k < n_pre;
     const uint2 d = in_pre ? pre : own;
     if (!in_pre) k -= n_pre;
-    if (d.y == ~0u) {
-        const size_t at = row + (in_pre ? (size_t)a.b.n_tok * a.n_head : 0);
-        return PaPart{pl.wo + at * a.p.hd, pl.wml + at};
-    }
-    const bool many = d.x & 1;
-    const int w = (int)(d.y >> 9) + k, wgs = many ? pl.many.wgs : pl.few.wgs, rows = many ? pl.many.rows : pl.few.rows;
-    const size_t s = (size_t)(2 * min(w, wgs - 1) + (k == 0 ? d.y >> 8 & 1 : 0)) * rows + (d.y & 255);
-    return PaPart{(many ? pl.many.o : pl.few.o) + s * a.p.hd, (many ? pl.many.ml : pl.few.ml) + s};
+    const bool whole = d.y == ~0u, by_many = d.x & 1;
+    const int w = min((int)(d.y >> 9) + k, (by_many ? many.wgs : few.wgs) - 1);
+    const size_t slot = (size_t)(2 * w + (k == 0 ? d.y >> 8 & 1 : 0)) * (by_many ? many.rows : few.rows) + (d.y & 255);
+    const size_t at = whole ? row + (in_pre ? (size_t)a.b.n_tok * a.n_head : 0) : slot;
+    return PaPart{(whole ? wo : by_many ? many.o : few.o) + at * hd, (whole ? wml : by_many ? many.ml : few.ml) + at};
+}
+
+// what one workgroup of a call does ahead of its pieces
+__device__ __forceinline__ void pa_rest(const PagedAttn &a, const PagedPlan &pl, int n_seq) {
+    const bool torn = n_seq < a.b.n_seq;
+    if (torn && threadIdx.x == 0) paged_flag(a.p, PAGED_BAD_BATCH);
+    if (torn || pl.own) pa_outside(a, pl, n_seq, threadIdx.x, blockDim.x);
 }
 
 // max of unsigned halves; the biased exponent of a (positive) half as a float

@@ -144,9 +144,10 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
     _Float16 *const qh = (_Float16 *)lds;
     float *const buf = (float *)lds;
 
-    int mine;
-    const int total = pa_total<false>(call.a, call.pl, mine), share = pa_share(call.pl.few, total);
+    int mine, n_seq;
+    const int total = pa_total<false>(call.a, call.pl, mine, n_seq), share = pa_share(call.pl.few, total);
     const int first = blockIdx.x * share, stop = min(first + share, total);
+    if (blockIdx.x == 0 && call.pl.many.rows == 0) pa_rest(call.a, call.pl, n_seq);
     PaFind from;
     for (int u = first; u < stop;) {
         const PagedCall call = pa_fresh();
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         const PagedBatch &b = a.b;
         const int tid = pa_thread(), lane = tid & 63, wave = pa_uniform(tid >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, pw = wave / ES;
         const int G = a.grp, rc = ST ? c & 7 : c;
-        const PaPiece x = pa_piece<false>(a, pl, mine, from, blockIdx.x, u, first, stop);
+        const PaPiece x = pa_piece<false>(a, pl, mine, n_seq, from, blockIdx.x, u, first, stop);
         u += x.took;
         if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                 rhi = hi0 + i;
                 rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
             } else if (a.window) {
-                rlo = max(0, pa_token_pos(p, b, sq.t0 + i) + 1 - a.window);
+                rlo = max(0, pa_token_pos(p, b, n_seq, sq.t0 + i) + 1 - a.window);
             }
         }
 
@@ -514,9 +515,10 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                 }
                 s *= VS;
                 const int i = (int)(r * pl.grp_inv >> 16), tok = sq.t0 + i, head = kvh * G + (r - i * G);
-                const PaSink to = pa_sink<false>(a, pl, x, share, r, tok, head, e4 == 0);
+                const bool none = !sq.bad && hi0 + i < 0;
+                const PaSink to = pa_sink<false>(a, pl, x, share, r, tok, head, none, e4 == 0);
                 if (to.out) {
-                    s = !sq.bad && hi0 + i < 0 ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / ls);
+                    s = none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / ls);
                     pa_store4(to.o + e4, s);
                 } else {
                     *(pa_v4f *)(to.o + e4) = s;

@@ -259,9 +259,10 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
     // Workgroups of one XCD (every eighth) take neighbouring shares: row tiles
     // that read the same K and V find them in its L2.
     const int per = (call.pl.many.wgs + 7) >> 3, wg = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    int mine;
-    const int total = pa_total<true>(call.a, call.pl, mine), share = pa_share(call.pl.many, total);
+    int mine, n_seq;
+    const int total = pa_total<true>(call.a, call.pl, mine, n_seq), share = pa_share(call.pl.many, total);
     const int first = wg * share, stop = wg < call.pl.many.wgs ? min(first + share, total) : 0;
+    if (blockIdx.x == 0) pa_rest(call.a, call.pl, n_seq);
     PaFind from;
     for (int u = first; u < stop;) {
         const PagedCall call = pa_fresh();
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         const int G = a.grp, R = pl.many.rows;
         float *const tr = (float *)lds + wave * PM_TR;
         const float capl = a.cap * 1.4426950408889634f;
-        const PaPiece x = pa_piece<true>(a, pl, mine, from, wg, u, first, stop);
+        const PaPiece x = pa_piece<true>(a, pl, mine, n_seq, from, wg, u, first, stop);
         u += x.took;
         if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                 rhi = sq.len - sq.nq + ri;
                 rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
             } else if (a.window) {
-                rlo = max(0, pa_token_pos(p, b, tok) + 1 - a.window);
+                rlo = max(0, pa_token_pos(p, b, n_seq, tok) + 1 - a.window);
             }
         }
         __syncthreads();                                     // the previous piece's tiles and rows are used
@@ -545,12 +546,13 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         // out through LDS as the queries came in
         __syncthreads();                                     // the tiles are used
         if (!busy) continue;
+        const bool nowhere = !sq.bad && sq.len - sq.nq + ri < 0;
         float *to[2];
         bool out = false;
         if (g == 0) {
             PaSink k = {nullptr, nullptr, false};
             if (ok) {
-                k = pa_sink<true>(a, pl, x, share, r0 + c - x.tile * R, tok, head, ew == 0);
+                k = pa_sink<true>(a, pl, x, share, r0 + c - x.tile * R, tok, head, nowhere, ew == 0);
                 if (!k.out && ew == 0) *k.ml = make_float2(m, l);
             }
             out = k.out;
@@ -561,7 +563,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
         for (int k = 0; k < 2; k++) to[k] = *(float **)(tr + (8 * k + (lane >> 3)) * PM_COLS);
         constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
-        const bool none = out && !sq.bad && sq.len - sq.nq + ri < 0;
+        const bool none = out && nowhere;
         const float f = none ? 0.0f : out ? VS / l : VS;
 #pragma unroll
         for (int s = 0; s < NS; s++) {                       // 32 elements at a time: value tiles 2 s, 2 s + 1

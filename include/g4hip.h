@@ -297,7 +297,9 @@ typedef struct {
  * [0, n_pages) where a position is stored or read; a length outside [0,
  * max_len] or past the table's table_stride pages, offsets that descend or
  * leave [0, n_tok].  Such rows are not appended, and read as NaN by the
- * attention; nothing outside the pools and the given arrays is touched. */
+ * attention, which ends the batch at the first sequence of such offsets: every
+ * row from there on reads as NaN.  Nothing outside the pools and the given
+ * arrays is touched. */
 enum { G4H_PAGED_BAD_PAGE = 1, G4H_PAGED_BAD_BATCH = 2 };
 /* The batch.  Its arrays live on the device, so that a captured graph is
  * replayed with other lengths and pages; the host values bound them.  Sequence

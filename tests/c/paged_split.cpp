@@ -5,8 +5,10 @@
 // Reads batches from stdin, one a line of whole numbers:
 //   kv_type n_head n_kv hd page max_len n_prefix window n_seq n_tok table_stride has_off,
 //   n_seq lengths, and with has_off n_seq + 1 offsets.
-// Prints a line a batch: "ok" and counts, or what is wrong with the split.  Rows of
-// tokens that no sequence holds must not be noted as if they had results.
+// Prints a line a batch: "ok" and counts, or what is wrong with the split.  The
+// workspace starts with notes that lead out of it: what the join reads has to have
+// been noted by the call, for rows of no sequence too.
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -46,6 +48,7 @@ struct Run {
     std::unordered_map<size_t, Part> places;                 // byte offset in the workspace
     std::vector<int> out;                                    // times a row was written out
     long pieces = 0;
+    int n_seq = 0;                                           // before the first torn one
 };
 
 template <bool MANY>
@@ -54,12 +57,12 @@ void follow(Run &r) {
     const PagedPlan &pl = r.pl;
     const PagedList &y = pa_list<MANY>(pl);
     std::vector<int64_t> upto(1, 0);                         // steps before each sequence
-    for (int s = 0; s < a.b.n_seq; s++) upto.push_back(upto.back() + (int64_t)pa_steps<MANY>(a, pl, s) * a.p.n_kv);
+    for (int s = 0; s < r.n_seq; s++) upto.push_back(upto.back() + (int64_t)pa_steps<MANY>(a, pl, paged_seq(a.p, a.b, s)) * a.p.n_kv);
     const int64_t all = upto.back() + (int64_t)y.pre_tiles * y.pre_steps * a.p.n_kv;
     if (all > 0x7fffffff) wrong("%lld steps do not fit 32 bits", (long long)all);
     const int total = (int)all, share = pa_share(y, total);
     auto find = [&](int u, int &seq, int &before) {
-        int lo = 0, hi = a.b.n_seq;                          // the last with upto <= u
+        int lo = 0, hi = r.n_seq;                          // the last with upto <= u
         while (hi - lo > 1) (upto[(lo + hi) / 2] <= u ? lo : hi) = (lo + hi) / 2;
         seq = lo;
         before = (int)upto[lo];
@@ -67,7 +70,7 @@ void follow(Run &r) {
     for (int wg = 0; wg < y.wgs; wg++) {
         const int first = wg * share, stop = std::min(first + share, total);
         for (int u = first; u < stop;) {
-            const PaPiece x = pa_piece_by<MANY>(a, pl, wg, u, first, stop, find);
+            const PaPiece x = pa_piece_by<MANY>(a, pl, r.n_seq, wg, u, first, stop, find);
             if (x.took <= 0) wrong("a piece of no steps at %d", u);
             u += x.took;
             if (x.n == 0) {
@@ -83,7 +86,7 @@ void follow(Run &r) {
                 const int tok = x.sq.t0 + i / G, head = x.kvh * G + i % G;
                 if (tok < 0 || tok >= a.b.n_tok) wrong("token %d", tok);
                 const size_t row = (size_t)tok * a.n_head + head;
-                const PaSink to = pa_sink<MANY>(a, pl, x, share, i - r0, tok, head, true);
+                const PaSink to = pa_sink<MANY>(a, pl, x, share, i - r0, tok, head, !x.sq.bad && x.sq.len - x.sq.nq + i / G < 0, true);
                 if (to.out) {
                     r.out[row]++;
                     continue;
@@ -100,14 +103,18 @@ void follow(Run &r) {
 void joined(Run &r) {
     const PagedAttn &a = r.a;
     const int all = a.b.n_tok * a.n_head;
-    std::vector<char> held(a.b.n_tok, 0);
-    for (int s = 0; s < a.b.n_seq; s++) {
+    std::vector<char> held(a.b.n_tok, 0), none(a.b.n_tok, 0);
+    for (int s = 0; s < r.n_seq; s++) {
         const PagedSeq q = paged_seq(a.p, a.b, s);
-        for (int i = 0; i < q.nq; i++) held[q.t0 + i] = 1;
+        for (int i = 0; i < q.nq; i++) {
+            if (held[q.t0 + i]++) wrong("token %d is two sequences'", q.t0 + i);
+            none[q.t0 + i] = !q.bad && q.len - q.nq + i < 0;
+        }
     }
     for (int row = 0; row < all; row++) {
         if (!held[row / a.n_head]) {
             if (r.out[row]) wrong("row %d without a sequence is written", row);
+            if (r.y.join && r.own[row].x >> 2) wrong("row %d without a sequence is joined", row);
             continue;
         }
         if (!r.y.join) {
@@ -115,12 +122,13 @@ void joined(Run &r) {
             continue;
         }
         const uint2 own = r.own[row], pre = a.b.n_prefix > 0 ? r.pre[row] : make_uint2(0, 0);
-        const int n_pre = pre.x >> 1, n_own = own.x >> 1;
+        const int n_pre = pre.x >> 2, n_own = own.x >> 2;
         if (n_own == 0) {
             if (r.out[row] != 1) wrong("row %d is written %d times", row, r.out[row]);
             continue;
         }
         if (r.out[row]) wrong("row %d is written and joined", row);
+        if ((own.x >> 1 & 1) != (none[row / a.n_head])) wrong("row %d is noted as %s a position", row, own.x & 2 ? "without" : "with");
         if (n_pre > 4096 || n_own > 4096) wrong("row %d of %d + %d pieces", row, n_pre, n_own);
         int at = 0;                                          // steps so far, of the prefix's tile, then of the own one
         bool in_pre = n_pre > 0;
@@ -182,7 +190,14 @@ int main() {
         r.out.assign((size_t)n_tok * n_head, 0);
         if (r.y.join) r.pl.own = r.own.data();
         r.pl.pre = r.pre.data();
+        // the batch ends at its first torn sequence, behind which rows become NaN
+        while (r.n_seq < n_seq && !paged_seq(a.p, a.b, r.n_seq).torn) r.n_seq++;
+        std::vector<float> out(r.n_seq < n_seq ? (size_t)n_tok * n_head * hd : 0, 1.0f);
+        a.out = out.data();
         try {
+            pa_outside(a, r.pl, r.n_seq, 0, 1);
+            for (size_t i = 0; i < out.size(); i++)
+                if (std::isnan(out[i]) != (i >= (size_t)pa_tokens(a.b, r.n_seq) * n_head * hd)) wrong("element %zu behind a torn sequence", i);
             if (r.pl.many.rows) follow<true>(r);
             if (r.pl.few.rows) follow<false>(r);
             joined(r);

@@ -1,0 +1,81 @@
+"""The paged KV cache's calls at the edges of what the header allows: offsets that
+are not a whole batch's, and offsets that are wrong."""
+import numpy as np
+import pytest
+
+from paged_util import F16, Q4_0, Q8_0, Case
+
+pytestmark = pytest.mark.gpu
+TYPES = [F16, Q8_0, Q4_0]
+IDS = ["f16", "q8_0", "q4_0"]
+
+
+def _guarded(G, c, scale, **more):
+    """Attention into rows with more behind them, which have to stay."""
+    out = G.Buffer.from_array(np.full((c.n_tok + 5, c.n_head, c.hd), 7.5, np.float32))
+    need = G.paged_attn_workspace_bytes(c.kv, c.batch, c.n_head)
+    ws = G.Buffer.from_array(np.full(need + 4096, 0x7f, np.uint8))
+    G.paged_attn(c.kv, c.batch, c.d["q"], c.n_head, out, scale=scale, ws=ws.ptr, **more)
+    got = out.download(np.float32, (c.n_tok + 5, c.n_head, c.hd))
+    assert np.all(got[c.n_tok:] == 7.5) and np.all(ws.download(np.uint8, (ws.nbytes,))[need:] == 0x7f)
+    return got[:c.n_tok]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("n_prefix", [0, 40, 700])
+@pytest.mark.parametrize("heads", [(2, 1), (40, 2)])
+@pytest.mark.parametrize("offs,good", [
+    ([0, 2, 9, 6, 8], 2),                                  # past n_tok, then descending
+    ([0, 5, 2, 6, 3], 5),                                  # tokens of two sequences each
+    ([0, 8, 0, 8, 0], 8),
+    ([-1, 2, 3, 4, 8], 0),
+    ([1 << 30, 2, 3, 4, 8], 0),
+    ([0, 1, 2, 5, -1 << 31], 5),
+])
+def test_rows_from_torn_offsets_on_read_as_nan(gpu, t, n_prefix, heads, offs, good):
+    new = [offs[i + 1] - offs[i] if 0 <= offs[i] <= offs[i + 1] <= 8 else 1 for i in range(4)]
+    c = Case(gpu, t, *heads, 64, 16, [300, 290, 310, 200], new=new, pad=8 - sum(new) if sum(new) < 8 else 0, n_prefix=n_prefix, seed=60)
+    c.n_tok = c.batch.struct.n_tok = 8
+    c.q = c.rng.standard_normal((8, heads[0], 64)).astype(np.float32)
+    c.d["q"] = gpu.Buffer.from_array(c.q)
+    c.off = np.asarray(offs, np.int32)
+    c.d["off"].upload(c.off)
+    last = next(s for s in range(4) if not 0 <= offs[s] <= offs[s + 1] <= 8)
+    c.new, c.lens = new[:last], c.lens[:last]
+    want, tol = c.expect(0.125)
+    got = _guarded(gpu, c, 0.125)
+    assert c.kv.status() == gpu.PAGED_BAD_BATCH
+    assert np.all(np.abs(got[:good] - want[:good]) <= tol[:good])
+    assert np.isnan(got[good:]).all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("n_prefix,window", [(0, 0), (40, 0), (700, 100)])
+def test_offsets_torn_behind_many_sequences(gpu, t, n_prefix, window):
+    # the first bad offset lies past the 64 sequences that are looked at at once
+    n = 150
+    new = [i % 3 for i in range(n)]
+    c = Case(gpu, t, 4, 2, 64, 16, [v + 7 * i % 90 for i, v in enumerate(new)], new=new, n_prefix=n_prefix, seed=61)
+    want, tol = c.expect(0.125, window=window)
+    off = c.off.copy()
+    off[132] = off[130] - 1
+    c.d["off"].upload(off)
+    got, end = _guarded(gpu, c, 0.125, window=window), int(off[131])
+    assert c.kv.status() == gpu.PAGED_BAD_BATCH
+    assert np.all(np.abs(got[:end] - want[:end]) <= tol[:end]) and np.isnan(got[end:]).all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("n_prefix", [0, 40])
+@pytest.mark.parametrize("lens,new", [([300, 290, 310, 200], [4, 1, 2, 1]), ([90, 150, 60, 70], [60, 70, 30, 2])])
+def test_a_part_of_a_batch(gpu, t, n_prefix, lens, new):
+    # sequences 1 and 2 of four, over the same arrays: rows of the others are left
+    c = Case(gpu, t, 4, 2, 64, 16, lens, new=new, pad=1, n_prefix=n_prefix, seed=62)
+    want, tol = c.expect(0.125)
+    s = c.batch.struct
+    s.n_seq, s.q_off_dev, s.len_dev, s.table_dev = 2, s.q_off_dev + 4, s.len_dev + 4, s.table_dev + 4 * c.stride
+    got = _guarded(gpu, c, 0.125)
+    a, b = int(c.off[1]), int(c.off[3])
+    assert np.all(np.abs(got[a:b] - want[a:b]) <= tol[a:b])
+    assert np.all(got[:a] == 7.5) and np.all(got[b:] == 7.5)
+    assert c.kv.status() == 0

@@ -30,12 +30,12 @@ def split(tmp_path_factory):
     return run
 
 
-def batch(t, n_head, n_kv, hd, lens, new=None, pad=0, n_prefix=0, window=0, page=16, max_len=None, offs=None):
+def batch(t, n_head, n_kv, hd, lens, new=None, pad=0, n_prefix=0, window=0, page=16, max_len=None, offs=None, n_tok=None):
     """One line of tests/c/paged_split.cpp; new None: one token each."""
     max_len = max(lens, default=0) if max_len is None else max_len
     if offs is None and new is not None:
         offs = [0] + [int(x) for x in np.cumsum(new)]
-    n_tok = (offs[-1] if offs is not None else len(lens)) + pad
+    n_tok = (offs[-1] if offs is not None else len(lens)) + pad if n_tok is None else n_tok
     head = [t, n_head, n_kv, hd, page, max_len, n_prefix, window, len(lens), n_tok, -(-max_len // page), int(offs is not None)]
     return " ".join(str(int(x)) for x in head + list(lens) + list(offs or []))
 
@@ -84,3 +84,41 @@ def test_any_batch(split, seed):
                              n_prefix=int(rng.choice([0, log(1, 20000), log(1, 200)])), window=int(rng.choice([0, 0, 1, log(1, 30000)])),
                              max_len=max(lens) + int(rng.integers(0, 300))))
     _good(split, batches)
+
+
+def test_torn_offsets(split):
+    # offsets that descend, leave the tokens or give them to several sequences: no
+    # more steps than the host counted, and no row joined that was not noted
+    many = [0, 4096] * 700
+    _good(split, [
+        batch(F16, 2, 1, 64, [60] * 4, n_prefix=20, offs=[0, 5, 2, 6, 3], n_tok=6),
+        batch(F16, 2, 1, 64, [60, 40, 20], offs=[0, 2, 9, 6], n_tok=6),
+        batch(F16, 2, 1, 64, [6000] * 4, n_prefix=20, offs=[0, 5, 2, 6, 3], n_tok=6),
+        batch(F16, 2, 1, 64, [60] * 2, n_prefix=20, offs=[-3, 4, 6], n_tok=6),
+        batch(F16, 2, 1, 64, [600] * 2, n_prefix=20, offs=[1 << 30, 4, 6], n_tok=6),
+        batch(F16, 2, 1, 64, [600] * 2, n_prefix=20, offs=[0, 0, 7], n_tok=6),
+        batch(F16, 2, 1, 64, [600] * 2, n_prefix=20, offs=[0, 6, -1 << 31], n_tok=6),
+        batch(F16, 4, 4, 64, [1 << 20] * (len(many) - 1), n_prefix=20, offs=many, n_tok=4096),
+        batch(F16, 4, 4, 64, [1 << 20] * (len(many) - 1), offs=many, n_tok=4096),
+    ])
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_any_offsets(split, seed):
+    rng = np.random.default_rng(100 + seed)
+    batches = []
+    for _ in range(150):
+        n_seq, n_tok, n_kv, hd = int(rng.integers(1, 130)), int(rng.integers(1, 60)), int(rng.choice([1, 3])), int(rng.choice([64, 512]))
+        offs = np.sort(rng.integers(0, n_tok + 1, n_seq + 1))
+        for _ in range(int(rng.integers(0, 3))):
+            offs[rng.integers(0, n_seq + 1)] = rng.integers(-5, n_tok + 6)
+        lens = [int(n) for n in rng.integers(-2, 600, n_seq)]
+        batches.append(batch(F16, n_kv * int(rng.choice([1, 4, 20])), n_kv, hd, lens, n_prefix=int(rng.choice([0, 30, 900])), max_len=560,
+                             window=int(rng.choice([0, 50])), offs=[int(x) for x in offs], n_tok=n_tok))
+    _good(split, batches)
+
+
+def test_rows_before_and_behind_the_sequences(split):
+    # a batch that is a part of a longer one's offsets
+    _good(split, [batch(t, 8, 2, 128, [700, 600, 3], n_prefix=p, offs=[4, 5, 5 + n, 7 + n], n_tok=20 + n)
+                  for t in (F16, Q8_0) for p in (0, 50, 3000) for n in (1, 2, 50)])
