@@ -70,7 +70,9 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
 
 }  // namespace
 
-size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head) { return paged_layout(p, b, n_head / p.n_kv, 0).total; }
+size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head) {
+    return b.n_tok == 0 || b.n_seq == 0 ? 0 : paged_layout(p, b, n_head / p.n_kv, 0).total;
+}
 
 hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s) {
     const PagedPool &p = a.p;

@@ -15,7 +15,7 @@ struct PagedLayout {
     bool join;
     size_t fo, fml, mo, mml, own, pre, wo, wml, total;
 };
-// window 0 gives the most workspace
+// of a batch with tokens and sequences; window 0 gives the most workspace
 inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
     PagedLayout y;
     PagedPlan &pl = y.pl;
