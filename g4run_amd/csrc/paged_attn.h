@@ -178,9 +178,22 @@ __device__ __forceinline__ PaUnits pa_units(const PagedPool &p, const int *table
     x.row = kvh * p.page + (u - ent * p.units) * 16;
     return x;
 }
-// before their first use (not with the load, which would be waited for there)
-__device__ __forceinline__ void pa_check(const PagedPool &p, PaUnits &x, bool &bad) {
-    if ((uint64_t)(int64_t)x.id >= (uint64_t)p.n_pages) { bad = true; x.id = 0; }
+// before their first use (not with the load, which would be waited for there): the
+// lanes whose page lies outside the pool, read as page 0 instead
+__device__ __forceinline__ uint64_t pa_check(const PagedPool &p, PaUnits &x) {
+    const bool out = (uint64_t)(int64_t)x.id >= (uint64_t)p.n_pages;
+    if (out) x.id = 0;
+    return __ballot(out);
+}
+// whether the lane's row, of positions [rlo, rhi], attends one of them; a page that
+// it does not attend (before its window, say, and given away) may be any
+__device__ __forceinline__ bool pa_hits(uint64_t out, int first, int stride, int last, int rlo, int rhi) {
+    bool hit = false;
+    for (; out; out &= out - 1) {
+        const int k = __ffsll((unsigned long long)out) - 1, pos = 16 * min(first + stride * (k >> 1) + (k & 1), last);
+        hit |= rlo <= pos + 15 && rhi >= pos;
+    }
+    return hit;
 }
 // the offset of a unit's rows in the pools and, quantized, of their scales
 struct PaUnit {

@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         int base = start + 32 * pw;
         if (iters) {
             us = pa_units(p, x.table, base >> 4, 2 * PW, last, kvh);
-            pa_check(p, us, bad);
+            bad |= pa_hits(pa_check(p, us), base >> 4, 2 * PW, last, rlo, rhi);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             if constexpr (KVT != F16) pa_load_scales<HD, HE, KVT>(kv, p, nx, lane, ew);
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
             un[1] = nx[1];
             if ((it & 31) == 31 && it + 1 < iters) {
                 us = more_us;
-                pa_check(p, us, bad);
+                bad |= pa_hits(pa_check(p, us), (base >> 4) + 2 * PW, 2 * PW, last, rlo, rhi);
             }
             if (more) {
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
@@ -471,9 +471,10 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                 }
             }
         }
+        bad &= rc < rows;
         if (__any(bad)) {
             if (lane == 0 && !sq.bad) paged_flag(p, PAGED_BAD_PAGE);
-            l = __builtin_nanf("");
+            if (bad) l = __builtin_nanf("");
         }
 
         // the position waves' results joined in order, 8 rows at a time

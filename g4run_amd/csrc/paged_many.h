@@ -305,9 +305,10 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         PmStage<HD, KVT> st;
         PaUnits us, more_us;                                 // of 32 steps, and of the next 32
         PaUnit un[2], nx[2];
+        uint64_t outside = 0;                                // of the first 32 steps
         if (iters) {
             us = pa_units(p, x.table, start >> 4, 2, last, kvh);
-            pa_check(p, us, bad);
+            outside = pa_check(p, us);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             pm_load<HD, KVT>(st, p, nx, tid);
@@ -324,6 +325,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                 rlo = max(0, pa_token_pos(p, b, n_seq, tok) + 1 - a.window);
             }
         }
+        bad |= pa_hits(outside, start >> 4, 2, last, rlo, rhi);
         __syncthreads();                                     // the previous piece's tiles and rows are used
         // Queries, 32 elements at a time through the wave's part of LDS: whole lines
         // from memory, then the operand's 8 elements of one row.
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             un[1] = nx[1];
             if ((it & 31) == 31 && it + 1 < iters) {
                 us = more_us;
-                pa_check(p, us, bad);
+                bad |= pa_hits(pa_check(p, us), (base + 32) >> 4, 2, last, rlo, rhi);
             }
             if (it + 1 < iters) {
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
@@ -537,9 +539,10 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                 });
             }
         }
+        bad &= ok;
         if (__any(bad)) {
             if (lane == 0 && !sq.bad) paged_flag(p, PAGED_BAD_PAGE);
-            l = __builtin_nanf("");
+            if (bad) l = __builtin_nanf("");
         }
         l += partner<16>(l);
         l += partner<32>(l);

@@ -294,7 +294,8 @@ typedef struct {
     int *status_dev;       /* one device word that calls OR G4H_PAGED_* into, or NULL */
 } g4h_paged_kv;
 /* What a call found in the batch's device arrays: a page id outside
- * [0, n_pages) where a position is stored or read; a length outside [0,
+ * [0, n_pages) where a position is stored or a row attends (the ids of pages
+ * before all windows, or behind a sequence's end, may be any); a length outside [0,
  * max_len] or past the table's table_stride pages, offsets that descend or
  * leave [0, n_tok].  Such rows are not appended, and read as NaN by the
  * attention, which ends the batch at the first sequence of such offsets: every

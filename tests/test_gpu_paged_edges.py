@@ -79,3 +79,52 @@ def test_a_part_of_a_batch(gpu, t, n_prefix, lens, new):
     assert np.all(np.abs(got[a:b] - want[a:b]) <= tol[a:b])
     assert np.all(got[:a] == 7.5) and np.all(got[b:] == 7.5)
     assert c.kv.status() == 0
+
+
+# -------------------------------------------------------------- pages given away
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd,n_head,n_kv", [(64, 4, 2), (128, 8, 4), (256, 4, 2), (512, 2, 1), (64, 40, 2)])
+@pytest.mark.parametrize("page", [16, 48])
+@pytest.mark.parametrize("new", [None, [2, 1, 3, 1], [70, 100, 1, 64]])
+def test_pages_before_the_window_may_be_given_away(gpu, t, hd, n_head, n_kv, page, new):
+    window, lens = 50, [150, 113, 99, 49]
+    c = Case(gpu, t, n_head, n_kv, hd, page, lens, new=[min(n, m) for n, m in zip(new, lens)] if new else None, seed=hd + page)
+    gone = 0
+    for s, (n, m) in enumerate(zip(c.lens, c.new)):
+        k = max(0, n - m + 1 - window) // page             # whole pages that no token of the call attends
+        c.table[s, :k] = -1 if s % 2 else c.pool.n_pages
+        gone += k
+    assert gone
+    c.d["table"].upload(c.table)
+    c.check(window=window)
+    c.check(window=window, cap=20.0)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("n_seq", [1, 30])
+@pytest.mark.parametrize("own", [60, 200])
+def test_a_prefix_before_all_windows_may_be_given_away(gpu, t, n_seq, own):
+    # its last pages are still attended by the shorter sequences
+    c = Case(gpu, t, 4, 2, 64, 16, [own + i % 7 for i in range(n_seq)], n_prefix=150, seed=63)
+    k = max(0, 150 + own - 100) // 16
+    c.prefix[:k] = -1
+    c.d["pre"].upload(c.prefix)
+    c.check(window=100)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd,n_head,n_kv", [(64, 4, 2), (256, 4, 2), (512, 2, 1)])
+@pytest.mark.parametrize("n,window", [(3, 0), (90, 0), (90, 20), (6, 20)])
+def test_a_bad_page_reaches_only_the_rows_that_attend_it(gpu, t, hd, n_head, n_kv, n, window):
+    # a chunk of n tokens; the page of positions 112 .. 127 is wrong
+    c = Case(gpu, t, n_head, n_kv, hd, 16, [130, 130], new=[n, n], seed=64)
+    c.table[0, 7] = -5
+    c.d["table"].upload(c.table)
+    want, tol = c.expect(0.1, window=window)
+    got = c.attn(0.1, window=window)
+    hit = np.zeros(c.n_tok, bool)
+    pos = 130 - n + np.arange(n)
+    hit[:n] = (pos >= 112) & ((pos - window < 127) if window else True)
+    assert np.isnan(got[hit]).all()
+    assert np.all(np.abs(got - want)[~hit] <= tol[~hit])
+    assert c.kv.status() == gpu.PAGED_BAD_PAGE
