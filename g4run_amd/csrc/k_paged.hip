@@ -74,10 +74,11 @@ size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head)
     return b.n_tok == 0 || b.n_seq == 0 ? 0 : paged_layout(p, b, n_head / p.n_kv, 0).total;
 }
 
-hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s) {
+hipError_t launch_paged_attn(PagedAttn a, hipStream_t s) {
     const PagedPool &p = a.p;
     const PagedBatch &b = a.b;
     if (b.n_tok == 0 || b.n_seq == 0) return hipSuccess;
+    a.window = paged_window(b, a.window);
     const PagedLayout y = paged_layout(p, b, a.grp, a.window);
     const PagedPlan pl = paged_places(y, a.ws);
     if (pl.many.rows)

@@ -133,6 +133,6 @@ struct PagedAttn {
 // workspace of a call: the workgroups' partial results and where each (token, head)
 // row's lie, 0 where a call writes its outputs directly
 size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head);
-hipError_t launch_paged_attn(const PagedAttn &a, hipStream_t s);
+hipError_t launch_paged_attn(PagedAttn a, hipStream_t s);
 
 }  // namespace g4

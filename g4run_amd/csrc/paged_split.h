@@ -10,6 +10,10 @@ namespace g4 {
 
 inline int pa_ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// A window that hides no position is none; with any other the device's sums of
+// positions and windows fit 32 bits (a token before position 0 counts from below 0).
+inline int paged_window(const PagedBatch &b, int window) { return window >= b.n_prefix + b.max_len ? 0 : window; }
+
 struct PagedLayout {
     PagedPlan pl;
     bool join;

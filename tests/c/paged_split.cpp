@@ -80,6 +80,10 @@ void follow(Run &r) {
             r.pieces++;
             if (x.kvh >= a.p.n_kv || x.step < 0 || x.step + x.n > x.all) wrong("steps %d + %d of %d of head %d", x.step, x.n, x.all, x.kvh);
             if (x.end > x.start && (x.start < 0 || x.end > x.seglen)) wrong("positions %d .. %d of %d", x.start, x.end, x.seglen);
+            if (!x.pre && !x.sq.bad) {                       // lowest position of the tile's first token: this piece's start, but for its steps
+                const int64_t p0 = (int64_t)x.sq.len - x.sq.nq + (MANY ? (int64_t)x.tile * y.toks : 0), lo = std::max<int64_t>(0, a.window ? p0 + 1 - a.window : 0);
+                if (x.start != (lo & ~31) + ((int64_t)x.step << y.shift)) wrong("a piece starts at %d, its tile at %lld", x.start, (long long)lo);
+            }
             const int G = a.grp, r0 = MANY ? x.tile * y.rows : 0, r1 = MANY ? std::min(x.sq.nq * G, r0 + y.rows) : x.sq.nq * G;
             if (!MANY && r1 > y.rows) wrong("%d rows of a tile of %d", r1, y.rows);
             for (int i = r0; i < r1; i++) {
@@ -176,9 +180,9 @@ int main() {
         a.n_head = n_head;
         a.grp = n_head / n_kv;
         a.os = (size_t)n_head * hd;
-        a.window = window;
+        a.window = paged_window(a.b, window);
         a.ws = (uint8_t *)0x100000000;                       // never read or written
-        r.y = paged_layout(a.p, a.b, a.grp, window);
+        r.y = paged_layout(a.p, a.b, a.grp, a.window);
         if (r.y.total > paged_layout(a.p, a.b, a.grp, 0).total) {
             printf("a window needs more workspace\n");
             continue;

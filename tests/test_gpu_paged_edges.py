@@ -128,3 +128,14 @@ def test_a_bad_page_reaches_only_the_rows_that_attend_it(gpu, t, hd, n_head, n_k
     assert np.isnan(got[hit]).all()
     assert np.all(np.abs(got - want)[~hit] <= tol[~hit])
     assert c.kv.status() == gpu.PAGED_BAD_PAGE
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("n_prefix", [0, 40])
+@pytest.mark.parametrize("heads", [(2, 1), (40, 2)])
+def test_the_largest_window_with_padded_slots(gpu, t, n_prefix, heads):
+    # tokens before position 0 among others, and a window as large as an int
+    for lens, new in (([0, 5, 40], [3, 9, 40]), ([5, 70, 0], [9, 60, 2]), ([0, 3, 2, 60], [2, 4, 5, 1])):
+        c = Case(gpu, t, *heads, 64, 16, lens, new=new, n_prefix=n_prefix, seed=65)
+        for window in ((1 << 31) - 1, (1 << 31) - 3, n_prefix + max(lens), n_prefix + max(lens) - 1):
+            c.check(window=window)

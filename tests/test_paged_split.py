@@ -122,3 +122,11 @@ def test_rows_before_and_behind_the_sequences(split):
     # a batch that is a part of a longer one's offsets
     _good(split, [batch(t, 8, 2, 128, [700, 600, 3], n_prefix=p, offs=[4, 5, 5 + n, 7 + n], n_tok=20 + n)
                   for t in (F16, Q8_0) for p in (0, 50, 3000) for n in (1, 2, 50)])
+
+
+@pytest.mark.parametrize("t", [F16, Q8_0])
+def test_windows_of_any_size(split, t):
+    # padded slots hold tokens before position 0: a window as large as an int is no window
+    for window in (1 << 26, (1 << 31) - 2, (1 << 31) - 1):
+        _good(split, [batch(t, n_head, 2, 64, lens, new=new, n_prefix=p, window=window)
+                      for n_head in (2, 40) for p in (0, 50) for lens, new in (([0, 5, 40], [3, 9, 40]), ([5, 700, 0], [200, 600, 200]), ([3] * 9, [4] * 9))])
