@@ -979,6 +979,18 @@ static int paged_rows(const char *fn, const char *what, const void *ptr, size_t 
     if (stride < row && n_tok > 1) return fail(G4H_ERR_ARG, "%s: %s stride %zu is smaller than a row of %zu", fn, what, stride, row);
     return G4H_OK;
 }
+// Whether rows of one array overlap rows of another.  Of one stride they may be
+// columns of one array; of two strides whose ranges meet they are taken to overlap.
+static bool paged_overlap(const float *a, size_t a_stride, size_t a_row, const float *b, size_t b_stride, size_t b_row, int n) {
+    if (n <= 0) return false;
+    typedef __int128 wide;                                   // strides may be anything
+    const wide d = ((wide)(uintptr_t)b - (wide)(uintptr_t)a) / 4, last = n - 1;
+    if (d >= last * (wide)a_stride + (wide)a_row || d + last * (wide)b_stride + (wide)b_row <= 0) return false;
+    if (n == 1 || a_stride != b_stride) return true;
+    const wide s = a_stride, k = d >= 0 ? d / s : -((s - 1 - d) / s), r = d - k * s;       // b's row j starts r behind a's row j + k
+    auto meets = [&](wide by) { return by >= -last && by <= last; };
+    return (meets(k) && r < (wide)a_row) || (meets(k + 1) && s - r < (wide)b_row);
+}
 
 extern "C" int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_rope *rope, int n_head, const float *q,
                                 size_t q_stride, float *q_out, size_t q_out_stride, const float *k, size_t k_stride, const float *v,
@@ -1066,10 +1078,7 @@ extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *bat
     if (!cap_ok || !std::isfinite(scale * 1024.0f) || (softcap && !std::isfinite(scale * 1024.0f / softcap)) || window < 0)
         return fail(G4H_ERR_ARG, "%s: scale=%g softcap=%g window=%d", fn, scale, softcap, window);
     if (a.b.n_prefix && !a.b.prefix) return fail(G4H_ERR_ARG, "%s: a prefix of %d positions needs its pages", fn, a.b.n_prefix);
-    if (a.b.n_tok) {
-        const size_t n = a.b.n_tok - 1;
-        if (q < out + n * out_stride + row && out < q + n * q_stride + row) return fail(G4H_ERR_ARG, "%s: q and out overlap", fn);
-    }
+    if (paged_overlap(q, q_stride, row, out, out_stride, row, a.b.n_tok)) return fail(G4H_ERR_ARG, "%s: q and out overlap", fn);
     const size_t need = paged_attn_workspace(a.p, a.b, n_head);
     if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
         return fail(G4H_ERR_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, ws ? ws_bytes : (size_t)0);

@@ -359,7 +359,8 @@ int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out
  * finite.
  * q / out: fp32 [n_tok][n_head][hd], at q_stride / out_stride floats per token
  * (0: packed); query head h reads KV head h / (n_head / n_kv), up to 128 heads a
- * KV head (64 of hd 512).  All in fp32
+ * KV head (64 of hd 512).  No row of out may overlap one of q: both may be
+ * columns of one array, at the same stride.  All in fp32
  * precision (queries and weights enter the matrix cores as two halves each),
  * unlike g4h_attn_decode, which rounds as the reference does.  The prefix's
  * rows are read once for the whole batch.  A non-finite cached value reaches

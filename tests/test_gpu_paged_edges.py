@@ -139,3 +139,22 @@ def test_the_largest_window_with_padded_slots(gpu, t, n_prefix, heads):
         c = Case(gpu, t, *heads, 64, 16, lens, new=new, n_prefix=n_prefix, seed=65)
         for window in ((1 << 31) - 1, (1 << 31) - 3, n_prefix + max(lens), n_prefix + max(lens) - 1):
             c.check(window=window)
+
+
+# ------------------------------------------------------------ fused rows
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("new", [None, [30, 2, 60]])
+def test_outputs_beside_the_queries_of_a_fused_row(gpu, t, new):
+    G = gpu
+    c = Case(G, t, 4, 2, 64, 16, [70, 5, 90], new=new, pad=1 if new else 0, n_prefix=20, seed=66)
+    w = 2 * 256 + 12
+    x = np.full((c.n_tok, w), 3.0, np.float32)
+    x[:, :256] = c.q.reshape(c.n_tok, 256)
+    b = G.Buffer.from_array(x)
+    G.paged_attn(c.kv, c.batch, b, 4, b.ptr + 4 * 260, scale=0.125, q_stride=w, out_stride=w)
+    got = b.download(np.float32, x.shape)
+    want, tol = c.expect(0.125)
+    n = c.n_tok - c.pad
+    assert np.all(np.abs(got[:n, 260:516].reshape(n, 4, 64) - want[:n]) <= tol[:n])
+    got[:n, 260:516] = 3.0
+    assert np.array_equal(got, x)

@@ -19,3 +19,24 @@ def test_an_empty_batch_needs_no_workspace(abi, n_seq, n_tok, q_off, n_prefix, n
     assert L.g4h_paged_attn_workspace_bytes(C.byref(kv), C.byref(b), n_head) == 0
     if not G._inited:
         assert _attn(L, kv, b, n_head=n_head, ws=None, wsb=0) == G.ERR_DEVICE
+
+
+def _rows(at, stride, row, n):
+    return [(at + i * stride, at + i * stride + row) for i in range(n)]
+
+
+@pytest.mark.parametrize("q_stride,out_stride", [(128, 128), (256, 256), (300, 300), (513, 513), (128, 256)])
+def test_queries_and_outputs_may_be_columns_of_one_array(abi, q_stride, out_stride):  # noqa: F811
+    G, L = abi
+    if G._inited:
+        pytest.skip("would run on the device")
+    kv, base, n, row = _kv(G), 1 << 20, 5, 128
+    b = _batch(G, n_tok=n)
+    for shift in list(range(-700, 701, 20)) + [127, 128, 129, 172, 255, 256, 385, -127, -128, -129, 1153, 1664]:
+        meet = any(x < d and c < y for x, y in _rows(0, q_stride, row, n) for c, d in _rows(shift, out_stride, row, n))
+        ranges = shift < (n - 1) * q_stride + row and shift + (n - 1) * out_stride + row > 0
+        rc = _attn(L, kv, b, q=base, qs=q_stride, out=base + 4 * shift, os=out_stride)
+        refused = meet if q_stride == out_stride else ranges
+        assert rc == (G.ERR_ARG if refused else G.ERR_DEVICE), (shift, meet)
+    assert _attn(L, kv, _batch(G, n_tok=1), q=base, qs=1 << 62, out=base + 4 * 128, os=1 << 62) == G.ERR_DEVICE
+    assert _attn(L, kv, b, q=base, qs=1 << 62, out=base + 4 * 128, os=1 << 62) == G.ERR_DEVICE
