@@ -1006,6 +1006,9 @@ extern "C" int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *b
         if (int rc = paged_rows(fn, "q", q, q_stride, qrow, a.b.n_tok)) return rc;
         if (int rc = paged_rows(fn, "q_out", q_out, q_out_stride, qrow, a.b.n_tok)) return rc;
         if (q == q_out && q_stride != q_out_stride && a.b.n_tok > 1) return fail(G4H_ERR_ARG, "%s: q rotated in place keeps its stride", fn);
+        if ((q != q_out && paged_overlap(q, q_stride, qrow, q_out, q_out_stride, qrow, a.b.n_tok)) ||
+            paged_overlap(k, k_stride, row, q_out, q_out_stride, qrow, a.b.n_tok) || paged_overlap(v, v_stride, row, q_out, q_out_stride, qrow, a.b.n_tok))
+            return fail(G4H_ERR_ARG, "%s: q_out overlaps what the call reads", fn);
     }
     a.r.n_rot = 0;
     a.r.interleaved = 0;

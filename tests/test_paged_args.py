@@ -40,3 +40,20 @@ def test_queries_and_outputs_may_be_columns_of_one_array(abi, q_stride, out_stri
         assert rc == (G.ERR_ARG if refused else G.ERR_DEVICE), (shift, meet)
     assert _attn(L, kv, _batch(G, n_tok=1), q=base, qs=1 << 62, out=base + 4 * 128, os=1 << 62) == G.ERR_DEVICE
     assert _attn(L, kv, b, q=base, qs=1 << 62, out=base + 4 * 128, os=1 << 62) == G.ERR_DEVICE
+
+
+def test_append_refuses_rotated_queries_over_what_it_reads(abi):  # noqa: F811
+    # n_head 2, n_kv 2, hd 64: rows of 128 floats each, three tokens
+    G, L = abi
+    kv, b, base, w = _kv(G), _batch(G), 1 << 20, 128 * 4 + 4
+    at = lambda col: base + 4 * col  # noqa: E731
+    fused = dict(q=at(0), qs=w, k=at(128), ks=w, v=at(256), vs=w)
+    for kw in [dict(qo=at(4), qos=w), dict(qo=at(100), qos=w), dict(qo=at(255), qos=w), dict(qo=at(300), qos=w), dict(qo=at(w - 1), qos=w),
+               dict(qo=at(-100), qos=w), dict(qo=at(-w - 127), qos=w), dict(qo=at(384), qos=w + 4)]:
+        assert _append(L, kv, b, **(fused | kw)) == G.ERR_ARG, kw
+    assert _append(L, kv, b, q=at(0), qo=at(64)) == G.ERR_ARG
+    assert _append(L, kv, b, q=at(0), qo=at(10000), k=at(10000), v=at(0)) == G.ERR_ARG
+    if not G._inited:
+        for kw in [dict(qo=at(0), qos=w), dict(qo=at(384), qos=w), dict(qo=at(388), qos=w), dict(qo=at(388 - w), qos=w), dict(qo=at(5000), qos=0)]:
+            assert _append(L, kv, b, **(fused | kw)) == G.ERR_DEVICE, kw
+        assert _append(L, kv, b, n_head=0, **(fused | dict(qo=at(100)))) == G.ERR_DEVICE
