@@ -972,9 +972,12 @@ static int paged_args(const char *fn, const g4h_paged_kv *kv, const g4h_paged_ba
     b.prefix = batch->prefix_dev;
     return G4H_OK;
 }
+// nothing to do: the arrays of no rows may be null
+static bool paged_empty(const PagedBatch &b) { return b.n_tok == 0 || b.n_seq == 0; }
 // a row array's stride: packed for 0, else at least a row; 4-byte aligned
-static int paged_rows(const char *fn, const char *what, const void *ptr, size_t &stride, size_t row, int n_tok) {
-    if (!ptr || (uintptr_t)ptr % 4) return fail(G4H_ERR_ARG, "%s: %s must be 4-byte aligned device memory", fn, what);
+static int paged_rows(const char *fn, const char *what, const void *ptr, size_t &stride, size_t row, const PagedBatch &b) {
+    const int n_tok = b.n_tok;
+    if ((!ptr && !paged_empty(b)) || (uintptr_t)ptr % 4) return fail(G4H_ERR_ARG, "%s: %s must be 4-byte aligned device memory", fn, what);
     if (stride == 0) stride = row;
     if (stride < row && n_tok > 1) return fail(G4H_ERR_ARG, "%s: %s stride %zu is smaller than a row of %zu", fn, what, stride, row);
     return G4H_OK;
@@ -1000,14 +1003,14 @@ extern "C" int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *b
     if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
     if (n_head < 0 || n_head > 65536) return fail(G4H_ERR_ARG, "%s: n_head=%d", fn, n_head);
     const size_t row = (size_t)a.p.n_kv * a.p.hd, qrow = (size_t)n_head * a.p.hd;
-    if (int rc = paged_rows(fn, "k", k, k_stride, row, a.b.n_tok)) return rc;
-    if (int rc = paged_rows(fn, "v", v, v_stride, row, a.b.n_tok)) return rc;
+    if (int rc = paged_rows(fn, "k", k, k_stride, row, a.b)) return rc;
+    if (int rc = paged_rows(fn, "v", v, v_stride, row, a.b)) return rc;
     if (n_head) {
-        if (int rc = paged_rows(fn, "q", q, q_stride, qrow, a.b.n_tok)) return rc;
-        if (int rc = paged_rows(fn, "q_out", q_out, q_out_stride, qrow, a.b.n_tok)) return rc;
+        if (int rc = paged_rows(fn, "q", q, q_stride, qrow, a.b)) return rc;
+        if (int rc = paged_rows(fn, "q_out", q_out, q_out_stride, qrow, a.b)) return rc;
         if (q == q_out && q_stride != q_out_stride && a.b.n_tok > 1) return fail(G4H_ERR_ARG, "%s: q rotated in place keeps its stride", fn);
-        if ((q != q_out && paged_overlap(q, q_stride, qrow, q_out, q_out_stride, qrow, a.b.n_tok)) ||
-            paged_overlap(k, k_stride, row, q_out, q_out_stride, qrow, a.b.n_tok) || paged_overlap(v, v_stride, row, q_out, q_out_stride, qrow, a.b.n_tok))
+        if (!paged_empty(a.b) && ((q != q_out && paged_overlap(q, q_stride, qrow, q_out, q_out_stride, qrow, a.b.n_tok)) ||
+            paged_overlap(k, k_stride, row, q_out, q_out_stride, qrow, a.b.n_tok) || paged_overlap(v, v_stride, row, q_out, q_out_stride, qrow, a.b.n_tok)))
             return fail(G4H_ERR_ARG, "%s: q_out overlaps what the call reads", fn);
     }
     a.r.n_rot = 0;
@@ -1044,7 +1047,7 @@ extern "C" int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *bat
     if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
     if (out_type != F16 && out_type != F32) return fail(G4H_ERR_TYPE, "%s: output type %d unsupported (f32, f16)", fn, out_type);
     const uintptr_t al = out_type == F16 ? 2 : 4;
-    if ((!k_out && !v_out) || (uintptr_t)k_out % al || (uintptr_t)v_out % al) return fail(G4H_ERR_ARG, "%s: null or misaligned outputs", fn);
+    if ((!k_out && !v_out && !paged_empty(a.b)) || (uintptr_t)k_out % al || (uintptr_t)v_out % al) return fail(G4H_ERR_ARG, "%s: null or misaligned outputs", fn);
     a.k_out = k_out;
     a.v_out = v_out;
     a.f16 = out_type == F16;
@@ -1074,14 +1077,14 @@ extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *bat
     if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
     if (int rc = check_paged_heads(fn, a.p, a.b, n_head)) return rc;
     const size_t row = (size_t)n_head * a.p.hd;
-    if (int rc = paged_rows(fn, "q", q, q_stride, row, a.b.n_tok)) return rc;
-    if (int rc = paged_rows(fn, "out", out, out_stride, row, a.b.n_tok)) return rc;
+    if (int rc = paged_rows(fn, "q", q, q_stride, row, a.b)) return rc;
+    if (int rc = paged_rows(fn, "out", out, out_stride, row, a.b)) return rc;
     // scores are taken in log2 units and for 8-bit pages by 512 times the scale
     const bool cap_ok = softcap == 0.0f || (softcap >= 0x1p-100f && softcap <= 0x1p100f);
     if (!cap_ok || !std::isfinite(scale * 1024.0f) || (softcap && !std::isfinite(scale * 1024.0f / softcap)) || window < 0)
         return fail(G4H_ERR_ARG, "%s: scale=%g softcap=%g window=%d", fn, scale, softcap, window);
-    if (a.b.n_prefix && !a.b.prefix) return fail(G4H_ERR_ARG, "%s: a prefix of %d positions needs its pages", fn, a.b.n_prefix);
-    if (paged_overlap(q, q_stride, row, out, out_stride, row, a.b.n_tok)) return fail(G4H_ERR_ARG, "%s: q and out overlap", fn);
+    if (a.b.n_prefix && !a.b.prefix && !paged_empty(a.b)) return fail(G4H_ERR_ARG, "%s: a prefix of %d positions needs its pages", fn, a.b.n_prefix);
+    if (!paged_empty(a.b) && paged_overlap(q, q_stride, row, out, out_stride, row, a.b.n_tok)) return fail(G4H_ERR_ARG, "%s: q and out overlap", fn);
     const size_t need = paged_attn_workspace(a.p, a.b, n_head);
     if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
         return fail(G4H_ERR_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, ws ? ws_bytes : (size_t)0);

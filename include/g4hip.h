@@ -313,7 +313,8 @@ enum { G4H_PAGED_BAD_PAGE = 1, G4H_PAGED_BAD_BATCH = 2 };
  * rows are in the pages prefix_dev[0 .. ceil(n_prefix / page)), shared by all:
  * own position p is position n_prefix + p. */
 typedef struct {
-    int n_seq, n_tok;          /* sequences; rows of the activations (any counts >= 0) */
+    int n_seq, n_tok;          /* sequences; rows of the activations (any counts >= 0; with none
+                                * of either a call does nothing, and its arrays may be NULL) */
     const int *q_off_dev;      /* n_seq + 1 ascending offsets, or NULL */
     const int *len_dev;        /* n_seq lengths, 0 .. max_len */
     const int *table_dev;      /* n_seq rows of table_stride page ids, position p in entry p / page */

@@ -158,3 +158,18 @@ def test_outputs_beside_the_queries_of_a_fused_row(gpu, t, new):
     assert np.all(np.abs(got[:n, 260:516].reshape(n, 4, 64) - want[:n]) <= tol[:n])
     got[:n, 260:516] = 3.0
     assert np.array_equal(got, x)
+
+
+@pytest.mark.parametrize("n_seq,n_tok", [(0, 0), (3, 0), (0, 3)])
+def test_an_empty_batch_does_nothing(gpu, n_seq, n_tok):
+    G = gpu
+    kv = G.PagedKV(Q8_0, 2, 64, 16, 4)
+    for n_prefix in (0, 20):
+        b = G.PagedBatch(n_seq, n_tok, None, None, 2, 32, n_prefix=n_prefix)
+        for n_head in (2, 40):
+            G.paged_append(kv, b, None, None, n_head=n_head, rope=G.Rope(64, 1e4))
+            G.paged_attn(kv, b, None, n_head, None)
+            G.paged_read(kv, b)
+    out = G.Buffer.from_array(np.full((3, 2, 64), 7.5, np.float32))
+    G.paged_attn(kv, b, out.ptr, 2, out.ptr)
+    assert np.all(out.download(np.float32, (3, 2, 64)) == 7.5) and kv.status() == 0

@@ -57,3 +57,19 @@ def test_append_refuses_rotated_queries_over_what_it_reads(abi):  # noqa: F811
         for kw in [dict(qo=at(0), qos=w), dict(qo=at(384), qos=w), dict(qo=at(388), qos=w), dict(qo=at(388 - w), qos=w), dict(qo=at(5000), qos=0)]:
             assert _append(L, kv, b, **(fused | kw)) == G.ERR_DEVICE, kw
         assert _append(L, kv, b, n_head=0, **(fused | dict(qo=at(100)))) == G.ERR_DEVICE
+
+
+@pytest.mark.parametrize("n_seq,n_tok", EMPTY)
+@pytest.mark.parametrize("n_prefix", [0, 5])
+def test_an_empty_batch_may_have_null_arrays(abi, n_seq, n_tok, n_prefix):  # noqa: F811
+    G, L = abi
+    kv, b = _kv(G), _batch(G, n_seq=n_seq, n_tok=n_tok, n_prefix=n_prefix, q_off_dev=None, len_dev=None, table_dev=None, prefix_dev=None)
+    calls = [lambda: _append(L, kv, b, q=None, qo=None, k=None, v=None), lambda: _attn(L, kv, b, q=None, out=None, ws=None, wsb=0),
+             lambda: L.g4h_paged_read(C.byref(kv), C.byref(b), G.F32, None, None, None)]
+    if G._inited:
+        assert [f() for f in calls] == [G.OK] * 3
+    else:
+        assert [f() for f in calls] == [G.ERR_DEVICE] * 3
+    # other arguments are still looked at
+    assert _append(L, kv, b, n_head=-1) == G.ERR_ARG and _attn(L, kv, b, window=-1) == G.ERR_ARG
+    assert L.g4h_paged_read(C.byref(kv), C.byref(b), G.Q8_0, None, None, None) == G.ERR_TYPE
