@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a) {
         const PagedSeq sq = paged_seq(p, a.b, seq);
         const int own = sq.len - sq.nq + (t - sq.t0);
         if (sq.bad || t < sq.t0 || t >= sq.t0 + sq.nq) {
-            if (threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
+            if (threadIdx.x == 0 && !paged_before(sq, seq, t)) paged_flag(p, PAGED_BAD_BATCH);
             continue;
         }
         if (own < 0) continue;
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedRead a) {
     const PagedSeq sq = paged_seq(p, a.b, seq);
     const int own = sq.len - sq.nq + (t - sq.t0);
     if (sq.bad || t < sq.t0 || t >= sq.t0 + sq.nq) {
-        if (threadIdx.x == 0) paged_flag(p, PAGED_BAD_BATCH);
+        if (threadIdx.x == 0 && !paged_before(sq, seq, t)) paged_flag(p, PAGED_BAD_BATCH);
         return;
     }
     if (own < 0) return;

@@ -99,6 +99,9 @@ __device__ __forceinline__ int paged_find(const PagedBatch &b, int t) {
     return lo + __popcll(__ballot(s <= hi && paged_ld(b.q_off, min(s, hi)) <= t));
 }
 
+// whether paged_find's sequence `seq` stands for none: t lies before all of them
+__device__ __forceinline__ bool paged_before(const PagedSeq &q, int seq, int t) { return seq == 0 && !q.torn && t < q.t0; }
+
 struct PagedAppend {
     PagedPool p;
     PagedBatch b;

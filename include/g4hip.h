@@ -308,7 +308,8 @@ enum { G4H_PAGED_BAD_PAGE = 1, G4H_PAGED_BAD_BATCH = 2 };
  * (q_off_dev NULL: one each, row s), and len[s] positions in its own pages, the
  * new tokens last: token i of n sits at len - n + i.  A token before position 0
  * (a slot of a padded batch with len 0) has no position: it is not appended and
- * attends nothing.  Rows behind the last sequence's are left as they were.
+ * attends nothing.  Rows before the first sequence's and behind the last's are
+ * left as they were (the arrays may be parts of a longer batch's).
  * With n_prefix, every sequence continues a prefix of n_prefix positions whose
  * rows are in the pages prefix_dev[0 .. ceil(n_prefix / page)), shared by all:
  * own position p is position n_prefix + p. */

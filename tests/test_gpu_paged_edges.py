@@ -3,7 +3,7 @@ are not a whole batch's, and offsets that are wrong."""
 import numpy as np
 import pytest
 
-from paged_util import F16, Q4_0, Q8_0, Case
+from paged_util import F16, Q4_0, Q8_0, Case, turn, values
 
 pytestmark = pytest.mark.gpu
 TYPES = [F16, Q8_0, Q4_0]
@@ -173,3 +173,30 @@ def test_an_empty_batch_does_nothing(gpu, n_seq, n_tok):
     out = G.Buffer.from_array(np.full((3, 2, 64), 7.5, np.float32))
     G.paged_attn(kv, b, out.ptr, 2, out.ptr)
     assert np.all(out.download(np.float32, (3, 2, 64)) == 7.5) and kv.status() == 0
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("new", [[4, 1, 2, 1], [300, 700, 600, 500]])
+def test_append_and_read_of_a_part_of_a_batch(gpu, t, new):
+    # rows of sequences 1 and 2 of four are stored, rotated and read, the others left, and nothing is flagged
+    G = gpu
+    c = Case(G, t, 2, 1, 64, 16, [n + 20 for n in new], new=new, pad=2, seed=67)
+    s = c.batch.struct
+    s.n_seq, s.q_off_dev, s.len_dev, s.table_dev = 2, s.q_off_dev + 4, s.len_dev + 4, s.table_dev + 4 * c.stride
+    a, b = int(c.off[1]), int(c.off[3])
+    k, v = (c.rng.standard_normal((c.n_tok, 1, 64)).astype(np.float32) for _ in range(2))
+    kb, vb, qo = G.Buffer.from_array(k), G.Buffer.from_array(v), G.Buffer.from_array(np.full_like(c.q, 7.5))
+    G.paged_append(c.kv, c.batch, kb, vb, q=c.d["q"], q_out=qo, n_head=2, rope=G.Rope(64, 1e4))
+    ko, vo = (G.Buffer.from_array(np.full(k.shape, 7.5, np.float32)) for _ in range(2))
+    G.paged_read(c.kv, c.batch, ko, vo)
+    assert c.kv.status() == 0
+    pos = np.zeros(c.n_tok)
+    pos[a:b] = np.concatenate([c.lens[i] - c.new[i] + np.arange(c.new[i]) for i in (1, 2)])
+    q, gk, gv = qo.download(np.float32, c.q.shape), ko.download(np.float32, k.shape), vo.download(np.float32, v.shape)
+    for x in (q, gk, gv):
+        assert np.all(x[:a] == 7.5) and np.all(x[b:] == 7.5)
+    want = turn(c.q, pos, 64, 1e4)
+    assert np.all(np.abs(q - want)[a:b] <= np.abs(c.q).max() * 2.0 ** -20)
+    assert np.array_equal(gv[a:b], values(t, v)[a:b].astype(np.float32))
+    changed = (c.kv.v.download(np.uint8, c.pool.v.shape) != c.pool.v).any(1)
+    assert set(np.flatnonzero(changed)) <= {int(p) for i in (1, 2) for p in c.table[i]}
