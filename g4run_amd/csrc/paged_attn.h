@@ -57,6 +57,7 @@ struct PagedList {
 };
 struct PagedPlan {
     PagedList few, many;             // rows 0: the kernel does not run
+    int all;                         // (token, head) rows of the call
     uint32_t grp_inv;                // rows to tokens: r / grp == r * grp_inv >> 16 for r < 16
     // where a (token, head) row's partial results lie, own positions and prefix:
     // count << 2 | whether it has no position << 1 | kernel (0 few), slot << 8 | row of
@@ -453,7 +454,7 @@ __host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const Pag
         s.ml = nullptr;
         if (note && pl.own) pl.own[row] = make_uint2(0, 0);
     } else if (whole) {
-        const size_t at = row + (x.pre ? (size_t)a.b.n_tok * a.n_head : 0);
+        const size_t at = row + (x.pre ? pl.all : 0);
         s.o = pl.wo + at * a.p.hd;
         s.ml = pl.wml + at;
         if (note) (x.pre ? pl.pre : pl.own)[row] = make_uint2(4 | none << 1 | MANY, ~0u);
@@ -501,7 +502,7 @@ __host__ __device__ __forceinline__ PaPart pa_part(const PagedAttn &a, const Pag
     const bool whole = d.y == ~0u, by_many = d.x & 1;
     const int w = min((int)(d.y >> 9) + k, (by_many ? many.wgs : few.wgs) - 1);
     const size_t slot = (size_t)(2 * w + (k == 0 ? d.y >> 8 & 1 : 0)) * (by_many ? many.rows : few.rows) + (d.y & 255);
-    const size_t at = whole ? row + (in_pre ? (size_t)a.b.n_tok * a.n_head : 0) : slot;
+    const size_t at = whole ? row + (in_pre ? pl.all : 0) : slot;
     return PaPart{(whole ? wo : by_many ? many.o : few.o) + at * hd, (whole ? wml : by_many ? many.ml : few.ml) + at};
 }
 

@@ -25,6 +25,7 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
     PagedPlan &pl = y.pl;
     PagedList &few = pl.few, &many = pl.many;
     const int64_t rows = (int64_t)b.n_tok * grp;             // of one KV head
+    pl.all = (int)(rows * p.n_kv);                           // up to 2^24
     pl.grp_inv = 65536 / grp + 1;
     many.toks = 1;
     many.toks_inv = 0;
