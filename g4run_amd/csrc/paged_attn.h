@@ -8,13 +8,19 @@
 // a lane then holds scores of one row at positions whose order is that of the
 // second product's operand, so the weights never leave their registers.
 //
-// Precision: fp32.  K and V enter exactly (halves, or the integers of the block
-// formats, their scales applied in fp32 to the scores and to the weights).  A
-// query row is scaled by a power of two to [2^14, 2^15) and split into two
-// halves (22 bits), a weight likewise.  Weights are exp2(s - m + 6), for
-// quantized values with m over s + the exponent of the position's largest
-// scale, so weight x scale neither overflows nor falls among the halves'
-// subnormals while it matters.
+// Precision: sums, scores and weights in fp32.  K and V enter the products exactly
+// (halves, or the integers of the block formats, their scales applied in fp32 to the
+// scores and to the weights); what they are multiplied with enters as two halves,
+// cut off.  A query row is scaled by a power of two to [2^14, 2^15): an element is
+// off by up to 2^-21 of itself and 2^-38 of the row's largest (the halves' smallest
+// step, 2^-24).  Weights are exp2(s - m + 6), for quantized values with m over s + the
+// exponent of the position's largest scale, so that weight x scale does not overflow:
+// one is off by up to 2^-21 of itself and 2^-30 of the row's largest (quantized:
+// weight times scale by 2^-29 of the largest such product, scales below 2^-14
+// counting as that).  Where one position has nearly all the weight and a value near
+// zero, the others' cut is what the result's error is made of: weights of 2^-17 of
+// the largest lose 6e-5 of themselves on average.  A third half of the weights would
+// cost a quarter more matrix instructions.
 //
 // Two kernels share a call:
 //   k_paged_few   row tiles of up to 16 rows (single tokens; the prefix of a small
@@ -560,8 +566,10 @@ __device__ __forceinline__ void pa_store4(float *to, pa_v4f s) {
     else { d[0] = s[0]; d[1] = s[1]; d[2] = s[2]; d[3] = s[3]; }
 }
 
-// the few-row kernel's workgroups per CU: what its registers allow (3 of 8-bit
-// heads of 128 fit with 32 bytes of spills: 73 us for 70, more results to join)
+// The few-row kernel's workgroups per CU: what its registers allow, but for 4-bit
+// heads of 128 and more, of which 3 would fit (16 windows of 1024, heads of 512: 19.7
+// us with 3, 19.4 with 2).  3 of 8-bit heads of 128 fit with 32 bytes of spills: 73 us
+// for 70, more results to join.
 __host__ __device__ constexpr int pa_few_per_cu(int type, int hd, bool st) {
     return hd == 64 ? 4 : type == F16 && hd == 128 && st ? 3 : 2;
 }

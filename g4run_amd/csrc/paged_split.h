@@ -32,7 +32,10 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
     // Sequences of at most few.rows rows are the few-row kernel's: 8 (one matrix
     // instruction per operand) where no sequence can have more, else 16.
     // None where sequences have 64 tokens on average: the other kernel then takes the
-    // short ones among them too, and a launch is saved (four prompts: 82 -> 77 us).
+    // short ones among them too, and a launch is saved (four prompts of up to 509: 80.8
+    // us with that launch, 79.0 without).  The rule goes by the average, which the host
+    // knows: single tokens over long caches beside one very long prompt are the many-row
+    // kernel's too, where one takes about twice its time in the other.
     few.rows = grp > 16 || (b.q_off && b.n_tok >= 64 * (int64_t)b.n_seq) ? 0 : (b.q_off ? rows : grp) <= 8 ? 8 : 16;
     if (b.n_prefix && few.rows == 8 && rows > 8 && rows <= 16) few.rows = 16;
     few.toks = few.rows / grp;
@@ -45,8 +48,8 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
     auto span = [&](int tokens) { return window ? std::min<int64_t>(b.max_len, (int64_t)window + 32 + tokens) : (int64_t)b.max_len; };
     const int64_t fspan = span(16);
     // A step is what a workgroup takes at once (of heads of 512 its four waves share
-    // 32 positions; with steps of 128, 16 windows of 1024 took 23.3 us, now 21.7); up to 256 positions stay
-    // one step, so that no join is launched for them.  A sequence's tile counts as
+    // 32 positions: 16 windows of 1024 take 19.3 us, with steps of 128 20.1); up to 256
+    // positions stay one step, so that no join is launched for them.  A sequence's tile counts as
     // `lead` steps more, for its queries, first loads and results: 64 sequences of
     // 2000 of 4096 positions, 8 KV heads of 128, 8 bits, take 75 us with a lead of 1, 73
     // with 2, 93 without; a lead of 2 is slower where steps are few (the shares' last
@@ -64,8 +67,10 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
     // Many rows: tiles of whole tokens, up to 128 rows (64 of heads of 512), evenly
     // filled; as many workgroups as fit on the device at once.  Steps of 32 positions,
     // each its workgroup where they are few (24 rows of 256 over 76 positions: 22 us,
-    // with shares of 2 at least 29.6), a lead of 5 (four prompts of 509 behind 3800, 4
-    // KV heads of 256: 91 us with 2, 83 with 4, 80 with 6; the same order for heads of 64).
+    // with shares of 2 at least 29.6).  A lead of 5 lies between what long and short
+    // tiles want (leads of 4, 5, 6; 32 / 8 heads of 128, f16: one prompt of 2000 158,
+    // 150, 141 us; four of 256 behind a prefix of 100 37.5, 37.6, 42.2; eight of 128 in
+    // windows of 512 40.5, 39.8, 40.7).
     many.rows = 0;
     many.pre_tiles = many.lead = 0;
     if (many_own || many_pre) {

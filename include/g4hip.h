@@ -295,9 +295,9 @@ typedef struct {
 } g4h_paged_kv;
 /* What a call found in the batch's device arrays: a page id outside
  * [0, n_pages) where a position is stored or a row attends (the ids of pages
- * before all windows, or behind a sequence's end, may be any); a length outside [0,
- * max_len] or past the table's table_stride pages, offsets that descend or
- * leave [0, n_tok].  Such rows are not appended, and read as NaN by the
+ * before all windows, or behind a sequence's end, may be any); a length
+ * outside [0, max_len] or past the table's table_stride pages, offsets that
+ * descend or leave [0, n_tok].  Such rows are not appended, and read as NaN by the
  * attention, which ends the batch at the first sequence of such offsets: every
  * row from there on reads as NaN.  Nothing outside the pools and the given
  * arrays is touched. */
@@ -314,8 +314,9 @@ enum { G4H_PAGED_BAD_PAGE = 1, G4H_PAGED_BAD_BATCH = 2 };
  * rows are in the pages prefix_dev[0 .. ceil(n_prefix / page)), shared by all:
  * own position p is position n_prefix + p. */
 typedef struct {
-    int n_seq, n_tok;          /* sequences; rows of the activations (any counts >= 0; with none
-                                * of either a call does nothing, and its arrays may be NULL) */
+    int n_seq, n_tok;          /* sequences, n_seq * n_kv up to 2^22; rows of the activations, up
+                                * to 2^24 (attention: n_tok * n_head up to 2^24).  With none of
+                                * either a call does nothing, and its arrays may be NULL */
     const int *q_off_dev;      /* n_seq + 1 ascending offsets, or NULL */
     const int *len_dev;        /* n_seq lengths, 0 .. max_len */
     const int *table_dev;      /* n_seq rows of table_stride page ids, position p in entry p / page */
@@ -362,13 +363,17 @@ int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out
  * q / out: fp32 [n_tok][n_head][hd], at q_stride / out_stride floats per token
  * (0: packed); query head h reads KV head h / (n_head / n_kv), up to 128 heads a
  * KV head (64 of hd 512).  No row of out may overlap one of q: both may be
- * columns of one array, at the same stride.  All in fp32
- * precision (queries and weights enter the matrix cores as two halves each),
- * unlike g4h_attn_decode, which rounds as the reference does.  The prefix's
- * rows are read once for the whole batch.  A non-finite cached value reaches
- * the rows that attend it and no others.  ws: g4h_paged_attn_workspace_bytes()
- * of caller-owned scratch, 16-byte aligned; it needs no initial contents and
- * keeps nothing from call to call, but calls that overlap must not share it.
+ * columns of one array, at the same stride.  Sums, scores and weights are fp32,
+ * unlike g4h_attn_decode's, which rounds as the reference does; queries and
+ * weights enter the matrix cores as two halves each, cut off: a weight to 2^-21
+ * of itself and 2^-30 of its row's largest (quantized values: weight times
+ * scale, 2^-29), a query element to 2^-21 of itself.  The prefix's rows are read
+ * for tiles of up to 128 query rows of a KV head (64 of hd 512), not for every
+ * sequence; all of them are, those that every window hides too.  A non-finite
+ * cached value reaches the rows that attend it and no others, as an infinity or
+ * as NaN.  ws: g4h_paged_attn_workspace_bytes() of caller-owned scratch, 16-byte
+ * aligned; it needs no initial contents and keeps nothing from call to call, but
+ * calls that overlap must not share it.
  * Asynchronous, capturable.  A row's bits depend on the batch it runs in (on
  * how the positions are split), not on the run. */
 size_t g4h_paged_attn_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head);
