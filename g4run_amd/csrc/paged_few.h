@@ -6,7 +6,7 @@
 // the device at once, and their shares of the list of steps are equal, so ragged
 // lengths leave none idle.  Reached: 32 sequences of up to 8192 positions, 8 q / 4
 // kv heads of 256, f16: 101 us, 5.3 TB/s; 64 of up to 4096, 32 / 8 heads of 128, 8
-// bits, capped: 70 to 73 us, 3.9 to 4.1 TB/s; 16 windows of 1024, 8 / 2 heads of 512,
+// bits, capped: 72 to 75 us, 3.8 to 4.0 TB/s; 16 windows of 1024, 8 / 2 heads of 512,
 // 4 bits: 19 us (joins included).
 //
 // A workgroup's 4 waves take 32 positions each of a step of 128, on

@@ -18,7 +18,7 @@
 // 32 positions of 128 rows of 256 take 2.06 us of a workgroup per CU: the matrix
 // cores at 1.04 PFLOP/s, a large f16 product of the library reaches 1.17.  A call of
 // four prompts of up to 509 tokens behind up to 3800 positions, 8 q / 4 kv heads,
-// capped, takes 78 us: the rest is each piece's start and end (8 us), the shares'
+// capped, takes 79 us: the rest is each piece's start and end (8 us), the shares'
 // rest, and the sums of the split tiles out and in again (about 60 MB each way, the join
 // 11 us).  Few rows do not make a tile cheaper (20 rows of 256: 1.4 us for 32
 // positions): it is then one wave's chain from the staging to its second product.
