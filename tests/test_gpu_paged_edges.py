@@ -200,3 +200,21 @@ def test_append_and_read_of_a_part_of_a_batch(gpu, t, new):
     assert np.array_equal(gv[a:b], values(t, v)[a:b].astype(np.float32))
     changed = (c.kv.v.download(np.uint8, c.pool.v.shape) != c.pool.v).any(1)
     assert set(np.flatnonzero(changed)) <= {int(p) for i in (1, 2) for p in c.table[i]}
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+def test_no_status_word(gpu, t):
+    # a cache without one: bad pages and offsets are read as they are with it
+    c = Case(gpu, t, 4, 2, 64, 16, [60, 40, 20], new=[1, 2, 1], n_prefix=20, seed=68)
+    c.table[0, 1] = -1
+    c.d["table"].upload(c.table)
+    c.kv.struct.status_dev = None
+    want, tol = c.expect(0.1)
+    got = c.attn(0.1)
+    assert np.isnan(got[0]).all() and np.all(np.abs(got[1:] - want[1:]) <= tol[1:])
+    c.d["off"].upload(np.asarray([0, 1, 9, 4], np.int32))
+    got = c.attn(0.1)
+    assert np.isnan(got).all()
+    k = gpu.Buffer.from_array(c.rng.standard_normal((4, 2, 64)).astype(np.float32))
+    gpu.paged_append(c.kv, c.batch, k, k)
+    gpu.synchronize()

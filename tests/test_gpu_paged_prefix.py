@@ -52,3 +52,27 @@ def test_prompts_behind_a_short_prefix(gpu, t, hd, n_head, n_kv, window):
 def test_prompts_behind_a_prefix_of_hundreds(gpu, t):
     # shares of a part of a prefix tile, whole ones, and own tiles
     LongCase(gpu, t, 16, 4, 128, 32, [200] * 6, new=[200, 150, 3, 1, 200, 90], n_prefix=333, seed=51).check(cap=30.0)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+def test_graph_replays_with_other_shares(gpu, t):
+    """A captured call whose shares hold whole tiles of the prefix, or parts, as the
+    lengths change; eager calls over a workspace of their own between the replays."""
+    G = gpu
+    full = [8000, 7000, 6500, 5]
+    c = LongCase(G, t, 16, 8, 128, 64, full, n_prefix=40, seed=52)
+    s, rows = G.Stream(), [x[:] for x in c.rows]
+    ws = G.Buffer.from_array(np.full(G.paged_attn_workspace_bytes(c.kv, c.batch, 16), 0xff, np.uint8))
+    out = G.Buffer.from_array(np.full((4, 16, 128), 7.5, np.float32))
+    g = G.Graph(s.ptr, lambda: G.paged_attn(c.kv, c.batch, c.d["q"], 16, out, scale=0.1, ws=ws, stream=s.ptr))
+    for step, lens in enumerate([full, [60, 5, 0, 1], [8000, 1, 6000, 5], full]):
+        c.lens = lens
+        c.rows = [[w[:n] for w in x] for x, n in zip(rows, lens)]
+        c.d["lens"].upload(np.asarray(lens + [0], np.int32), s.ptr)
+        g.launch(s.ptr)
+        s.synchronize()
+        got = out.download(np.float32, (4, 16, 128))
+        want, tol = c.expect(0.1)
+        assert np.all(np.abs(got - want) <= tol), step
+        assert np.array_equal(c.attn(0.1), got), step
+    assert c.kv.status() == 0
