@@ -341,8 +341,9 @@ size_t g4h_paged_pool_bytes(int kv_type, int n_kv, int hd, int page, int64_t n_p
  * fp32 [n_tok][n_kv][hd] at k_stride / v_stride floats per token (0: packed),
  * rounded to the cache's type as g4h_kv_store does; and, with n_head > 0, the
  * queries q [n_tok][n_head][hd] rotated into q_out (q itself, at the same
- * stride, or rows that overlap none of q, k and v).  Strides let all of them be
- * parts of one fused projection's rows.  Two tokens of one batch must not share
+ * stride, or rows that overlap none of q, k and v; at another stride than
+ * theirs, an array apart).  Strides let all of them be parts of one fused
+ * projection's rows.  Two tokens of one batch must not share
  * a slot.  Asynchronous, capturable, needs no workspace. */
 int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_rope *rope, int n_head, const float *q_dev,
                      size_t q_stride, float *q_out_dev, size_t q_out_stride, const float *k_dev, size_t k_stride,
