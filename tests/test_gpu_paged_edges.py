@@ -218,3 +218,47 @@ def test_no_status_word(gpu, t):
     k = gpu.Buffer.from_array(c.rng.standard_normal((4, 2, 64)).astype(np.float32))
     gpu.paged_append(c.kv, c.batch, k, k)
     gpu.synchronize()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_append_rounds_as_kv_store(gpu, t, hd):
+    # every bit that a stored row's values depend on, of blocks of any size
+    G, n = gpu, 96
+    c = Case(G, t, 1, 1, hd, 16, [n], new=[n], seed=69)
+    x = (c.rng.standard_normal((n, 1, hd)) * np.exp2(c.rng.integers(-40, 20, (n, 1, hd // 32))).repeat(32, -1)).astype(np.float32)
+    x[1] = 0
+    x[2] = np.float32(1e-42)
+    x[3] *= np.float32(1e30)
+    x[4] = np.sign(x[4])
+    x[5, 0, :32] = np.arange(-16, 16) / 16
+    x[6] = -np.abs(x[6])
+    x[7, 0, ::2] = -x[7, 0, 1::2]
+    b = G.Buffer.from_array(x)
+    G.paged_append(c.kv, c.batch, b, b)
+    size = {F16: 2 * hd, Q8_0: hd // 32 * 34, Q4_0: hd // 32 * 18}[t]
+    flat = G.Buffer(n * size)
+    G.kv_store(t, b, flat, hd, n)
+    G.synchronize()
+    want = flat.download(np.uint8, (n, size))
+    c.pool.k, c.pool.v = c.kv.k.download(np.uint8, c.pool.k.shape), c.kv.v.download(np.uint8, c.pool.v.shape)
+    row = hd * 2 if t == F16 else hd if t == Q8_0 else hd // 2
+    for p in range(n):
+        pg, slot = c.table[0, p // 16], p % 16
+        for raw, at in ((c.pool.k, "k"), (c.pool.v, "v")):
+            bytes_ = raw[pg, slot * row:(slot + 1) * row]
+            if t == F16:
+                assert np.array_equal(bytes_, want[p])
+                continue
+            scales = raw[pg, 16 * row + slot * (hd // 16):16 * row + (slot + 1) * (hd // 16)].reshape(-1, 2)
+            blocks = want[p].reshape(hd // 32, -1)
+            assert np.array_equal(scales, blocks[:, :2]), (p, at)
+            if t == Q8_0:
+                q = bytes_[getattr(c.pool, at + "8")].astype(np.int32) - 128
+                w = blocks[:, 2:].view(np.int8).astype(np.int32).reshape(-1)
+            else:
+                q = np.stack([bytes_ & 15, bytes_ >> 4], -1).reshape(-1)[getattr(c.pool, at + "4")].astype(np.int32)
+                w = np.concatenate([blocks[:, 2:] & 15, blocks[:, 2:] >> 4], 1).astype(np.int32).reshape(-1)
+            # of a zero scale (one below 2^-25) every quant is the value 0: 1 / d may be infinite there
+            held = np.repeat(scales.copy().view(np.float16)[:, 0] != 0, 32)
+            assert np.array_equal(q[held], w[held]), (p, at)
