@@ -96,6 +96,15 @@ _SIGS = [
     ("g4h_paged_read", _int, [_vp, _vp, _int, _vp, _vp, _vp]),
     ("g4h_paged_attn_workspace_bytes", _sz, [_vp, _vp, _int]),
     ("g4h_paged_attn", _int, [_vp, _vp, _int, _vp, _sz, C.c_float, C.c_float, _int, _vp, _sz, _vp, _sz, _vp]),
+    ("g4h_paged_tree_build", _int, [_vp, _vp, _int, _vp, _vp, _vp, _vp]),
+    ("g4h_paged_append_tree", _int, [_vp, _vp, _vp, _vp, _int, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
+    ("g4h_paged_attn_tree_workspace_bytes", _sz, [_vp, _vp, _int]),
+    ("g4h_paged_attn_tree", _int, [_vp, _vp, _vp, _int, _vp, _sz, C.c_float, C.c_float, _int, _vp, _sz, _vp, _sz, _vp]),
+    ("g4h_paged_tree_accept", _int, [_vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp]),
+    ("g4h_paged_keep", _int, [_vp, _int, _vp, _vp, _vp, _int, _vp]),
+    ("g4h_paged_fork", _int, [_vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _int, _vp]),
+    ("g4h_beam_workspace_bytes", _sz, [_int, _int, _int, _int]),
+    ("g4h_beam_select", _int, [_vp, _sz, _int, _int, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
     ("g4h_kv_store", _int, [_int, _vp, _vp, _int, _int, _sz, _vp]),
     ("g4h_model_create", _int, [_vp, C.c_uint64, C.POINTER(_vp)]),
     ("g4h_model_free", _int, [_vp]),
@@ -564,6 +573,96 @@ def paged_attn(kv: PagedKV, batch: PagedBatch, q, n_head: int, out, scale: float
                                ws.nbytes if isinstance(ws, Buffer) else need, stream))
     if made:
         synchronize(stream)                          # before the workspace goes
+
+
+# -------------------------------------------- drafts that are trees, and beams
+class _PagedTree(C.Structure):
+    _fields_ = [("words", _int), ("mask_dev", _vp), ("depth_dev", _vp)]
+
+
+class PagedTree:
+    """A batch's trees of new tokens (g4h_paged_tree): mask [n_tok][words] and
+    depth [n_tok] are device arrays, written by paged_tree_build or by the caller."""
+
+    def __init__(self, words: int, mask, depth):
+        self.keep = (mask, depth)
+        self.struct = _PagedTree(words, _p(mask), _p(depth))
+        self.ref = C.byref(self.struct)
+
+
+class PagedCaches:
+    """The paged caches of a model's layers, all of one shape, as paged_keep and
+    paged_fork take them; flags go to the first one's status word."""
+
+    def __init__(self, caches):
+        self.keep = list(caches)
+        self.array = (_PagedKV * max(1, len(self.keep)))(*[x.struct for x in self.keep])
+
+
+def paged_tree_build(batch: PagedBatch, parent, words: int, mask, depth, status=None, stream=None) -> None:
+    """Masks and depths of a batch's new tokens from their parents."""
+    check(lib().g4h_paged_tree_build(batch.ref, _p(parent), words, _p(mask), _p(depth), _p(status), stream))
+
+
+def paged_append_tree(kv: PagedKV, batch: PagedBatch, tree: PagedTree, k, v, q=None, q_out=None, n_head: int = 0, rope=None, q_stride: int = 0,
+                      q_out_stride: int = 0, k_stride: int = 0, v_stride: int = 0, stream=None) -> None:
+    """paged_append, rotated as the tokens' depths say."""
+    check(lib().g4h_paged_append_tree(kv.ref, batch.ref, tree.ref, rope.ref if rope else None, n_head, _p(q), q_stride, _p(q_out), q_out_stride,
+                                      _p(k), k_stride, _p(v), v_stride, stream))
+
+
+def paged_attn_tree_workspace_bytes(kv: PagedKV, batch: PagedBatch, n_head: int) -> int:
+    return lib().g4h_paged_attn_tree_workspace_bytes(kv.ref, batch.ref, n_head)
+
+
+def paged_attn_tree(kv: PagedKV, batch: PagedBatch, tree: PagedTree, q, n_head: int, out, scale: float = 1.0, softcap: float = 0.0,
+                    window: int = 0, ws=None, q_stride: int = 0, out_stride: int = 0, stream=None) -> None:
+    """Attention of a tree's tokens: the cached positions, and the new tokens of
+    their masks; ws as paged_attn's, of paged_attn_tree_workspace_bytes."""
+    need = 0 if isinstance(ws, Buffer) else paged_attn_tree_workspace_bytes(kv, batch, n_head)
+    made = ws is None and need > 0
+    if made:
+        ws = Buffer(need)
+    check(lib().g4h_paged_attn_tree(kv.ref, batch.ref, tree.ref, n_head, _p(q), q_stride, scale, softcap, window, _p(out), out_stride, _p(ws),
+                                    ws.nbytes if isinstance(ws, Buffer) else need, stream))
+    if made:
+        synchronize(stream)                          # before the workspace goes
+
+
+def paged_tree_accept(batch: PagedBatch, parent, token, choice, most: int, n_keep, keep, next_out=None, len_out=None, status=None,
+                      stream=None) -> None:
+    """The path of each sequence's tree that the choices made at its tokens confirm."""
+    check(lib().g4h_paged_tree_accept(batch.ref, _p(parent), _p(token), _p(choice), most, _p(n_keep), _p(keep), _p(next_out), _p(len_out),
+                                      _p(status), stream))
+
+
+def paged_keep(caches: PagedCaches, batch: PagedBatch, n_keep, keep, most: int, stream=None) -> None:
+    """Move the kept new tokens' rows together, in all caches."""
+    check(lib().g4h_paged_keep(caches.array, len(caches.keep), batch.ref, _p(n_keep), _p(keep), most, stream))
+
+
+def paged_fork(caches: PagedCaches, batch: PagedBatch, n_out: int, parent, fresh, len_out, table_out, out_stride: int, stream=None) -> None:
+    """Lengths, page tables and part-filled pages of rows that continue rows of the batch."""
+    check(lib().g4h_paged_fork(caches.array, len(caches.keep), batch.ref, n_out, _p(parent), _p(fresh), _p(len_out), _p(table_out), out_stride,
+                               stream))
+
+
+def beam_workspace_bytes(n_group: int, n_beam: int, n_vocab: int, n_out: int) -> int:
+    return lib().g4h_beam_workspace_bytes(n_group, n_beam, n_vocab, n_out)
+
+
+def beam_select(logits, n_group: int, n_beam: int, n_vocab: int, score, n_out: int, score_out, row_out, token_out, ended=None, stride: int = 0,
+                ws=None, stream=None) -> None:
+    """The n_out best continuations of each group of beams; ws: a Buffer of
+    beam_workspace_bytes (allocated here, and the stream waited for, if not given)."""
+    need = 0 if isinstance(ws, Buffer) else beam_workspace_bytes(n_group, n_beam, n_vocab, n_out)
+    made = ws is None and need > 0
+    if made:
+        ws = Buffer(need)
+    check(lib().g4h_beam_select(_p(logits), stride, n_group, n_beam, n_vocab, _p(score), _p(ended), n_out, _p(score_out), _p(row_out), _p(token_out),
+                                _p(ws), ws.nbytes if isinstance(ws, Buffer) else need, stream))
+    if made:
+        synchronize(stream)
 
 
 # ---------------------------------------------------------------- decode step

@@ -2,6 +2,7 @@
 // resident-tensor management and dispatch to the gfx950 kernels.
 #include "../../include/g4hip.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdarg>
@@ -11,6 +12,7 @@
 #include <unordered_map>
 
 #include "kernels.h"
+#include "beam.h"
 #include "paged.h"
 
 using namespace g4;
@@ -995,12 +997,12 @@ static bool paged_overlap(const float *a, size_t a_stride, size_t a_row, const f
     return (meets(k) && r < (wide)a_row) || (meets(k + 1) && s - r < (wide)b_row);
 }
 
-extern "C" int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_rope *rope, int n_head, const float *q,
-                                size_t q_stride, float *q_out, size_t q_out_stride, const float *k, size_t k_stride, const float *v,
-                                size_t v_stride, void *stream) {
-    const char *fn = "g4h_paged_append";
+static int paged_append(const char *fn, const g4h_paged_kv *kv, const g4h_paged_batch *batch, const int *depth, const g4h_rope *rope, int n_head,
+                        const float *q, size_t q_stride, float *q_out, size_t q_out_stride, const float *k, size_t k_stride, const float *v,
+                        size_t v_stride, void *stream) {
     PagedAppend a;
     if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
+    a.depth = depth;
     if (n_head < 0 || n_head > 65536) return fail(G4H_ERR_ARG, "%s: n_head=%d", fn, n_head);
     const size_t row = (size_t)a.p.n_kv * a.p.hd, qrow = (size_t)n_head * a.p.hd;
     if (int rc = paged_rows(fn, "k", k, k_stride, row, a.b)) return rc;
@@ -1040,6 +1042,11 @@ extern "C" int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *b
     G4_HIP(launch_paged_append(a, (hipStream_t)stream));
     return G4H_OK;
 }
+extern "C" int g4h_paged_append(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_rope *rope, int n_head, const float *q,
+                                size_t q_stride, float *q_out, size_t q_out_stride, const float *k, size_t k_stride, const float *v,
+                                size_t v_stride, void *stream) {
+    return paged_append("g4h_paged_append", kv, batch, nullptr, rope, n_head, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride, stream);
+}
 
 extern "C" int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out_type, void *k_out, void *v_out, void *stream) {
     const char *fn = "g4h_paged_read";
@@ -1070,9 +1077,9 @@ extern "C" size_t g4h_paged_attn_workspace_bytes(const g4h_paged_kv *kv, const g
     if (paged_args(fn, kv, batch, p, b, true) || check_paged_heads(fn, p, b, n_head)) return 0;
     return paged_attn_workspace(p, b, n_head);
 }
-extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head, const float *q, size_t q_stride, float scale,
-                              float softcap, int window, float *out, size_t out_stride, void *ws, size_t ws_bytes, void *stream) {
-    const char *fn = "g4h_paged_attn";
+static int paged_attn(const char *fn, const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_paged_tree *tree, int n_head, const float *q,
+                      size_t q_stride, float scale, float softcap, int window, float *out, size_t out_stride, void *ws, size_t ws_bytes,
+                      void *stream) {
     PagedAttn a;
     if (int rc = paged_args(fn, kv, batch, a.p, a.b)) return rc;
     if (int rc = check_paged_heads(fn, a.p, a.b, n_head)) return rc;
@@ -1085,7 +1092,7 @@ extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *bat
         return fail(G4H_ERR_ARG, "%s: scale=%g softcap=%g window=%d", fn, scale, softcap, window);
     if (a.b.n_prefix && !a.b.prefix && !paged_empty(a.b)) return fail(G4H_ERR_ARG, "%s: a prefix of %d positions needs its pages", fn, a.b.n_prefix);
     if (!paged_empty(a.b) && paged_overlap(q, q_stride, row, out, out_stride, row, a.b.n_tok)) return fail(G4H_ERR_ARG, "%s: q and out overlap", fn);
-    const size_t need = paged_attn_workspace(a.p, a.b, n_head);
+    const size_t need = tree ? paged_attn_tree_workspace(a.p, a.b, n_head) : paged_attn_workspace(a.p, a.b, n_head);
     if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
         return fail(G4H_ERR_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, ws ? ws_bytes : (size_t)0);
     a.n_head = n_head;
@@ -1098,7 +1105,231 @@ extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *bat
     a.cap = softcap;
     a.window = window;
     a.ws = (uint8_t *)ws;
+    a.mask = tree ? tree->mask_dev : nullptr;
+    a.depth = tree ? tree->depth_dev : nullptr;
+    a.words = tree ? tree->words : 0;
     G4_NEED_INIT();
-    G4_HIP(launch_paged_attn(a, (hipStream_t)stream));
+    if (tree) G4_HIP(launch_paged_attn_tree(a, (hipStream_t)stream));
+    else G4_HIP(launch_paged_attn(a, (hipStream_t)stream));
+    return G4H_OK;
+}
+extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head, const float *q, size_t q_stride, float scale,
+                              float softcap, int window, float *out, size_t out_stride, void *ws, size_t ws_bytes, void *stream) {
+    return paged_attn("g4h_paged_attn", kv, batch, nullptr, n_head, q, q_stride, scale, softcap, window, out, out_stride, ws, ws_bytes, stream);
+}
+
+// ------------------------------------------- trees of drafted tokens, beams ----
+static bool ranges_meet(const void *a, size_t an, const void *b, size_t bn) {
+    return a && b && an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+static int check_tree(const char *fn, const g4h_paged_batch *batch, const g4h_paged_tree *tree, bool mask) {
+    if (!batch || !tree) return fail(G4H_ERR_ARG, "%s: null pointer", fn);
+    if (tree->words < 1 || tree->words > PAGED_TREE_WORDS) return fail(G4H_ERR_ARG, "%s: words=%d (1 .. %d)", fn, tree->words, PAGED_TREE_WORDS);
+    const bool any = batch->n_seq > 0 && batch->n_tok > 0;
+    if ((any && !tree->depth_dev) || (uintptr_t)tree->depth_dev % 4 || (mask && any && !tree->mask_dev) || (uintptr_t)tree->mask_dev % 4)
+        return fail(G4H_ERR_ARG, "%s: masks and depths must be 4-byte aligned device memory", fn);
+    return G4H_OK;
+}
+extern "C" int g4h_paged_append_tree(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_paged_tree *tree, const g4h_rope *rope,
+                                     int n_head, const float *q, size_t q_stride, float *q_out, size_t q_out_stride, const float *k,
+                                     size_t k_stride, const float *v, size_t v_stride, void *stream) {
+    const char *fn = "g4h_paged_append_tree";
+    if (int rc = check_tree(fn, batch, tree, false)) return rc;
+    return paged_append(fn, kv, batch, tree->depth_dev, rope, n_head, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride, stream);
+}
+extern "C" size_t g4h_paged_attn_tree_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head) {
+    const char *fn = "g4h_paged_attn_tree_workspace_bytes";
+    PagedPool p;
+    PagedBatch b;
+    if (paged_args(fn, kv, batch, p, b, true) || check_paged_heads(fn, p, b, n_head)) return 0;
+    return paged_attn_tree_workspace(p, b, n_head);
+}
+extern "C" int g4h_paged_attn_tree(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_paged_tree *tree, int n_head, const float *q,
+                                   size_t q_stride, float scale, float softcap, int window, float *out, size_t out_stride, void *ws,
+                                   size_t ws_bytes, void *stream) {
+    const char *fn = "g4h_paged_attn_tree";
+    if (int rc = check_tree(fn, batch, tree, true)) return rc;
+    return paged_attn(fn, kv, batch, tree, n_head, q, q_stride, scale, softcap, window, out, out_stride, ws, ws_bytes, stream);
+}
+// a batch of which no cache is given
+static int tree_batch(const char *fn, const g4h_paged_batch *batch, PagedBatch &b, bool lengths, const int *status) {
+    if (!batch) return fail(G4H_ERR_ARG, "%s: null pointer", fn);
+    if (batch->n_seq < 0 || batch->n_seq > 1 << 22 || batch->n_tok < 0 || batch->n_tok > 1 << 24 || batch->max_len < 0 || batch->max_len > PAGED_MAX_POS)
+        return fail(G4H_ERR_ARG, "%s: n_seq=%d (up to 2^22) n_tok=%d (up to 2^24) max_len=%d", fn, batch->n_seq, batch->n_tok, batch->max_len);
+    if ((lengths && batch->n_seq && !batch->len_dev) || (uintptr_t)batch->len_dev % 4 || (uintptr_t)batch->q_off_dev % 4 || (uintptr_t)status % 4)
+        return fail(G4H_ERR_ARG, "%s: null lengths or a misaligned array", fn);
+    b = PagedBatch{batch->n_seq, batch->n_tok, batch->q_off_dev, batch->len_dev, nullptr, 0, batch->max_len, 0, nullptr};
+    return G4H_OK;
+}
+static bool null_or_odd(const void *p, bool needed) { return (needed && !p) || (uintptr_t)p % 4; }
+extern "C" int g4h_paged_tree_build(const g4h_paged_batch *batch, const int *parent, int words, uint32_t *mask, int *depth, int *status,
+                                    void *stream) {
+    const char *fn = "g4h_paged_tree_build";
+    PagedTreeBuild a;
+    if (int rc = tree_batch(fn, batch, a.b, false, status)) return rc;
+    if (words < 1 || words > PAGED_TREE_WORDS) return fail(G4H_ERR_ARG, "%s: words=%d (1 .. %d)", fn, words, PAGED_TREE_WORDS);
+    const bool any = !paged_empty(a.b);
+    if (null_or_odd(parent, any) || null_or_odd(mask, any) || null_or_odd(depth, any)) return fail(G4H_ERR_ARG, "%s: null or misaligned array", fn);
+    const size_t n = (size_t)a.b.n_tok * 4, off = ((size_t)a.b.n_seq + 1) * 4;
+    if (any && (ranges_meet(mask, n * words, depth, n) || ranges_meet(mask, n * words, parent, n) || ranges_meet(depth, n, parent, n) ||
+                ranges_meet(mask, n * words, a.b.q_off, off) || ranges_meet(depth, n, a.b.q_off, off)))
+        return fail(G4H_ERR_ARG, "%s: masks or depths overlap another array", fn);
+    a.parent = parent;
+    a.words = words;
+    a.mask = mask;
+    a.depth = depth;
+    a.status = status;
+    G4_NEED_INIT();
+    G4_HIP(launch_paged_tree_build(a, (hipStream_t)stream));
+    return G4H_OK;
+}
+extern "C" int g4h_paged_tree_accept(const g4h_paged_batch *batch, const int *parent, const int *token, const int *choice, int most, int *n_keep,
+                                     int *keep, int *next, int *len_out, int *status, void *stream) {
+    const char *fn = "g4h_paged_tree_accept";
+    PagedTreeAccept a;
+    if (int rc = tree_batch(fn, batch, a.b, true, status)) return rc;
+    if (most < 1 || most > 32 * PAGED_TREE_WORDS) return fail(G4H_ERR_ARG, "%s: most=%d (1 .. %d)", fn, most, 32 * PAGED_TREE_WORDS);
+    const bool any = a.b.n_seq > 0, tokens = any && a.b.n_tok > 0;
+    if (null_or_odd(parent, tokens) || null_or_odd(token, tokens) || null_or_odd(choice, tokens) || null_or_odd(n_keep, any) || null_or_odd(keep, any) ||
+        null_or_odd(next, false) || null_or_odd(len_out, false))
+        return fail(G4H_ERR_ARG, "%s: null or misaligned array", fn);
+    const size_t n = (size_t)a.b.n_tok * 4, ns = (size_t)a.b.n_seq * 4;
+    const struct { const void *p; size_t n; } out[] = {{n_keep, ns}, {keep, ns * most}, {next, ns}, {len_out, ns}},
+        in[] = {{parent, n}, {token, n}, {choice, n}, {a.b.len, ns}, {a.b.q_off, ns + 4}};
+    for (int i = 0; any && i < 4; i++) {
+        for (int j = 0; j < i; j++)
+            if (ranges_meet(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(G4H_ERR_ARG, "%s: outputs overlap", fn);
+        for (const auto &y : in)
+            if (ranges_meet(out[i].p, out[i].n, y.p, y.n)) return fail(G4H_ERR_ARG, "%s: an output overlaps what the call reads", fn);
+    }
+    a.parent = parent;
+    a.token = token;
+    a.choice = choice;
+    a.most = most;
+    a.n_keep = n_keep;
+    a.keep = keep;
+    a.next = next;
+    a.len_out = len_out;
+    a.status = status;
+    G4_NEED_INIT();
+    G4_HIP(launch_paged_tree_accept(a, (hipStream_t)stream));
+    return G4H_OK;
+}
+// the caches of a call, all of one shape; p: the first
+static int paged_caches(const char *fn, const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *batch, PagedPool &p, PagedBatch &b) {
+    if (!kv || n_cache < 1 || n_cache > 65536) return fail(G4H_ERR_ARG, "%s: n_cache=%d (1 .. 65536)", fn, n_cache);
+    for (int i = n_cache - 1; i >= 0; i--) {
+        if (int rc = paged_args(fn, kv + i, batch, p, b)) return rc;
+        if (kv[i].kv_type != kv->kv_type || kv[i].n_kv != kv->n_kv || kv[i].hd != kv->hd || kv[i].page != kv->page || kv[i].n_pages != kv->n_pages)
+            return fail(G4H_ERR_SHAPE, "%s: cache %d has another shape than the first", fn, i);
+    }
+    return G4H_OK;
+}
+static int paged_pools(const g4h_paged_kv *kv, int n_cache, int c0, PagedPools &pools) {
+    const int n = std::min(n_cache - c0, PAGED_CACHES);
+    for (int i = 0; i < n; i++) {
+        pools.k[i] = (uint8_t *)kv[c0 + i].k_dev;
+        pools.v[i] = (uint8_t *)kv[c0 + i].v_dev;
+    }
+    return n;
+}
+extern "C" int g4h_paged_keep(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *batch, const int *n_keep, const int *keep, int most,
+                              void *stream) {
+    const char *fn = "g4h_paged_keep";
+    PagedKeep a;
+    if (int rc = paged_caches(fn, kv, n_cache, batch, a.p, a.b)) return rc;
+    if (most < 1 || most > 1 << 24) return fail(G4H_ERR_ARG, "%s: most=%d (1 .. 2^24)", fn, most);
+    if (null_or_odd(n_keep, !paged_empty(a.b)) || null_or_odd(keep, !paged_empty(a.b))) return fail(G4H_ERR_ARG, "%s: null or misaligned array", fn);
+    a.n_keep = n_keep;
+    a.keep = keep;
+    a.most = most;
+    G4_NEED_INIT();
+    PagedPools pools = {};
+    for (int c0 = 0; c0 < n_cache; c0 += PAGED_CACHES) {
+        a.n_cache = paged_pools(kv, n_cache, c0, pools);
+        G4_HIP(launch_paged_keep(a, pools, (hipStream_t)stream));
+    }
+    return G4H_OK;
+}
+extern "C" int g4h_paged_fork(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *batch, int n_out, const int *parent, const int *fresh,
+                              int *len_out, int *table_out, int out_stride, void *stream) {
+    const char *fn = "g4h_paged_fork";
+    PagedFork a;
+    if (!batch) return fail(G4H_ERR_ARG, "%s: null pointer", fn);
+    g4h_paged_batch seqs = *batch;                           // its sequences: tokens are not looked at
+    seqs.n_tok = std::max(0, std::min(batch->n_seq, 1 << 24));
+    seqs.q_off_dev = nullptr;
+    if (int rc = paged_caches(fn, kv, n_cache, &seqs, a.p, a.b)) return rc;
+    if (n_out < 0 || (int64_t)n_out * a.p.n_kv > 1 << 22 || out_stride < 0 || (!table_out != !len_out))
+        return fail(G4H_ERR_ARG, "%s: n_out=%d (n_out * n_kv up to 2^22) out_stride=%d, lengths and tables go together", fn, n_out, out_stride);
+    if (null_or_odd(parent, n_out > 0) || null_or_odd(fresh, n_out > 0) || null_or_odd(len_out, false) || null_or_odd(table_out, false))
+        return fail(G4H_ERR_ARG, "%s: null or misaligned array", fn);
+    const size_t ns = (size_t)a.b.n_seq * 4, no = (size_t)n_out * 4, to = no * out_stride;
+    const struct { const void *p; size_t n; } in[] = {{parent, no}, {fresh, no}, {a.b.len, ns}, {a.b.table, ns * a.b.table_stride}};
+    for (const auto &y : in)
+        if (ranges_meet(len_out, no, y.p, y.n) || ranges_meet(table_out, to, y.p, y.n)) return fail(G4H_ERR_ARG, "%s: an output overlaps what the call reads", fn);
+    if (ranges_meet(len_out, no, table_out, to)) return fail(G4H_ERR_ARG, "%s: outputs overlap", fn);
+    a.n_out = n_out;
+    a.parent = parent;
+    a.fresh = fresh;
+    a.len_out = len_out;
+    a.table_out = table_out;
+    a.out_stride = out_stride;
+    G4_NEED_INIT();
+    PagedPools pools = {};
+    for (int c0 = 0; c0 < n_cache; c0 += PAGED_CACHES) {
+        a.n_cache = paged_pools(kv, n_cache, c0, pools);
+        G4_HIP(launch_paged_fork(a, pools, (hipStream_t)stream));
+    }
+    return G4H_OK;
+}
+
+// -------------------------------------------------------- beam search ----
+static int check_beam(const char *fn, int n_group, int n_beam, int n_vocab, int n_out) {
+    if (n_group < 0 || n_beam < 1 || n_beam > BEAM_MOST || n_out < 1 || n_out > BEAM_MOST || n_vocab < 1 || n_vocab > BEAM_VOCAB ||
+        (int64_t)n_group * n_beam > 1 << 20)
+        return fail(G4H_ERR_ARG, "%s: n_group=%d (n_group * n_beam up to 2^20) n_beam=%d n_out=%d (1 .. %d) n_vocab=%d (1 .. 2^24)", fn, n_group, n_beam,
+                    n_out, BEAM_MOST, n_vocab);
+    return G4H_OK;
+}
+extern "C" size_t g4h_beam_workspace_bytes(int n_group, int n_beam, int n_vocab, int n_out) {
+    return check_beam("g4h_beam_workspace_bytes", n_group, n_beam, n_vocab, n_out) ? 0 : beam_workspace(n_group, n_beam, n_vocab, n_out);
+}
+extern "C" int g4h_beam_select(const float *logits, size_t stride, int n_group, int n_beam, int n_vocab, const float *score, const int *ended,
+                               int n_out, float *score_out, int *row_out, int *token_out, void *ws, size_t ws_bytes, void *stream) {
+    const char *fn = "g4h_beam_select";
+    if (int rc = check_beam(fn, n_group, n_beam, n_vocab, n_out)) return rc;
+    const bool any = n_group > 0;
+    if (null_or_odd(logits, any) || null_or_odd(score, any) || null_or_odd(ended, false) || null_or_odd(score_out, any) || null_or_odd(row_out, any) ||
+        null_or_odd(token_out, any))
+        return fail(G4H_ERR_ARG, "%s: null or misaligned array", fn);
+    if (stride == 0) stride = n_vocab;
+    if (stride < (size_t)n_vocab || stride > (size_t)1 << 40) return fail(G4H_ERR_ARG, "%s: stride %zu for rows of %d", fn, stride, n_vocab);
+    const size_t rows = (size_t)n_group * n_beam, no = (size_t)n_group * n_out * 4, need = beam_workspace(n_group, n_beam, n_vocab, n_out);
+    if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
+        return fail(G4H_ERR_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, ws ? ws_bytes : (size_t)0);
+    const struct { const void *p; size_t n; } out[] = {{score_out, no}, {row_out, no}, {token_out, no}, {ws, need}},
+        in[] = {{logits, any ? ((rows - 1) * stride + n_vocab) * 4 : 0}, {score, rows * 4}, {ended, rows * 4}};
+    for (int i = 0; any && i < 4; i++) {
+        for (int j = 0; j < i; j++)
+            if (ranges_meet(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(G4H_ERR_ARG, "%s: outputs or the workspace overlap", fn);
+        for (const auto &y : in)
+            if (ranges_meet(out[i].p, out[i].n, y.p, y.n) && !(i == 0 && y.p == score && score_out == score && n_out == n_beam))
+                return fail(G4H_ERR_ARG, "%s: an output or the workspace overlaps what the call reads", fn);
+    }
+    BeamSelect a = {};
+    a.x = logits;
+    a.stride = stride;
+    a.n_group = n_group;
+    a.n_beam = n_beam;
+    a.n_vocab = n_vocab;
+    a.n_out = n_out;
+    a.score = score;
+    a.ended = ended;
+    a.score_out = score_out;
+    a.row_out = row_out;
+    a.token_out = token_out;
+    G4_NEED_INIT();
+    G4_HIP(launch_beam_select(a, (uint8_t *)ws, (hipStream_t)stream));
     return G4H_OK;
 }

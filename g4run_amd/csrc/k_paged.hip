@@ -73,6 +73,21 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan pl) {
 size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head) {
     return b.n_tok == 0 || b.n_seq == 0 ? 0 : paged_layout(p, b, n_head / p.n_kv, 0).total;
 }
+size_t paged_attn_tree_workspace(const PagedPool &p, const PagedBatch &b, int n_head) {
+    return b.n_tok == 0 || b.n_seq == 0 ? 0 : paged_layout(p, b, n_head / p.n_kv, 0, true).total;
+}
+
+namespace {
+
+hipError_t join(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
+    const int64_t rows = (int64_t)a.b.n_tok * a.n_head;
+    const int hd = a.p.hd;
+    if (rows <= 2048) hipLaunchKernelGGL(k_paged_join<true>, dim3((unsigned)rows, rows * (hd / 64) <= 512 ? hd / 64 : 1), dim3(256), 0, s, a, pl);
+    else hipLaunchKernelGGL(k_paged_join<false>, dim3(pa_ceil_div(rows, 256 / (hd / 4))), dim3(256), 0, s, a, pl);
+    return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_paged_attn(PagedAttn a, hipStream_t s) {
     const PagedPool &p = a.p;
@@ -85,13 +100,22 @@ hipError_t launch_paged_attn(PagedAttn a, hipStream_t s) {
         if (hipError_t e = p.type == F16 ? pa_many_f16(a, pl, s) : p.type == Q8_0 ? pa_many_q8(a, pl, s) : pa_many_q4(a, pl, s)) return e;
     if (pl.few.rows)
         if (hipError_t e = p.type == F16 ? pa_few_f16(a, pl, s) : p.type == Q8_0 ? pa_few_q8(a, pl, s) : pa_few_q4(a, pl, s)) return e;
-    if (y.join) {
-        const int64_t rows = (int64_t)b.n_tok * a.n_head;
-        if (rows <= 2048) hipLaunchKernelGGL(k_paged_join<true>, dim3((unsigned)rows, rows * (p.hd / 64) <= 512 ? p.hd / 64 : 1), dim3(256), 0, s, a, pl);
-        else hipLaunchKernelGGL(k_paged_join<false>, dim3(pa_ceil_div(rows, 256 / (p.hd / 4))), dim3(256), 0, s, a, pl);
-        return hipGetLastError();
-    }
-    return hipSuccess;
+    return y.join ? join(a, pl, s) : hipSuccess;
+}
+
+// The same kernels, rows differing in which new tokens they attend.
+hipError_t launch_paged_attn_tree(PagedAttn a, hipStream_t s) {
+    const PagedPool &p = a.p;
+    const PagedBatch &b = a.b;
+    if (b.n_tok == 0 || b.n_seq == 0) return hipSuccess;
+    a.window = paged_window(b, a.window);
+    const PagedLayout y = paged_layout(p, b, a.grp, a.window, true);
+    const PagedPlan pl = paged_places(y, a.ws);
+    if (pl.many.rows)
+        if (hipError_t e = p.type == F16 ? pa_many_tree_f16(a, pl, s) : p.type == Q8_0 ? pa_many_tree_q8(a, pl, s) : pa_many_tree_q4(a, pl, s)) return e;
+    if (pl.few.rows)
+        if (hipError_t e = p.type == F16 ? pa_few_tree_f16(a, pl, s) : p.type == Q8_0 ? pa_few_tree_q8(a, pl, s) : pa_few_tree_q4(a, pl, s)) return e;
+    return y.join ? join(a, pl, s) : hipSuccess;
 }
 
 }  // namespace g4

@@ -75,7 +75,9 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a) {
         if (half) {
             __syncthreads();                         // the previous token's angles are used
             if ((int)threadIdx.x < half) {
-                const double x = turns * (double)((int64_t)a.b.n_prefix + own);
+                // a tree's token is where its depth puts it, whatever its slot
+                const int at = a.depth ? sq.len - sq.nq + paged_depth(paged_ld(a.depth, t), sq.nq) : own;
+                const double x = turns * (double)((int64_t)a.b.n_prefix + at);
                 const float f = (float)(2.0 * (x - rint(x)));
                 float sn, cn;
                 sincospif(f, &sn, &cn);

@@ -1,0 +1,8 @@
+// k_paged_few_tree_f16.hip -- k_paged_few (paged_few.h) over trees of new tokens and F16 pages
+#include "paged_few.h"
+
+namespace g4 {
+
+hipError_t pa_few_tree_f16(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) { return pa_few<F16, true>(a, pl, s); }
+
+}  // namespace g4

@@ -1,0 +1,8 @@
+// k_paged_many_tree_q4.hip -- k_paged_many (paged_many.h) over trees of new tokens and Q4_0 pages
+#include "paged_many.h"
+
+namespace g4 {
+
+hipError_t pa_many_tree_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) { return pa_many<Q4_0, true>(a, pl, s); }
+
+}  // namespace g4

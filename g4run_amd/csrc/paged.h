@@ -111,6 +111,7 @@ struct PagedAppend {
     const float *q, *k, *v;
     float *q_out;
     size_t qs, qos, ks, vs;
+    const int *depth;                // of a tree's tokens (k_paged_tree.hip), or null: they follow each other
 };
 hipError_t launch_paged_append(const PagedAppend &a, hipStream_t s);
 
@@ -132,10 +133,63 @@ struct PagedAttn {
     float scale, cap;
     int window;
     uint8_t *ws;
+    const uint32_t *mask;            // trees of new tokens: rows of `words` words, and the tokens' depths
+    const int *depth;
+    int words;
 };
 // workspace of a call: the workgroups' partial results and where each (token, head)
 // row's lie, 0 where a call writes its outputs directly
 size_t paged_attn_workspace(const PagedPool &p, const PagedBatch &b, int n_head);
 hipError_t launch_paged_attn(PagedAttn a, hipStream_t s);
+// of trees of new tokens (a.mask): a split of its own
+size_t paged_attn_tree_workspace(const PagedPool &p, const PagedBatch &b, int n_head);
+hipError_t launch_paged_attn_tree(PagedAttn a, hipStream_t s);
+
+// ---- trees of drafted tokens, and rows moved within the caches (k_paged_tree.hip, k_paged_move.hip) ----
+constexpr int PAGED_TREE_WORDS = 32;             // words of a mask row at most
+constexpr int PAGED_CACHES = 64;                 // caches of one launch
+
+// the depth of new token i of n as a call may use it
+__host__ __device__ __forceinline__ int paged_depth(int depth, int n) { return min(max(depth, 0), max(n, 1) - 1); }
+
+struct PagedTreeBuild {
+    PagedBatch b;
+    const int *parent;
+    int words;
+    uint32_t *mask;
+    int *depth, *status;
+};
+hipError_t launch_paged_tree_build(const PagedTreeBuild &a, hipStream_t s);
+
+struct PagedTreeAccept {
+    PagedBatch b;
+    const int *parent, *token, *choice;
+    int most;
+    int *n_keep, *keep, *next, *len_out, *status;
+};
+hipError_t launch_paged_tree_accept(const PagedTreeAccept &a, hipStream_t s);
+
+// The pools of up to PAGED_CACHES caches of one shape: `p` describes each of them, its
+// k and v are the first one's.
+struct PagedPools {
+    uint8_t *k[PAGED_CACHES], *v[PAGED_CACHES];
+};
+struct PagedKeep {
+    PagedPool p;
+    PagedBatch b;
+    int n_cache, most;
+    const int *n_keep, *keep;
+};
+hipError_t launch_paged_keep(const PagedKeep &a, const PagedPools &pools, hipStream_t s);
+
+struct PagedFork {
+    PagedPool p;
+    PagedBatch b;
+    int n_cache, n_out;
+    const int *parent, *fresh;
+    int *len_out, *table_out;
+    int out_stride;
+};
+hipError_t launch_paged_fork(const PagedFork &a, const PagedPools &pools, hipStream_t s);
 
 }  // namespace g4

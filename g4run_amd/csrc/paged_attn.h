@@ -108,6 +108,8 @@ __device__ __forceinline__ PagedCall pa_fresh() {
     pa_global(k.a.p.status);
     pa_global(k.a.q);
     pa_global(k.a.out);
+    pa_global(k.a.mask);
+    pa_global(k.a.depth);
     pa_global(k.pl.few.o);
     pa_global(k.pl.few.ml);
     pa_global(k.pl.many.o);
@@ -202,6 +204,39 @@ __device__ __forceinline__ bool pa_hits(uint64_t out, int first, int stride, int
     }
     return hit;
 }
+// 32 bits of a tree's mask row from bit `off` on (off may be anything): 0 outside of it
+__device__ __forceinline__ uint32_t pa_bits(const uint32_t *mask, int words, int off) {
+    const int w = off >> 5;
+    const uint32_t lo = w >= 0 && w < words ? mask[w] : 0u, hi = w + 1 >= 0 && w + 1 < words ? mask[w + 1] : 0u;
+    return (uint32_t)(((uint64_t)hi << 32 | lo) >> (off & 31));
+}
+// Whether a tree's row attends nothing: no position of the prefix, no cached one, no
+// new token that has a position.
+__device__ __forceinline__ bool pa_tree_nothing(const PagedAttn &a, const PagedSeq &q, int tok) {
+    const int first_new = q.len - q.nq;
+    if (first_new + (tok - q.t0) < 0) return true;
+    const int low = a.window ? first_new + paged_depth(a.depth[tok], q.nq) + 1 - a.window : -0x7fffffff;       // first position, the prefix's below 0
+    if ((a.b.n_prefix > 0 && low < 0) || (first_new > 0 && low < first_new)) return false;
+    const uint32_t *mask = a.mask + (size_t)tok * a.words;
+    for (int w = 0; w < a.words; w++) {
+        const int n = q.nq - 32 * w, gone = -first_new - 32 * w;             // tokens from this word on; of them before position 0
+        uint32_t bits = n >= 32 ? mask[w] : n > 0 ? mask[w] & ((1u << n) - 1) : 0u;
+        if (gone > 0) bits = gone >= 32 ? 0u : bits & ~((1u << gone) - 1);
+        if (bits) return false;
+    }
+    return true;
+}
+// pa_hits of a tree's row: cached positions [rlo, rhi], or new tokens; of those,
+// bits(pos) has in its low 16 bits which of the positions from pos on it attends
+template <typename F>
+__device__ __forceinline__ bool pa_tree_hits(uint64_t out, int first, int stride, int last, int rlo, int rhi, F bits) {
+    bool hit = false;
+    for (; out; out &= out - 1) {
+        const int k = __ffsll((unsigned long long)out) - 1, pos = 16 * min(first + stride * (k >> 1) + (k & 1), last);
+        hit |= (rlo <= pos + 15 && rhi >= pos) || (bits(pos) & 0xffffu);
+    }
+    return hit;
+}
 // the offset of a unit's rows in the pools and, quantized, of their scales
 struct PaUnit {
     size_t row, sc;
@@ -250,8 +285,9 @@ __host__ __device__ __forceinline__ int pa_tokens(const PagedBatch &b, int n_seq
 // first own position that tokens from `first` on attend, rounded down to 32
 __host__ __device__ __forceinline__ int pa_low(int first, int window) { return window ? max(0, first + 1 - window) & ~31 : 0; }
 
-// position of global token tok (prefix included), its sequence looked up
-__device__ __forceinline__ int pa_token_pos(const PagedPool &p, const PagedBatch &b, int n_seq, int tok) {
+// position of global token tok (prefix included), its sequence looked up; a tree's
+// (depth given) as its depth says
+__device__ __forceinline__ int pa_token_pos(const PagedPool &p, const PagedBatch &b, int n_seq, int tok, const int *depth = nullptr) {
     int s = tok;
     if (b.q_off) {
         int x = 0, y = n_seq;                                // last s with q_off[s] <= tok
@@ -263,7 +299,7 @@ __device__ __forceinline__ int pa_token_pos(const PagedPool &p, const PagedBatch
         s = x;
     }
     const PagedSeq o = paged_seq(p, b, s);
-    return b.n_prefix + o.len - o.nq + (tok - o.t0);
+    return b.n_prefix + o.len - o.nq + (depth ? paged_depth(depth[tok], o.nq) : tok - o.t0);
 }
 
 // inclusive sum over the lanes of a wave: within each row of 16, then the rows'
@@ -293,33 +329,34 @@ __host__ __device__ __forceinline__ int pa_tiles(const PagedPlan &pl, const Page
     const uint32_t n = q.nq + pl.many.toks - 1;
     return pl.many.toks_inv ? (int)((uint64_t)n * pl.many.toks_inv >> 32) : (int)n;
 }
-template <bool MANY>
+// A tree's tokens (TREE) may all attend all new tokens, and start with the first one's window.
+template <bool MANY, bool TREE = false>
 __host__ __device__ __forceinline__ void pa_tile_span(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile, int &lo, int &hi) {
-    const int first = q.len - q.nq + (MANY ? tile * pl.many.toks : 0);
+    const int first = q.len - q.nq + (MANY && !TREE ? tile * pl.many.toks : 0);
     lo = pa_low(first, a.window);
-    hi = MANY ? min(q.len, first + pl.many.toks) - 1 : q.len - 1;
+    hi = MANY && !TREE ? min(q.len, first + pl.many.toks) - 1 : q.len - 1;
 }
-template <bool MANY>
+template <bool MANY, bool TREE = false>
 __host__ __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile) {
     if (q.bad) return 1;
     const PagedList &y = pa_list<MANY>(pl);
     int lo, hi;
-    pa_tile_span<MANY>(a, pl, q, tile, lo, hi);
+    pa_tile_span<MANY, TREE>(a, pl, q, tile, lo, hi);
     return max(1, (hi - lo + y.unit) >> y.shift);
 }
 // steps of a sequence for one KV head
-template <bool MANY>
+template <bool MANY, bool TREE = false>
 __host__ __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q) {
     const int tiles = pa_tiles<MANY>(pl, q);
     int n = 0;
-    for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY>(a, pl, q, t);
+    for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY, TREE>(a, pl, q, t);
     return n + tiles * pa_list<MANY>(pl).lead;
 }
 // All steps of the list (wave-uniform; the whole wave calls it), 64 sequences at a
 // time; the lane's own of the first 64 in `mine`.  The batch ends at the first torn
 // sequence, n_seq: offsets that descend would give tokens to several sequences, and
 // more steps than the host counted.
-template <bool MANY>
+template <bool MANY, bool TREE = false>
 __device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl, int &mine, int &n_seq) {
     const PagedList &y = pa_list<MANY>(pl);
     const int lane = threadIdx.x & 63;
@@ -333,7 +370,7 @@ __device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl,
                 if (s0 + lane >= n_seq) q.nq = 0;
             }
         }
-        return pa_steps<MANY>(a, pl, q);
+        return pa_steps<MANY, TREE>(a, pl, q);
     };
     n_seq = a.b.n_seq;
     mine = at(0);
@@ -349,11 +386,11 @@ __device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl,
 struct PaFind {
     int s0 = 0, before = 0;
 };
-template <bool MANY>
+template <bool MANY, bool TREE = false>
 __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan &pl, int mine, int u, PaFind &from, int &seq, int &before) {
     const int lane = threadIdx.x & 63;
     for (; from.s0 < a.b.n_seq; from.s0 += 64) {
-        const int n = (from.s0 == 0 ? mine : from.s0 + lane < a.b.n_seq ? pa_steps<MANY>(a, pl, paged_seq(a.p, a.b, from.s0 + lane)) : 0) * a.p.n_kv;
+        const int n = (from.s0 == 0 ? mine : from.s0 + lane < a.b.n_seq ? pa_steps<MANY, TREE>(a, pl, paged_seq(a.p, a.b, from.s0 + lane)) : 0) * a.p.n_kv;
         const int incl = pa_scan(n);
         const uint64_t past = __ballot(from.before + incl > u);
         if (past) {
@@ -376,13 +413,14 @@ struct PaPiece {
     int kvh, tile, step, n, all;
     int took;                        // of the share: n and what it holds of the lead; n is 0 where it ends in that
     int seglen, start, end;          // positions of the segment; the piece's [start, end)
-    int hi0, hi1, lo0, lo1;          // the first and the last row's last and first positions
+    int hi0, hi1, lo0, lo1;          // the first and the last row's last and first positions (a tree: hi0 the first new token's,
+                                     // hi1 the last's; lo0 and lo1 as if its depths were 0 and the most)
     int slot;                        // of its sums
     const int *table;
     bool pre;
 };
 // the piece at step u of a share [first, stop); find(u, seq, before) as pa_find_step
-template <bool MANY, typename F>
+template <bool MANY, bool TREE = false, typename F>
 __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, const PagedPlan &pl, int n_seq, int wg, int u, int first, int stop, F find) {
     const PagedList &y = pa_list<MANY>(pl);
     const PagedBatch &b = a.b;
@@ -413,17 +451,17 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
         if constexpr (MANY) {
             const int tiles = pa_tiles<MANY>(pl, x.sq);
             int head = tiles * y.lead;                       // steps of one KV head
-            for (int t = 0; t < tiles; t++) head += pa_tile_steps<MANY>(a, pl, x.sq, t);
+            for (int t = 0; t < tiles; t++) head += pa_tile_steps<MANY, TREE>(a, pl, x.sq, t);
             for (x.kvh = 0; v >= head; x.kvh++) v -= head;
             x.tile = 0;
-            for (x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0); v >= y.lead + x.all; x.all = pa_tile_steps<MANY>(a, pl, x.sq, ++x.tile)) v -= y.lead + x.all;
+            for (x.all = pa_tile_steps<MANY, TREE>(a, pl, x.sq, 0); v >= y.lead + x.all; x.all = pa_tile_steps<MANY, TREE>(a, pl, x.sq, ++x.tile)) v -= y.lead + x.all;
         } else {
-            x.all = pa_tile_steps<MANY>(a, pl, x.sq, 0);
+            x.all = pa_tile_steps<MANY, TREE>(a, pl, x.sq, 0);
             x.tile = 0;
             for (x.kvh = 0; v >= y.lead + x.all; x.kvh++) v -= y.lead + x.all;
         }
-        pa_tile_span<MANY>(a, pl, x.sq, x.tile, base, x.hi1);
-        x.hi0 = x.sq.len - x.sq.nq + (MANY ? x.tile * pl.many.toks : 0);
+        pa_tile_span<MANY, TREE>(a, pl, x.sq, x.tile, base, x.hi1);
+        x.hi0 = x.sq.len - x.sq.nq + (MANY && !TREE ? x.tile * pl.many.toks : 0);
         x.lo0 = a.window ? max(0, x.hi0 + 1 - a.window) : 0;
         x.lo1 = a.window ? max(0, x.hi1 + 1 - a.window) : 0;
         x.seglen = x.sq.bad ? 0 : x.sq.len;
@@ -437,9 +475,9 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
     x.slot = 2 * wg + (u != first);
     return x;
 }
-template <bool MANY>
+template <bool MANY, bool TREE = false>
 __device__ __forceinline__ PaPiece pa_piece(const PagedAttn &a, const PagedPlan &pl, int mine, int n_seq, PaFind &from, int wg, int u, int first, int stop) {
-    return pa_piece_by<MANY>(a, pl, n_seq, wg, u, first, stop, [&](int v, int &seq, int &before) { pa_find_step<MANY>(a, pl, mine, v, from, seq, before); });
+    return pa_piece_by<MANY, TREE>(a, pl, n_seq, wg, u, first, stop, [&](int v, int &seq, int &before) { pa_find_step<MANY, TREE>(a, pl, mine, v, from, seq, before); });
 }
 // Where row r (of its tile) of a piece puts its sums: out (normalised), or `o` and
 // `ml`; and, from a tile's first piece, where k_paged_join finds them.
@@ -581,5 +619,12 @@ hipError_t pa_few_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
 hipError_t pa_many_f16(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
 hipError_t pa_many_q8(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
 hipError_t pa_many_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+// and over trees of new tokens
+hipError_t pa_few_tree_f16(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+hipError_t pa_few_tree_q8(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+hipError_t pa_few_tree_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+hipError_t pa_many_tree_f16(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+hipError_t pa_many_tree_q8(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
+hipError_t pa_many_tree_q4(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);
 
 }  // namespace g4

@@ -131,7 +131,7 @@ __device__ __forceinline__ int pa_elem(int m, int x) {
     return KVT != F16 ? 16 * m + x : HE == 64 ? 4 * x + m : 128 * (m >> 3) + 8 * x + (m & 7);
 }
 
-template <int HD, int KVT, bool ST>
+template <int HD, int KVT, bool ST, bool TREE>
 __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(PagedCall call) {
     constexpr int R = ST ? 8 : 16, HE = HD > 128 ? 128 : HD, ES = HD / HE, PW = 4 / ES, NS = HE / 32, NM = HE / 16;
     constexpr int QP = HD + 8;                               // padded query row
@@ -141,11 +141,12 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
     __shared__ float2 wml[4][R];                             // two waves of one tile may differ in m (by their elements' scales)
     __shared__ __align__(16) float xs[ES > 1 ? 2 : 1][ES > 1 ? 4 : 1][ES > 1 ? 64 : 1][8];   // partial scores of the waves of one tile
     __shared__ __align__(16) PaScales<HE> scl[KVT == F16 ? 1 : 4];           // of a wave
+    __shared__ int nothing[TREE ? R : 1];                    // whether a tree's row attends nothing
     _Float16 *const qh = (_Float16 *)lds;
     float *const buf = (float *)lds;
 
     int mine, n_seq;
-    const int total = pa_total<false>(call.a, call.pl, mine, n_seq), share = pa_share(call.pl.few, total);
+    const int total = pa_total<false, TREE>(call.a, call.pl, mine, n_seq), share = pa_share(call.pl.few, total);
     const int first = blockIdx.x * share, stop = min(first + share, total);
     if (blockIdx.x == 0 && call.pl.many.rows == 0) pa_rest(call.a, call.pl, n_seq);
     PaFind from;
@@ -157,14 +158,16 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         const PagedBatch &b = a.b;
         const int tid = pa_thread(), lane = tid & 63, wave = pa_uniform(tid >> 6), c = lane & 15, g = lane >> 4, ew = wave % ES, pw = wave / ES;
         const int G = a.grp, rc = ST ? c & 7 : c;
-        const PaPiece x = pa_piece<false>(a, pl, mine, n_seq, from, blockIdx.x, u, first, stop);
+        const PaPiece x = pa_piece<false, TREE>(a, pl, mine, n_seq, from, blockIdx.x, u, first, stop);
         u += x.took;
         if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;
         const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = sq.nq * G;
         bool bad = sq.bad;
         if (bad && tid == 0) paged_flag(p, PAGED_BAD_BATCH);
-        const bool mixed = hi0 != x.hi1 || lo0 != lo1;       // whether the rows differ in what they attend
+        const bool tree = TREE && !x.pre;
+        const bool mixed = tree || hi0 != x.hi1 || lo0 != lo1;           // whether the rows differ in what they attend
+        const int full = tree ? hi0 - 1 : hi0;               // the last position that all rows attend, windows apart
         const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 32 * PW - 1) / (32 * PW) : 0;
 
         // queries: loaded first, ahead of the stream
@@ -187,15 +190,28 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         }
         // the lane's row: positions [rlo, rhi]
         int rlo = lo0, rhi = hi0;
+        uint32_t bits = 0;                                   // a tree's row: its new tokens (16 at most), from position hi0 on
         if (rc < rows) {
             const int i = (int)(rc * pl.grp_inv >> 16);
-            if (!x.pre) {
+            if (tree) {
+                rhi = hi0 + i < 0 ? -1 : hi0 - 1;
+                if (hi0 + i >= 0) bits = a.mask[(size_t)(sq.t0 + i) * a.words];
+                rlo = a.window ? max(0, hi0 + paged_depth(a.depth[sq.t0 + i], sq.nq) + 1 - a.window) : 0;
+            } else if (!x.pre) {
                 rhi = hi0 + i;
                 rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
             } else if (a.window) {
-                rlo = max(0, pa_token_pos(p, b, n_seq, sq.t0 + i) + 1 - a.window);
+                rlo = max(0, pa_token_pos(p, b, n_seq, sq.t0 + i, TREE ? a.depth : nullptr) + 1 - a.window);
             }
         }
+        auto row_bits = [&](int pos) {                       // from position pos on
+            const int off = pos - hi0;
+            return off <= -32 || off >= 32 ? 0u : off < 0 ? bits << -off : bits >> off;
+        };
+        auto row_hits = [&](uint64_t out, int first, int stride) {
+            if constexpr (TREE) return pa_tree_hits(out, first, stride, last, rlo, rhi, row_bits);
+            else return pa_hits(out, first, stride, last, rlo, rhi);
+        };
 
         PaTile<HE, KVT> kv;
         PaUnit un[2], nx[2];
@@ -203,7 +219,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         int base = start + 32 * pw;
         if (iters) {
             us = pa_units(p, x.table, base >> 4, 2 * PW, last, kvh);
-            bad |= pa_hits(pa_check(p, us), base >> 4, 2 * PW, last, rlo, rhi);
+            bad |= row_hits(pa_check(p, us), base >> 4, 2 * PW);
             nx[0] = pa_unit<HD, KVT>(p, us, 0);
             nx[1] = pa_unit<HD, KVT>(p, us, 1);
             if constexpr (KVT != F16) pa_load_scales<HD, HE, KVT>(kv, p, nx, lane, ew);
@@ -211,6 +227,9 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
             pa_load_v<HD, HE, KVT>(kv, p, nx, c, g, ew);
         }
         lds_barrier();                                       // the previous piece's sums are read
+        if constexpr (TREE) {
+            if (tid < R) nothing[tid] = tid < rows && !x.pre && !sq.bad && pa_tree_nothing(a, sq, sq.t0 + (int)(tid * pl.grp_inv >> 16));
+        }
         {
             float am = 0.0f;
 #pragma unroll
@@ -254,14 +273,19 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
             un[1] = nx[1];
             if ((it & 31) == 31 && it + 1 < iters) {
                 us = more_us;
-                bad |= pa_hits(pa_check(p, us), (base >> 4) + 2 * PW, 2 * PW, last, rlo, rhi);
+                bad |= row_hits(pa_check(p, us), (base >> 4) + 2 * PW, 2 * PW);
             }
             if (more) {
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
                 nx[1] = pa_unit<HD, KVT>(p, us, (2 * (it + 1) & 63) + 1);
             }
             if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units(p, x.table, (base >> 4) + 64 * PW, 2 * PW, last, kvh);
-            const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
+            const bool edge = base + 31 > full || base < lo1 || base + 32 > end;
+            const uint32_t vis = TREE ? row_bits(base) : 0u;
+            auto seen = [&](int pos) {                       // by the lane's row
+                if constexpr (TREE) return ((pos >= rlo && pos <= rhi) || (vis >> (pos - base) & 1)) && pos < end;
+                else return pos >= rlo && pos <= rhi && pos < end;
+            };
             constexpr int DW = PaTile<HE, KVT>::DW;
             uint32_t dk[8][DW], dv[8][DW];                   // of the lane's 8 positions
             PaScales<HE> &sl = scl[KVT == F16 ? 0 : wave];
@@ -344,7 +368,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int pos = base + 16 * (j >> 2) + 4 * g + (j & 3);
-                    w[j] = pos >= rlo && pos <= rhi && pos < end ? w[j] : -__builtin_inff();
+                    w[j] = seen(pos) ? w[j] : -__builtin_inff();
                 }
             }
             if constexpr (KVT == F16) {
@@ -420,7 +444,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const int pos = base + 16 * (j >> 2) + 4 * g + (j & 3);
-                        const uint32_t live = pos >= rlo && pos <= rhi && pos < end ? ~0u : 0u;
+                        const uint32_t live = seen(pos) ? ~0u : 0u;
 #pragma unroll
                         for (int d = 0; d < DW; d++) dv[j][d] &= live;
                     }
@@ -458,7 +482,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                             const float v = __shfl(w[j], 16 * ((k & 15) >> 2) + c, 64);
                             if (j == 4 * (k >> 4) + (k & 3)) wx = v;
                         }
-                        const bool sees = pos >= rlo && pos <= rhi && !(ST && c >= 8);
+                        const bool sees = seen(pos) && !(ST && c >= 8);
 #pragma unroll
                         for (int e = 0; e < NM; e++)
 #pragma unroll
@@ -516,7 +540,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                 }
                 s *= VS;
                 const int i = (int)(r * pl.grp_inv >> 16), tok = sq.t0 + i, head = kvh * G + (r - i * G);
-                const bool none = !sq.bad && hi0 + i < 0;
+                const bool none = TREE ? nothing[r] : !sq.bad && hi0 + i < 0;
                 const PaSink to = pa_sink<false>(a, pl, x, share, r, tok, head, none, e4 == 0);
                 if (to.out) {
                     s = none ? pa_v4f{0.0f, 0.0f, 0.0f, 0.0f} : s * (1.0f / ls);
@@ -530,20 +554,20 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
     }
 }
 
-template <int KVT, int HD>
+template <int KVT, int HD, bool TREE>
 hipError_t pa_few_hd(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
     const dim3 grid(pl.few.wgs), wg(256);
-    if (pl.few.rows <= 8) hipLaunchKernelGGL((k_paged_few<HD, KVT, true>), grid, wg, 0, s, PagedCall{a, pl});
-    else hipLaunchKernelGGL((k_paged_few<HD, KVT, false>), grid, wg, 0, s, PagedCall{a, pl});
+    if (pl.few.rows <= 8) hipLaunchKernelGGL((k_paged_few<HD, KVT, true, TREE>), grid, wg, 0, s, PagedCall{a, pl});
+    else hipLaunchKernelGGL((k_paged_few<HD, KVT, false, TREE>), grid, wg, 0, s, PagedCall{a, pl});
     return hipGetLastError();
 }
-template <int KVT>
+template <int KVT, bool TREE = false>
 hipError_t pa_few(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
     switch (a.p.hd) {
-    case 64: return pa_few_hd<KVT, 64>(a, pl, s);
-    case 128: return pa_few_hd<KVT, 128>(a, pl, s);
-    case 256: return pa_few_hd<KVT, 256>(a, pl, s);
-    case 512: return pa_few_hd<KVT, 512>(a, pl, s);
+    case 64: return pa_few_hd<KVT, 64, TREE>(a, pl, s);
+    case 128: return pa_few_hd<KVT, 128, TREE>(a, pl, s);
+    case 256: return pa_few_hd<KVT, 256, TREE>(a, pl, s);
+    case 512: return pa_few_hd<KVT, 512, TREE>(a, pl, s);
     }
     return hipErrorInvalidValue;
 }

@@ -20,7 +20,8 @@ struct PagedLayout {
     size_t fo, fml, mo, mml, own, pre, wo, wml, total;
 };
 // of a batch with tokens and sequences; window 0 gives the most workspace
-inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp, int window) {
+// (tree: of trees of new tokens, whose tiles all end with the last one)
+inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp, int window, bool tree = false) {
     PagedLayout y;
     PagedPlan &pl = y.pl;
     PagedList &few = pl.few, &many = pl.many;
@@ -80,7 +81,7 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
         many.rows = many.toks * grp;
         many.pre_tiles = many_pre ? pa_ceil_div(b.n_tok, many.toks) : 0;
         const int64_t own = !many_own ? 0 : b.q_off ? pa_ceil_div(b.n_tok, many.toks) + std::min(b.n_seq, b.n_tok / (few.toks + 1)) : b.n_seq;
-        const int64_t mspan = span(many.toks);
+        const int64_t mspan = span(tree ? b.n_tok : many.toks);
         for (many.shift = 5;; many.shift++) {
             many.unit = 1 << many.shift;
             many.pre_steps = many_pre ? pa_ceil_div(b.n_prefix, many.unit) : 0;

@@ -382,6 +382,113 @@ int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_h
                    float scale, float softcap, int window, float *out_dev, size_t out_stride, void *ws_dev, size_t ws_bytes,
                    void *stream);
 
+/* ------------------------------------- drafts that are trees, and beams ---- */
+/* More than one continuation of a sequence at a time over the paged cache (no
+ * counterpart in the reference, which verifies one row of drafted tokens,
+ * main.c:383-397).  A draft is a tree: a sequence's new tokens (g4h_paged_batch)
+ * continue each other by their parents, in the batch's slots one behind the
+ * other, and each attends the cached positions and its own ancestors only.  With
+ * `first` = len - n, the position of a sequence's first new token, a step is
+ *   g4h_paged_tree_build     masks and depths from the parents, once;
+ *   g4h_paged_append_tree    per layer: token i into slot first + i, rotated by
+ *                            position first + depth[i];
+ *   g4h_paged_attn_tree      per layer;
+ *   g4h_paged_tree_accept    which tokens the target model's choices confirm;
+ *   g4h_paged_keep           their rows moved to first, first + 1, .. in all
+ *                            layers, where their rotation puts them.
+ * All are asynchronous and capturable. */
+typedef struct {
+    int words;                 /* 32-bit words of a mask row, 1 .. 32 */
+    const uint32_t *mask_dev;  /* [n_tok][words]: bit j of a token's row: it attends its sequence's new token j */
+    const int *depth_dev;      /* [n_tok]: its position over the sequence's first new token */
+} g4h_paged_tree;
+/* parent_dev[t]: the number, within its sequence, of the token that token t
+ * continues, smaller than its own, or -1: the cached positions.  A mask holds the
+ * token's own bit and its ancestors', a depth counts these.  Any other parent sets
+ * G4H_PAGED_BAD_BATCH in *status_dev (may be NULL) and counts as -1; so does a
+ * sequence of more than 32 words tokens, of which those behind get no bit and depth
+ * 0.  With offsets that descend or leave [0, n_tok] (flagged too) the masks and
+ * depths of the whole batch are undefined, as are those of rows of no sequence
+ * without them: those are left as they were.  Only n_seq, n_tok and q_off_dev of the
+ * batch are used. */
+int g4h_paged_tree_build(const g4h_paged_batch *batch, const int *parent_dev, int words, uint32_t *mask_dev, int *depth_dev,
+                         int *status_dev, void *stream);
+/* g4h_paged_append with the rotations of positions first + depth (a depth outside
+ * 0 .. n - 1 counts as the nearest); the masks are not used and may be NULL. */
+int g4h_paged_append_tree(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_paged_tree *tree, const g4h_rope *rope, int n_head,
+                          const float *q_dev, size_t q_stride, float *q_out_dev, size_t q_out_stride, const float *k_dev, size_t k_stride,
+                          const float *v_dev, size_t v_stride, void *stream);
+/* g4h_paged_attn of a tree's tokens: a token attends the prefix's and the cached
+ * positions before its sequence's first new one -- with a window those after first
+ * + depth - window -- and of the new tokens those whose bits are set, its own among
+ * them only if set, whatever their order; bits of tokens that the sequence does not
+ * have mean nothing, and the window hides none of them.  Zeros for a token that
+ * attends nothing, as for one without a position.  Everything else as there, with a
+ * workspace of its own size. */
+size_t g4h_paged_attn_tree_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head);
+int g4h_paged_attn_tree(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_paged_tree *tree, int n_head, const float *q_dev,
+                        size_t q_stride, float scale, float softcap, int window, float *out_dev, size_t out_stride, void *ws_dev,
+                        size_t ws_bytes, void *stream);
+/* The walk that verifies a draft: from a sequence's new token 0 (the last one that
+ * is certain) on to the first child (the lowest j with parent[j] the present token)
+ * whose token_dev is the choice_dev made at the present one (g4h_argmax_rows, or a
+ * sampler's draw), until there is none or `most` (1 .. 1024) are kept.
+ *   n_keep[s], keep[s][most]: their numbers, ascending, then -1;
+ *   next[s] (may be NULL): the choice at the last of them, the next step's token 0;
+ *   len_out[s] (may be NULL): the sequence's positions without the others.
+ * A sequence without new tokens, or with fewer positions than those, keeps none and
+ * has next -1.  Lengths outside [0, max_len] and offsets that descend or leave
+ * [0, n_tok] are flagged; such sequences keep none and get len_out 0. */
+int g4h_paged_tree_accept(const g4h_paged_batch *batch, const int *parent_dev, const int *token_dev, const int *choice_dev, int most,
+                          int *n_keep_dev, int *keep_dev, int *next_dev, int *len_out_dev, int *status_dev, void *stream);
+/* Moves, in n_cache caches of one shape (kv[0 .. n_cache), a model's layers; flags go
+ * to the first one's status word), the keys and values of each sequence's new tokens
+ * keep[s][k], k < n_keep[s], to the slots first + k, bit for bit.  Lists ascend
+ * (keep_dev [n_seq][most], as g4h_paged_tree_accept writes them): from the first
+ * entry that does not, or that the sequence does not have, on nothing is moved
+ * (G4H_PAGED_BAD_BATCH); a row whose page or whose place's page is outside the pool is
+ * left where it is (G4H_PAGED_BAD_PAGE).  The batch is the one that was appended, its
+ * lengths unchanged; a sequence with fewer positions than new tokens is left alone.
+ * Slots behind the kept ones keep what they hold. */
+int g4h_paged_keep(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *batch, const int *n_keep_dev, const int *keep_dev, int most,
+                   void *stream);
+/* Rows of a new batch that continue rows of the present one, as a beam selection
+ * leaves them: for i < n_out, with len = len[parent[i]],
+ *   len_out[i] = len;
+ *   table_out[i]: the parent's len / page whole pages, shared with it, then
+ *     fresh[i], in all n_cache caches (kv[0 .. n_cache), of one shape) holding
+ *     copies of the parent's len % page rows behind those.  Later entries keep what
+ *     they hold.
+ * parent -1: no row (len_out 0, its table left as it was); so are, flagged, any other
+ * parent outside [0, n_seq), a length outside its bounds and one of more than
+ * out_stride pages.  Pages outside the pool are flagged where rows would be copied,
+ * and not copied.  fresh[i] may be the parent's own last page, which then goes on in
+ * place -- for one of its rows at most; no other fresh page may be one that a row of
+ * the present batch reads or another row's fresh one.  Of the batch n_seq, len_dev,
+ * table_dev, table_stride and max_len are used; the outputs may not overlap them.
+ * len_out and table_out may both be NULL, where the caches of another shape have had
+ * them. */
+int g4h_paged_fork(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *batch, int n_out, const int *parent_dev, const int *fresh_dev,
+                   int *len_out_dev, int *table_out_dev, int out_stride, void *stream);
+/* Beam search's selection.  Of each of n_group groups of n_beam rows of logits
+ * (stride floats apart, 0: n_vocab; 4-byte aligned) the n_out (1 .. 64) largest of
+ *   score[row] + logits[row][v] - log sum_u exp(logits[row][u])
+ * in descending order: score_out, row_out (the row's number among all n_group *
+ * n_beam, g4h_paged_fork's parent) and token_out, each [n_group][n_out].  Equal ones
+ * go by row, then by token (equal logits of a row: by token); rows are compared by
+ * scores in 64 bits, whose normalisers carry an fp32 sum's error.  A row whose
+ * ended_dev (may be NULL) is not 0 competes once, with its score as it is and token
+ * -1; its logits are not read.  Tokens at -inf, rows at score -inf and rows with a
+ * NaN or +inf among their logits, or in their score, are never selected; where fewer
+ * than n_out can be, the rest has score -inf, row -1 and token -1.  n_out == n_beam:
+ * score_out may be score.  Up to 2^20 rows of up to 2^24 logits, 64 beams a group.
+ * ws: g4h_beam_workspace_bytes() of caller-owned scratch, 16-byte aligned, without
+ * initial contents; calls that overlap must not share it.  Asynchronous, capturable;
+ * runs repeat bit for bit. */
+size_t g4h_beam_workspace_bytes(int n_group, int n_beam, int n_vocab, int n_out);
+int g4h_beam_select(const float *logits_dev, size_t stride, int n_group, int n_beam, int n_vocab, const float *score_dev, const int *ended_dev,
+                    int n_out, float *score_out_dev, int *row_out_dev, int *token_out_dev, void *ws_dev, size_t ws_bytes, void *stream);
+
 /* -------------------------------------------------------- decode step ---- */
 /* A gemma-style decoder resident on the device (the model behind
  * g4_ctx_init / g4_forward, g4run.h:303-311): layer order of model.c:647-736
