@@ -112,7 +112,7 @@ hipError_t launch_paged_attn_tree(PagedAttn a, hipStream_t s) {
     const PagedLayout y = paged_layout(p, b, a.grp, a.window, true);
     const PagedPlan pl = paged_places(y, a.ws);
     if (pl.many.rows)
-        if (hipError_t e = p.type == F16 ? pa_many_tree_f16(a, pl, s) : p.type == Q8_0 ? pa_many_tree_q8(a, pl, s) : pa_many_tree_q4(a, pl, s)) return e;
+        if (hipError_t e = p.type == F16 ? pa_tree_f16(a, pl, y.wide, s) : p.type == Q8_0 ? pa_tree_q8(a, pl, y.wide, s) : pa_tree_q4(a, pl, y.wide, s)) return e;
     if (pl.few.rows)
         if (hipError_t e = p.type == F16 ? pa_few_tree_f16(a, pl, s) : p.type == Q8_0 ? pa_few_tree_q8(a, pl, s) : pa_few_tree_q4(a, pl, s)) return e;
     return y.join ? join(a, pl, s) : hipSuccess;

@@ -247,7 +247,7 @@ __device__ __forceinline__ void pm_wave() { asm volatile("s_waitcnt lgkmcnt(0)" 
 // a wave's 16 rows of 32 floats on their way between memory and operands, padded
 constexpr int PM_COLS = 36, PM_TR = 16 * PM_COLS;
 
-template <int HD, int KVT, bool TREE>
+template <int HD, int KVT>
 __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(PagedCall call) {
     constexpr int HE = HD > 256 ? 256 : HD, ES = HD / HE, NS = HE / 32, NM = HE / 16, NB = HD > 256 ? 1 : 2, AHEAD = HD == 64 || HD == 512 ? 2 : 4, BLOCKS = HD > 64 ? 2 : 1;    // NB: buffers
     constexpr size_t TB = sizeof(PmTile<HD, KVT>) * NB, RB = (size_t)8 * PM_TR * 4;
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
     // that read the same K and V find them in its L2.
     const int per = (call.pl.many.wgs + 7) >> 3, wg = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     int mine, n_seq;
-    const int total = pa_total<true, TREE>(call.a, call.pl, mine, n_seq), share = pa_share(call.pl.many, total);
+    const int total = pa_total<true>(call.a, call.pl, mine, n_seq), share = pa_share(call.pl.many, total);
     const int first = wg * share, stop = wg < call.pl.many.wgs ? min(first + share, total) : 0;
     if (blockIdx.x == 0) pa_rest(call.a, call.pl, n_seq);
     PaFind from;
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         const int G = a.grp, R = pl.many.rows;
         float *const tr = (float *)lds + wave * PM_TR;
         const float capl = a.cap * 1.4426950408889634f;
-        const PaPiece x = pa_piece<true, TREE>(a, pl, mine, n_seq, from, wg, u, first, stop);
+        const PaPiece x = pa_piece<true>(a, pl, mine, n_seq, from, wg, u, first, stop);
         u += x.took;
         if (x.n == 0) break;                                 // the share ends in a tile's lead
         const PagedSeq &sq = x.sq;
@@ -282,8 +282,6 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         bool bad = sq.bad;
         if (bad && tid == 0) paged_flag(p, PAGED_BAD_BATCH);
         const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 31) / 32 : 0;
-        const bool tree = TREE && !x.pre;
-        const int full = tree ? hi0 - 1 : hi0;               // the last position that all rows attend, windows apart
 
         // The queries first (rows 8 k + lane / 8 of the wave's, elements 32 s + 4 (lane %
         // 8) ..): they are back with the page ids, and used while the first keys and values come.
@@ -319,24 +317,15 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         const bool busy = r0 < rows, ok = r0 + c < rows;
         const int ri = ok ? (r0 + c) / G : 0, head = kvh * G + (ok ? r0 + c - ri * G : 0), tok = sq.t0 + ri;
         int rlo = lo0, rhi = hi0;                            // the lane's row attends [rlo, rhi]
-        const uint32_t *mask = nullptr;                      // a tree's row: its new tokens, from position hi0 on
         if (ok) {
-            if (tree) {
-                rhi = hi0 + ri < 0 ? -1 : hi0 - 1;
-                if (hi0 + ri >= 0) mask = a.mask + (size_t)tok * a.words;
-                rlo = a.window ? max(0, hi0 + paged_depth(a.depth[tok], sq.nq) + 1 - a.window) : 0;
-            } else if (!x.pre) {
+            if (!x.pre) {
                 rhi = sq.len - sq.nq + ri;
                 rlo = a.window ? max(0, rhi + 1 - a.window) : 0;
             } else if (a.window) {
-                rlo = max(0, pa_token_pos(p, b, n_seq, tok, TREE ? a.depth : nullptr) + 1 - a.window);
+                rlo = max(0, pa_token_pos(p, b, n_seq, tok) + 1 - a.window);
             }
         }
-        auto row_hits = [&](uint64_t out, int first) {
-            if constexpr (TREE) return pa_tree_hits(out, first, 2, last, rlo, rhi, [&](int pos) { return mask ? pa_bits(mask, a.words, pos - hi0) : 0u; });
-            else return pa_hits(out, first, 2, last, rlo, rhi);
-        };
-        bad |= row_hits(outside, start >> 4);
+        bad |= pa_hits(outside, start >> 4, 2, last, rlo, rhi);
         __syncthreads();                                     // the previous piece's tiles and rows are used
         // Queries, 32 elements at a time through the wave's part of LDS: whole lines
         // from memory, then the operand's 8 elements of one row.
@@ -386,15 +375,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 
         for (int it = 0, turn = 0; it < iters; it++, turn = turn == 2 ? 0 : turn + 1) {
             const int base = start + 32 * it;
-            const bool edge = base + 31 > full || base < lo1 || base + 32 > end;
-            uint32_t vis = 0;
-            if constexpr (TREE) {
-                if (edge && mask && base + 31 >= hi0) vis = pa_bits(mask, a.words, base - hi0);
-            }
-            auto seen = [&](int pos) {                       // by the lane's row
-                if constexpr (TREE) return ((pos >= rlo && pos <= rhi) || (vis >> (pos - base) & 1)) && pos < end;
-                else return pos >= rlo && pos <= rhi && pos < end;
-            };
+            const bool edge = base + 31 > hi0 || base < lo1 || base + 32 > end;
             PmTile<HD, KVT> &d = tiles[NB == 2 ? it & 1 : 0];
             if (NB == 1 && it) __syncthreads();              // one buffer: the previous positions are used
             if (pm_store<HD, KVT>(d, st, edge, lo0 - base, end - base, tid)) odds[turn] = 1;
@@ -402,7 +383,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
             un[1] = nx[1];
             if ((it & 31) == 31 && it + 1 < iters) {
                 us = more_us;
-                bad |= row_hits(pa_check(p, us), (base + 32) >> 4);
+                bad |= pa_hits(pa_check(p, us), (base + 32) >> 4, 2, last, rlo, rhi);
             }
             if (it + 1 < iters) {
                 nx[0] = pa_unit<HD, KVT>(p, us, 2 * (it + 1) & 63);
@@ -461,7 +442,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int pos = base + pm_pos(g, j);
-                    w[j] = seen(pos) ? w[j] : -__builtin_inff();
+                    w[j] = pos >= rlo && pos <= rhi && pos < end ? w[j] : -__builtin_inff();
                 }
             }
             float mt = -__builtin_inff();
@@ -515,7 +496,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
                             const float v = __shfl(w[j], 16 * ((k & 15) >> 2) + c, 64);
                             if (j == 4 * (k >> 4) + (k & 3)) wx = v;
                         }
-                        const bool sees = seen(pos);
+                        const bool sees = pos >= rlo && pos <= rhi;
 #pragma unroll
                         for (int e = 0; e < NM; e++) {
                             const uint2 hv = *(const uint2 *)(row + 16 * e + 4 * g);
@@ -535,7 +516,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const int pos = base + pm_pos(g, j);
-                        if (!seen(pos)) live[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
+                        if (!(pos >= rlo && pos <= rhi && pos < end)) live[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
                     }
                 }
                 // blocks of 32 elements: value tiles 2 s, 2 s + 1
@@ -568,7 +549,7 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
         // out through LDS as the queries came in
         __syncthreads();                                     // the tiles are used
         if (!busy) continue;
-        const bool nowhere = TREE ? ok && !x.pre && !sq.bad && pa_tree_nothing(a, sq, tok) : !sq.bad && sq.len - sq.nq + ri < 0;
+        const bool nowhere = !sq.bad && sq.len - sq.nq + ri < 0;
         float *to[2];
         bool out = false;
         if (g == 0) {
@@ -600,14 +581,14 @@ __global__ __launch_bounds__(PM_THREADS, HD >= 128 ? 2 : 4) void k_paged_many(Pa
     }
 }
 
-template <int KVT, bool TREE = false>
+template <int KVT>
 hipError_t pa_many(const PagedAttn &a, const PagedPlan &pl, hipStream_t s) {
     const dim3 grid((pl.many.wgs + 7) / 8 * 8), wg(PM_THREADS);
     switch (a.p.hd) {
-    case 64: hipLaunchKernelGGL((k_paged_many<64, KVT, TREE>), grid, wg, 0, s, PagedCall{a, pl}); break;
-    case 128: hipLaunchKernelGGL((k_paged_many<128, KVT, TREE>), grid, wg, 0, s, PagedCall{a, pl}); break;
-    case 256: hipLaunchKernelGGL((k_paged_many<256, KVT, TREE>), grid, wg, 0, s, PagedCall{a, pl}); break;
-    case 512: hipLaunchKernelGGL((k_paged_many<512, KVT, TREE>), grid, wg, 0, s, PagedCall{a, pl}); break;
+    case 64: hipLaunchKernelGGL((k_paged_many<64, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
+    case 128: hipLaunchKernelGGL((k_paged_many<128, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
+    case 256: hipLaunchKernelGGL((k_paged_many<256, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
+    case 512: hipLaunchKernelGGL((k_paged_many<512, KVT>), grid, wg, 0, s, PagedCall{a, pl}); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

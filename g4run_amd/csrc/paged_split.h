@@ -17,6 +17,7 @@ inline int paged_window(const PagedBatch &b, int window) { return window >= b.n_
 struct PagedLayout {
     PagedPlan pl;
     bool join;
+    bool wide;                       // trees: k_paged_tree's form
     size_t fo, fml, mo, mml, own, pre, wo, wml, total;
 };
 // of a batch with tokens and sequences; window 0 gives the most workspace
@@ -39,6 +40,13 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
     // kernel's too, where one takes about twice its time in the other.
     few.rows = grp > 16 || (b.q_off && b.n_tok >= 64 * (int64_t)b.n_seq) ? 0 : (b.q_off ? rows : grp) <= 8 ? 8 : 16;
     if (b.n_prefix && few.rows == 8 && rows > 8 && rows <= 16) few.rows = 16;
+    // Trees: all in one kernel, this one where no sequence can have more than its rows,
+    // else k_paged_tree.
+    y.wide = tree && grp > pt_rows(p.hd, false);
+    if (tree) {
+        const int64_t bound = b.q_off ? rows : grp;
+        few.rows = grp > 16 || bound > 16 ? 0 : bound <= 8 && !(b.n_prefix && rows > 8) ? 8 : 16;
+    }
     few.toks = few.rows / grp;
     const bool few_pre = b.n_prefix && few.rows && rows <= few.rows;
     const bool many_own = b.q_off ? b.n_tok > few.toks : !few.rows;
@@ -75,21 +83,21 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
     many.rows = 0;
     many.pre_tiles = many.lead = 0;
     if (many_own || many_pre) {
-        const int most = paged_most_group(p.hd) / grp, toks = b.q_off || many_pre ? b.n_tok : 1;
-        many.toks = pa_ceil_div(toks, pa_ceil_div(toks, most));
+        const int most = (tree ? pt_rows(p.hd, y.wide) : paged_most_group(p.hd)) / grp, toks = b.q_off || many_pre ? b.n_tok : 1;
+        many.toks = tree ? std::min(toks, most) : pa_ceil_div(toks, pa_ceil_div(toks, most));
         many.toks_inv = many.toks == 1 ? 0 : (uint32_t)(0x100000000ull / many.toks + 1);
         many.rows = many.toks * grp;
         many.pre_tiles = many_pre ? pa_ceil_div(b.n_tok, many.toks) : 0;
         const int64_t own = !many_own ? 0 : b.q_off ? pa_ceil_div(b.n_tok, many.toks) + std::min(b.n_seq, b.n_tok / (few.toks + 1)) : b.n_seq;
         const int64_t mspan = span(tree ? b.n_tok : many.toks);
-        for (many.shift = 5;; many.shift++) {
+        for (many.shift = tree ? pt_shift(p.hd) : 5;; many.shift++) {
             many.unit = 1 << many.shift;
             many.pre_steps = many_pre ? pa_ceil_div(b.n_prefix, many.unit) : 0;
             steps = (own * std::max(1, pa_ceil_div(mspan, many.unit)) + (int64_t)many.pre_tiles * many.pre_steps) * p.n_kv;
             if (steps < (1 << 27)) break;
         }
-        many.wgs = (int)std::min<int64_t>(p.hd >= 128 ? 256 : 512, steps);
-        many.lead = steps > many.wgs ? 5 : 0;
+        many.wgs = (int)std::min<int64_t>(p.hd >= 128 || tree ? 256 : 512, steps);
+        many.lead = steps > many.wgs ? tree ? 3 : 5 : 0;
         y.join |= mspan > many.unit;
     }
     const size_t all = y.join ? (size_t)b.n_tok * p.n_kv * grp : 0, whole = b.n_prefix ? all : 0;
