@@ -615,7 +615,7 @@ __host__ __device__ constexpr int pa_few_per_cu(int type, int hd, bool st) {
 // k_paged_tree (paged_tree.h): rows of a tile at most, and the log2 of the positions
 // that a workgroup takes at a time.  wide: for more query heads a KV head than its rows
 __host__ __device__ constexpr int pt_rows(int hd, bool wide) { return (hd == 512 ? 32 : hd == 256 ? 64 : 128) << wide; }
-__host__ __device__ constexpr int pt_shift(int hd) { return hd <= 128 ? 7 : hd == 256 ? 6 : 5; }
+__host__ __device__ constexpr int pt_shift(int type, int hd) { return hd <= 128 ? 7 : hd == 256 && type != F16 ? 6 : 5; }
 
 // launches of one cache type; the few-row variants hold 8 or 16 rows
 hipError_t pa_few_f16(const PagedAttn &a, const PagedPlan &pl, hipStream_t s);

@@ -90,7 +90,7 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
         many.pre_tiles = many_pre ? pa_ceil_div(b.n_tok, many.toks) : 0;
         const int64_t own = !many_own ? 0 : b.q_off ? pa_ceil_div(b.n_tok, many.toks) + std::min(b.n_seq, b.n_tok / (few.toks + 1)) : b.n_seq;
         const int64_t mspan = span(tree ? b.n_tok : many.toks);
-        for (many.shift = tree ? pt_shift(p.hd) : 5;; many.shift++) {
+        for (many.shift = tree ? pt_shift(p.type, p.hd) : 5;; many.shift++) {
             many.unit = 1 << many.shift;
             many.pre_steps = many_pre ? pa_ceil_div(b.n_prefix, many.unit) : 0;
             steps = (own * std::max(1, pa_ceil_div(mspan, many.unit)) + (int64_t)many.pre_tiles * many.pre_steps) * p.n_kv;

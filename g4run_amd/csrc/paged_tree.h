@@ -14,6 +14,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_few.h"
 #include "paged_many.h"
@@ -47,8 +48,8 @@ struct PtShape {
     static constexpr int HE = HD <= 128 ? HD : WIDE ? 256 : 128, ES = HD / HE, ZW = 8 / ES;
     static constexpr int RB = paged_row_bytes(KVT, HD), CPR = RB / 16, WIN = RB < 256 ? 256 / RB : 1, FM = (CPR < 16 ? CPR : 16) - 1;
     static constexpr int SCB = KVT == F16 ? 0 : HD / 16;                                 // scale bytes of a row
-    static constexpr int TILE = 64 * RB + 64 * SCB, TILES = HD <= 128 ? 4 : HD == 256 ? 2 : 1, SLOT = TILES * TILE;
-    static constexpr int DEPTH = std::max(2, std::min(6, 132 * 1024 / SLOT));            // slots
+    static constexpr int TILE = 64 * RB + 64 * SCB, TILES = HD <= 128 ? 4 : HD == 256 && KVT != F16 ? 2 : 1, SLOT = TILES * TILE;
+    static constexpr int DEPTH = std::max(2, std::min(6, (ES > 1 ? 112 : 132) * 1024 / SLOT));        // slots
     static constexpr int LOADS = 2 * (RB / 32) * TILES, PER = LOADS >= 8 ? LOADS / 8 : 1;            // of 1 KB, K and V; a wave's
     static constexpr int SLOADS = KVT == F16 ? 0 : TILES * (HD == 512 ? 2 : 1);          // of scales, the last waves'
     static constexpr int TRB = 8 * PM_TR * 4, BP = HE + 4;
@@ -118,8 +119,8 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
     constexpr int PG = S::TILES, HE = S::HE, ES = S::ES, ZW = S::ZW, NS = HE / 32, NM = HE / 16, RB = S::RB, BP = S::BP, TURN = 32 / PG;   // TURN: iterations of 64 units
     constexpr int AHEAD = HE == 64 ? 2 : 4;
     __shared__ __align__(16) uint8_t lds[S::LDS];            // the ring; before it, where it is filled last, queries on their way; after it sums
-    __shared__ __align__(16) float xs[ES > 1 ? 8 : 1][ES > 1 ? 64 : 1][8];   // partial scores of the waves of one tile
-    __shared__ __align__(16) float ex[KVT == F16 ? 1 : 8][32];               // of a wave: pa_exponent of its positions' largest V scales
+    __shared__ __align__(16) float xs[ES > 1 ? 8 : 1][ES > 1 ? PG : 1][ES > 1 ? 64 : 1][8];      // partial scores of the waves of one tile
+    __shared__ __align__(16) float ex[KVT == F16 ? 1 : 8][ES > 1 ? PG : 1][32];            // of a wave and tile: pa_exponent of its positions' largest V scales
     __shared__ int ids[8][64];                               // of a wave: the next page ids
     __shared__ float2 wml[8][16];
     __shared__ int nothing[16 * ZW];                         // whether a row attends nothing
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
         const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = min(sq.nq * G, (x.tile + 1) * R);     // the tile's rows end at `rows`
         // row groups: a power of two that the tile's rows need; position groups: the rest
         const int need = (rows - x.tile * R + 15) >> 4, rgl = need <= 1 ? 0 : 32 - __builtin_clz(need - 1), rw = z & ((1 << rgl) - 1), pg = z >> rgl;
-        const int groups = min(ZW >> rgl, PG), turns = PG / groups;          // position groups (other waves have none); tiles of a slot for each
+        const int groups = min(ZW >> rgl, PG), turns = PG / groups;          // position groups (other waves have none); tiles of a slot for each: of heads of 256 and 512 one or two
         bool bad = sq.bad;
         if (bad && tid == 0) paged_flag(p, PAGED_BAD_BATCH);
         const int last = (x.seglen - 1) >> 4, iters = end > start ? (end - start + 32 * PG - 1) / (32 * PG) : 0;
@@ -292,116 +293,128 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
                 load(far);
             }
             if (!busy) {                                     // waves that share scores all meet
-                if constexpr (ES > 1)
-                    for (int turn = 0; turn < turns << (turns > 1); turn++) lds_barrier();
+                if constexpr (ES > 1) lds_barrier();
                 continue;
             }
-            for (int turn = 0; turn < turns; turn++) {
-                const int q = turn * groups + (pg & (groups - 1)), base = start + 32 * (PG * it + q);
-                if (base >= end && ES == 1) break;
-                const uint8_t *const d = slot + q * S::TILE;
-                const bool edge = base + 31 > full || base < lo1 || base + 32 > end;
-                const uint32_t vis = edge && base + 31 >= hi0 ? row_bits(base) : 0u;           // the row's bits of these positions
-                auto seen = [&](int pos) { return ((pos >= rlo && pos <= full) || (vis >> (pos - base) & 1)) && pos < end; };
-                // scores of row c at positions base + pm_pos(g, j)
-                pa_v4f sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}, s2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-                constexpr int DW = HE / 64;                      // dwords of a row's scales
-                PaTile<HE, KVT> kv;
-                uint32_t dv[8][DW];
-                if constexpr (KVT == F16) {
-                    const uint8_t *const kr = d + c * RB + HE * 2 * ew;
-                    const uint32_t k0 = 16 * (g ^ kc);
-                    // high and low halves apart, so that no instruction waits for the one before it
-                    pm_pipeline<2 * NS, AHEAD>([&](int i) { return *(const pa_v8h *)(kr + (i & 1) * 16 * RB + (k0 ^ (64 * (i >> 1)))); }, [&](int i, pa_v8h ko) {
-                        sc[i & 1] = pa_mma(ko, q0[i >> 1], sc[i & 1]);
-                        s2[i & 1] = pa_mma(ko, q1[i >> 1], s2[i & 1]);
-                    });
-                    sc[0] += s2[0];
-                    sc[1] += s2[1];
-                } else {
-                    // the lane's runs, as k_paged_few's
-                    constexpr int KW = PaTile<HE, KVT>::KW, VW = PaTile<HE, KVT>::VW;
-                    uint32_t dk[8][DW];
+            // NT tiles at once, q, q + groups: one exchange of scores and one maximum for both
+            // (heads of 64 and 128 exchange none, and two at once spill: 113 us for 69)
+            auto step = [&](auto nt, int q) {
+                constexpr int NT = decltype(nt)::value, DW = HE / 64;        // DW: dwords of a row's scales
+                const int base0 = start + 32 * (PG * it + q);
+                const uint8_t *const d0 = slot + q * S::TILE;
+                auto base_of = [&](int t) { return base0 + 32 * groups * t; };
+                auto tile_of = [&](int t) { return d0 + t * groups * S::TILE; };
+                const bool edge = base_of(NT - 1) + 31 > full || base0 < lo1 || base_of(NT - 1) + 32 > end;
+                uint32_t vis[NT];                            // the row's bits of these positions
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint8_t *const kr = d + (16 * h + c) * RB;
-                        const uint32_t byte = 4 * KW * ((HD / HE) * g + ew);
-                        if constexpr (KW >= 4) {
+                for (int t = 0; t < NT; t++) vis[t] = edge && base_of(t) + 31 >= hi0 ? row_bits(base_of(t)) : 0u;
+                auto seen = [&](int t, int k) {              // position k of tile t
+                    const int pos = base_of(t) + k;
+                    return ((pos >= rlo && pos <= full) || (vis[t] >> k & 1)) && pos < end;
+                };
+                // scores of row c at positions pm_pos(g, j)
+                pa_v4f sc[NT][2];
 #pragma unroll
-                            for (int k = 0; k < KW / 4; k++) pa_load<4>(kv.k[h] + 4 * k, kr + 16 * ((byte / 16 + k) ^ kc));
-                        } else pa_load<KW>(kv.k[h], kr + 16 * (byte / 16 ^ kc) + byte % 16);
-                    }
-                    const uint8_t *const sp = d + 64 * RB + HE / 16 * ew;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) pa_load<DW>(dk[j], sp + pm_pos(g, j) * S::SCB);
-                    // the largest V scale of each position, as an exponent: a position a lane
-                    if (lane < 32) {
-                        uint32_t w[DW], top = 0;
-                        pa_load<DW>(w, sp + (32 + lane) * S::SCB);
-#pragma unroll
-                        for (int k = 0; k < DW; k++) top = pa_pkmax(top, w[k] & 0x7fff7fffu);
-                        ex[wave][lane] = pa_exponent(max(top << 16, top), 1);
-                    }
-                    asm volatile("" ::: "memory");               // a wave's LDS accesses complete in order
-#pragma unroll
-                    for (int s = 0; s < NS; s++)
+                for (int t = 0; t < NT; t++) {
+                    const uint8_t *const d = tile_of(t);
+                    sc[t][0] = sc[t][1] = pa_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (KVT == F16) {
+                        pa_v4f s2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                        const uint8_t *const kr = d + c * RB + HE * 2 * ew;
+                        const uint32_t k0 = 16 * (g ^ kc);
+                        // high and low halves apart, so that no instruction waits for the one before it
+                        pm_pipeline<2 * NS, AHEAD>([&](int i) { return *(const pa_v8h *)(kr + (i & 1) * 16 * RB + (k0 ^ (64 * (i >> 1)))); }, [&](int i, pa_v8h ko) {
+                            sc[t][i & 1] = pa_mma(ko, q0[i >> 1], sc[t][i & 1]);
+                            s2[i & 1] = pa_mma(ko, q1[i >> 1], s2[i & 1]);
+                        });
+                        sc[t][0] += s2[0];
+                        sc[t][1] += s2[1];
+                    } else {
+                        // the lane's runs, as k_paged_few's
+                        constexpr int KW = PaTile<HE, KVT>::KW;
+                        PaTile<HE, KVT> kv;
+                        uint32_t dk[8][DW];
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const pa_v8h ko = pa_key<HE, KVT>(kv, h, s);
-                            const pa_v4f y = pa_mma(ko, q1[s], pa_mma(ko, q0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f}));
+                            const uint8_t *const kr = d + (16 * h + c) * RB;
+                            const uint32_t byte = 4 * KW * ((HD / HE) * g + ew);
+                            if constexpr (KW >= 4) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) sc[h][i] = __builtin_fmaf(pa_scale(dk[4 * h + i], s), y[i], sc[h][i]);
+                                for (int k = 0; k < KW / 4; k++) pa_load<4>(kv.k[h] + 4 * k, kr + 16 * ((byte / 16 + k) ^ kc));
+                            } else pa_load<KW>(kv.k[h], kr + 16 * (byte / 16 ^ kc) + byte % 16);
                         }
+                        const uint8_t *const sp = d + 64 * RB + HE / 16 * ew;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int pos = pm_pos(g, j);
-                        const uint8_t *const row = d + (32 + pos) * RB;
-                        if constexpr (KVT == Q4_0 && HE == 64) kv.v[j][0] = *(const uint16_t *)(row + 2 * c);
-                        else pa_load<VW>(kv.v[j], row + 4 * VW * ((HD / HE) * c + ew));
-                        pa_load<DW>(dv[j], sp + (32 + pos) * S::SCB);
+                        for (int j = 0; j < 8; j++) pa_load<DW>(dk[j], sp + pm_pos(g, j) * S::SCB);
+                        // the largest V scale of each position, as an exponent: a position a lane
+                        if (lane < 32) {
+                            uint32_t w[DW], top = 0;
+                            pa_load<DW>(w, sp + (32 + lane) * S::SCB);
+#pragma unroll
+                            for (int k = 0; k < DW; k++) top = pa_pkmax(top, w[k] & 0x7fff7fffu);
+                            ex[wave][t][lane] = pa_exponent(max(top << 16, top), 1);
+                        }
+                        asm volatile("" ::: "memory");       // a wave's LDS accesses complete in order
+#pragma unroll
+                        for (int s = 0; s < NS; s++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const pa_v8h ko = pa_key<HE, KVT>(kv, h, s);
+                                const pa_v4f y = pa_mma(ko, q1[s], pa_mma(ko, q0[s], pa_v4f{0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+                                for (int i = 0; i < 4; i++) sc[t][h][i] = __builtin_fmaf(pa_scale(dk[4 * h + i], s), y[i], sc[t][h][i]);
+                            }
                     }
                 }
                 if constexpr (ES > 1) {
-                    *(pa_v4f *)xs[wave][lane] = sc[0];
-                    *(pa_v4f *)(xs[wave][lane] + 4) = sc[1];
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        *(pa_v4f *)xs[wave][t][lane] = sc[t][0];
+                        *(pa_v4f *)(xs[wave][t][lane] + 4) = sc[t][1];
+                    }
                     lds_barrier();
-                    const int w0 = wave & ~(ES - 1);             // in one order for all of them
-                    sc[0] = *(const pa_v4f *)xs[w0][lane];
-                    sc[1] = *(const pa_v4f *)(xs[w0][lane] + 4);
+                    const int w0 = wave & ~(ES - 1);         // in one order for all of them
 #pragma unroll
-                    for (int k = 1; k < ES; k++) {
-                        sc[0] += *(const pa_v4f *)xs[w0 + k][lane];
-                        sc[1] += *(const pa_v4f *)(xs[w0 + k][lane] + 4);
-                    }
-                    if (turns > 1) lds_barrier();                // read before the next tile's are written
-                }
-                float w[8];
+                    for (int t = 0; t < NT; t++) {
+                        sc[t][0] = *(const pa_v4f *)xs[w0][t][lane];
+                        sc[t][1] = *(const pa_v4f *)(xs[w0][t][lane] + 4);
 #pragma unroll
-                for (int j = 0; j < 8; j++) w[j] = sc[j >> 2][j & 3] * qs;
-                if (a.cap > 0.0f) {
-                    pt_tanh(w);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) w[j] *= capl;
-                }
-                uint32_t live = 0xffu;                           // bit j: the row attends position j
-                if (edge) {
-                    live = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const bool sees = seen(base + pm_pos(g, j));
-                        live |= (uint32_t)sees << j;
-                        w[j] = sees ? w[j] : -__builtin_inff();
+                        for (int k = 1; k < ES; k++) {
+                            sc[t][0] += *(const pa_v4f *)xs[w0 + k][t][lane];
+                            sc[t][1] += *(const pa_v4f *)(xs[w0 + k][t][lane] + 4);
+                        }
                     }
                 }
-                float mt = -__builtin_inff();
-                if constexpr (KVT == F16) {
+                float w[NT][8], mt = -__builtin_inff();
+                uint32_t live[NT];                           // bit j: the row attends position j
 #pragma unroll
-                    for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j]);
-                } else {
-                    // + the exponent of the position's largest value scale
-                    const pa_v4f e[2] = {*(const pa_v4f *)&ex[wave][4 * g], *(const pa_v4f *)&ex[wave][16 + 4 * g]};
+                for (int t = 0; t < NT; t++) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[j] + e[j >> 2][j & 3]);
+                    for (int j = 0; j < 8; j++) w[t][j] = sc[t][j >> 2][j & 3] * qs;
+                    if (a.cap > 0.0f) {
+                        pt_tanh(w[t]);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) w[t][j] *= capl;
+                    }
+                    live[t] = 0xffu;
+                    if (edge) {
+                        live[t] = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const bool sees = seen(t, pm_pos(g, j));
+                            live[t] |= (uint32_t)sees << j;
+                            w[t][j] = sees ? w[t][j] : -__builtin_inff();
+                        }
+                    }
+                    if constexpr (KVT == F16) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[t][j]);
+                    } else {
+                        // + the exponent of the position's largest value scale
+                        const pa_v4f e[2] = {*(const pa_v4f *)&ex[wave][t][4 * g], *(const pa_v4f *)&ex[wave][t][16 + 4 * g]};
+#pragma unroll
+                        for (int j = 0; j < 8; j++) mt = fmaxf(mt, w[t][j] + e[j >> 2][j & 3]);
+                    }
                 }
                 mt = fmaxf(mt, partner<16>(mt));
                 mt = fmaxf(mt, partner<32>(mt));
@@ -414,99 +427,125 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
                 }
                 const float mr = m == -__builtin_inff() ? 0.0f : m - pa_shift_of<KVT>();
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    w[j] = __builtin_amdgcn_exp2f(w[j] - mr);
-                    l += w[j];
-                }
-                if constexpr (KVT == F16) {
-                    uint32_t hi[4], lo[4];
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) pa_split(w[2 * k], w[2 * k + 1], hi[k], lo[k]);
-                    const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
-                    const uint8_t *const vt = d + (32 + vr) * RB + HE * 2 * ew + 8 * (c & 1);
-                    const uint32_t v0 = 16 * ((c & 3) >> 1 ^ S::value(vr));
-                    // 16 lanes give 4 positions of 16 elements and get 4 positions of their own
-                    auto turned = [&](int e) { return pm_turned((const _Float16 *)(vt + (v0 ^ (32 * e))), (const _Float16 *)(vt + 16 * RB + (v0 ^ (32 * e)))); };
-                    if (edge) {
-                        // Positions that no row of the tile attends may hold anything: zeros for
-                        // them.  Non-finite values that some rows attend and some do not are taken
-                        // out and added to those that do (rare, one by one).
-                        uint32_t mask4[4], nf = 0;
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const int pos = base + pm_pos(g, 2 * k);
-                            mask4[k] = (pos >= lo0 && pos < end ? 0xffffu : 0u) | (pos + 1 >= lo0 && pos + 1 < end ? 0xffff0000u : 0u);
-                        }
-#pragma unroll
-                        for (int e = 0; e < NM; e++) {
-                            pa_v4u va = __builtin_bit_cast(pa_v4u, turned(e));
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const uint32_t v = va[k] & mask4[k];
-                                nf |= (v & 0x7c007c00u) + 0x04000400u;                       // bit 15 or 31 where an exponent is all ones
-                                va[k] = pa_finite(v);
-                            }
-                            const pa_v8h vo = __builtin_bit_cast(pa_v8h, va);
-                            o[e] = pa_mma(vo, b0, o[e]);
-                            o[e] = pa_mma(vo, b1, o[e]);
-                        }
-                        if (__any(nf & 0x80008000u)) {
-                            for (int k = 0; k < 32; k++) {
-                                const int pos = base + k;
-                                if (pos < lo0 || pos >= end) continue;
-                                const uint8_t *const row = d + (32 + k) * RB + HE * 2 * ew;
-                                const uint32_t f = S::value(k);
-                                float wx = 0.0f;
-#pragma unroll
-                                for (int j = 0; j < 8; j++) {
-                                    const float v = __shfl(w[j], 16 * ((k & 15) >> 2) + c, 64);
-                                    if (j == 4 * (k >> 4) + (k & 3)) wx = v;
-                                }
-                                const bool sees = seen(pos);
-#pragma unroll
-                                for (int e = 0; e < NM; e++) {
-                                    const uint2 hv = *(const uint2 *)(row + 16 * ((2 * e + (g >> 1)) ^ f) + 8 * (g & 1));
-#pragma unroll
-                                    for (int i = 0; i < 4; i++) {
-                                        const uint32_t v = (i < 2 ? hv.x : hv.y) >> (16 * (i & 1)) & 0xffffu;
-                                        if (sees && (v & 0x7c00) == 0x7c00) o[e][i] += wx * h2f((uint16_t)v);
-                                    }
-                                    __builtin_amdgcn_sched_barrier(0);
-                                }
-                            }
-                        }
-                    } else {
-                        pa_v8h before;                           // low halves one operand later
-                        pm_pipeline<NM, AHEAD>(turned, [&](int e, pa_v8h va) {
-                            o[e] = pa_mma(va, b0, o[e]);
-                            if (e) o[e - 1] = pa_mma(before, b1, o[e - 1]);
-                            before = va;
-                        });
-                        o[NM - 1] = pa_mma(before, b1, o[NM - 1]);
-                    }
-                } else {
-                    // a scale of a position that the row does not attend may be anything
-                    if (edge) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-#pragma unroll
-                            for (int k = 0; k < DW; k++) dv[j][k] = live >> j & 1 ? dv[j][k] : 0u;
+                    for (int j = 0; j < 8; j++) {
+                        w[t][j] = __builtin_amdgcn_exp2f(w[t][j] - mr);
+                        l += w[t][j];
                     }
 #pragma unroll
-                    for (int s = 0; s < NS; s++) {               // blocks of 32 elements: value tiles 2 s, 2 s + 1
+                for (int t = 0; t < NT; t++) {
+                    const uint8_t *const d = tile_of(t);
+                    if constexpr (KVT == F16) {
                         uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            pa_split(__builtin_fmaf(pa_scale(dv[2 * k], s), w[2 * k], 0.0f), __builtin_fmaf(pa_scale(dv[2 * k + 1], s), w[2 * k + 1], 0.0f), hi[k], lo[k]);
+                        for (int k = 0; k < 4; k++) pa_split(w[t][2 * k], w[t][2 * k + 1], hi[k], lo[k]);
                         const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
-                        const pa_v8h x0 = pa_value<HE, KVT>(kv, 2 * s), x1 = pa_value<HE, KVT>(kv, 2 * s + 1);
-                        o[2 * s] = pa_mma(x0, b0, o[2 * s]);
-                        o[2 * s + 1] = pa_mma(x1, b0, o[2 * s + 1]);
-                        o[2 * s] = pa_mma(x0, b1, o[2 * s]);
-                        o[2 * s + 1] = pa_mma(x1, b1, o[2 * s + 1]);
+                        const uint8_t *const vt = d + (32 + vr) * RB + HE * 2 * ew + 8 * (c & 1);
+                        const uint32_t v0 = 16 * ((c & 3) >> 1 ^ S::value(vr));
+                        // 16 lanes give 4 positions of 16 elements and get 4 positions of their own
+                        auto turned = [&](int e) { return pm_turned((const _Float16 *)(vt + (v0 ^ (32 * e))), (const _Float16 *)(vt + 16 * RB + (v0 ^ (32 * e)))); };
+                        if (edge) {
+                            // Positions that no row of the tile attends may hold anything: zeros
+                            // for them.  Non-finite values that some rows attend and some do not
+                            // are taken out and added to those that do (rare, one by one).
+                            uint32_t mask4[4], nf = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const int pos = base_of(t) + pm_pos(g, 2 * k);
+                                mask4[k] = (pos >= lo0 && pos < end ? 0xffffu : 0u) | (pos + 1 >= lo0 && pos + 1 < end ? 0xffff0000u : 0u);
+                            }
+#pragma unroll
+                            for (int e = 0; e < NM; e++) {
+                                pa_v4u va = __builtin_bit_cast(pa_v4u, turned(e));
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const uint32_t v = va[k] & mask4[k];
+                                    nf |= (v & 0x7c007c00u) + 0x04000400u;               // bit 15 or 31 where an exponent is all ones
+                                    va[k] = pa_finite(v);
+                                }
+                                const pa_v8h vo = __builtin_bit_cast(pa_v8h, va);
+                                o[e] = pa_mma(vo, b0, o[e]);
+                                o[e] = pa_mma(vo, b1, o[e]);
+                            }
+                            if (__any(nf & 0x80008000u)) {
+                                for (int k = 0; k < 32; k++) {
+                                    const int pos = base_of(t) + k;
+                                    if (pos < lo0 || pos >= end) continue;
+                                    const uint8_t *const row = d + (32 + k) * RB + HE * 2 * ew;
+                                    const uint32_t f = S::value(k);
+                                    float wx = 0.0f;
+#pragma unroll
+                                    for (int j = 0; j < 8; j++) {
+                                        const float v = __shfl(w[t][j], 16 * ((k & 15) >> 2) + c, 64);
+                                        if (j == 4 * (k >> 4) + (k & 3)) wx = v;
+                                    }
+                                    const bool sees = seen(t, k);
+#pragma unroll
+                                    for (int e = 0; e < NM; e++) {
+                                        const uint2 hv = *(const uint2 *)(row + 16 * ((2 * e + (g >> 1)) ^ f) + 8 * (g & 1));
+#pragma unroll
+                                        for (int i = 0; i < 4; i++) {
+                                            const uint32_t v = (i < 2 ? hv.x : hv.y) >> (16 * (i & 1)) & 0xffffu;
+                                            if (sees && (v & 0x7c00) == 0x7c00) o[e][i] += wx * h2f((uint16_t)v);
+                                        }
+                                        __builtin_amdgcn_sched_barrier(0);
+                                    }
+                                }
+                            }
+                        } else {
+                            pa_v8h before;                   // low halves one operand later
+                            pm_pipeline<NM, AHEAD>(turned, [&](int e, pa_v8h va) {
+                                o[e] = pa_mma(va, b0, o[e]);
+                                if (e) o[e - 1] = pa_mma(before, b1, o[e - 1]);
+                                before = va;
+                            });
+                            o[NM - 1] = pa_mma(before, b1, o[NM - 1]);
+                        }
+                    } else {
+                        constexpr int VW = PaTile<HE, KVT>::VW;
+                        PaTile<HE, KVT> kv;
+                        uint32_t dv[8][DW];
+                        const uint8_t *const sp = d + 64 * RB + HE / 16 * ew;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const int pos = pm_pos(g, j);
+                            const uint8_t *const row = d + (32 + pos) * RB;
+                            if constexpr (KVT == Q4_0 && HE == 64) kv.v[j][0] = *(const uint16_t *)(row + 2 * c);
+                            else pa_load<VW>(kv.v[j], row + 4 * VW * ((HD / HE) * c + ew));
+                            pa_load<DW>(dv[j], sp + (32 + pos) * S::SCB);
+                        }
+                        // a scale of a position that the row does not attend may be anything
+                        if (edge) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+#pragma unroll
+                                for (int k = 0; k < DW; k++) dv[j][k] = live[t] >> j & 1 ? dv[j][k] : 0u;
+                        }
+#pragma unroll
+                        for (int s = 0; s < NS; s++) {       // blocks of 32 elements: value tiles 2 s, 2 s + 1
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                pa_split(__builtin_fmaf(pa_scale(dv[2 * k], s), w[t][2 * k], 0.0f), __builtin_fmaf(pa_scale(dv[2 * k + 1], s), w[t][2 * k + 1], 0.0f), hi[k], lo[k]);
+                            const pa_v8h b0 = pa_op(hi[0], hi[1], hi[2], hi[3]), b1 = pa_op(lo[0], lo[1], lo[2], lo[3]);
+                            const pa_v8h x0 = pa_value<HE, KVT>(kv, 2 * s), x1 = pa_value<HE, KVT>(kv, 2 * s + 1);
+                            o[2 * s] = pa_mma(x0, b0, o[2 * s]);
+                            o[2 * s + 1] = pa_mma(x1, b0, o[2 * s + 1]);
+                            o[2 * s] = pa_mma(x0, b1, o[2 * s]);
+                            o[2 * s + 1] = pa_mma(x1, b1, o[2 * s + 1]);
+                        }
                     }
                 }
+            };
+            if constexpr (ES > 1 && PG > 1) {
+                if (turns > 1) {
+                    step(std::integral_constant<int, 2>(), pg & (groups - 1));
+                    continue;
+                }
             }
+            for (int q = pg & (groups - 1); q < PG; q += groups)
+                if (ES > 1 || start + 32 * (PG * it + q) < end) step(std::integral_constant<int, 1>(), q);
         }
         bad &= ok;
         if (__any(bad)) {
