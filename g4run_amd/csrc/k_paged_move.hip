@@ -13,6 +13,8 @@ namespace g4 {
 
 namespace {
 
+typedef uint32_t pv_v4 __attribute__((ext_vector_type(4)));      // (arrays of HIP's uint4 end up in LDS or scratch)
+
 // The rows of one sequence and one cache's keys or values: a thread carries the same
 // 16 bytes (of quantized rows' scales: 4) of every kept row, so that the moves of a
 // thread need only be in their own order.  Entries ascend and entry k is at least k:
@@ -62,30 +64,41 @@ __global__ __launch_bounds__(256) void k_paged_keep(PagedKeep a, PagedPools pool
             const int h = x / cols, c = x - h * cols, row = h * p.page;
             const bool sc = c >= wide;
             const size_t at = sc ? p.sc_off + (size_t)row * (p.hd / 16) + (c - wide) * 4 : (size_t)row * rb + c * 16;
-            const int step = sc ? p.hd / 16 : rb;
+            auto place = [&](int l, size_t page, int r) {
+                const size_t b = (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)page, l) | (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(page >> 32), l) << 32;
+                return b + (size_t)__builtin_amdgcn_readlane(r, l) * rb;
+            };
+            auto scales = [&](int l, size_t page, int r) {
+                const size_t b = (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)page, l) | (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(page >> 32), l) << 32;
+                return b + (size_t)__builtin_amdgcn_readlane(r, l) * (p.hd / 16);
+            };
+            // eight rows read, then written: the last one again where fewer are left
             for (uint64_t left = todo; left;) {
                 constexpr int N = 8;
-                uint4 v[N];
-                uint8_t *to[N];
-                int m = 0;
+                size_t f[N], t[N], fs[N], ts[N];
+                int l = 0;
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    if (!left) break;
-                    const int l = __ffsll((unsigned long long)left) - 1;
+                    if (left) l = __ffsll((unsigned long long)left) - 1;
                     left &= left - 1;
-                    const size_t f = (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)src, l) | (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(src >> 32), l) << 32;
-                    const size_t t = (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)dst, l) | (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(dst >> 32), l) << 32;
-                    const uint8_t *d = pool + f + at + (size_t)__builtin_amdgcn_readlane(src_row, l) * step;
-                    to[i] = pool + t + at + (size_t)__builtin_amdgcn_readlane(dst_row, l) * step;
-                    if (live && sc) v[i].x = *(const uint32_t *)d;
-                    else if (live) v[i] = *(const uint4 *)d;
-                    m = i + 1;
+                    f[i] = place(l, src, src_row);
+                    t[i] = place(l, dst, dst_row);
+                    fs[i] = scales(l, src, src_row);
+                    ts[i] = scales(l, dst, dst_row);
                 }
+                if (!live) continue;
+                if (sc) {
+                    uint32_t v[N];
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    if (i >= m) break;
-                    if (live && sc) *(uint32_t *)to[i] = v[i].x;
-                    else if (live) *(uint4 *)to[i] = v[i];
+                    for (int i = 0; i < N; i++) v[i] = *(const uint32_t *)(pool + at + fs[i]);
+#pragma unroll
+                    for (int i = 0; i < N; i++) *(uint32_t *)(pool + at + ts[i]) = v[i];
+                } else {
+                    pv_v4 v[N];
+#pragma unroll
+                    for (int i = 0; i < N; i++) v[i] = *(const pv_v4 *)(pool + at + f[i]);
+#pragma unroll
+                    for (int i = 0; i < N; i++) *(pv_v4 *)(pool + at + t[i]) = v[i];
                 }
             }
         }
@@ -138,18 +151,16 @@ __global__ __launch_bounds__(256) void k_paged_fork(PagedFork a, PagedPools pool
     uint8_t *const pool = value ? pools.v[blockIdx.y] : pools.k[blockIdx.y];
     const int rb = paged_row_bytes(p.type, p.hd);
     const size_t src = (size_t)from * p.page_bytes, dst = (size_t)fresh * p.page_bytes, row = (size_t)h * p.page;
-    const int n = part * rb;                                 // up to 4096 * 1024
-    {
-        const uint4 *const f = (const uint4 *)(pool + src + row * rb);
-        uint4 *const t = (uint4 *)(pool + dst + row * rb);
-        uint4 v[4];
-        const int at = piece * (PF_BYTES / 16) + threadIdx.x;
+    const int n = part * rb / 16, at = piece * (PF_BYTES / 16) + threadIdx.x;            // up to 4096 * 64
+    if (piece * (PF_BYTES / 16) < n) {
+        const pv_v4 *const f = (const pv_v4 *)(pool + src + row * rb);
+        pv_v4 *const t = (pv_v4 *)(pool + dst + row * rb);
+        pv_v4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = f[min(at + 256 * k, n - 1)];
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (at + 256 * k < n / 16) v[k] = f[at + 256 * k];
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (at + 256 * k < n / 16) t[at + 256 * k] = v[k];
+            if (at + 256 * k < n) t[at + 256 * k] = v[k];
     }
     if (p.type != F16 && piece == 0) {
         const size_t at = p.sc_off + row * (p.hd / 16);
