@@ -16,9 +16,9 @@ struct BeamSelect {
     const int *ended;                            // or null
     float *score_out;
     int *row_out, *token_out;
-    int chunks;                                  // of a row
-    float2 *ms;                                  // [row][chunk] maximum, sum of exp(x - maximum)
-    uint64_t *top;                               // [row][chunk][n_out] candidates, descending; 0: none
+    int lists, span;                             // workgroups a row, and the tokens of each
+    float2 *ms;                                  // [row][list] maximum, sum of exp(x - maximum)
+    uint64_t *top;                               // [row][list][n_out] candidates, descending; 0: none
 };
 size_t beam_workspace(int n_group, int n_beam, int n_vocab, int n_out);
 hipError_t launch_beam_select(BeamSelect a, uint8_t *ws, hipStream_t s);

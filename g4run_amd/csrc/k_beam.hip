@@ -4,15 +4,15 @@
 //
 // Within a row the order is that of its logits, so one pass over a row finds both
 // what its normaliser is made of and its n_out best tokens; scores are only computed
-// for those.  k_beam_rows reads the logits once, a workgroup a chunk of a row, and
-// keeps per chunk the maximum, the sum and the n_out best; k_beam_join takes a row's
-// from its chunks', then a group's from its rows'.  Bound by the logits' bytes where
-// they are many, by the two launches and the selection's chains where they are few.
+// for those.  k_beam_rows reads the logits once, a workgroup a part of a row, and
+// leaves the part's maximum, sum and n_out best; k_beam_join takes a row's from its
+// parts', then a group's from its rows'.  Bound by the logits' bytes where they are
+// many, by the two launches and the selection's chains where they are few.
 //
 // Exactness: candidates are compared as (logit, lowest token) within a row and as
-// (score in 64 bits, lowest beam) between rows.  Sums of exponentials are fp32
-// within a thread's elements, the threads' fp32 sums added in a fixed order; chunks
-// and scores in 64 bits.
+// (score in 64 bits, lowest beam) between rows.  Sums of exponentials are fp32, under
+// each thread's running maximum, added up over the threads in a fixed order; over the
+// parts, and scores, in 64 bits.
 #include <algorithm>
 
 #include "beam.h"
@@ -40,130 +40,205 @@ __device__ __forceinline__ double bs_value(uint64_t o) {
 __device__ __forceinline__ uint64_t bs_key(float x, int v) {
     return x > -__builtin_inff() ? (uint64_t)bs_order(x) << 32 | (uint32_t)~v : 0;
 }
-__device__ __forceinline__ uint64_t wave_umax64(uint64_t v) {
+// The largest of the wave's values and the first lane that has it: one round over the
+// upper halves, a second where several lanes share the largest.
+__device__ __forceinline__ uint64_t bs_largest(uint64_t v, int &lane) {
     const uint32_t hi = wave_umax((uint32_t)(v >> 32));
-    return (uint64_t)hi << 32 | wave_umax((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    uint64_t who = __ballot((uint32_t)(v >> 32) == hi);
+    uint32_t lo;
+    if (who & (who - 1)) {
+        const bool tied = (uint32_t)(v >> 32) == hi;
+        lo = wave_umax(tied ? (uint32_t)v : 0u);
+        who = __ballot(tied && (uint32_t)v == lo);
+        lane = __ffsll((unsigned long long)who) - 1;
+    } else {
+        lane = __ffsll((unsigned long long)who) - 1;
+        lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    }
+    return (uint64_t)hi << 32 | lo;
 }
 
 // four elements from 4-byte aligned addresses on
 typedef float bs_v4 __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int BR_CAP = 1024;                     // candidates kept for the ranking
+constexpr int BR_CAP = 1024;                     // new candidates of a chunk
 
-// One chunk of 256 E elements: thread t has the elements 4 (t + 256 i) + j.  A wave's
-// n_out largest thread maxima bound the chunk's n_out largest elements from below
-// (each is an element): what reaches the best wave's bound is ranked by counting.
+// A part of a row in chunks of 256 E elements, the next one's loads under way while one
+// is looked through: thread t has a chunk's elements 4 (t + 256 i) + j.  Elements above
+// the n_out-th best so far join the list, few after the first chunk; in the first one
+// a wave's n_out-th largest thread maximum bounds the n_out-th largest element from
+// below (each maximum is an element), and the best of four waves' bounds counts.
 template <int E>
 __global__ __launch_bounds__(256) void k_beam_rows(BeamSelect a) {
     __shared__ float red[8];
     __shared__ uint32_t bound[4];
-    __shared__ int count, ones[4];
-    __shared__ uint64_t cand[BR_CAP];
+    __shared__ int counts[2], ones[4];                       // of a chunk's candidates: one of the two, in turn
+    __shared__ uint64_t cand[BR_CAP], best[2][BEAM_MOST];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, k = a.n_out;
     if (a.ended && a.ended[row]) return;                     // its logits do not count
-    const int v0 = blockIdx.y * 256 * E, n = min(a.n_vocab - v0, 256 * E);
+    const int v0 = blockIdx.y * a.span, n = min(a.n_vocab - v0, a.span);
     const float *const x = a.x + (size_t)row * a.stride + v0;
-    float e[E];
+    constexpr float LOWEST = -3.4028234664e38f;
+    float e[E], more[E];
+    auto load = [&](float(&to)[E], int c0) {
 #pragma unroll
-    for (int i = 0; i < E / 4; i++) {
-        const int at = 4 * (tid + 256 * i);
-        if (at + 3 < n) {
-            const bs_v4 y = *(const bs_v4 *)(x + at);
-            e[4 * i] = y.x; e[4 * i + 1] = y.y; e[4 * i + 2] = y.z; e[4 * i + 3] = y.w;
-        } else {
+        for (int i = 0; i < E / 4; i++) {
+            const int at = c0 + 4 * (tid + 256 * i);
+            if (at + 3 < n) {
+                const bs_v4 y = *(const bs_v4 *)(x + at);
+                to[4 * i] = y.x; to[4 * i + 1] = y.y; to[4 * i + 2] = y.z; to[4 * i + 3] = y.w;
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) e[4 * i + j] = at + j < n ? x[at + j] : -__builtin_inff();
+                for (int j = 0; j < 4; j++) to[4 * i + j] = at + j < n ? x[at + j] : -__builtin_inff();
+            }
         }
-    }
-    float m = e[0];
+    };
+    if (tid < 2) counts[tid] = 0;
+    load(more, 0);
+    float m = -__builtin_inff(), s = 0.0f, least = LOWEST;
+    int kept = 0, side = 0, turn = 0;
+    for (int c0 = 0; c0 < n; c0 += 256 * E, turn ^= 1) {
+        // a thread that finds no candidate goes on while others still read that: the next
+        // chunk counts elsewhere, and the one behind it after another barrier
+        int &count = counts[turn];
 #pragma unroll
-    for (int i = 1; i < E; i++) m = fmaxf(m, e[i]);          // a NaN only where all are
-    // the wave's k-th largest thread maximum, bit by bit
-    const uint32_t mo = m > -__builtin_inff() ? bs_order(m) : 0u;
-    uint32_t t = 0;
-    for (int b = 31; b >= 0; b--) {
-        const uint32_t u = t | 1u << b;
-        if (__popcll(__ballot(mo >= u)) >= k) t = u;
-    }
-    const float wm = group_max<64>(m);
-    if (tid == 0) count = 0;
-    if (lane == 0) {
-        bound[wave] = t;
-        red[wave] = wm;
-    }
-    __syncthreads();
-    t = max(max(bound[0], bound[1]), max(bound[2], bound[3]));
-    const float least = t > bs_order(-3.4028234664e38f) ? bs_value(t) : -3.4028234664e38f;
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mm = m > -__builtin_inff() ? m : 0.0f;       // nothing but -inf and NaN
-    float s = 0.0f;
+        for (int i = 0; i < E; i++) e[i] = more[i];
+        if (c0 + 256 * E < n) load(more, c0 + 256 * E);
+        float cm = e[0];
 #pragma unroll
-    for (int i = 0; i < E; i++) s += __expf(e[i] - mm);
-    s = group_sum<64>(s);
-    if (lane == 0) red[4 + wave] = s;
-    auto key = [&](int i) { return bs_key(e[i], v0 + 4 * (tid + 256 * (i >> 2)) + (i & 3)); };
-#pragma unroll
-    for (int i = 0; i < E; i++) {
-        if (e[i] >= least) {
-            const int at = atomicAdd(&count, 1);
-            if (at < BR_CAP) cand[at] = key(i);
+        for (int i = 1; i < E; i++) cm = fmaxf(cm, e[i]);    // a NaN only where all are
+        if (cm > m) {
+            s *= __expf(m - cm);                             // from -inf: 0 (or a NaN's NaN)
+            m = cm;
         }
-    }
-    __syncthreads();
-    const size_t chunk = (size_t)row * a.chunks + blockIdx.y;
-    if (tid == 0) a.ms[chunk] = make_float2(m, red[4] + red[5] + red[6] + red[7]);
-    int c = count;
-    if (c > BR_CAP) {
-        // too many alike: the k-th largest candidate itself, bit by bit
-        uint64_t low = 0;
-        for (int b = 63; b >= 0; b--) {
-            const uint64_t u = low | 1ull << b;
-            int n1 = 0;
+        const float mm = m > -__builtin_inff() ? m : 0.0f;   // nothing but -inf and NaN
+        float cs = 0.0f;                                     // a chunk's apart: few roundings in a long row
 #pragma unroll
-            for (int i = 0; i < E; i++) n1 += key(i) >= u;
-            n1 = group_isum<64>(n1);
+        for (int i = 0; i < E; i++) cs += __expf(e[i] - mm);
+        s += cs;
+        if (kept < k) {
+            // the wave's k-th largest thread maximum, its upper half bit by bit
+            const uint32_t mo = cm > -__builtin_inff() ? bs_order(cm) : 0u;
+            uint32_t t = 0;
+            for (int b = 31; b >= 16; b--) {
+                const uint32_t u = t | 1u << b;
+                if (__popcll(__ballot(mo >= u)) >= k) t = u;
+            }
+            if (lane == 0) bound[wave] = t;
             __syncthreads();
-            if (lane == 0) ones[wave] = n1;
+            t = max(max(bound[0], bound[1]), max(bound[2], bound[3]));
+            least = t > bs_order(LOWEST) ? bs_value(t) : LOWEST;
+        }
+        auto key = [&](int i) { return bs_key(e[i], v0 + c0 + 4 * (tid + 256 * (i >> 2)) + (i & 3)); };
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            if (e[i] >= least) {
+                const int at = atomicAdd(&count, 1);
+                if (at < BR_CAP) cand[at] = key(i);
+            }
+        }
+        __syncthreads();
+        int c = count;
+        if (c > BR_CAP) {
+            // too many alike: the k-th largest candidate itself, bit by bit
+            uint64_t low = 0;
+            for (int b = 63; b >= 0; b--) {
+                const uint64_t u = low | 1ull << b;
+                int n1 = 0;
+#pragma unroll
+                for (int i = 0; i < E; i++) n1 += key(i) >= u;
+                n1 = group_isum<64>(n1);
+                __syncthreads();
+                if (lane == 0) ones[wave] = n1;
+                __syncthreads();
+                if (ones[0] + ones[1] + ones[2] + ones[3] >= k) low = u;
+            }
             __syncthreads();
-            if (ones[0] + ones[1] + ones[2] + ones[3] >= k) low = u;
+            if (tid == 0) count = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const uint64_t y = key(i);
+                if (y >= low && y) cand[atomicAdd(&count, 1)] = y;       // k of them: keys differ
+            }
+            __syncthreads();
+            c = count;
+        }
+        if (c == 0) continue;
+        // ranks among those kept and the new ones, by counting
+        const uint64_t *const old = best[side];
+        uint64_t *const now = best[side ^ 1];
+        for (int i = tid; i < kept + c; i += 256) {
+            const uint64_t y = i < kept ? old[i] : cand[i - kept];
+            int rank = i < kept ? i : 0;
+            if (i >= kept)
+                for (int j = 0; j < kept; j++) rank += old[j] > y;
+            for (int j = 0; j < c; j++) rank += cand[j] > y;
+            if (rank < k) now[rank] = y;
         }
         __syncthreads();
         if (tid == 0) count = 0;
-        __syncthreads();
-        for (int i = 0; i < E; i++) {
-            const uint64_t y = key(i);
-            if (y >= low && y) cand[atomicAdd(&count, 1)] = y;  // k of them: keys differ
+        kept = min(kept + c, k);
+        side ^= 1;
+        if (kept == k) {
+            // only what is above the k-th: an equal one has a higher token
+            const float kth = bs_value((uint32_t)(now[k - 1] >> 32));
+            least = kth < __builtin_inff() ? bs_value(bs_order(kth) + 1) : __builtin_nanf("");
         }
         __syncthreads();
-        c = count;
     }
-    uint64_t *const top = a.top + chunk * k;
-    for (int i = tid; i < c; i += 256) {
-        const uint64_t y = cand[i];
-        int rank = 0;
-        for (int j = 0; j < c; j++) rank += cand[j] > y;
-        if (rank < k) top[rank] = y;
+    const float wm = group_max<64>(m);
+    s = m > -__builtin_inff() ? s * __expf(m - wm) : s;
+    s = group_sum<64>(s);
+    if (lane == 0) {
+        red[wave] = wm;
+        red[4 + wave] = s;
     }
-    for (int i = c + tid; i < k; i += 256) top[i] = 0;
+    __syncthreads();
+    const size_t list = (size_t)row * a.lists + blockIdx.y;
+    if (tid == 0) {
+        const float top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        float sum = 0.0f;
+        for (int w = 0; w < 4; w++) sum += red[w] > -__builtin_inff() ? red[4 + w] * __expf(red[w] - top) : red[4 + w];
+        a.ms[list] = make_float2(top, sum);
+    }
+    for (int i = tid; i < k; i += 256) a.top[list * k + i] = i < kept ? best[side][i] : 0;
 }
 
-// The k largest of `lists` descending lists of k in memory, lists l, l + 64, .. a
-// lane's: k times the largest head.  put(i, candidate) for i < k, by the whole wave.
+// The first entries of a lane's list in registers.
+struct BsHeads {
+    uint64_t h[4];
+};
+__device__ __forceinline__ BsHeads bs_heads(const uint64_t *list, bool is, int k) {
+    BsHeads x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x.h[i] = is && i < k ? list[i] : 0;
+    return x;
+}
+// k times the largest head of up to 64 descending lists of k, one a lane's, its first
+// entries in x: put(i, entry, lane), by the whole wave.  Ties go to the first lane.
 template <typename F>
-__device__ __forceinline__ void bs_merge(const uint64_t *lists, int n, int k, F put) {
+__device__ __forceinline__ void bs_merge(const uint64_t *list, BsHeads x, int k, F put) {
     const int lane = threadIdx.x & 63;
-    if (n <= 64) {
-        const uint64_t *at = lists + (size_t)min(lane, n - 1) * k, *const end = at + k;
-        uint64_t head = lane < n ? *at : 0;
-        for (int i = 0; i < k; i++) {
-            const uint64_t best = wave_umax64(head);
-            put(i, best);
-            if (best == 0) continue;
-            if (head == best) head = ++at < end ? *at : 0;
+    int taken = 0;
+    for (int i = 0; i < k; i++) {
+        int who;
+        const uint64_t best = bs_largest(x.h[0], who);
+        put(i, best, who);
+        if (best && lane == who) {
+            taken++;
+            x.h[0] = x.h[1];
+            x.h[1] = x.h[2];
+            x.h[2] = x.h[3];
+            x.h[3] = taken + 3 < k ? list[taken + 3] : 0;
         }
-        return;
     }
-    // more lists than lanes: the best below the last one, looked for in all of the lane's
+}
+// The same of more lists than lanes, in memory: the best below the last one, looked for
+// in all of the lane's lists.
+template <typename F>
+__device__ __forceinline__ void bs_merge_many(const uint64_t *lists, int n, int k, F put) {
+    const int lane = threadIdx.x & 63;
     uint64_t last = ~0ull;
     for (int i = 0; i < k; i++) {
         uint64_t mine = 0;
@@ -175,97 +250,105 @@ __device__ __forceinline__ void bs_merge(const uint64_t *lists, int n, int k, F 
                 if (j < k && at[j] > mine) mine = at[j];
             }
         }
-        last = wave_umax64(mine);
-        put(i, last);
+        int who;
+        last = bs_largest(mine, who);
+        put(i, last, who);
     }
 }
 
-// A workgroup a group: its waves merge the rows' chunks, then the first wave the rows.
+// A workgroup a group: its waves merge the rows' lists, all threads turn the rows' best
+// into scores, the first wave merges the rows.
 __global__ __launch_bounds__(1024) void k_beam_join(BeamSelect a) {
-    extern __shared__ uint64_t tops[];                       // [beam][n_out]
+    extern __shared__ uint64_t tops[];                       // [beam][n_out] candidates, then their scores; behind them the tokens
     __shared__ double norm[BEAM_MOST];                       // what a logit's score is above it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, k = a.n_out, g = blockIdx.x;
+    int *const tokens = (int *)(tops + a.n_beam * k);
     for (int b = wave; b < a.n_beam; b += waves) {
         const int row = g * a.n_beam + b;
-        if (a.ended && a.ended[row]) {
+        // all that the row needs at once: the first reads are what this kernel waits for
+        const bool over = a.ended && a.ended[row];
+        const float score = a.score[row];
+        const float2 *const ms = a.ms + (size_t)row * a.lists;
+        const uint64_t *const top = a.top + (size_t)row * a.lists * k, *const list = top + (size_t)min(lane, a.lists - 1) * k;
+        const float2 first = ms[min(lane, a.lists - 1)];
+        const BsHeads heads = bs_heads(list, lane < a.lists, k);
+        if (over) {
             for (int i = lane; i < k; i += 64) tops[b * k + i] = i == 0 ? 1 : 0;
-            if (lane == 0) norm[b] = a.score[row];
+            if (lane == 0) norm[b] = score;
             continue;
         }
-        const float2 *const ms = a.ms + (size_t)row * a.chunks;
-        float m = -__builtin_inff();
-        for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, ms[c].x);
+        float m = first.x;
+        for (int c = lane + 64; c < a.lists; c += 64) m = fmaxf(m, ms[c].x);
         m = group_max<64>(m);
-        double s = 0.0;
-        for (int c = lane; c < a.chunks; c += 64) {
-            const float2 y = ms[c];
-            s += y.y == 0.0f ? 0.0 : (double)y.y * exp((double)y.x - (double)m);        // a NaN stays
-        }
+        auto term = [&](float2 y) { return y.y == 0.0f ? 0.0 : (double)y.y * exp((double)y.x - (double)m); };      // a NaN stays
+        double s = lane < a.lists ? term(first) : 0.0;
+        for (int c = lane + 64; c < a.lists; c += 64) s += term(ms[c]);
         s = group_sum_t<64>(s);
-        if (lane == 0) norm[b] = (double)a.score[row] - ((double)m + log(s));
-        bs_merge(a.top + (size_t)row * a.chunks * k, a.chunks, k, [&](int i, uint64_t y) {
+        if (lane == 0) norm[b] = (double)score - ((double)m + log(s));
+        auto put = [&](int i, uint64_t y, int) {
             if (lane == 0) tops[b * k + i] = y;
-        });
+        };
+        if (a.lists <= 64) bs_merge(list, heads, k, put);
+        else bs_merge_many(top, a.lists, k, put);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.n_beam * k; i += blockDim.x) {
+        const int b = i / k;
+        const uint64_t y = tops[i];
+        const double v = y == 1 ? norm[b] : norm[b] + (double)bs_value((uint32_t)(y >> 32));         // (1: no logit's)
+        tops[i] = y && v > -__builtin_inf() ? bs_order(v) : 0;           // nor a NaN
+        tokens[i] = y == 1 ? -1 : (int)~(uint32_t)y;
     }
     __syncthreads();
     if (wave) return;
-    // lane: a beam; its next candidate's score, and whether that is one
-    const bool mine = lane < a.n_beam;
-    const double base = mine ? norm[lane] : 0.0;
-    const bool over = mine && a.ended && a.ended[g * a.n_beam + lane];
-    int at = 0;
-    auto next = [&]() -> uint64_t {
-        if (!mine || at == k) return 0;
-        const uint64_t y = tops[lane * k + at];
-        if (y == 0) return 0;
-        const double v = over ? base : base + (double)bs_value((uint32_t)(y >> 32));
-        return v > -__builtin_inf() ? bs_order(v) : 0;       // nor a NaN
-    };
-    uint64_t head = next();
-    for (int i = 0; i < k; i++) {
-        const uint64_t best = wave_umax64(head);
-        const uint64_t hit = __ballot(head == best);
-        const int b = __ffsll((unsigned long long)hit) - 1;  // the lowest of equal ones
+    const bool mine = lane < a.n_beam;                       // lane: a beam
+    const uint64_t *const list = tops + (mine ? lane : 0) * k;
+    int at = 0;                                              // of its candidates
+    bs_merge(list, bs_heads(list, mine, k), k, [&](int i, uint64_t best, int who) {
         const size_t out = (size_t)g * k + i;
-        if (best == 0) {
-            if (lane == 0) {
-                a.score_out[out] = -__builtin_inff();
-                a.row_out[out] = -1;
-                a.token_out[out] = -1;
-            }
-            continue;
-        }
-        if (lane == b) {
-            a.score_out[out] = (float)bs_value(best);
-            a.row_out[out] = g * a.n_beam + b;
-            a.token_out[out] = over ? -1 : (int)~(uint32_t)tops[lane * k + at];
-            at++;
-            head = next();
-        }
-    }
+        if (lane != who) return;
+        const int token = tokens[lane * k + at++];
+        a.score_out[out] = best ? (float)bs_value(best) : -__builtin_inff();
+        a.row_out[out] = best ? g * a.n_beam + lane : -1;
+        a.token_out[out] = best ? token : -1;
+    });
 }
 
-// Elements of a thread: 32 where that leaves two workgroups a CU, else 8.
-int beam_elements(int rows, int n_vocab) { return (int64_t)rows * ((n_vocab + 8191) / 8192) >= 512 ? 32 : 8; }
+// How a row is cut: 4 workgroups a CU in all where its parts stay 4096 tokens or more,
+// else parts of 2048, one chunk of 8 elements a thread.
+struct BeamSplit {
+    int lists, span, e;
+};
+BeamSplit beam_split(int rows, int n_vocab) {
+    BeamSplit y;
+    const int most = (n_vocab + 4095) / 4096, want = std::max(1, 1024 / std::max(1, rows));
+    y.e = want >= most ? 8 : 16;
+    const int lists = y.e == 8 ? (n_vocab + 2047) / 2048 : want;
+    y.span = ((n_vocab + lists - 1) / lists + 1023) / 1024 * 1024;
+    y.lists = (n_vocab + y.span - 1) / y.span;
+    return y;
+}
 
 }  // namespace
 
 size_t beam_workspace(int n_group, int n_beam, int n_vocab, int n_out) {
-    const int rows = n_group * n_beam, chunk = 256 * beam_elements(rows, n_vocab);
-    const size_t chunks = (size_t)rows * ((n_vocab + chunk - 1) / chunk);
-    return chunks * (sizeof(float2) + (size_t)n_out * sizeof(uint64_t));
+    const int rows = n_group * n_beam;
+    const size_t lists = (size_t)rows * beam_split(rows, n_vocab).lists;
+    return lists * (sizeof(float2) + (size_t)n_out * sizeof(uint64_t));
 }
 hipError_t launch_beam_select(BeamSelect a, uint8_t *ws, hipStream_t s) {
-    const int rows = a.n_group * a.n_beam, e = beam_elements(rows, a.n_vocab), chunk = 256 * e;
+    const int rows = a.n_group * a.n_beam;
     if (rows == 0) return hipSuccess;
-    a.chunks = (a.n_vocab + chunk - 1) / chunk;
+    const BeamSplit y = beam_split(rows, a.n_vocab);
+    a.lists = y.lists;
+    a.span = y.span;
     a.top = (uint64_t *)ws;
-    a.ms = (float2 *)(ws + (size_t)rows * a.chunks * a.n_out * sizeof(uint64_t));
-    if (e == 32) hipLaunchKernelGGL(k_beam_rows<32>, dim3(rows, a.chunks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(k_beam_rows<8>, dim3(rows, a.chunks), dim3(256), 0, s, a);
+    a.ms = (float2 *)(ws + (size_t)rows * a.lists * a.n_out * sizeof(uint64_t));
+    if (y.e == 16) hipLaunchKernelGGL(k_beam_rows<16>, dim3(rows, a.lists), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(k_beam_rows<8>, dim3(rows, a.lists), dim3(256), 0, s, a);
     if (hipError_t err = hipGetLastError()) return err;
     const int waves = std::min(16, a.n_beam);
-    hipLaunchKernelGGL(k_beam_join, dim3(a.n_group), dim3(64 * waves), (size_t)a.n_beam * a.n_out * sizeof(uint64_t), s, a);
+    hipLaunchKernelGGL(k_beam_join, dim3(a.n_group), dim3(64 * waves), (size_t)a.n_beam * a.n_out * (sizeof(uint64_t) + sizeof(int)), s, a);
     return hipGetLastError();
 }
 

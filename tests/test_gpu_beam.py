@@ -61,6 +61,29 @@ def test_select_of_a_long_row(gpu):
     _check(gpu, x, [-1.0, -1.25], 2, 40)
 
 
+@pytest.mark.parametrize("order", ["rising", "falling", "nothing first", "level", "steps"])
+@pytest.mark.parametrize("rows,vocab,n_out", [(300, 20011, 7), (512, 16385, 64), (1024, 12289, 1)])
+def test_rows_of_several_chunks(gpu, order, rows, vocab, n_out):
+    # many rows: a workgroup looks through several chunks of one, its bound rising as it goes
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((rows, vocab), np.float32)
+    if order in ("rising", "falling"):
+        x.sort(axis=1)
+    if order == "falling":
+        x = x[:, ::-1]
+    if order == "nothing first":
+        x[:, :9000] = -np.inf
+        x[::2, :4500] = np.nan
+        x[::3, 9000:12288] = -np.inf
+    if order == "level":
+        x[:] = 0.5
+        x[::2, 4096:] = 0.75                                 # above what the first chunk left, all of it
+    if order == "steps":
+        x = np.floor(np.arange(vocab) / 1000 + x).astype(np.float32) / 4
+    # beams far enough apart that no two rows' normalisers decide
+    _check(gpu, np.ascontiguousarray(x), np.tile([0.0, -60.0, -120.0, -180.0], rows // 4), 4, n_out)
+
+
 @pytest.mark.parametrize("stride,shift", [(1009, 0), (1001, 1), (0, 3), (1003, 2)])
 def test_rows_of_any_stride_and_alignment(gpu, stride, shift):
     rng = np.random.default_rng(stride + shift)
