@@ -25,9 +25,13 @@ __device__ __forceinline__ PtSpan pt_span(const PagedBatch &b, int s) {
 }
 
 // mask = the token's own bit and its ancestors', depth = their number.  A workgroup a
-// sequence, a thread a (token, word): each follows its token's chain in LDS.
+// sequence, its tokens in blocks of 32 (a mask's words).  First a thread a token: the
+// token's line within its block, and the ancestor at which it leaves the block.  Then a
+// thread a (token, word), from block to block down to the word's: at most 32 steps of
+// each kind, where a line followed token by token takes a thousand.
 __global__ __launch_bounds__(256) void k_paged_tree_build(PagedTreeBuild a) {
-    __shared__ int up[PT_TOKENS];
+    __shared__ int up[PT_TOKENS], out[PT_TOKENS];
+    __shared__ uint32_t line[PT_TOKENS];
     const PtSpan q = pt_span(a.b, blockIdx.x);
     const int most = 32 * a.words, n = min(q.nq, most);
     bool bad = q.torn || q.nq > most;
@@ -41,16 +45,23 @@ __global__ __launch_bounds__(256) void k_paged_tree_build(PagedTreeBuild a) {
     }
     if (__any(bad) && (threadIdx.x & 63) == 0) pt_flag(a.status);
     __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 256) {
+        uint32_t bits = 0;
+        int j = i;
+        for (; j >= 0 && j >> 5 == i >> 5; j = up[j]) bits |= 1u << (j & 31);            // descends: the block ends it
+        line[i] = bits;
+        out[i] = j;
+    }
+    __syncthreads();
     for (int64_t x = threadIdx.x; x < (int64_t)q.nq * a.words; x += 256) {
         const int i = (int)(x / a.words), w = (int)(x - (int64_t)i * a.words);
         uint32_t bits = 0;
         int depth = 0;
         if (i < n) {
-            depth = -1;
-            for (int j = i; j >= 0; j = up[j]) {             // descends: at most i + 1 steps
-                if (j >> 5 == w) bits |= 1u << (j & 31);
-                depth++;
-            }
+            int j = i;
+            for (depth = -1; j >= 0 && j >> 5 > w; j = out[j]) depth += __popc(line[j]);
+            if (j >= 0 && j >> 5 == w) bits = line[j];
+            depth += __popc(bits);                           // of word 0: all of them
         }
         a.mask[(size_t)(q.t0 + i) * a.words + w] = bits;
         if (w == 0) a.depth[q.t0 + i] = depth;

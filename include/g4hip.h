@@ -407,10 +407,9 @@ typedef struct {
  * token's own bit and its ancestors', a depth counts these.  Any other parent sets
  * G4H_PAGED_BAD_BATCH in *status_dev (may be NULL) and counts as -1; so does a
  * sequence of more than 32 words tokens, of which those behind get no bit and depth
- * 0.  With offsets that descend or leave [0, n_tok] (flagged too) the masks and
- * depths of the whole batch are undefined, as are those of rows of no sequence
- * without them: those are left as they were.  Only n_seq, n_tok and q_off_dev of the
- * batch are used. */
+ * 0.  Masks and depths of rows of no sequence are left as they were.  Offsets that
+ * descend or leave [0, n_tok] are flagged too, and the whole batch's masks and depths
+ * are undefined then.  Only n_seq, n_tok and q_off_dev of the batch are used. */
 int g4h_paged_tree_build(const g4h_paged_batch *batch, const int *parent_dev, int words, uint32_t *mask_dev, int *depth_dev,
                          int *status_dev, void *stream);
 /* g4h_paged_append with the rotations of positions first + depth (a depth outside
@@ -446,7 +445,8 @@ int g4h_paged_tree_accept(const g4h_paged_batch *batch, const int *parent_dev, c
  * keep[s][k], k < n_keep[s], to the slots first + k, bit for bit.  Lists ascend
  * (keep_dev [n_seq][most], as g4h_paged_tree_accept writes them): from the first
  * entry that does not, or that the sequence does not have, on nothing is moved
- * (G4H_PAGED_BAD_BATCH); a row whose page or whose place's page is outside the pool is
+ * (G4H_PAGED_BAD_BATCH), and nothing at all where n_keep is below 0 or above `most` or
+ * the sequence's new tokens (likewise); a row whose page or whose place's page is outside the pool is
  * left where it is (G4H_PAGED_BAD_PAGE).  The batch is the one that was appended, its
  * lengths unchanged; a sequence with fewer positions than new tokens is left alone.
  * Slots behind the kept ones keep what they hold. */
@@ -478,8 +478,8 @@ int g4h_paged_fork(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *b
  * go by row, then by token (equal logits of a row: by token); rows are compared by
  * scores in 64 bits, whose normalisers carry an fp32 sum's error.  A row whose
  * ended_dev (may be NULL) is not 0 competes once, with its score as it is and token
- * -1; its logits are not read.  Tokens at -inf, rows at score -inf and rows with a
- * NaN or +inf among their logits, or in their score, are never selected; where fewer
+ * -1; its logits are not read.  Tokens at -inf, rows with a score of -inf or NaN and
+ * rows with a NaN or +inf among their logits are never selected; where fewer
  * than n_out can be, the rest has score -inf, row -1 and token -1.  n_out == n_beam:
  * score_out may be score.  Up to 2^20 rows of up to 2^24 logits, 64 beams a group.
  * ws: g4h_beam_workspace_bytes() of caller-owned scratch, 16-byte aligned, without
