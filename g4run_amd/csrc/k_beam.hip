@@ -234,28 +234,6 @@ __device__ __forceinline__ void bs_merge(const uint64_t *list, BsHeads x, int k,
         }
     }
 }
-// The same of more lists than lanes, in memory: the best below the last one, looked for
-// in all of the lane's lists.
-template <typename F>
-__device__ __forceinline__ void bs_merge_many(const uint64_t *lists, int n, int k, F put) {
-    const int lane = threadIdx.x & 63;
-    uint64_t last = ~0ull;
-    for (int i = 0; i < k; i++) {
-        uint64_t mine = 0;
-        if (last) {
-            for (int l = lane; l < n; l += 64) {
-                const uint64_t *at = lists + (size_t)l * k;
-                int j = 0;
-                while (j < k && at[j] >= last) j++;          // descending: the first below
-                if (j < k && at[j] > mine) mine = at[j];
-            }
-        }
-        int who;
-        last = bs_largest(mine, who);
-        put(i, last, who);
-    }
-}
-
 // A workgroup a group: its waves merge the rows' lists, all threads turn the rows' best
 // into scores, the first wave merges the rows.
 __global__ __launch_bounds__(1024) void k_beam_join(BeamSelect a) {
@@ -269,27 +247,21 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamSelect a) {
         const bool over = a.ended && a.ended[row];
         const float score = a.score[row];
         const float2 *const ms = a.ms + (size_t)row * a.lists;
-        const uint64_t *const top = a.top + (size_t)row * a.lists * k, *const list = top + (size_t)min(lane, a.lists - 1) * k;
-        const float2 first = ms[min(lane, a.lists - 1)];
+        const uint64_t *const list = a.top + ((size_t)row * a.lists + min(lane, a.lists - 1)) * k;
+        const float2 first = ms[min(lane, a.lists - 1)];     // lane: a list
         const BsHeads heads = bs_heads(list, lane < a.lists, k);
         if (over) {
             for (int i = lane; i < k; i += 64) tops[b * k + i] = i == 0 ? 1 : 0;
             if (lane == 0) norm[b] = score;
             continue;
         }
-        float m = first.x;
-        for (int c = lane + 64; c < a.lists; c += 64) m = fmaxf(m, ms[c].x);
-        m = group_max<64>(m);
-        auto term = [&](float2 y) { return y.y == 0.0f ? 0.0 : (double)y.y * exp((double)y.x - (double)m); };      // a NaN stays
-        double s = lane < a.lists ? term(first) : 0.0;
-        for (int c = lane + 64; c < a.lists; c += 64) s += term(ms[c]);
-        s = group_sum_t<64>(s);
+        const float m = group_max<64>(first.x);
+        // (a NaN stays one)
+        const double s = group_sum_t<64>(lane < a.lists && first.y != 0.0f ? (double)first.y * exp((double)first.x - (double)m) : 0.0);
         if (lane == 0) norm[b] = (double)score - ((double)m + log(s));
-        auto put = [&](int i, uint64_t y, int) {
+        bs_merge(list, heads, k, [&](int i, uint64_t y, int) {
             if (lane == 0) tops[b * k + i] = y;
-        };
-        if (a.lists <= 64) bs_merge(list, heads, k, put);
-        else bs_merge_many(top, a.lists, k, put);
+        });
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.n_beam * k; i += blockDim.x) {
@@ -315,15 +287,17 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamSelect a) {
 }
 
 // How a row is cut: 4 workgroups a CU in all where its parts stay 4096 tokens or more,
-// else parts of 2048, one chunk of 8 elements a thread.
+// else parts of 2048, one chunk of 8 elements a thread; never more parts than a wave of
+// k_beam_join has lanes.
+constexpr int BEAM_LISTS = 64;
 struct BeamSplit {
     int lists, span, e;
 };
 BeamSplit beam_split(int rows, int n_vocab) {
     BeamSplit y;
-    const int most = (n_vocab + 4095) / 4096, want = std::max(1, 1024 / std::max(1, rows));
-    y.e = want >= most ? 8 : 16;
-    const int lists = y.e == 8 ? (n_vocab + 2047) / 2048 : want;
+    const int most = (n_vocab + 4095) / 4096, want = std::max(1, 1024 / std::max(1, rows)), small = (n_vocab + 2047) / 2048;
+    y.e = want >= most && small <= BEAM_LISTS ? 8 : 16;
+    const int lists = y.e == 8 ? small : std::min(std::min(want, most), BEAM_LISTS);
     y.span = ((n_vocab + lists - 1) / lists + 1023) / 1024 * 1024;
     y.lists = (n_vocab + y.span - 1) / y.span;
     return y;
