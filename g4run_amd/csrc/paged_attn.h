@@ -211,13 +211,12 @@ __device__ __forceinline__ uint32_t pa_bits(const uint32_t *mask, int words, int
     return (uint32_t)(((uint64_t)hi << 32 | lo) >> (off & 31));
 }
 // Whether a tree's row attends nothing: no position of the prefix, no cached one, no
-// new token that has a position.
-__device__ __forceinline__ bool pa_tree_nothing(const PagedAttn &a, const PagedSeq &q, int tok) {
+// new token that has a position.  mask: its row.
+__device__ __forceinline__ bool pa_tree_nothing(const PagedAttn &a, const PagedSeq &q, int tok, const uint32_t *mask) {
     const int first_new = q.len - q.nq;
     if (first_new + (tok - q.t0) < 0) return true;
     const int low = a.window ? first_new + paged_depth(a.depth[tok], q.nq) + 1 - a.window : -0x7fffffff;       // first position, the prefix's below 0
     if ((a.b.n_prefix > 0 && low < 0) || (first_new > 0 && low < first_new)) return false;
-    const uint32_t *mask = a.mask + (size_t)tok * a.words;
     for (int w = 0; w < a.words; w++) {
         const int n = q.nq - 32 * w, gone = -first_new - 32 * w;             // tokens from this word on; of them before position 0
         uint32_t bits = n >= 32 ? mask[w] : n > 0 ? mask[w] & ((1u << n) - 1) : 0u;

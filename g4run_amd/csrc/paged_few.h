@@ -228,7 +228,10 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
         }
         lds_barrier();                                       // the previous piece's sums are read
         if constexpr (TREE) {
-            if (tid < R) nothing[tid] = tid < rows && !x.pre && !sq.bad && pa_tree_nothing(a, sq, sq.t0 + (int)(tid * pl.grp_inv >> 16));
+            if (tid < R) {
+                const int tok = sq.t0 + (int)(tid * pl.grp_inv >> 16);
+                nothing[tid] = tid < rows && !x.pre && !sq.bad && pa_tree_nothing(a, sq, tok, a.mask + (size_t)tok * a.words);
+            }
         }
         {
             float am = 0.0f;

@@ -63,6 +63,8 @@ struct PtShape {
 template <typename S, int HD, int KVT>
 __device__ __forceinline__ void pt_load(const PagedPool &p, const PaUnits &us, int l0, uint32_t slot, int wave, int lane) {
     constexpr int T = S::RB / 32;
+    uintptr_t pk = (uintptr_t)p.k, pv = (uintptr_t)p.v;      // chosen between by value, not by place
+    asm volatile("" : "+s"(pk), "+s"(pv));
 #pragma unroll
     for (int n = 0; n < S::PER; n++) {
         const int idx = wave + 8 * n;
@@ -76,7 +78,7 @@ __device__ __forceinline__ void pt_load(const PagedPool &p, const PaUnits &us, i
             const size_t u0 = pa_unit<HD, KVT>(p, us, l0 + 2 * q).row, u1 = pa_unit<HD, KVT>(p, us, l0 + 2 * q + 1).row;
             unit = row < 16 ? u0 : u1;
         }
-        pt_async16((value ? p.v : p.k) + unit + (uint32_t)((row & 15) * S::RB + 16 * chunk), slot + q * S::TILE + (value ? 32 * S::RB : 0) + 1024 * w);
+        pt_async16((const uint8_t *)(value ? pv : pk) + unit + (uint32_t)((row & 15) * S::RB + 16 * chunk), slot + q * S::TILE + (value ? 32 * S::RB : 0) + 1024 * w);
     }
     if constexpr (S::SLOADS > 0) {
         if (wave >= 8 - S::SLOADS) {
@@ -123,7 +125,6 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
     __shared__ __align__(16) float ex[KVT == F16 ? 1 : 8][ES > 1 ? PG : 1][32];            // of a wave and tile: pa_exponent of its positions' largest V scales
     __shared__ int ids[8][64];                               // of a wave: the next page ids
     __shared__ float2 wml[8][16];
-    __shared__ int nothing[16 * ZW];                         // whether a row attends nothing
     __shared__ uint32_t bits[PT_BITS];                       // the tile's masks
     __shared__ float part[8][16];                            // at the end: each wave's factor of its rows
     __shared__ float *dst[16 * ZW];                          // and where the rows go
@@ -199,7 +200,6 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
         auto row_hits = [&](uint64_t out, int unit) { return out ? pa_tree_hits(out, unit, 2, last, rlo, full, row_bits) : false; };
         uint32_t my_bits = 0;
         if (in_lds && tid < held) my_bits = a.mask[(size_t)(sq.t0 + tok0) * words + tid];
-        const bool none = ok && tree && !sq.bad && pg == 0 && ew == 0 && g == 0 && pa_tree_nothing(a, sq, tok);
 
         PaUnits us = {0, 0};                                 // 64 units; their successors' ids in ids[wave]
         uint64_t outside = 0;
@@ -209,7 +209,12 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
         }
         __syncthreads();                                     // the previous piece's sums are used
         if (in_lds && tid < held) bits[tid] = my_bits;
-        if (pg == 0 && ew == 0 && g == 0) nothing[16 * rw + c] = none;
+        // The queries, older than the page ids, are here too: said now, as a wait of the
+        // compiler's for them behind the loads below would be for those as well.
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) asm volatile("" : "+v"(y[s][k]));
         issue_order();
         // the ids of the 64 units from `unit` on, on their way
         auto ask = [&](int unit) { pt_async4(x.table + paged_entry(p, min(unit + lane, last)), pt_lds(ids[wave])); };
@@ -554,17 +559,26 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
         }
         l += partner<16>(l);
         l += partner<32>(l);
-        // out through LDS, the position groups' results joined in order
+        // Out through LDS, the position groups' results joined in order.  A row a thread
+        // finds its place meanwhile.
+        constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
+        const int r00 = x.tile * R, count = rows - r00;      // rows of the tile
+        PaSink sink = {nullptr, nullptr, false};
+        bool zero = false;
+        if (tid < count) {
+            const int i = (r00 + tid) / G, head = kvh * G + (r00 + tid - i * G), tok = sq.t0 + i;
+            zero = tree && !sq.bad && pa_tree_nothing(a, sq, tok, in_lds ? bits + (i - tok0) * words : a.mask + (size_t)tok * words);
+            sink = pa_sink<true>(a, pl, x, share, tid, tok, head, zero, true);
+            dst[tid] = sink.o;
+        }
         __syncthreads();                                     // the ring is used
         if (g == 0) wml[wave][c] = make_float2(m, l);
 #pragma unroll
         for (int e = 0; e < NM; e++) *(pa_v4f *)&buf[(wave * 16 + c) * BP + 16 * e + 4 * g] = o[e];
         __syncthreads();
-        // a row a thread: its waves' factors, its sums' place; then four elements a thread
-        constexpr float VS = KVT == Q8_0 ? 512.0f : 1.0f;
-        const int r00 = x.tile * R, count = rows - r00;      // rows of the tile
+        // a row a thread: its waves' factors; then four elements a thread
         if (tid < count) {
-            const int w0 = (tid >> 4) * ES, step = ES << rgl, i = (r00 + tid) / G, head = kvh * G + (r00 + tid - i * G), cc = tid & 15;
+            const int w0 = (tid >> 4) * ES, step = ES << rgl, cc = tid & 15;
             float mm = -__builtin_inff(), ls = 0.0f;
             for (int k = 0; k < groups; k++)
 #pragma unroll
@@ -574,14 +588,11 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
                 const float v = wml[w0 + k * step][cc].y;
                 ls += v == v ? factor(w0 + k * step) * v : v;            // a bad page's NaN stays
             }
-            const bool zero = nothing[tid];
-            const PaSink to = pa_sink<true>(a, pl, x, share, tid, sq.t0 + i, head, zero, true);
-            const float f = !to.out ? VS : zero ? 0.0f : VS / ls;
+            const float f = !sink.out ? VS : zero ? 0.0f : VS / ls;
             for (int k = 0; k < groups; k++)
 #pragma unroll
                 for (int n = 0; n < ES; n++) part[w0 + k * step + n][cc] = f * factor(w0 + k * step + n);
-            dst[tid] = to.o;
-            if (!to.out) *to.ml = make_float2(mm, ls);
+            if (!sink.out) *sink.ml = make_float2(mm, ls);
         }
         __syncthreads();
         for (int y = tid; y < count * (HD / 4); y += PM_THREADS) {
