@@ -57,6 +57,7 @@ struct PagedList {
     int wgs;                         // workgroups
     int unit, shift;                 // positions of a step, and their log2
     int lead;                        // steps that the start of a sequence's tile counts as
+    int cost[3];                     // trees: what a step of a tile of up to 32, up to 64 and more rows counts as
     int pre_tiles, pre_steps;        // the prefix's tiles (0: not this kernel's), and steps of each
     float *o;                        // [2 wgs][rows][hd] unnormalised sums
     float2 *ml;                      // [2 wgs][rows] maximum (log2), sum
@@ -343,12 +344,25 @@ __host__ __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const 
     pa_tile_span<MANY, TREE>(a, pl, q, tile, lo, hi);
     return max(1, (hi - lo + y.unit) >> y.shift);
 }
-// steps of a sequence for one KV head
+// What a step of a tile of `toks` tokens counts as: 1, but in k_paged_tree, whose time
+// for a step goes by the rows (pt_cost).
+template <bool MANY, bool TREE = false>
+__host__ __device__ __forceinline__ int pa_cost(const PagedAttn &a, const PagedPlan &pl, int toks) {
+    if constexpr (!MANY || !TREE) return 1;
+    const int rows = toks * a.grp, c0 = pl.many.cost[0], c1 = pl.many.cost[1], c2 = pl.many.cost[2];       // (loaded, then chosen between)
+    return rows <= 32 ? c0 : rows <= 64 ? c1 : c2;
+}
+template <bool MANY, bool TREE = false>
+__host__ __device__ __forceinline__ int pa_tile_cost(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile) {
+    if constexpr (!MANY || !TREE) return 1;
+    return pa_cost<MANY, TREE>(a, pl, min(q.nq - tile * pl.many.toks, pl.many.toks));
+}
+// steps of a sequence for one KV head, by what they count as
 template <bool MANY, bool TREE = false>
 __host__ __device__ __forceinline__ int pa_steps(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q) {
     const int tiles = pa_tiles<MANY>(pl, q);
     int n = 0;
-    for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY, TREE>(a, pl, q, t);
+    for (int t = 0; t < tiles; t++) n += pa_tile_steps<MANY, TREE>(a, pl, q, t) * pa_tile_cost<MANY, TREE>(a, pl, q, t);
     return n + tiles * pa_list<MANY>(pl).lead;
 }
 // All steps of the list (wave-uniform; the whole wave calls it), 64 sequences at a
@@ -377,7 +391,7 @@ __device__ __forceinline__ int pa_total(const PagedAttn &a, const PagedPlan &pl,
     for (int s0 = 64; s0 < n_seq; s0 += 64) n += at(s0);
     n_seq = pa_uniform(n_seq);
     n = pa_uniform(group_isum<64>(n));
-    return (n + y.pre_tiles * y.pre_steps) * a.p.n_kv;
+    return (n + y.pre_tiles * y.pre_steps * pa_cost<MANY, TREE>(a, pl, y.toks)) * a.p.n_kv;
 }
 // The sequence whose steps hold step u (counted without the prefix's) and the
 // number of steps before it.  A workgroup asks for ascending u: the search goes on
@@ -404,27 +418,45 @@ __device__ __forceinline__ void pa_find_step(const PagedAttn &a, const PagedPlan
     before = from.before;
 }
 __host__ __device__ __forceinline__ int pa_share(const PagedList &y, int total) { return (total + y.wgs - 1) / y.wgs; }
+// Of trees no less than the dearest step: every share of a tile's then begins one.
+__device__ __forceinline__ int pa_tree_share(const PagedAttn &a, const PagedPlan &pl, int total, int n_seq) {
+    const PagedList &y = pl.many;
+    int most = y.pre_tiles ? y.toks : 0;                     // tokens of a tile
+    for (int s = threadIdx.x & 63; s < n_seq; s += 64) most = max(most, min(paged_seq(a.p, a.b, s).nq, y.toks));
+    return max(pa_share(y, total), pa_cost<true, true>(a, pl, pa_uniform((int)wave_umax((uint32_t)most))));
+}
 
 // A piece: steps [step, step + n) of the `all` of one tile of one KV head.  (The
 // lead comes before step 0, so the shares of the list stay contiguous.)
 struct PaPiece {
     PagedSeq sq;                     // the prefix: all tokens of the batch
     int kvh, tile, step, n, all;
-    int took;                        // of the share: n and what it holds of the lead; n is 0 where it ends in that
+    int took;                        // of the share: n and what it holds of the lead; n is 0 where it ends in that (a tree: or begins behind its last step)
     int seglen, start, end;          // positions of the segment; the piece's [start, end)
     int hi0, hi1, lo0, lo1;          // the first and the last row's last and first positions (a tree: hi0 the first new token's,
                                      // hi1 the last's; lo0 and lo1 as if its depths were 0 and the most)
     int slot;                        // of its sums
+    int after;                       // what lies between the piece's end and the last step's start
     const int *table;
     bool pre;
 };
+// steps that begin before `end`, `cost` apart; wave-uniform
+__host__ __device__ __forceinline__ int pa_steps_in(int end, int cost) {
+    const int n = (end + cost - 1) / cost;
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_readfirstlane(n);
+#else
+    return n;
+#endif
+}
 // the piece at step u of a share [first, stop); find(u, seq, before) as pa_find_step
 template <bool MANY, bool TREE = false, typename F>
 __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, const PagedPlan &pl, int n_seq, int wg, int u, int first, int stop, F find) {
     const PagedList &y = pa_list<MANY>(pl);
     const PagedBatch &b = a.b;
     PaPiece x;
-    const int pre_all = y.pre_tiles * y.pre_steps * a.p.n_kv;
+    int cost = pa_cost<MANY, TREE>(a, pl, y.toks);
+    const int pre_all = y.pre_tiles * y.pre_steps * cost * a.p.n_kv;
     x.pre = u < pre_all;
     int base, v, lead = 0;                                   // v: the step of the tile, its lead counted
     if (x.pre) {
@@ -433,8 +465,8 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
         x.sq.len = x.seglen = b.n_prefix;
         x.sq.bad = false;
         x.all = y.pre_steps;
-        const int t = u / x.all;
-        v = u - t * x.all;
+        const int t = u / (x.all * cost);
+        v = u - t * x.all * cost;
         x.kvh = y.pre_tiles == 1 ? t : t / y.pre_tiles;
         x.tile = t - x.kvh * y.pre_tiles;
         x.table = b.prefix;
@@ -450,12 +482,17 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
         if constexpr (MANY) {
             const int tiles = pa_tiles<MANY>(pl, x.sq);
             int head = tiles * y.lead;                       // steps of one KV head
-            for (int t = 0; t < tiles; t++) head += pa_tile_steps<MANY, TREE>(a, pl, x.sq, t);
+            for (int t = 0; t < tiles; t++) head += pa_tile_steps<MANY, TREE>(a, pl, x.sq, t) * pa_tile_cost<MANY, TREE>(a, pl, x.sq, t);
             for (x.kvh = 0; v >= head; x.kvh++) v -= head;
-            x.tile = 0;
-            for (x.all = pa_tile_steps<MANY, TREE>(a, pl, x.sq, 0); v >= y.lead + x.all; x.all = pa_tile_steps<MANY, TREE>(a, pl, x.sq, ++x.tile)) v -= y.lead + x.all;
+            for (x.tile = 0;; x.tile++) {
+                x.all = pa_tile_steps<MANY, TREE>(a, pl, x.sq, x.tile);
+                cost = pa_tile_cost<MANY, TREE>(a, pl, x.sq, x.tile);
+                if (v < y.lead + x.all * cost) break;
+                v -= y.lead + x.all * cost;
+            }
         } else {
             x.all = pa_tile_steps<MANY, TREE>(a, pl, x.sq, 0);
+            cost = 1;
             x.tile = 0;
             for (x.kvh = 0; v >= y.lead + x.all; x.kvh++) v -= y.lead + x.all;
         }
@@ -466,9 +503,16 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
         x.seglen = x.sq.bad ? 0 : x.sq.len;
         x.table = b.table + (size_t)seq * b.table_stride;
     }
-    x.step = max(0, v - lead);
-    x.took = min(lead + x.all - v, stop - u);
-    x.n = max(0, v + x.took - lead) - x.step;
+    x.took = min(lead + x.all * cost - v, stop - u);
+    const int end = max(0, v + x.took - lead);               // steps that begin before it
+    if constexpr (MANY && TREE) {
+        x.step = pa_steps_in(max(0, v - lead), cost);
+        x.n = pa_steps_in(end, cost) - x.step;
+    } else {
+        x.step = max(0, v - lead);
+        x.n = end - x.step;
+    }
+    x.after = (x.all - 1) * cost - end;
     x.start = base + (x.step << y.shift);
     x.end = min(x.start + (x.n << y.shift), min(x.hi1 + 1, x.seglen));
     x.slot = 2 * wg + (u != first);
@@ -507,7 +551,7 @@ __host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const Pag
         s.ml = y.ml + at;
         if (note && x.step == 0) {
             // later pieces start the next workgroups' shares
-            const int rest = x.all - x.n, count = 1 + (rest + share - 1) / share;
+            const int count = 2 + x.after / share;
             (x.pre ? pl.pre : pl.own)[row] = make_uint2((uint32_t)count << 2 | none << 1 | MANY, (uint32_t)x.slot << 8 | (uint32_t)r);
         }
     }
@@ -610,6 +654,16 @@ __device__ __forceinline__ void pa_store4(float *to, pa_v4f s) {
 __host__ __device__ constexpr int pa_few_per_cu(int type, int hd, bool st) {
     return hd == 64 ? 4 : type == F16 && hd == 128 && st ? 3 : 2;
 }
+
+// k_paged_tree: what a step of a tile of up to 32 (k 0), up to 64 (1) and more rows
+// counts as (PagedList::cost), and what a tile's start.  Its 8 waves take a step's rows
+// and positions in 1, 2 or 4 turns, which hide behind f16's bytes more than behind
+// fewer ones.  (Steps alike, a lead of 3 of them, against these, with drafts of 1 to 33
+// tokens: 32 over up to 4096 positions, 8 / 4 heads of 256, 8 bits 114.6 and 94.5 us, f16
+// 143.8 and 130.1; 24 over up to 6000, 32 / 8 heads of 128, 8 bits 181.6 and 137.0, 4 bits
+// 198.5 and 144.2; 16 of up to 16 over 8192, f16, 69.5 and 67.0.)
+__host__ __device__ constexpr int pt_cost(int type, int k) { return type == F16 ? k == 0 ? 4 : k == 1 ? 5 : 9 : k == 0 ? 3 : k == 1 ? 5 : 8; }
+__host__ __device__ constexpr int pt_lead(int type) { return type == F16 ? 16 : 9; }
 
 // k_paged_tree (paged_tree.h): rows of a tile at most, and the log2 of the positions
 // that a workgroup takes at a time.  wide: for more query heads a KV head than its rows

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
     // that read the same K and V find them in its L2.
     const int per = (call.pl.many.wgs + 7) >> 3, wg = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     int mine, n_seq;
-    const int total = pa_total<true, true>(call.a, call.pl, mine, n_seq), share = pa_share(call.pl.many, total);
+    const int total = pa_total<true, true>(call.a, call.pl, mine, n_seq), share = pa_tree_share(call.a, call.pl, total, n_seq);
     const int first = wg * share, stop = wg < call.pl.many.wgs ? min(first + share, total) : 0;
     if (blockIdx.x == 0) pa_rest(call.a, call.pl, n_seq);
     PaFind from;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
         const float capl = a.cap * 1.4426950408889634f;
         const PaPiece x = pa_piece<true, true>(a, pl, mine, n_seq, from, wg, u, first, stop);
         u += x.took;
-        if (x.n == 0) break;                                 // the share ends in a tile's lead
+        if (x.n == 0) continue;                              // the share ends in a tile's lead, or begins behind a last step
         const PagedSeq &sq = x.sq;
         const int kvh = x.kvh, hi0 = x.hi0, lo0 = x.lo0, lo1 = x.lo1, start = x.start, end = x.end, rows = min(sq.nq * G, (x.tile + 1) * R);     // the tile's rows end at `rows`
         // row groups: a power of two that the tile's rows need; position groups: the rest
