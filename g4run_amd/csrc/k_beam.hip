@@ -226,11 +226,14 @@ __device__ __forceinline__ void bs_merge(const uint64_t *list, BsHeads x, int k,
         const uint64_t best = bs_largest(x.h[0], who);
         put(i, best, who);
         if (best && lane == who) {
-            taken++;
             x.h[0] = x.h[1];
             x.h[1] = x.h[2];
             x.h[2] = x.h[3];
-            x.h[3] = taken + 3 < k ? list[taken + 3] : 0;
+            x.h[3] = 0;
+            if ((++taken & 3) == 0) {                        // four at a time: a load a round would be waited for in each
+#pragma unroll
+                for (int j = 0; j < 4; j++) x.h[j] = taken + j < k ? list[taken + j] : 0;
+            }
         }
     }
 }
