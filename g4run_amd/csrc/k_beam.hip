@@ -215,17 +215,24 @@ __device__ __forceinline__ BsHeads bs_heads(const uint64_t *list, bool is, int k
     for (int i = 0; i < 4; i++) x.h[i] = is && i < k ? list[i] : 0;
     return x;
 }
-// k times the largest head of up to 64 descending lists of k, one a lane's, its first
-// entries in x: put(i, entry, lane), by the whole wave.  Ties go to the first lane.
-template <typename F>
-__device__ __forceinline__ void bs_merge(const uint64_t *list, BsHeads x, int k, F put) {
+// The k largest of up to 64 descending lists of k, one a lane's, its first entries in
+// x, by the whole wave: lane i gets the i-th, the list it is from and its place there.
+// Ties go to the first list.
+struct BsBest {
+    uint64_t entry;
+    int list, at;
+};
+__device__ __forceinline__ BsBest bs_merge(const uint64_t *list, BsHeads x, int k) {
     const int lane = threadIdx.x & 63;
+    BsBest y = {0, 0, 0};
     int taken = 0;
     for (int i = 0; i < k; i++) {
         int who;
         const uint64_t best = bs_largest(x.h[0], who);
-        put(i, best, who);
-        if (best && lane == who) {
+        if (best == 0) break;
+        const int at = __builtin_amdgcn_readlane(taken, who);
+        if (lane == i) y = BsBest{best, who, at};
+        if (lane == who) {
             x.h[0] = x.h[1];
             x.h[1] = x.h[2];
             x.h[2] = x.h[3];
@@ -236,7 +243,9 @@ __device__ __forceinline__ void bs_merge(const uint64_t *list, BsHeads x, int k,
             }
         }
     }
+    return y;
 }
+
 // A workgroup a group: its waves merge the rows' lists, all threads turn the rows' best
 // into scores, the first wave merges the rows.
 __global__ __launch_bounds__(1024) void k_beam_join(BeamSelect a) {
@@ -262,9 +271,8 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamSelect a) {
         // (a NaN stays one)
         const double s = group_sum_t<64>(lane < a.lists && first.y != 0.0f ? (double)first.y * exp((double)first.x - (double)m) : 0.0);
         if (lane == 0) norm[b] = (double)score - ((double)m + log(s));
-        bs_merge(list, heads, k, [&](int i, uint64_t y, int) {
-            if (lane == 0) tops[b * k + i] = y;
-        });
+        const BsBest y = bs_merge(list, heads, k);
+        if (lane < k) tops[b * k + lane] = y.entry;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.n_beam * k; i += blockDim.x) {
@@ -278,15 +286,12 @@ __global__ __launch_bounds__(1024) void k_beam_join(BeamSelect a) {
     if (wave) return;
     const bool mine = lane < a.n_beam;                       // lane: a beam
     const uint64_t *const list = tops + (mine ? lane : 0) * k;
-    int at = 0;                                              // of its candidates
-    bs_merge(list, bs_heads(list, mine, k), k, [&](int i, uint64_t best, int who) {
-        const size_t out = (size_t)g * k + i;
-        if (lane != who) return;
-        const int token = tokens[lane * k + at++];
-        a.score_out[out] = best ? (float)bs_value(best) : -__builtin_inff();
-        a.row_out[out] = best ? g * a.n_beam + lane : -1;
-        a.token_out[out] = best ? token : -1;
-    });
+    const BsBest y = bs_merge(list, bs_heads(list, mine, k), k);
+    if (lane >= k) return;
+    const size_t out = (size_t)g * k + lane;
+    a.score_out[out] = y.entry ? (float)bs_value(y.entry) : -__builtin_inff();
+    a.row_out[out] = y.entry ? g * a.n_beam + y.list : -1;
+    a.token_out[out] = y.entry ? tokens[y.list * k + y.at] : -1;
 }
 
 // How a row is cut: 4 workgroups a CU in all where its parts stay 4096 tokens or more,
