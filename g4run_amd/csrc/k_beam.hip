@@ -7,7 +7,9 @@
 // for those.  k_beam_rows reads the logits once, a workgroup a part of a row, and
 // leaves the part's maximum, sum and n_out best; k_beam_join takes a row's from its
 // parts', then a group's from its rows'.  Bound by the logits' bytes where they are
-// many, by the two launches and the selection's chains where they are few.
+// many (16 groups of 8 beams of 262144, 16 outputs: 37 us of k_beam_rows, 3.6 TB/s, and
+// 10 of k_beam_join, whose two merges are a chain of 32 rounds), by the two launches and
+// the selection's chains where they are few (4 beams of 32768, 8 outputs: 6 and 6 us).
 //
 // Exactness: candidates are compared as (logit, lowest token) within a row and as
 // (score in 64 bits, lowest beam) between rows.  Sums of exponentials are fp32, under
@@ -68,6 +70,8 @@ constexpr int BR_CAP = 1024;                     // new candidates of a chunk
 // the n_out-th best so far join the list, few after the first chunk; in the first one
 // a wave's n_out-th largest thread maximum bounds the n_out-th largest element from
 // below (each maximum is an element), and the best of four waves' bounds counts.
+// (Parts of one chunk, each with a bound of its own: 2048 workgroups 42 us, 1024 of
+// eight chunks 37.)
 template <int E>
 __global__ __launch_bounds__(256) void k_beam_rows(BeamSelect a) {
     __shared__ float red[8];

@@ -103,7 +103,10 @@ hipError_t launch_paged_attn(PagedAttn a, hipStream_t s) {
     return y.join ? join(a, pl, s) : hipSuccess;
 }
 
-// The same kernels, rows differing in which new tokens they attend.
+// Trees of new tokens: all sequences in one kernel, k_paged_few's form for trees where
+// no sequence can have more than 16 rows of a KV head (8 tokens of 2 query heads over
+// 100 positions of 256, f16, 11.3 us; k_paged_tree 12.7, and with its shorter steps a
+// join of 4), else k_paged_tree.
 hipError_t launch_paged_attn_tree(PagedAttn a, hipStream_t s) {
     const PagedPool &p = a.p;
     const PagedBatch &b = a.b;

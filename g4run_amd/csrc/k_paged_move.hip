@@ -3,8 +3,10 @@
 // a selection kept given tables and pages of their own (g4h_paged_fork).
 //
 // Copies: bound by memory where there is much of it (each byte read and written
-// once), else by a launch and a chain of dependent reads (offsets and lengths, page
-// ids, rows).  One launch serves all layers' caches of one shape.
+// once: 32 new beams' pages of 64 x 4 heads of 256 in 26 f16 caches, 257 MB in 46 us,
+// 5.6 TB/s), else by a launch and a chain of dependent reads (offsets and lengths, page
+// ids, rows: 4 beams in 26 caches 5.7 us; one accepted path 4.5, 32 of them in 8-bit
+// caches 7.9).  One launch serves all layers' caches of one shape.
 #include <algorithm>
 
 #include "paged.h"
@@ -57,7 +59,8 @@ __global__ __launch_bounds__(256) void k_paged_keep(PagedKeep a, PagedPools pool
             }
         }
         const uint64_t todo = __ballot(moves);
-        // whole waves: all lanes have to be there where one's move is read
+        // whole waves: all lanes have to be there where one's move is read (in divergent code
+        // the reads became a loop over lanes: 13.6 us, with this 7.9)
         for (int x0 = threadIdx.x & ~63; x0 < p.n_kv * cols; x0 += 256) {
             const int x = min(x0 + lane, p.n_kv * cols - 1);
             const bool live = x == x0 + lane;

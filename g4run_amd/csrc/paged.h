@@ -111,7 +111,7 @@ struct PagedAppend {
     const float *q, *k, *v;
     float *q_out;
     size_t qs, qos, ks, vs;
-    const int *depth;                // of a tree's tokens (k_paged_tree.hip), or null: they follow each other
+    const int *depth;                // of a tree's tokens (g4h_paged_tree), or null: they follow each other
 };
 hipError_t launch_paged_append(const PagedAppend &a, hipStream_t s);
 

@@ -28,6 +28,10 @@
 //   k_paged_many  sequences of more rows (prompt chunks; the prefix of a large
 //                 batch): bound by the matrix cores.  K and V pass through LDS
 //                 once for up to 128 rows.
+// Calls with trees of new tokens (PagedAttn::mask) take one of two:
+//   k_paged_few   in a form whose rows look at their masks, where all tiles are small;
+//   k_paged_tree  else (paged_tree.h): a few to 128 rows, bound by the cache's bytes
+//                 (f16) or by what makes operands of them.
 #pragma once
 
 #include "paged.h"
@@ -42,7 +46,8 @@ typedef uint32_t pa_v4u __attribute__((ext_vector_type(4)));
 
 // The split of a call.  Each kernel's work is one list of steps (`unit` positions
 // of one row tile of one KV head: the prefix's tiles, then the sequences' in
-// order), cut into equal shares for its workgroups.  A piece -- the part of a
+// order), cut into equal shares for its workgroups; k_paged_tree's steps count by
+// their tiles' rows, so that its shares take equal time.  A piece -- the part of a
 // share that lies in one tile of one head -- is written out where it is the whole
 // tile and there is no prefix; else its sums go to the workspace.  A whole tile's
 // have a place by row, one for the prefix's tile and one for the row's own.  Of the
@@ -57,7 +62,6 @@ struct PagedList {
     int wgs;                         // workgroups
     int unit, shift;                 // positions of a step, and their log2
     int lead;                        // steps that the start of a sequence's tile counts as
-    int cost[3];                     // trees: what a step of a tile of up to 32, up to 64 and more rows counts as
     int pre_tiles, pre_steps;        // the prefix's tiles (0: not this kernel's), and steps of each
     float *o;                        // [2 wgs][rows][hd] unnormalised sums
     float2 *ml;                      // [2 wgs][rows] maximum (log2), sum
@@ -94,6 +98,7 @@ __device__ __forceinline__ void pa_global(T *&p) {
     asm("" : "+s"(g));
     p = (T *)g;
 }
+template <bool TREE = false>
 __device__ __forceinline__ PagedCall pa_fresh() {
     static_assert(sizeof(PagedCall) % 4 == 0, "read by dwords");
     auto *p = (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
@@ -109,8 +114,10 @@ __device__ __forceinline__ PagedCall pa_fresh() {
     pa_global(k.a.p.status);
     pa_global(k.a.q);
     pa_global(k.a.out);
-    pa_global(k.a.mask);
-    pa_global(k.a.depth);
+    if constexpr (TREE) {                                    // (said of what a kernel does not use, it is held all the same)
+        pa_global(k.a.mask);
+        pa_global(k.a.depth);
+    }
     pa_global(k.pl.few.o);
     pa_global(k.pl.few.ml);
     pa_global(k.pl.many.o);
@@ -210,6 +217,12 @@ __device__ __forceinline__ uint32_t pa_bits(const uint32_t *mask, int words, int
     const int w = off >> 5;
     const uint32_t lo = w >= 0 && w < words ? mask[w] : 0u, hi = w + 1 >= 0 && w + 1 < words ? mask[w + 1] : 0u;
     return (uint32_t)(((uint64_t)hi << 32 | lo) >> (off & 31));
+}
+// which of the 32 positions from base on a tree's row attends: cached ones in [rlo, rhi],
+// new ones by its bits from base on, before end
+__device__ __forceinline__ uint32_t pa_tree_seen(int base, int rlo, int rhi, uint32_t bits, int end) {
+    auto below = [&](int pos) { return pos <= base ? 0u : pos >= base + 32 ? ~0u : (1u << (pos - base)) - 1; };
+    return ((below(rhi + 1) & ~below(rlo)) | bits) & below(end);
 }
 // Whether a tree's row attends nothing: no position of the prefix, no cached one, no
 // new token that has a position.  mask: its row.
@@ -344,13 +357,23 @@ __host__ __device__ __forceinline__ int pa_tile_steps(const PagedAttn &a, const 
     pa_tile_span<MANY, TREE>(a, pl, q, tile, lo, hi);
     return max(1, (hi - lo + y.unit) >> y.shift);
 }
+// k_paged_tree: what a step of a tile of up to 32 (k 0), up to 64 (1) and more rows
+// counts as (pa_cost), and what a tile's start.  Its 8 waves take a step's rows
+// and positions in 1, 2 or 4 turns, which hide behind f16's bytes more than behind
+// fewer ones.  (Steps alike, a lead of 3 of them, against these, with drafts of 1 to 33
+// tokens: 32 over up to 4096 positions, 8 / 4 heads of 256, 8 bits 114.6 and 94.5 us, f16
+// 143.8 and 130.1; 24 over up to 6000, 32 / 8 heads of 128, 8 bits 181.6 and 137.0, 4 bits
+// 198.5 and 144.2; 16 of up to 16 over 8192, f16, 69.5 and 67.0.)
+__host__ __device__ constexpr int pt_cost(int type, int k) { return type == F16 ? k == 0 ? 4 : k == 1 ? 5 : 9 : k == 0 ? 3 : k == 1 ? 5 : 8; }
+__host__ __device__ constexpr int pt_lead(int type) { return type == F16 ? 16 : 9; }
+
 // What a step of a tile of `toks` tokens counts as: 1, but in k_paged_tree, whose time
 // for a step goes by the rows (pt_cost).
 template <bool MANY, bool TREE = false>
 __host__ __device__ __forceinline__ int pa_cost(const PagedAttn &a, const PagedPlan &pl, int toks) {
     if constexpr (!MANY || !TREE) return 1;
-    const int rows = toks * a.grp, c0 = pl.many.cost[0], c1 = pl.many.cost[1], c2 = pl.many.cost[2];       // (loaded, then chosen between)
-    return rows <= 32 ? c0 : rows <= 64 ? c1 : c2;
+    const int rows = toks * a.grp;
+    return pt_cost(a.p.type, rows <= 32 ? 0 : rows <= 64 ? 1 : 2);
 }
 template <bool MANY, bool TREE = false>
 __host__ __device__ __forceinline__ int pa_tile_cost(const PagedAttn &a, const PagedPlan &pl, const PagedSeq &q, int tile) {
@@ -436,7 +459,7 @@ struct PaPiece {
     int hi0, hi1, lo0, lo1;          // the first and the last row's last and first positions (a tree: hi0 the first new token's,
                                      // hi1 the last's; lo0 and lo1 as if its depths were 0 and the most)
     int slot;                        // of its sums
-    int after;                       // what lies between the piece's end and the last step's start
+    int after;                       // k_paged_tree: what lies between the piece's end and the last step's start
     const int *table;
     bool pre;
 };
@@ -503,16 +526,17 @@ __host__ __device__ __forceinline__ PaPiece pa_piece_by(const PagedAttn &a, cons
         x.seglen = x.sq.bad ? 0 : x.sq.len;
         x.table = b.table + (size_t)seq * b.table_stride;
     }
-    x.took = min(lead + x.all * cost - v, stop - u);
-    const int end = max(0, v + x.took - lead);               // steps that begin before it
     if constexpr (MANY && TREE) {
+        x.took = min(lead + x.all * cost - v, stop - u);
+        const int end = max(0, v + x.took - lead);           // steps that begin before it
         x.step = pa_steps_in(max(0, v - lead), cost);
         x.n = pa_steps_in(end, cost) - x.step;
+        x.after = (x.all - 1) * cost - end;
     } else {
         x.step = max(0, v - lead);
-        x.n = end - x.step;
+        x.took = min(lead + x.all - v, stop - u);
+        x.n = max(0, v + x.took - lead) - x.step;
     }
-    x.after = (x.all - 1) * cost - end;
     x.start = base + (x.step << y.shift);
     x.end = min(x.start + (x.n << y.shift), min(x.hi1 + 1, x.seglen));
     x.slot = 2 * wg + (u != first);
@@ -529,7 +553,7 @@ struct PaSink {
     float2 *ml;
     bool out;
 };
-template <bool MANY>
+template <bool MANY, bool TREE = false>
 __host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const PagedPlan &pl, const PaPiece &x, int share, int r, int tok, int head, uint32_t none, bool note) {
     const PagedList &y = pa_list<MANY>(pl);
     const size_t row = (size_t)tok * a.n_head + head;
@@ -551,7 +575,7 @@ __host__ __device__ __forceinline__ PaSink pa_sink(const PagedAttn &a, const Pag
         s.ml = y.ml + at;
         if (note && x.step == 0) {
             // later pieces start the next workgroups' shares
-            const int count = 2 + x.after / share;
+            const int rest = x.all - x.n, count = MANY && TREE ? 2 + x.after / share : 1 + (rest + share - 1) / share;
             (x.pre ? pl.pre : pl.own)[row] = make_uint2((uint32_t)count << 2 | none << 1 | MANY, (uint32_t)x.slot << 8 | (uint32_t)r);
         }
     }
@@ -654,16 +678,6 @@ __device__ __forceinline__ void pa_store4(float *to, pa_v4f s) {
 __host__ __device__ constexpr int pa_few_per_cu(int type, int hd, bool st) {
     return hd == 64 ? 4 : type == F16 && hd == 128 && st ? 3 : 2;
 }
-
-// k_paged_tree: what a step of a tile of up to 32 (k 0), up to 64 (1) and more rows
-// counts as (PagedList::cost), and what a tile's start.  Its 8 waves take a step's rows
-// and positions in 1, 2 or 4 turns, which hide behind f16's bytes more than behind
-// fewer ones.  (Steps alike, a lead of 3 of them, against these, with drafts of 1 to 33
-// tokens: 32 over up to 4096 positions, 8 / 4 heads of 256, 8 bits 114.6 and 94.5 us, f16
-// 143.8 and 130.1; 24 over up to 6000, 32 / 8 heads of 128, 8 bits 181.6 and 137.0, 4 bits
-// 198.5 and 144.2; 16 of up to 16 over 8192, f16, 69.5 and 67.0.)
-__host__ __device__ constexpr int pt_cost(int type, int k) { return type == F16 ? k == 0 ? 4 : k == 1 ? 5 : 9 : k == 0 ? 3 : k == 1 ? 5 : 8; }
-__host__ __device__ constexpr int pt_lead(int type) { return type == F16 ? 16 : 9; }
 
 // k_paged_tree (paged_tree.h): rows of a tile at most, and the log2 of the positions
 // that a workgroup takes at a time.  wide: for more query heads a KV head than its rows

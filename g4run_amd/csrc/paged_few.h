@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
     if (blockIdx.x == 0 && call.pl.many.rows == 0) pa_rest(call.a, call.pl, n_seq);
     PaFind from;
     for (int u = first; u < stop;) {
-        const PagedCall call = pa_fresh();
+        const PagedCall call = pa_fresh<TREE>();
         const PagedAttn &a = call.a;
         const PagedPlan &pl = call.pl;
         const PagedPool &p = a.p;
@@ -284,11 +284,8 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
             }
             if ((it & 31) == 0 && it + 32 < iters) more_us = pa_units(p, x.table, (base >> 4) + 64 * PW, 2 * PW, last, kvh);
             const bool edge = base + 31 > full || base < lo1 || base + 32 > end;
-            const uint32_t vis = TREE ? row_bits(base) : 0u;
-            auto seen = [&](int pos) {                       // by the lane's row
-                if constexpr (TREE) return ((pos >= rlo && pos <= rhi) || (vis >> (pos - base) & 1)) && pos < end;
-                else return pos >= rlo && pos <= rhi && pos < end;
-            };
+            const uint32_t att = TREE ? pa_tree_seen(base, rlo, rhi, row_bits(base), end) : 0u;
+            auto seen = [&](int pos) { return (att >> (pos - base) & 1) != 0; };         // by a tree's row
             constexpr int DW = PaTile<HE, KVT>::DW;
             uint32_t dk[8][DW], dv[8][DW];                   // of the lane's 8 positions
             PaScales<HE> &sl = scl[KVT == F16 ? 0 : wave];
@@ -371,7 +368,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int pos = base + 16 * (j >> 2) + 4 * g + (j & 3);
-                    w[j] = seen(pos) ? w[j] : -__builtin_inff();
+                    w[j] = (TREE ? seen(pos) : pos >= rlo && pos <= rhi && pos < end) ? w[j] : -__builtin_inff();
                 }
             }
             if constexpr (KVT == F16) {
@@ -447,7 +444,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const int pos = base + 16 * (j >> 2) + 4 * g + (j & 3);
-                        const uint32_t live = seen(pos) ? ~0u : 0u;
+                        const uint32_t live = (TREE ? seen(pos) : pos >= rlo && pos <= rhi && pos < end) ? ~0u : 0u;
 #pragma unroll
                         for (int d = 0; d < DW; d++) dv[j][d] &= live;
                     }
@@ -485,7 +482,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
                             const float v = __shfl(w[j], 16 * ((k & 15) >> 2) + c, 64);
                             if (j == 4 * (k >> 4) + (k & 3)) wx = v;
                         }
-                        const bool sees = seen(pos) && !(ST && c >= 8);
+                        const bool sees = (TREE ? seen(pos) : pos >= rlo && pos <= rhi) && !(ST && c >= 8);
 #pragma unroll
                         for (int e = 0; e < NM; e++)
 #pragma unroll

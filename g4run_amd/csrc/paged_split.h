@@ -82,7 +82,6 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
     // windows of 512 40.5, 39.8, 40.7).
     many.rows = 0;
     many.pre_tiles = many.lead = 0;
-    for (int k = 0; k < 3; k++) many.cost[k] = tree ? pt_cost(p.type, k) : 1;
     if (many_own || many_pre) {
         const int most = (tree ? pt_rows(p.hd, y.wide) : paged_most_group(p.hd)) / grp, toks = b.q_off || many_pre ? b.n_tok : 1;
         many.toks = tree ? std::min(toks, most) : pa_ceil_div(toks, pa_ceil_div(toks, most));
@@ -95,7 +94,7 @@ inline PagedLayout paged_layout(const PagedPool &p, const PagedBatch &b, int grp
             many.unit = 1 << many.shift;
             many.pre_steps = many_pre ? pa_ceil_div(b.n_prefix, many.unit) : 0;
             steps = (own * std::max(1, pa_ceil_div(mspan, many.unit)) + (int64_t)many.pre_tiles * many.pre_steps) * p.n_kv;
-            if (steps * many.cost[2] < (1 << 27)) break;
+            if (steps * (tree ? pt_cost(p.type, 2) : 1) < (1 << 27)) break;
         }
         many.wgs = (int)std::min<int64_t>(p.hd >= 128 || tree ? 256 : 512, steps);
         many.lead = steps > many.wgs ? tree ? pt_lead(p.type) : 5 : 0;

@@ -10,7 +10,16 @@
 // 2 fours, each wave with 128 of the elements, their scores added through LDS) are
 // 1, 2, 4 or 8 row groups times as many position groups as are left, as the tile's
 // rows need, so that drafts of all sizes share a call.  The position groups' sums are
-// joined at a piece's end.
+// joined at a piece's end.  (A kernel with k_paged_few's register loads for more row
+// groups took 91 us for 16 drafts of up to 16 tokens over 8192 positions, 32 / 8 heads
+// of 128, f16; this one 67: 3.8 TB/s of pages in the call, 5.5 in its steps.  Two row
+// groups a wave, one operand for both, halve the LDS traffic and the conversions of
+// quantized rows, but a wave then starts and ends with twice the state: 82 us there.)
+//
+// Quantized rows are bound by the VALU: of a tile of 16 rows x 32 positions x 128
+// elements (8 bits) 380 instructions and 24 transcendental ones beside 32 matrix
+// instructions; 32 drafts of up to 33 tokens over 4096 positions, 8 / 4 heads of 256,
+// capped, take 95 us, their bytes 30.
 #pragma once
 
 #include <algorithm>
@@ -139,7 +148,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
     if (blockIdx.x == 0) pa_rest(call.a, call.pl, n_seq);
     PaFind from;
     for (int u = first; u < stop;) {
-        const PagedCall call = pa_fresh();
+        const PagedCall call = pa_fresh<true>();
         const PagedAttn &a = call.a;
         const PagedPlan &pl = call.pl;
         const PagedPool &p = a.p;
@@ -310,13 +319,11 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
                 auto base_of = [&](int t) { return base0 + 32 * groups * t; };
                 auto tile_of = [&](int t) { return d0 + t * groups * S::TILE; };
                 const bool edge = base_of(NT - 1) + 31 > full || base0 < lo1 || base_of(NT - 1) + 32 > end;
-                uint32_t vis[NT];                            // the row's bits of these positions
+                uint32_t att[NT];                            // which of these positions the row attends
 #pragma unroll
-                for (int t = 0; t < NT; t++) vis[t] = edge && base_of(t) + 31 >= hi0 ? row_bits(base_of(t)) : 0u;
-                auto seen = [&](int t, int k) {              // position k of tile t
-                    const int pos = base_of(t) + k;
-                    return ((pos >= rlo && pos <= full) || (vis[t] >> k & 1)) && pos < end;
-                };
+                for (int t = 0; t < NT; t++)
+                    att[t] = edge ? pa_tree_seen(base_of(t), rlo, full, base_of(t) + 31 >= hi0 ? row_bits(base_of(t)) : 0u, end) : ~0u;
+                auto seen = [&](int t, int k) { return (att[t] >> k & 1) != 0; };        // position k of tile t
                 // scores of row c at positions pm_pos(g, j)
                 pa_v4f sc[NT][2];
 #pragma unroll
@@ -401,15 +408,11 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
 #pragma unroll
                         for (int j = 0; j < 8; j++) w[t][j] *= capl;
                     }
-                    live[t] = 0xffu;
+                    // (positions pm_pos(g, j): 4 g .. 4 g + 3 and 16 further)
+                    live[t] = (att[t] >> (4 * g) & 15) | (att[t] >> (4 * g + 12) & 240);
                     if (edge) {
-                        live[t] = 0;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const bool sees = seen(t, pm_pos(g, j));
-                            live[t] |= (uint32_t)sees << j;
-                            w[t][j] = sees ? w[t][j] : -__builtin_inff();
-                        }
+                        for (int j = 0; j < 8; j++) w[t][j] = live[t] >> j & 1 ? w[t][j] : -__builtin_inff();
                     }
                     if constexpr (KVT == F16) {
 #pragma unroll
@@ -568,7 +571,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
         if (tid < count) {
             const int i = (r00 + tid) / G, head = kvh * G + (r00 + tid - i * G), tok = sq.t0 + i;
             zero = tree && !sq.bad && pa_tree_nothing(a, sq, tok, in_lds ? bits + (i - tok0) * words : a.mask + (size_t)tok * words);
-            sink = pa_sink<true>(a, pl, x, share, tid, tok, head, zero, true);
+            sink = pa_sink<true, true>(a, pl, x, share, tid, tok, head, zero, true);
             dst[tid] = sink.o;
         }
         __syncthreads();                                     // the ring is used

@@ -54,7 +54,7 @@ void follow_trees(Run &r) {
                 const int tok = x.sq.t0 + i / G, head = x.kvh * G + i % G;
                 if (tok < 0 || tok >= a.b.n_tok) wrong("token %d", tok);
                 const size_t row = (size_t)tok * a.n_head + head;
-                const PaSink to = pa_sink<MANY>(a, pl, x, share, i - r0, tok, head, !x.sq.bad && x.sq.len - x.sq.nq + i / G < 0, true);
+                const PaSink to = pa_sink<MANY, true>(a, pl, x, share, i - r0, tok, head, !x.sq.bad && x.sq.len - x.sq.nq + i / G < 0, true);
                 if (to.out) {
                     r.out[row]++;
                     continue;
