@@ -997,6 +997,9 @@ static bool paged_overlap(const float *a, size_t a_stride, size_t a_row, const f
     return (meets(k) && r < (wide)a_row) || (meets(k + 1) && s - r < (wide)b_row);
 }
 
+static bool ranges_meet(const void *a, size_t an, const void *b, size_t bn) {
+    return a && b && an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
 static int paged_append(const char *fn, const g4h_paged_kv *kv, const g4h_paged_batch *batch, const int *depth, const g4h_rope *rope, int n_head,
                         const float *q, size_t q_stride, float *q_out, size_t q_out_stride, const float *k, size_t k_stride, const float *v,
                         size_t v_stride, void *stream) {
@@ -1014,6 +1017,8 @@ static int paged_append(const char *fn, const g4h_paged_kv *kv, const g4h_paged_
         if (!paged_empty(a.b) && ((q != q_out && paged_overlap(q, q_stride, qrow, q_out, q_out_stride, qrow, a.b.n_tok)) ||
             paged_overlap(k, k_stride, row, q_out, q_out_stride, qrow, a.b.n_tok) || paged_overlap(v, v_stride, row, q_out, q_out_stride, qrow, a.b.n_tok)))
             return fail(G4H_ERR_ARG, "%s: q_out overlaps what the call reads", fn);
+        if (!paged_empty(a.b) && ranges_meet(q_out, (((size_t)a.b.n_tok - 1) * q_out_stride + qrow) * 4, depth, (size_t)a.b.n_tok * 4))
+            return fail(G4H_ERR_ARG, "%s: q_out overlaps the depths", fn);
     }
     a.r.n_rot = 0;
     a.r.interleaved = 0;
@@ -1095,6 +1100,12 @@ static int paged_attn(const char *fn, const g4h_paged_kv *kv, const g4h_paged_ba
     const size_t need = tree ? paged_attn_tree_workspace(a.p, a.b, n_head) : paged_attn_workspace(a.p, a.b, n_head);
     if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
         return fail(G4H_ERR_ARG, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, ws ? ws_bytes : (size_t)0);
+    if (tree && !paged_empty(a.b)) {
+        const size_t n = (size_t)a.b.n_tok * 4, masks = n * tree->words, outs = (((size_t)a.b.n_tok - 1) * out_stride + row) * 4;
+        if (ranges_meet(out, outs, tree->mask_dev, masks) || ranges_meet(out, outs, tree->depth_dev, n) || ranges_meet(ws, need, tree->mask_dev, masks) ||
+            ranges_meet(ws, need, tree->depth_dev, n))
+            return fail(G4H_ERR_ARG, "%s: out or the workspace overlaps masks or depths", fn);
+    }
     a.n_head = n_head;
     a.grp = n_head / a.p.n_kv;
     a.q = q;
@@ -1119,9 +1130,6 @@ extern "C" int g4h_paged_attn(const g4h_paged_kv *kv, const g4h_paged_batch *bat
 }
 
 // ------------------------------------------- trees of drafted tokens, beams ----
-static bool ranges_meet(const void *a, size_t an, const void *b, size_t bn) {
-    return a && b && an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
-}
 static int check_tree(const char *fn, const g4h_paged_batch *batch, const g4h_paged_tree *tree, bool mask) {
     if (!batch || !tree) return fail(G4H_ERR_ARG, "%s: null pointer", fn);
     if (tree->words < 1 || tree->words > PAGED_TREE_WORDS) return fail(G4H_ERR_ARG, "%s: words=%d (1 .. %d)", fn, tree->words, PAGED_TREE_WORDS);

@@ -54,6 +54,22 @@ def test_attention_and_append(abi):  # noqa: F811
     assert need(C.byref(kv), C.byref(big), 3) == 0 and need(None, C.byref(big), 2) == 0
 
 
+def test_outputs_apart_from_masks_and_depths(abi):  # noqa: F811
+    G, L = abi
+    kv, big = _kv(G), _batch(G, n_seq=2, n_tok=40, max_len=4000, table_stride=250)
+    n = L.g4h_paged_attn_tree_workspace_bytes(C.byref(kv), C.byref(big), 2)
+    row = 2 * kv.hd
+    for t in (_tree(G, mask_dev=A[4]), _tree(G, depth_dev=A[4]), _tree(G, mask_dev=A[4] + 40 * row * 4 - 4), _tree(G, depth_dev=A[4] - 4 * 39),
+              _tree(G, mask_dev=A[5] + n - 4), _tree(G, words=3, mask_dev=A[5] - 4 * 3 * 40 + 4), _tree(G, depth_dev=A[5])):
+        assert _attn(L, kv, big, t, wsb=n) == G.ERR_ARG
+    # a wider stride reaches further; right behind and right before is apart
+    assert _attn(L, kv, big, _tree(G, mask_dev=A[4] + 40 * row * 4), os=row + 8, wsb=n) == G.ERR_ARG
+    assert _append(L, kv, big, _tree(G, depth_dev=A[4] + 40 * row * 4 - 4)) == G.ERR_ARG
+    if not G._inited:
+        assert _attn(L, kv, big, _tree(G, mask_dev=A[4] + 40 * row * 4, depth_dev=A[4] - 4 * 40), wsb=n) == G.ERR_DEVICE
+        assert _append(L, kv, big, _tree(G, depth_dev=A[4] + 40 * row * 4)) == G.ERR_DEVICE
+
+
 @pytest.mark.parametrize("n_seq,n_tok", [(0, 0), (3, 0), (0, 3)])
 def test_an_empty_batch(abi, n_seq, n_tok):  # noqa: F811
     G, L = abi
