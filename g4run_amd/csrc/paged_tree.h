@@ -216,8 +216,10 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
             us = pa_units(p, x.table, start >> 4, 2, last, kvh);
             outside = pa_check(p, us);
         }
-        __syncthreads();                                     // the previous piece's sums are used
+        // The masks before the barrier: the previous piece has met behind its last look at its
+        // own, and this one's are there for all waves from the first units' check on.
         if (in_lds && tid < held) bits[tid] = my_bits;
+        __syncthreads();                                     // the previous piece's sums are used
         // The queries, older than the page ids, are here too: said now, as a wait of the
         // compiler's for them behind the loads below would be for those as well.
 #pragma unroll
