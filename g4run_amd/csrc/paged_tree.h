@@ -113,17 +113,6 @@ __device__ __forceinline__ void pt_arrived(int wave) {
 
 constexpr int PT_BITS = 512;                     // words of a tile's masks kept in LDS
 
-// tanh to half a step of 1: what a capped score, and with it a weight, is off by then
-// is less than the rounding of a score as large as the cap
-template <int N>
-__device__ __forceinline__ void pt_tanh(float (&x)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; j++) {
-        const float t = __builtin_amdgcn_exp2f(-2.885390081777927f * fabsf(x[j]));
-        x[j] = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x[j]);
-    }
-}
-
 template <int HD, int KVT, bool WIDE>
 __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
     using S = PtShape<HD, KVT, WIDE>;
@@ -406,7 +395,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) w[t][j] = sc[t][j >> 2][j & 3] * qs;
                     if (a.cap > 0.0f) {
-                        pt_tanh(w[t]);
+                        pa_tanh(w[t]);
 #pragma unroll
                         for (int j = 0; j < 8; j++) w[t][j] *= capl;
                     }

@@ -1,5 +1,5 @@
 """Draft trees over the paged KV cache where a call can go wrong unseen: pages outside
-the pool judged by the right masks."""
+the pool judged by the right masks, caps far above the scores."""
 import numpy as np
 import pytest
 
@@ -40,3 +40,81 @@ def test_bad_pages_of_drafts_with_unlike_masks(gpu, t, hd, n_head, n_kv, n):
         assert np.isnan(got[lost]).all()
         assert np.array_equal(got[~lost], clean[~lost])
         assert c.kv.status() == gpu.PAGED_BAD_PAGE
+
+
+def _capped(c, scale, cap):
+    """Outputs and tolerances as TreeCase.expect's, but with the cap's part relative to
+    the capped score, which is small where the cap is large.  tanh to 2^-20 of itself:
+    below 0.3 an odd polynomial leaves 9e-3 x^11 out, less than 2^-24 x there, and rounds
+    a few times; above it is (1 - t) / (1 + t) with t = exp(-2 x), whose numerator, 0.45
+    at least, is off by 2.2 steps of 2^-24 (exponent 0.6, exponential 1.1, difference
+    0.5), the rest by 4.4.  The argument's and the result's factors are two roundings more."""
+    grp = c.n_head // c.n_kv
+    out, tol = np.zeros((c.n_tok, c.n_head, c.hd)), np.zeros((c.n_tok, c.n_head, c.hd))
+    for s, n in enumerate(c.new):
+        for i in range(n):
+            t, at = c.off[s] + i, c.seen(s, i)
+            for h in range(c.n_head):
+                k, v = (c.rows[s][w][:, h // grp][at] for w in (0, 1))
+                q = c.q[t, h].astype(np.float64)
+                x = cap * np.tanh(k @ q * scale / cap)
+                size = (np.abs(k) @ np.abs(q) * scale).max()
+                d = size * (2.0 ** -21 + c.hd * 2.0 ** -24) + np.abs(x).max() * (2.0 ** -20 + 2.0 ** -22) + 2.0 ** -22
+                w = np.exp(x - x.max())
+                out[t, h] = w @ v / w.sum()
+                tol[t, h] = (2 * d + 2.0 ** -18) * (w @ np.abs(v)) / w.sum() + 2.0 ** -29 * len(v) * np.abs(v).max() / w.sum()
+    return out, tol
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [[3, 1], [20, 7]])
+@pytest.mark.parametrize("cap", [2.0 ** -100, 1e-3, 1.0, 50.0, 1e3, 1e4, 1e6, 1e8, 2.0 ** 100])
+def test_caps_of_any_size(gpu, t, hd, new, cap):
+    scale = hd ** -0.5
+    c = TreeCase(gpu, t, 4, 2, hd, 16, [n + 40 for n in new], new, sets=[set(range(i + 1)) for n in new for i in range(n)],
+                 depths=[i for n in new for i in range(n)], spread=1.5, seed=41)
+    want, tol = _capped(c, scale, cap)
+    got = c.attn(scale, cap=cap)
+    assert (np.abs(got - want) <= tol).all(), np.nanmax(np.abs(got - want) / tol)
+    # chains: as rows of tokens
+    same = gpu.Buffer(got.nbytes)
+    gpu.paged_attn(c.kv, c.batch, c.d["q"], 4, same, scale=scale, softcap=cap)
+    same = same.download(np.float32, got.shape)
+    assert (np.abs(same - want) <= tol).all(), np.nanmax(np.abs(same - want) / tol)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd,n_head", [(256, 65), (512, 33)])
+@pytest.mark.parametrize("cap", [1e5, 2.0 ** 100])
+def test_large_caps_of_many_query_heads(gpu, t, hd, n_head, cap):
+    c = TreeCase(gpu, t, n_head, 1, hd, 16, [40, 22], [2, 3], spread=1.5, seed=42)
+    want, tol = _capped(c, hd ** -0.5, cap)
+    got = c.attn(hd ** -0.5, cap=cap)
+    assert (np.abs(got - want) <= tol).all(), np.nanmax(np.abs(got - want) / tol)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [[3, 1], [20, 7]])
+@pytest.mark.parametrize("cap", [20.0, 300.0, 1e3, 1e4])
+def test_caps_of_scores_of_one_product(gpu, t, hd, new, cap):
+    """A query of one element: the score is one product of two halves, or of a quant and
+    its scale, and what is left to be wrong is the cap."""
+    c = TreeCase(gpu, t, 4, 2, hd, 16, [n + 40 for n in new], new, seed=43)
+    c.q[:] = 0.0
+    c.q[:, :, 37] = 1.0
+    c.d["q"].upload(c.q)
+    got = c.attn(1.0, cap=cap)
+    for s, n in enumerate(c.new):
+        for i in range(n):
+            at = c.seen(s, i)
+            for h in range(4):
+                k, v = (c.rows[s][w][:, h // 2][at] for w in (0, 1))
+                x = cap * np.tanh(k[:, 37] / cap)
+                w = np.exp(x - x.max())
+                # the product and its factors 2^-22 (four roundings), tanh 2^-20, the exponential 2^-22
+                d = np.abs(x).max() * (2.0 ** -20 + 2.0 ** -21) + 2.0 ** -22
+                tol = (2 * d + 2.0 ** -18) * (w @ np.abs(v)) / w.sum() + 2.0 ** -29 * len(v) * np.abs(v).max() / w.sum()
+                off = np.abs(got[c.off[s] + i, h] - w @ v / w.sum())
+                assert (off <= tol).all(), (s, i, h, (off / tol).max())
