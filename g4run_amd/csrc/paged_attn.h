@@ -239,14 +239,15 @@ __device__ __forceinline__ bool pa_tree_nothing(const PagedAttn &a, const PagedS
     }
     return true;
 }
-// pa_hits of a tree's row: cached positions [rlo, rhi], or new tokens; of those,
-// bits(pos) has in its low 16 bits which of the positions from pos on it attends
+// pa_hits of a tree's row, by what pa_tree_seen says that it attends of the segment's
+// `len` positions: a window may leave it no cached position (rlo behind rhi), and bits
+// of tokens that the sequence does not have mean nothing.  bits(pos): its bits from pos on
 template <typename F>
-__device__ __forceinline__ bool pa_tree_hits(uint64_t out, int first, int stride, int last, int rlo, int rhi, F bits) {
+__device__ __forceinline__ bool pa_tree_hits(uint64_t out, int first, int stride, int len, int rlo, int rhi, F bits) {
     bool hit = false;
     for (; out; out &= out - 1) {
-        const int k = __ffsll((unsigned long long)out) - 1, pos = 16 * min(first + stride * (k >> 1) + (k & 1), last);
-        hit |= (rlo <= pos + 15 && rhi >= pos) || (bits(pos) & 0xffffu);
+        const int k = __ffsll((unsigned long long)out) - 1, pos = 16 * min(first + stride * (k >> 1) + (k & 1), (len - 1) >> 4);
+        hit |= (pa_tree_seen(pos, rlo, rhi, bits(pos), len) & 0xffffu) != 0;
     }
     return hit;
 }

@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256, pa_few_per_cu(KVT, HD, ST)) void k_paged_few(P
             return off <= -32 || off >= 32 ? 0u : off < 0 ? bits << -off : bits >> off;
         };
         auto row_hits = [&](uint64_t out, int first, int stride) {
-            if constexpr (TREE) return pa_tree_hits(out, first, stride, last, rlo, rhi, row_bits);
+            if constexpr (TREE) return pa_tree_hits(out, first, stride, x.seglen, rlo, rhi, row_bits);
             else return pa_hits(out, first, stride, last, rlo, rhi);
         };
 

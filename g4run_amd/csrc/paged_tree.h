@@ -195,7 +195,7 @@ __global__ __launch_bounds__(PM_THREADS, 2) void k_paged_tree(PagedCall call) {
             }
         }
         auto row_bits = [&](int pos) { return mask ? pa_bits(mask, words, pos - hi0) : 0u; };
-        auto row_hits = [&](uint64_t out, int unit) { return out ? pa_tree_hits(out, unit, 2, last, rlo, full, row_bits) : false; };
+        auto row_hits = [&](uint64_t out, int unit) { return out ? pa_tree_hits(out, unit, 2, x.seglen, rlo, full, row_bits) : false; };
         uint32_t my_bits = 0;
         if (in_lds && tid < held) my_bits = a.mask[(size_t)(sq.t0 + tok0) * words + tid];
 

@@ -18,6 +18,32 @@ def _lose(c, entries):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("n,first,window", [(6, 29, 2), (6, 20, 0), (6, 16, 0), (7, 16, 3), (20, 18, 4), (20, 16, 0), (40, 27, 6), (40, 33, 30)])
+def test_a_bad_page_that_a_row_does_not_attend(gpu, t, hd, n, first, window):
+    """Windows that leave a row no cached position, and bits of tokens that the sequence
+    does not have: neither makes a row attend the page beside the positions it sees."""
+    rng = np.random.default_rng(n + first)
+    words = -(-n // 32)
+    sets = [{j for j in range(n) if rng.random() < 0.15} | {j for j in range(n, 32 * words) if rng.random() < 0.5} for _ in range(n)]
+    depths = [int(rng.integers(0, min(n, 14))) for _ in range(n)]
+    c = TreeCase(gpu, t, 2, 1, hd, 16, [first + n], [n], words=words, sets=sets, depths=depths, seed=44)
+    clean = c.attn(hd ** -0.5, window=window)
+    assert np.isfinite(clean).all() and c.kv.status() == 0
+    kept = 0
+    for page in range(-(-(first + n) // 16)):
+        _lose(c, [page])
+        got = c.attn(hd ** -0.5, window=window)
+        lost = np.array([any(p // 16 == page for p in c.seen(0, i, window)) for i in range(n)])
+        assert np.isnan(got[lost]).all()
+        assert np.array_equal(got[~lost], clean[~lost]), (page, np.argwhere(~np.isclose(got, clean).all((1, 2)) & ~lost).ravel())
+        assert c.kv.status() == (gpu.PAGED_BAD_PAGE if lost.any() else 0)
+        kept += (~lost).sum()
+    # (without a window all rows attend every page that holds a cached position)
+    assert kept or (window == 0 and (first + n - 1) // 16 == (first - 1) // 16)
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("hd,n_head,n_kv,n", [(64, 4, 2, 20), (128, 4, 2, 20), (256, 65, 1, 3), (512, 2, 1, 20)])
 def test_bad_pages_of_drafts_with_unlike_masks(gpu, t, hd, n_head, n_kv, n):
     """A workgroup goes through several drafts, each with a lost page among its first and
