@@ -203,12 +203,13 @@ __device__ __forceinline__ uint64_t pa_check(const PagedPool &p, PaUnits &x) {
     return __ballot(out);
 }
 // whether the lane's row, of positions [rlo, rhi], attends one of them; a page that
-// it does not attend (before its window, say, and given away) may be any
+// it does not attend (before its window, say, and given away) may be any.  A window
+// may hide the whole segment: rlo behind rhi
 __device__ __forceinline__ bool pa_hits(uint64_t out, int first, int stride, int last, int rlo, int rhi) {
     bool hit = false;
     for (; out; out &= out - 1) {
         const int k = __ffsll((unsigned long long)out) - 1, pos = 16 * min(first + stride * (k >> 1) + (k & 1), last);
-        hit |= rlo <= pos + 15 && rhi >= pos;
+        hit |= max(rlo, pos) <= min(rhi, pos + 15);
     }
     return hit;
 }

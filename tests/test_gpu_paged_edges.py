@@ -113,6 +113,19 @@ def test_a_prefix_before_all_windows_may_be_given_away(gpu, t, n_seq, own):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=IDS)
+@pytest.mark.parametrize("hd,n_head,n_kv", [(64, 4, 2), (128, 2, 1), (64, 40, 2), (512, 2, 1)])
+@pytest.mark.parametrize("own", [100, 105, 109, 110])
+@pytest.mark.parametrize("new", [1, 20])
+def test_all_of_a_prefix_before_all_windows_may_be_given_away(gpu, t, hd, n_head, n_kv, own, new):
+    # the first window begins in the 16 positions that the prefix's last ones are among, or right behind
+    own += new - 1
+    c = Case(gpu, t, n_head, n_kv, hd, 16, [own, own + 3], new=[new, new], n_prefix=150, seed=65)
+    c.prefix[:] = -1
+    c.d["pre"].upload(c.prefix)
+    c.check(window=100)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=IDS)
 @pytest.mark.parametrize("hd,n_head,n_kv", [(64, 4, 2), (256, 4, 2), (512, 2, 1)])
 @pytest.mark.parametrize("n,window", [(3, 0), (90, 0), (90, 20), (6, 20)])
 def test_a_bad_page_reaches_only_the_rows_that_attend_it(gpu, t, hd, n_head, n_kv, n, window):
