@@ -592,7 +592,8 @@ class PagedTree:
 
 class PagedCaches:
     """The paged caches of a model's layers, all of one shape, as paged_keep and
-    paged_fork take them; flags go to the first one's status word."""
+    paged_fork take them, one that layers share named once; flags go to the first one's
+    status word."""
 
     def __init__(self, caches):
         self.keep = list(caches)

@@ -8,7 +8,9 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <unordered_map>
 
 #include "kernels.h"
@@ -1233,6 +1235,22 @@ static int paged_caches(const char *fn, const g4h_paged_kv *kv, int n_cache, con
     }
     return G4H_OK;
 }
+// Whether two of the caches share memory: sorted by where they begin, pools of one size
+// that meet have neighbours of two caches that meet.  -1: no memory to find out.
+static int paged_shared(const g4h_paged_kv *kv, int n_cache, size_t bytes) {
+    struct Place { uintptr_t at; int cache; } few[2 * PAGED_CACHES];
+    std::unique_ptr<Place[]> many(n_cache > PAGED_CACHES ? new (std::nothrow) Place[2 * (size_t)n_cache] : nullptr);
+    if (n_cache > PAGED_CACHES && !many) return -1;
+    Place *const x = many ? many.get() : few;
+    for (int i = 0; i < n_cache; i++) {
+        x[2 * i] = {(uintptr_t)kv[i].k_dev, i};
+        x[2 * i + 1] = {(uintptr_t)kv[i].v_dev, i};
+    }
+    std::sort(x, x + 2 * n_cache, [](const Place &a, const Place &b) { return a.at < b.at; });
+    for (int i = 1; i < 2 * n_cache; i++)
+        if (x[i].cache != x[i - 1].cache && x[i].at - x[i - 1].at < bytes) return 1;
+    return 0;
+}
 static int paged_pools(const g4h_paged_kv *kv, int n_cache, int c0, PagedPools &pools) {
     const int n = std::min(n_cache - c0, PAGED_CACHES);
     for (int i = 0; i < n; i++) {
@@ -1248,6 +1266,9 @@ extern "C" int g4h_paged_keep(const g4h_paged_kv *kv, int n_cache, const g4h_pag
     if (int rc = paged_caches(fn, kv, n_cache, batch, a.p, a.b)) return rc;
     if (most < 1 || most > 1 << 24) return fail(G4H_ERR_ARG, "%s: most=%d (1 .. 2^24)", fn, most);
     if (null_or_odd(n_keep, !paged_empty(a.b)) || null_or_odd(keep, !paged_empty(a.b))) return fail(G4H_ERR_ARG, "%s: null or misaligned array", fn);
+    // rows move within a cache: two at once in one place would read what the other has written
+    if (const int y = n_cache > 1 && !paged_empty(a.b) ? paged_shared(kv, n_cache, a.p.page_bytes * (size_t)a.p.n_pages) : 0)
+        return y < 0 ? fail(G4H_ERR_NOMEM, "%s: no host memory for %d caches", fn, n_cache) : fail(G4H_ERR_ARG, "%s: two of the caches share memory", fn);
     a.n_keep = n_keep;
     a.keep = keep;
     a.most = most;

@@ -449,7 +449,8 @@ int g4h_paged_tree_accept(const g4h_paged_batch *batch, const int *parent_dev, c
  * the sequence's new tokens (likewise); a row whose page or whose place's page is outside the pool is
  * left where it is (G4H_PAGED_BAD_PAGE).  The batch is the one that was appended, its
  * lengths unchanged; a sequence with fewer positions than new tokens is left alone.
- * Slots behind the kept ones keep what they hold. */
+ * Slots behind the kept ones keep what they hold.  No two of the caches may share
+ * memory (G4H_ERR_ARG): layers that share a cache name it once. */
 int g4h_paged_keep(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *batch, const int *n_keep_dev, const int *keep_dev, int most,
                    void *stream);
 /* Rows of a new batch that continue rows of the present one, as a beam selection
@@ -467,7 +468,7 @@ int g4h_paged_keep(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *b
  * the present batch reads or another row's fresh one.  Of the batch n_seq, len_dev,
  * table_dev, table_stride and max_len are used; the outputs may not overlap them.
  * len_out and table_out may both be NULL, where the caches of another shape have had
- * them. */
+ * them.  A cache that is named twice is written twice, with the same bytes. */
 int g4h_paged_fork(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *batch, int n_out, const int *parent_dev, const int *fresh_dev,
                    int *len_out_dev, int *table_out_dev, int out_stride, void *stream);
 /* Beam search's selection.  Of each of n_group groups of n_beam rows of logits

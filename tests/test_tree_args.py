@@ -133,6 +133,36 @@ def test_keep(abi):  # noqa: F811
         assert call() == G.ERR_DEVICE
 
 
+def test_keep_of_caches_that_share_memory(abi):  # noqa: F811
+    """Rows moved in one place by two at once: refused, but where nothing is moved."""
+    G, L = abi
+    size = G.paged_pool_bytes(G.F16, 2, 64, 16, 4)
+    far = lambda i: 1 << 32 | i << 20  # noqa: E731
+    pools = [(far(2 * i), far(2 * i + 1)) for i in range(300)]
+
+    def call(pools, b=_batch(G)):
+        kvs = (G._PagedKV * len(pools))(*[_kv(G, k_dev=k, v_dev=v) for k, v in pools])
+        return L.g4h_paged_keep(kvs, len(pools), C.byref(b), A[1], A[2], 3, None)
+
+    apart = G.OK if G._inited else G.ERR_DEVICE
+    for n in (2, 3, 64, 65, 300):
+        few = pools[:n]
+        for i, j in ((0, 1), (0, n - 1), (n // 2, n - 1)):
+            if i == j:
+                continue
+            for pair in (few[i], few[i][::-1], (far(900), few[i][0]), (few[i][1], far(900)), (few[i][0] + size - 16, far(900)),
+                         (far(900), few[i][1] - size + 16)):
+                assert call(few[:j] + [pair] + few[j + 1:]) == G.ERR_ARG, (n, i, j)
+        if not G._inited:                                    # right behind and right before is apart; any order
+            assert call(few) == apart and call(few[::-1]) == apart
+            assert call([(few[0][0] + size, far(900))] + few) == apart and call(few + [(far(900), few[-1][1] - size)]) == apart
+    # nothing to move, and a fork, which only writes pages that nothing is read from
+    assert call([pools[0], pools[0]], _batch(G, n_tok=0)) == apart
+    if not G._inited:
+        kvs = (G._PagedKV * 2)(_kv(G), _kv(G))
+        assert L.g4h_paged_fork(kvs, 2, C.byref(_batch(G, n_tok=0, len_dev=A[6], table_dev=A[7])), 4, A[1], A[2], A[3], A[4], 2, None) == G.ERR_DEVICE
+
+
 def test_fork(abi):  # noqa: F811
     G, L = abi
 
