@@ -1322,7 +1322,7 @@ static int check_beam(const char *fn, int n_group, int n_beam, int n_vocab, int 
     return G4H_OK;
 }
 extern "C" size_t g4h_beam_workspace_bytes(int n_group, int n_beam, int n_vocab, int n_out) {
-    return check_beam("g4h_beam_workspace_bytes", n_group, n_beam, n_vocab, n_out) ? 0 : beam_workspace(n_group, n_beam, n_vocab, n_out);
+    return check_beam("g4h_beam_workspace_bytes", n_group, n_beam, n_vocab, n_out) ? 0 : beam_workspace_most(n_group, n_beam, n_vocab, n_out);
 }
 extern "C" int g4h_beam_select(const float *logits, size_t stride, int n_group, int n_beam, int n_vocab, const float *score, const int *ended,
                                int n_out, float *score_out, int *row_out, int *token_out, void *ws, size_t ws_bytes, void *stream) {

@@ -20,7 +20,9 @@ struct BeamSelect {
     float2 *ms;                                  // [row][list] maximum, sum of exp(x - maximum)
     uint64_t *top;                               // [row][list][n_out] candidates, descending; 0: none
 };
+// workspace of a call; and enough for it and all calls of fewer groups
 size_t beam_workspace(int n_group, int n_beam, int n_vocab, int n_out);
+size_t beam_workspace_most(int n_group, int n_beam, int n_vocab, int n_out);
 hipError_t launch_beam_select(BeamSelect a, uint8_t *ws, hipStream_t s);
 
 }  // namespace g4

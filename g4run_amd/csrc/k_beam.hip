@@ -315,13 +315,23 @@ BeamSplit beam_split(int rows, int n_vocab) {
     return y;
 }
 
+// lists of any call of up to `rows` rows at most: fewer rows may be cut into more parts
+size_t beam_lists_most(int rows, int n_vocab) {
+    const int most = (n_vocab + 4095) / 4096, small = (n_vocab + 2047) / 2048;
+    const int fine = small > BEAM_LISTS ? 0 : most == 1 ? rows : 1024 / most;            // rows up to which the parts are of 2048
+    const size_t few = (size_t)std::min(rows, fine) * small;
+    const size_t many = rows > fine ? std::min((size_t)rows * std::min(most, BEAM_LISTS), (size_t)std::max(1024, rows)) : 0;
+    return std::max(few, many);
+}
+size_t beam_bytes(size_t lists, int n_out) { return lists * (sizeof(float2) + (size_t)n_out * sizeof(uint64_t)); }
+
 }  // namespace
 
 size_t beam_workspace(int n_group, int n_beam, int n_vocab, int n_out) {
     const int rows = n_group * n_beam;
-    const size_t lists = (size_t)rows * beam_split(rows, n_vocab).lists;
-    return lists * (sizeof(float2) + (size_t)n_out * sizeof(uint64_t));
+    return beam_bytes((size_t)rows * beam_split(rows, n_vocab).lists, n_out);
 }
+size_t beam_workspace_most(int n_group, int n_beam, int n_vocab, int n_out) { return beam_bytes(beam_lists_most(n_group * n_beam, n_vocab), n_out); }
 hipError_t launch_beam_select(BeamSelect a, uint8_t *ws, hipStream_t s) {
     const int rows = a.n_group * a.n_beam;
     if (rows == 0) return hipSuccess;

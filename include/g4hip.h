@@ -484,8 +484,8 @@ int g4h_paged_fork(const g4h_paged_kv *kv, int n_cache, const g4h_paged_batch *b
  * than n_out can be, the rest has score -inf, row -1 and token -1.  n_out == n_beam:
  * score_out may be score.  Up to 2^20 rows of up to 2^24 logits, 64 beams a group.
  * ws: g4h_beam_workspace_bytes() of caller-owned scratch, 16-byte aligned, without
- * initial contents; calls that overlap must not share it.  Asynchronous, capturable;
- * runs repeat bit for bit. */
+ * initial contents; that of n_group groups is enough for fewer; calls that overlap must
+ * not share it.  Asynchronous, capturable; runs repeat bit for bit. */
 size_t g4h_beam_workspace_bytes(int n_group, int n_beam, int n_vocab, int n_out);
 int g4h_beam_select(const float *logits_dev, size_t stride, int n_group, int n_beam, int n_vocab, const float *score_dev, const int *ended_dev,
                     int n_out, float *score_out_dev, int *row_out_dev, int *token_out_dev, void *ws_dev, size_t ws_bytes, void *stream);

@@ -202,6 +202,29 @@ def test_beam_select(abi):  # noqa: F811
                   lambda: call(g=0, x=None, s=None, so=None, ro=None, to=None, ws=None, wsb=0)], G.ERR_DEVICE)
 
 
+@pytest.mark.parametrize("n_beam,n_out", [(1, 1), (4, 8), (8, 8), (64, 64)])
+@pytest.mark.parametrize("n_vocab", [1, 100, 2048, 2049, 4096, 4097, 20011, 32768, 50001, 100000, 131072, 131073, 262144, 1 << 24])
+def test_a_workspace_serves_smaller_batches(abi, n_vocab, n_beam, n_out):  # noqa: F811
+    """Requests end and the batch shrinks: what was enough for the largest is enough."""
+    G, L = abi
+    most = 0
+    for g in [*range(1, 600), 1023, 1024, 1025, 1 << 14, (1 << 20) // n_beam]:
+        need = L.g4h_beam_workspace_bytes(g, n_beam, n_vocab, n_out)
+        assert need >= most, (g, need, most)
+        most = need
+    # and not far more than 2048 lists, or two a row (rows of up to 4096 tokens in parts of 2048), take
+    assert most <= max(2 * g * n_beam, 2048) * (8 + 8 * n_out)
+
+    def call(g, wsb):
+        return L.g4h_beam_select(1 << 50, 0, g, n_beam, n_vocab, A[2], None, n_out, A[3], A[4], A[5], 1 << 52, wsb, None)
+
+    for g in (1, 2, 3, 10, 31, 32, 33, 100, 128, 129, 255, 256, 257, 500):
+        need = L.g4h_beam_workspace_bytes(g, n_beam, n_vocab, n_out)
+        assert call(g, 0) == call(g, 7) == G.ERR_ARG
+        if not G._inited:
+            assert call(g, need) == G.ERR_DEVICE, g
+
+
 def test_the_plain_model():
     sets, depth = ancestry([-1, 0, 0, 1, 3, -1])
     assert sets == [{0}, {0, 1}, {0, 2}, {0, 1, 3}, {0, 1, 3, 4}, {5}] and depth == [0, 1, 1, 2, 3, 0]
