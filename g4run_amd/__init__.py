@@ -618,8 +618,10 @@ def paged_attn_tree_workspace_bytes(kv: PagedKV, batch: PagedBatch, n_head: int)
 
 def paged_attn_tree(kv: PagedKV, batch: PagedBatch, tree: PagedTree, q, n_head: int, out, scale: float = 1.0, softcap: float = 0.0,
                     window: int = 0, ws=None, q_stride: int = 0, out_stride: int = 0, stream=None) -> None:
-    """Attention of a tree's tokens: the cached positions, and the new tokens of
-    their masks; ws as paged_attn's, of paged_attn_tree_workspace_bytes."""
+    """Attention of a tree's tokens: the cached positions (with a window those that it
+    leaves), and the new tokens of their masks, whatever the window: one that is not longer
+    than a draft is deep needs masks without the ancestors behind it; ws as paged_attn's, of
+    paged_attn_tree_workspace_bytes."""
     need = 0 if isinstance(ws, Buffer) else paged_attn_tree_workspace_bytes(kv, batch, n_head)
     made = ws is None and need > 0
     if made:

@@ -404,7 +404,8 @@ typedef struct {
 } g4h_paged_tree;
 /* parent_dev[t]: the number, within its sequence, of the token that token t
  * continues, smaller than its own, or -1: the cached positions.  A mask holds the
- * token's own bit and its ancestors', a depth counts these.  Any other parent sets
+ * token's own bit and all its ancestors' (for layers whose window is not longer than
+ * a draft is deep, see g4h_paged_attn_tree), a depth counts these.  Any other parent sets
  * G4H_PAGED_BAD_BATCH in *status_dev (may be NULL) and counts as -1; so does a
  * sequence of more than 32 words tokens, of which those behind get no bit and depth
  * 0.  Masks and depths of rows of no sequence are left as they were.  Offsets that
@@ -421,9 +422,12 @@ int g4h_paged_append_tree(const g4h_paged_kv *kv, const g4h_paged_batch *batch, 
  * positions before its sequence's first new one -- with a window those after first
  * + depth - window -- and of the new tokens those whose bits are set, its own among
  * them only if set, whatever their order; bits of tokens that the sequence does not
- * have mean nothing, and the window hides none of them.  Zeros for a token that
- * attends nothing, as for one without a position.  Everything else as there, with a
- * workspace of its own size. */
+ * have mean nothing, and the window hides none of them.  So a window that is not
+ * longer than a draft is deep needs masks of the caller's own, without the bits of
+ * ancestors `window` or more levels up (g4h_paged_tree_build keeps them all): a
+ * confirmed token's attention is then that of g4h_paged_attn with this window, and
+ * with them it is not.  Zeros for a token that attends nothing, as for one without a
+ * position.  Everything else as there, with a workspace of its own size. */
 size_t g4h_paged_attn_tree_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head);
 int g4h_paged_attn_tree(const g4h_paged_kv *kv, const g4h_paged_batch *batch, const g4h_paged_tree *tree, int n_head, const float *q_dev,
                         size_t q_stride, float scale, float softcap, int window, float *out_dev, size_t out_stride, void *ws_dev,

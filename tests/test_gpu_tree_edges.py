@@ -1,10 +1,10 @@
 """Draft trees over the paged KV cache where a call can go wrong unseen: pages outside
-the pool judged by the right masks, caps far above the scores."""
+the pool judged by the right masks, caps far above the scores, windows that a draft outgrows."""
 import numpy as np
 import pytest
 
-from paged_util import F16, Q4_0, Q8_0
-from tree_util import TreeCase
+from paged_util import F16, Q4_0, Q8_0, attend
+from tree_util import TreeCase, pack
 
 pytestmark = pytest.mark.gpu
 TYPES = [F16, Q8_0, Q4_0]
@@ -144,3 +144,37 @@ def test_caps_of_scores_of_one_product(gpu, t, hd, new, cap):
                 tol = (2 * d + 2.0 ** -18) * (w @ np.abs(v)) / w.sum() + 2.0 ** -29 * len(v) * np.abs(v).max() / w.sum()
                 off = np.abs(got[c.off[s] + i, h] - w @ v / w.sum())
                 assert (off <= tol).all(), (s, i, h, (off / tol).max())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("new,window", [([6], 3), ([6, 2], 6), ([40, 9], 8), ([40], 33), ([40], 39), ([40], 40)])
+@pytest.mark.parametrize("chain", [True, False])
+def test_a_window_that_a_draft_outgrows(gpu, t, new, window, chain):
+    """Masks without the ancestors that a token's window has left: its attention is that of
+    the row of tokens that it continues, with this window."""
+    c = TreeCase(gpu, t, 4, 2, 128, 16, [n + 50 for n in new], new, n_prefix=11, seed=45)
+    parents = [list(range(-1, n - 1)) if chain else [-1] + [max(0, i - 1 - (i * 7) % 3) for i in range(1, n)] for n in new]
+    paths, at = [], 0
+    for up in parents:
+        for i, x in enumerate(up):
+            paths.append((paths[at + x] if x >= 0 else []) + [i])
+        at += len(up)
+    c.sets, c.depths = [set(p[-window:]) for p in paths], [len(p) - 1 for p in paths]
+    assert max(c.depths) + 1 >= min(window, 3)
+    c.d["mask"].upload(pack(c.sets, c.words))
+    c.d["depth"].upload(np.asarray(c.depths, np.int32))
+    got = c.attn(0.1, window=window)
+    for s, n in enumerate(c.new):
+        first = c.n_prefix + c.lens[s] - n
+        for i in range(n):
+            tok = c.off[s] + i
+            row = list(range(first)) + [first + j for j in paths[tok]]
+            for h in range(4):
+                k, v = (np.concatenate([c.shared[w][:, h // 2], c.rows[s][w][:, h // 2]])[row] for w in (0, 1))
+                want, tol = attend(c.q[tok, h], k, v, len(row) - 1, 0.1, window=window)
+                assert (np.abs(got[tok, h] - want) <= tol).all(), (s, i, h)
+    if chain:
+        same = gpu.Buffer(got.nbytes)
+        gpu.paged_attn(c.kv, c.batch, c.d["q"], 4, same, scale=0.1, window=window)
+        want, tol = super(TreeCase, c).expect(0.1, window=window)
+        assert (np.abs(same.download(np.float32, got.shape) - got) <= 2 * tol).all()
