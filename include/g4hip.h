@@ -374,7 +374,9 @@ int g4h_paged_read(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int out
  * cached value reaches the rows that attend it and no others, as an infinity or
  * as NaN.  ws: g4h_paged_attn_workspace_bytes() of caller-owned scratch, 16-byte
  * aligned; it needs no initial contents and keeps nothing from call to call, but
- * calls that overlap must not share it.
+ * calls that overlap must not share it.  Its size goes by the batch's n_seq, n_tok,
+ * max_len and n_prefix and by whether it has offsets; a smaller batch may be split
+ * further and need more, so one workspace for several is the largest of theirs.
  * Asynchronous, capturable.  A row's bits depend on the batch it runs in (on
  * how the positions are split), not on the run. */
 size_t g4h_paged_attn_workspace_bytes(const g4h_paged_kv *kv, const g4h_paged_batch *batch, int n_head);
