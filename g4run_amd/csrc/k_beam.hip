@@ -9,7 +9,9 @@
 // parts', then a group's from its rows'.  Bound by the logits' bytes where they are
 // many (16 groups of 8 beams of 262144, 16 outputs: 37 us of k_beam_rows, 3.6 TB/s, and
 // 10 of k_beam_join, whose two merges are a chain of 32 rounds), by the two launches and
-// the selection's chains where they are few (4 beams of 32768, 8 outputs: 6 and 6 us).
+// the selection's chains where they are few (4 beams of 32768, 8 outputs: 6 and 6 us) or
+// the outputs many: the first bound is loose, and candidates are ranked by comparing all
+// with all (32 beams of 262144, both kernels: 8, 16, 32, 64 outputs 25, 35, 53, 245 us).
 //
 // Exactness: candidates are compared as (logit, lowest token) within a row and as
 // (score in 64 bits, lowest beam) between rows.  Sums of exponentials are fp32, under

@@ -16,10 +16,11 @@
 // groups a wave, one operand for both, halve the LDS traffic and the conversions of
 // quantized rows, but a wave then starts and ends with twice the state: 82 us there.)
 //
-// Quantized rows are bound by the VALU: of a tile of 16 rows x 32 positions x 128
-// elements (8 bits) 380 instructions and 24 transcendental ones beside 32 matrix
-// instructions; 32 drafts of up to 33 tokens over 4096 positions, 8 / 4 heads of 256,
-// capped, take 93 us, their bytes 30.
+// Quantized rows are VALU work first (operands from integers, scales, splits), and no one
+// limit: 32 drafts of up to 33 tokens over 4096 positions, 8 / 4 heads of 256, 8 bits,
+// capped, take 90 us, their bytes 30.  The VALU issues in 55 % of the SIMDs' time there,
+// the matrix cores are busy in 12 %, and the waves, two a SIMD with a barrier a step,
+// wait 45 % of theirs.  (Without a cap 87; where the scores reach the cap, 97.)
 #pragma once
 
 #include <algorithm>
